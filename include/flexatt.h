@@ -293,13 +293,153 @@ int flexatt_bwd_dkdv_ds(const flexatt_problem* p, const flexatt_tensor* q, const
 int flexatt_bwd_dq_ds(const flexatt_problem* p, const flexatt_tensor* k, const void* workspace,
                       size_t workspace_bytes, const flexatt_tensor* dq, void* stream);
 
+/* ---------------------------------------------------------------- positions
+ * and the K/V cache.  None of the entry points below has a counterpart in the
+ * reference, whose inputs are already positioned and which keeps no cache.
+ * `cache` tensors are [B, Hkv, cache_rows, D] views like any other; `lengths`
+ * is device int32 [B], the rows of each sequence that are in use. */
+
+/* Rotary positions.  Pair i of the first rotary_dim elements of a head, elements
+ * (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved, is turned by
+ * position * inv_freq[i] radians (the product in 64 bits) and scaled by
+ * magnitude; the other elements are copied.  Rounded once. */
+typedef struct flexatt_rotary {
+  int32_t dtype;        /* enum flexatt_dtype */
+  int32_t batch;        /* B */
+  int32_t heads_q;      /* Hq >= 1 */
+  int32_t heads_kv;     /* Hkv >= 0; 0: no k */
+  int32_t seqlen;       /* S, new tokens per sequence */
+  int32_t head_dim;     /* D in {32, 64, 128, 256} */
+  int32_t rotary_dim;   /* even, 0 .. D; 0: nothing is turned and inv_freq may be NULL */
+  int32_t interleaved;  /* 1: neighbouring elements are pairs */
+  int32_t inverse;      /* 1: turned backwards (the gradient) */
+  float magnitude;
+  const double* inv_freq; /* device [rotary_dim / 2] */
+  /* Position of token (b, s): positions[b * position_stride_b + s *
+   * position_stride_s], device integers of position_bytes (4 or 8) bytes.  NULL
+   * with position_bytes 0: s, or lengths[b] + s in flexatt_rotary_append. */
+  const void* positions;
+  int64_t position_stride_b, position_stride_s;
+  int32_t position_bytes;
+  int32_t reserved;     /* 0 */
+} flexatt_rotary;
+
+/* q_out = turned q [B, Hq, S, D] and k_out = turned k [B, Hkv, S, D] (both NULL
+ * when heads_kv is 0).  An output may be its own input. */
+int flexatt_rotary_apply(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* k,
+                         const flexatt_tensor* q_out, const flexatt_tensor* k_out, void* stream);
+
+/* q_out = turned q, and the rows lengths[b] .. lengths[b] + S - 1 of the cache
+ * receive turned k and v [B, Hkv, S, D].  A row outside [0, cache_rows) is not
+ * written.  `lengths` is not changed.  k and v may not overlap the cache. */
+int flexatt_rotary_append(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* k,
+                          const flexatt_tensor* v, const flexatt_tensor* q_out, const flexatt_tensor* k_cache,
+                          const flexatt_tensor* v_cache, int32_t cache_rows, const int32_t* lengths, void* stream);
+
+/* Attention of `tokens` (T) drafted tokens per sequence over the cache.  The keys
+ * of drafted token t of sequence b with n = lengths[b]: the cached rows j < n (with
+ * a window, n + depths[b][t] - j <= W), and the rows n + u, u < T, that hold the
+ * drafted tokens themselves, where tree_mask[b][t][u] is not 0 (no mask: u <= t).
+ * Scores, soft-cap, softmax and LSE as flexatt_fwd; a row without keys is 0 with
+ * LSE -inf.  A sequence with n < 0 or n + T > cache_rows gets NaN (o and lse).
+ * Rows of the cache from n + T on are not read. */
+typedef struct flexatt_tree {
+  int32_t dtype;
+  int32_t batch;
+  int32_t heads_q;
+  int32_t heads_kv;
+  int32_t tokens;         /* T >= 1 */
+  int32_t cache_rows;     /* >= 1 */
+  int32_t head_dim;
+  float scale;
+  float soft_cap;         /* 0: off */
+  int32_t sliding_window; /* W > 0; 0: off */
+  int32_t mask_batch;     /* tree_mask: 1 (one tree for all sequences) or batch; 0 with NULL */
+  int32_t reserved;       /* 0 */
+  const uint8_t* tree_mask; /* device [mask_batch][T][T], or NULL */
+  /* device int32 [B][T], depth of each token in its tree (0: directly behind the
+   * cached ones; less counts as 0); read with a window only.  NULL: t, which a
+   * window takes with a NULL tree_mask only. */
+  const int32_t* depths;
+  const int32_t* lengths;   /* device int32 [B] */
+} flexatt_tree;
+
+/* o [B, Hq, T, D] and lse fp32 [B, Hq, T].  `workspace`:
+ * flexatt_tree_fwd_workspace(p) bytes, 16-byte aligned, not zeroed, reusable once
+ * the call's work on `stream` is done; NULL when that is 0 (SIZE_MAX: p is
+ * rejected). */
+size_t flexatt_tree_fwd_workspace(const flexatt_tree* p);
+int flexatt_tree_fwd(const flexatt_tree* p, const flexatt_tensor* q, const flexatt_tensor* k_cache,
+                     const flexatt_tensor* v_cache, const flexatt_tensor* o, float* lse, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* The attention weight each key has received: sums[b][hk][j] = sum over the G
+ * query heads of KV head hk and the query rows i of exp(x_ij - lse_i), with the
+ * scores of flexatt_fwd; a masked pair and a row with lse -inf give 0.  Query row i
+ * of sequence b is at position start + i, start = query_starts[b] (NULL:
+ * query_start); causal keeps j <= start + i, a window start + i - j <= W.  Keys
+ * from lengths[b] on (NULL: seqlen_kv; values outside [0, seqlen_kv] count as the
+ * nearer end) get 0, with `accumulate` nothing. */
+typedef struct flexatt_weights {
+  int32_t dtype;
+  int32_t batch;
+  int32_t heads_q;
+  int32_t heads_kv;
+  int32_t seqlen_q;
+  int32_t seqlen_kv;
+  int32_t head_dim;
+  float scale;
+  float soft_cap;         /* 0: off */
+  int32_t causal;
+  int32_t sliding_window; /* 0: off */
+  int32_t query_start;
+  int32_t accumulate;     /* 1: added to sums */
+  int32_t reserved;       /* 0 */
+  const int32_t* query_starts; /* device int32 [B], or NULL */
+  const int32_t* lengths;      /* device int32 [B], or NULL */
+} flexatt_weights;
+
+/* sums: contiguous fp32 [B, Hkv, seqlen_kv].  `workspace` as in flexatt_tree_fwd. */
+size_t flexatt_weight_sums_workspace(const flexatt_weights* p);
+int flexatt_weight_sums(const flexatt_weights* p, const flexatt_tensor* q, const flexatt_tensor* k, const float* lse,
+                        float* sums, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Eviction.  Of the n = lengths[b] rows (clamped to [0, cache_rows]) of each KV
+ * head, n > keep, the first `sinks`, the last `recent` and the keep - sinks -
+ * recent others with the largest scores stay (of equal ones the lowest rows; NaN is
+ * the largest score), in row order; n <= keep: all stay.  They are copied to the
+ * first rows of k_out and v_out, their scores to scores_out, their rows' numbers
+ * to slots (-1 behind), and min(n, keep) to lengths_out.  Rows of k_out and v_out
+ * behind them are left as they were, or with `fill` zeroed up to row keep - 1;
+ * scores_out is 0 behind them. */
+typedef struct flexatt_evict {
+  int32_t dtype;
+  int32_t batch;
+  int32_t heads_kv;
+  int32_t cache_rows;
+  int32_t head_dim;
+  int32_t keep;      /* >= 1 */
+  int32_t recent;    /* >= 0 */
+  int32_t sinks;     /* >= 0; recent + sinks <= keep */
+  int32_t out_rows;  /* rows of k_out, v_out and scores_out, >= keep */
+  int32_t fill;
+  const int32_t* lengths; /* device int32 [B] */
+} flexatt_evict;
+
+/* scores: contiguous fp32 [B, Hkv, cache_rows]; scores_out [B, Hkv, out_rows];
+ * slots int32 [B, Hkv, keep]; lengths_out int32 [B].  No output may
+ * overlap an input. */
+int flexatt_evict_rows(const flexatt_evict* p, const flexatt_tensor* k_cache, const flexatt_tensor* v_cache,
+                       const float* scores, const flexatt_tensor* k_out, const flexatt_tensor* v_out,
+                       float* scores_out, int32_t* slots, int32_t* lengths_out, void* stream);
+
 /* Human-readable text for a status code (static storage). */
 const char* flexatt_status_string(int status);
 
 /* ABI version of this header (bumped on any signature change). */
 int flexatt_abi_version(void);
 
-#define FLEXATT_ABI_VERSION 8
+#define FLEXATT_ABI_VERSION 9
 
 #ifdef __cplusplus
 }

@@ -3,33 +3,14 @@
 #include <math.h>
 #include <stdint.h>
 
-#include <atomic>
 #include <mutex>
 
 #include "../../include/flexatt.h"
+#include "capi_checks.h"
 #include "flexatt_kernels.h"
 
 namespace {
 using namespace flexatt;
-
-size_t elt_size(int dt) {
-  switch (dt) {
-    case FLEXATT_F32: return 4;
-    case FLEXATT_F16:
-    case FLEXATT_BF16: return 2;
-    default: return 0;
-  }
-}
-
-int head_index(int d) {
-  switch (d) {
-    case 32: return 0;
-    case 64: return 1;
-    case 128: return 2;
-    case 256: return 3;
-    default: return -1;
-  }
-}
 
 int check_problem(const flexatt_problem* p) {
   if (!p) return FLEXATT_EINVAL;
@@ -52,49 +33,6 @@ int check_problem(const flexatt_problem* p) {
   const int64_t rows_q = (int64_t)p->batch * p->heads_q * p->seqlen_q;
   const int64_t rows_k = (int64_t)p->batch * p->heads_kv * p->seqlen_kv;
   if (rows_q > INT32_MAX || rows_k > INT32_MAX) return FLEXATT_ESHAPE;
-  return FLEXATT_OK;
-}
-
-#define FLEXATT_TRY_OK(x)               \
-  do {                                  \
-    const int rc_ = (x);                \
-    if (rc_ != FLEXATT_OK) return rc_;  \
-  } while (0)
-
-int check_tensor(const flexatt_tensor* t, int dt) {
-  if (!t || !t->data) return FLEXATT_EINVAL;
-  const int64_t es = (int64_t)elt_size(dt);
-  if (t->stride_d != 1) return FLEXATT_ELAYOUT;
-  if (t->stride_b < 0 || t->stride_h < 0 || t->stride_s < 0) return FLEXATT_ELAYOUT;
-  if (((uintptr_t)t->data) % 16 != 0) return FLEXATT_ELAYOUT;
-  if ((t->stride_b * es) % 16 || (t->stride_h * es) % 16 || (t->stride_s * es) % 16) return FLEXATT_ELAYOUT;
-  return FLEXATT_OK;
-}
-
-// Output tensors: the input rules, and no two elements of the [b, h, s, d]
-// index space may share an address (several workgroups would store to it,
-// and the results would depend on their order).  Sufficient test: over the
-// dimensions of extent > 1 sorted by stride, each stride exceeds the span of
-// the smaller ones.
-int check_out_tensor(const flexatt_tensor* t, int dt, int64_t n_b, int64_t n_h, int64_t n_s, int64_t n_d) {
-  FLEXATT_TRY_OK(check_tensor(t, dt));
-  int64_t st[4] = {t->stride_b, t->stride_h, t->stride_s, 1};
-  int64_t ext[4] = {n_b, n_h, n_s, n_d};
-  int order[4], n = 0;
-  for (int i = 0; i < 4; ++i)
-    if (ext[i] > 1) order[n++] = i;
-  for (int i = 1; i < n; ++i)  // insertion sort by stride
-    for (int j = i; j > 0 && st[order[j]] < st[order[j - 1]]; --j) {
-      const int x = order[j];
-      order[j] = order[j - 1];
-      order[j - 1] = x;
-    }
-  int64_t span = 0;  // largest offset reachable with the dims sorted so far
-  for (int i = 0; i < n; ++i) {
-    const int d = order[i];
-    if (st[d] <= span) return FLEXATT_ELAYOUT;
-    span += (ext[d] - 1) * st[d];
-  }
   return FLEXATT_OK;
 }
 
@@ -130,9 +68,6 @@ Shape make_shape(const flexatt_problem* p) {
   s.blk_nk = (p->seqlen_kv + kBlk - 1) / kBlk;
   return s;
 }
-
-View view(const flexatt_tensor* t) { return View{t->data, t->stride_b, t->stride_h, t->stride_s}; }
-MutView mview(const flexatt_tensor* t) { return MutView{t->data, t->stride_b, t->stride_h, t->stride_s}; }
 
 // [dtype][head index]
 const FwdLauncher kFwd[3][4] = {
@@ -219,7 +154,6 @@ int decode_run(const flexatt_problem* p, const DecodePlan& d, const flexatt_tens
 // the device address of each GPU's copy is looked up once, with that GPU
 // current, and kept in scratch_ptr.
 static __device__ __align__(256) unsigned char scratch[FLEXATT_NOALLOC_SCRATCH_BYTES];
-constexpr int kMaxDevices = 64;
 std::mutex scratch_mu;
 void* scratch_ptr[kMaxDevices] = {};
 
@@ -267,32 +201,6 @@ bool dq_fuses_delta(const flexatt_problem* p) {
   return f == bwd_q_bf16_d128 || f == bwd_q_f16_d128 || f == bwd_q_bf16_d64 || f == bwd_q_f16_d64;
 }
 BwdLauncher pick_dkdv(const flexatt_problem* p) { return kDkdv[p->dtype][head_index(p->head_dim)]; }
-
-#define FLEXATT_TRY(x)             \
-  do {                             \
-    const int rc_ = (x);           \
-    if (rc_ != FLEXATT_OK) return rc_; \
-  } while (0)
-
-// CUs of the current device (cached per device), 0 if unknown.  Host threads
-// may call the ABI concurrently: the cache is atomic (a racing first lookup
-// stores the same value twice).
-int cu_count() {
-  static std::atomic<int> cache[kMaxDevices];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) return 0;
-  int n = cache[dev].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 0;
-    cache[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
-
-int cus() {  // 256 if unknown
-  const int n = cu_count();
-  return n > 0 ? n : 256;
-}
 
 // Attended (query row, key) pairs of one head under the causal and window
 // masks (interval masks, whose bounds are on the device, not counted).

@@ -1,0 +1,306 @@
+// extern "C" entry points around positions and the K/V cache (declared in
+// include/flexatt.h): argument checks, then the kernel launchers.
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/flexatt.h"
+#include "capi_checks.h"
+#include "flexatt_kernels.h"
+
+namespace {
+using namespace flexatt;
+
+// The bytes a [b, h, s, d] view spans.
+struct Span {
+  uintptr_t lo, hi;
+};
+Span span_of(const flexatt_tensor* t, int dt, int64_t n_b, int64_t n_h, int64_t n_s, int64_t n_d) {
+  const int64_t last = (n_b - 1) * t->stride_b + (n_h - 1) * t->stride_h + (n_s - 1) * t->stride_s + n_d;
+  return Span{(uintptr_t)t->data, (uintptr_t)t->data + (uintptr_t)(last * (int64_t)elt_size(dt))};
+}
+Span span_of(const void* p, size_t bytes) { return Span{(uintptr_t)p, (uintptr_t)p + bytes}; }
+bool overlap(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
+
+int check_sizes(int dtype, int64_t b, int64_t h, int64_t s, int head_dim) {
+  if (elt_size(dtype) == 0) return FLEXATT_EDTYPE;
+  if (b <= 0 || h <= 0 || s <= 0) return FLEXATT_EINVAL;
+  if (head_index(head_dim) < 0) return FLEXATT_EHEADDIM;
+  if (b * h > INT32_MAX || b * h * s > INT32_MAX) return FLEXATT_ESHAPE;
+  return FLEXATT_OK;
+}
+
+int check_rotary(const flexatt_rotary* r) {
+  if (!r) return FLEXATT_EINVAL;
+  FLEXATT_TRY(check_sizes(r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
+  if (r->heads_kv < 0) return FLEXATT_EINVAL;
+  if (r->heads_kv > 0) FLEXATT_TRY(check_sizes(r->dtype, r->batch, r->heads_kv, r->seqlen, r->head_dim));
+  if (r->rotary_dim < 0 || r->rotary_dim > r->head_dim || r->rotary_dim % 2) return FLEXATT_EINVAL;
+  if (r->rotary_dim > 0 && !r->inv_freq) return FLEXATT_EINVAL;
+  if ((r->interleaved & ~1) || (r->inverse & ~1) || r->reserved != 0 || !isfinite(r->magnitude))
+    return FLEXATT_EINVAL;
+  if (r->positions ? r->position_bytes != 4 && r->position_bytes != 8 : r->position_bytes != 0) return FLEXATT_EINVAL;
+  if (((uintptr_t)r->inv_freq) % 8 || (r->positions && ((uintptr_t)r->positions) % r->position_bytes))
+    return FLEXATT_ELAYOUT;
+  return FLEXATT_OK;
+}
+
+RotaryArgs rotary_args(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* qo) {
+  RotaryArgs a = {};
+  a.q = view(q);
+  a.qo = mview(qo);
+  a.inv_freq = r->inv_freq;
+  a.positions = r->positions;
+  a.pos_sb = r->position_stride_b;
+  a.pos_ss = r->position_stride_s;
+  a.pos_bytes = r->position_bytes;
+  a.B = r->batch;
+  a.Hq = r->heads_q;
+  a.Hkv = r->heads_kv;
+  a.S = r->seqlen;
+  a.D = r->head_dim;
+  a.rotary = r->rotary_dim;
+  a.inter = r->interleaved;
+  a.mag = r->magnitude;
+  a.sign = r->inverse ? -1.0f : 1.0f;
+  a.heads = r->heads_q + r->heads_kv;
+  return a;
+}
+
+// [dtype][head index]
+const TreeLauncher kTree[3][4] = {
+    {tree_attn_f32_d32, tree_attn_f32_d64, tree_attn_f32_d128, tree_attn_f32_d256},
+    {tree_attn_f16_d32, tree_attn_f16_d64, tree_attn_f16_d128, tree_attn_f16_d256},
+    {tree_attn_bf16_d32, tree_attn_bf16_d64, tree_attn_bf16_d128, tree_attn_bf16_d256},
+};
+const WeightLauncher kWeights[3][4] = {
+    {weight_sums_f32_d32, weight_sums_f32_d64, weight_sums_f32_d128, weight_sums_f32_d256},
+    {weight_sums_f16_d32, weight_sums_f16_d64, weight_sums_f16_d128, weight_sums_f16_d256},
+    {weight_sums_bf16_d32, weight_sums_bf16_d64, weight_sums_bf16_d128, weight_sums_bf16_d256},
+};
+
+int check_scores(float scale, float cap, int window) {
+  if (!(cap >= 0.f) || !isfinite(cap) || !isfinite(scale) || window < 0) return FLEXATT_EINVAL;
+  return FLEXATT_OK;
+}
+
+// The score parameters of a Shape without causal, ALiBi, interval and block masks.
+Shape score_shape(int B, int Hq, int Hkv, int Sq, int Skv, float scale, float cap, int window) {
+  Shape s = {};
+  s.B = B;
+  s.Hq = Hq;
+  s.Hkv = Hkv;
+  s.G = Hq / Hkv;
+  s.Sq = Sq;
+  s.Skv = Skv;
+  s.scale = scale;
+  s.scale_log2 = scale * kLog2e;
+  s.window = window;
+  s.cap = cap;
+  s.inv_cap = cap > 0.f ? 1.0f / cap : 0.f;
+  s.tanh_k = cap > 0.f ? 2.0f * kLog2e * scale / cap : 0.f;
+  s.cap_log2 = cap * kLog2e;
+  s.blk_h = 1;
+  return s;
+}
+
+int check_tree(const flexatt_tree* p) {
+  if (!p) return FLEXATT_EINVAL;
+  FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_q, p->tokens, p->head_dim));
+  FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim));
+  if (p->heads_q % p->heads_kv != 0) return FLEXATT_ESHAPE;
+  FLEXATT_TRY(check_scores(p->scale, p->soft_cap, p->sliding_window));
+  if (p->reserved != 0 || !p->lengths) return FLEXATT_EINVAL;
+  if (p->tree_mask ? p->mask_batch != 1 && p->mask_batch != p->batch : p->mask_batch != 0) return FLEXATT_EINVAL;
+  if (p->sliding_window > 0 && p->tree_mask && !p->depths) return FLEXATT_EINVAL;
+  return FLEXATT_OK;
+}
+
+// Workgroups per row tile at most (each sequence takes as many of them as its own
+// length is worth, in the kernel): about two per CU in all, two tiles per wave at
+// least if the cache is full.
+int tree_splits(const flexatt_tree* p) {
+  const int64_t rows = (int64_t)(p->heads_q / p->heads_kv) * p->tokens;
+  const int64_t groups = (int64_t)p->batch * p->heads_kv * ((rows + 31) / 32);
+  const int nw = p->head_dim * elt_size(p->dtype) <= 512 ? 4 : 2;  // (TreeCfg)
+  int64_t ns = (512 + groups - 1) / groups;
+  const int64_t most = (p->cache_rows + 31) / 32 / (2 * nw);
+  if (ns > most) ns = most;
+  if (ns > 256) ns = 256;
+  return ns < 1 ? 1 : (int)ns;
+}
+
+int check_weights(const flexatt_weights* p) {
+  if (!p) return FLEXATT_EINVAL;
+  FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_q, p->seqlen_q, p->head_dim));
+  FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_kv, p->seqlen_kv, p->head_dim));
+  if (p->heads_q % p->heads_kv != 0) return FLEXATT_ESHAPE;
+  FLEXATT_TRY(check_scores(p->scale, p->soft_cap, p->sliding_window));
+  if ((p->causal & ~1) || (p->accumulate & ~1) || p->reserved != 0) return FLEXATT_EINVAL;
+  return FLEXATT_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int flexatt_rotary_apply(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* k,
+                         const flexatt_tensor* q_out, const flexatt_tensor* k_out, void* stream) {
+  FLEXATT_TRY(check_rotary(r));
+  FLEXATT_TRY(check_tensor(q, r->dtype));
+  FLEXATT_TRY(check_out_tensor(q_out, r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
+  if (r->heads_kv == 0 && (k || k_out)) return FLEXATT_EINVAL;
+  RotaryArgs a = rotary_args(r, q, q_out);
+  if (r->heads_kv > 0) {
+    FLEXATT_TRY(check_tensor(k, r->dtype));
+    FLEXATT_TRY(check_out_tensor(k_out, r->dtype, r->batch, r->heads_kv, r->seqlen, r->head_dim));
+    a.k = view(k);
+    a.ko = mview(k_out);
+  }
+  return (int)rotary_run(r->dtype, a, (hipStream_t)stream);
+}
+
+int flexatt_rotary_append(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* k,
+                          const flexatt_tensor* v, const flexatt_tensor* q_out, const flexatt_tensor* k_cache,
+                          const flexatt_tensor* v_cache, int32_t cache_rows, const int32_t* lengths, void* stream) {
+  FLEXATT_TRY(check_rotary(r));
+  if (r->heads_kv == 0 || cache_rows <= 0 || !lengths) return FLEXATT_EINVAL;
+  if ((int64_t)r->batch * r->heads_kv * cache_rows > INT32_MAX) return FLEXATT_ESHAPE;
+  FLEXATT_TRY(check_tensor(q, r->dtype));
+  FLEXATT_TRY(check_tensor(k, r->dtype));
+  FLEXATT_TRY(check_tensor(v, r->dtype));
+  FLEXATT_TRY(check_out_tensor(q_out, r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
+  FLEXATT_TRY(check_out_tensor(k_cache, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim));
+  FLEXATT_TRY(check_out_tensor(v_cache, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim));
+  for (const flexatt_tensor* x : {k, v})
+    for (const flexatt_tensor* y : {k_cache, v_cache})
+      if (overlap(span_of(x, r->dtype, r->batch, r->heads_kv, r->seqlen, r->head_dim),
+                  span_of(y, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim)))
+        return FLEXATT_ELAYOUT;
+  RotaryArgs a = rotary_args(r, q, q_out);
+  a.k = view(k);
+  a.v = view(v);
+  a.ko = mview(k_cache);
+  a.vo = mview(v_cache);
+  a.cache_rows = cache_rows;
+  a.lengths = lengths;
+  a.heads += r->heads_kv;
+  return (int)rotary_run(r->dtype, a, (hipStream_t)stream);
+}
+
+size_t flexatt_tree_fwd_workspace(const flexatt_tree* p) {
+  if (check_tree(p) != FLEXATT_OK) return SIZE_MAX;
+  const int ns = tree_splits(p);
+  if (ns == 1) return 0;
+  return (size_t)p->batch * p->heads_q * p->tokens * ns * (p->head_dim + 1) * sizeof(float);
+}
+
+int flexatt_tree_fwd(const flexatt_tree* p, const flexatt_tensor* q, const flexatt_tensor* k_cache,
+                     const flexatt_tensor* v_cache, const flexatt_tensor* o, float* lse, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  FLEXATT_TRY(check_tree(p));
+  FLEXATT_TRY(check_tensor(q, p->dtype));
+  FLEXATT_TRY(check_tensor(k_cache, p->dtype));
+  FLEXATT_TRY(check_tensor(v_cache, p->dtype));
+  FLEXATT_TRY(check_out_tensor(o, p->dtype, p->batch, p->heads_q, p->tokens, p->head_dim));
+  if (!lse) return FLEXATT_EINVAL;
+  const size_t need = flexatt_tree_fwd_workspace(p);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need) return FLEXATT_EINVAL;
+    if (((uintptr_t)workspace) % 16 != 0) return FLEXATT_ELAYOUT;
+  }
+  TreeArgs a = {};
+  a.q = view(q);
+  a.k = view(k_cache);
+  a.v = view(v_cache);
+  a.o = mview(o);
+  a.lse = lse;
+  a.nsplit = tree_splits(p);
+  a.part_o = (float*)workspace;
+  a.part_lse = a.nsplit > 1 ? a.part_o + (int64_t)p->batch * p->heads_q * p->tokens * a.nsplit * p->head_dim : nullptr;
+  a.lengths = p->lengths;
+  a.mask = p->tree_mask;
+  a.mask_sb = p->mask_batch > 1 ? (int64_t)p->tokens * p->tokens : 0;
+  a.depths = p->depths;
+  a.p = score_shape(p->batch, p->heads_q, p->heads_kv, p->tokens, p->cache_rows, p->scale, p->soft_cap,
+                    p->sliding_window);
+  return (int)kTree[p->dtype][head_index(p->head_dim)](a, (hipStream_t)stream);
+}
+
+size_t flexatt_weight_sums_workspace(const flexatt_weights* p) {
+  if (check_weights(p) != FLEXATT_OK) return SIZE_MAX;
+  return 0;
+}
+
+int flexatt_weight_sums(const flexatt_weights* p, const flexatt_tensor* q, const flexatt_tensor* k, const float* lse,
+                        float* sums, void* workspace, size_t workspace_bytes, void* stream) {
+  FLEXATT_TRY(check_weights(p));
+  FLEXATT_TRY(check_tensor(q, p->dtype));
+  FLEXATT_TRY(check_tensor(k, p->dtype));
+  if (!lse || !sums) return FLEXATT_EINVAL;
+  const size_t need = flexatt_weight_sums_workspace(p);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need) return FLEXATT_EINVAL;
+    if (((uintptr_t)workspace) % 16 != 0) return FLEXATT_ELAYOUT;
+  }
+  WeightArgs a = {};
+  a.q = view(q);
+  a.k = view(k);
+  a.lse = lse;
+  a.sums = sums;
+  a.lengths = p->lengths;
+  a.starts = p->query_starts;
+  a.start = p->query_start;
+  a.add = p->accumulate;
+  a.p = score_shape(p->batch, p->heads_q, p->heads_kv, p->seqlen_q, p->seqlen_kv, p->scale, p->soft_cap,
+                    p->sliding_window);
+  a.p.causal = p->causal;
+  return (int)kWeights[p->dtype][head_index(p->head_dim)](a, (hipStream_t)stream);
+}
+
+int flexatt_evict_rows(const flexatt_evict* p, const flexatt_tensor* k_cache, const flexatt_tensor* v_cache,
+                       const float* scores, const flexatt_tensor* k_out, const flexatt_tensor* v_out,
+                       float* scores_out, int32_t* slots, int32_t* lengths_out, void* stream) {
+  if (!p) return FLEXATT_EINVAL;
+  FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim));
+  if (p->keep < 1 || p->recent < 0 || p->sinks < 0 || p->out_rows < p->keep || (p->fill & ~1)) return FLEXATT_EINVAL;
+  if ((int64_t)p->recent + p->sinks > p->keep) return FLEXATT_EINVAL;
+  FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_kv, p->out_rows, p->head_dim));
+  if (!p->lengths || !scores || !scores_out || !slots || !lengths_out) return FLEXATT_EINVAL;
+  FLEXATT_TRY(check_tensor(k_cache, p->dtype));
+  FLEXATT_TRY(check_tensor(v_cache, p->dtype));
+  FLEXATT_TRY(check_out_tensor(k_out, p->dtype, p->batch, p->heads_kv, p->out_rows, p->head_dim));
+  FLEXATT_TRY(check_out_tensor(v_out, p->dtype, p->batch, p->heads_kv, p->out_rows, p->head_dim));
+  const int64_t bh = (int64_t)p->batch * p->heads_kv;
+  const Span in[] = {span_of(k_cache, p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim),
+                     span_of(v_cache, p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim),
+                     span_of(scores, bh * p->cache_rows * 4), span_of(p->lengths, p->batch * 4)};
+  const Span out[] = {span_of(k_out, p->dtype, p->batch, p->heads_kv, p->out_rows, p->head_dim),
+                      span_of(v_out, p->dtype, p->batch, p->heads_kv, p->out_rows, p->head_dim),
+                      span_of(scores_out, bh * p->out_rows * 4), span_of(slots, bh * p->keep * 4),
+                      span_of(lengths_out, p->batch * 4)};
+  for (const Span& x : in)
+    for (const Span& y : out)
+      if (overlap(x, y)) return FLEXATT_ELAYOUT;
+  EvictArgs a = {};
+  a.k = view(k_cache);
+  a.v = view(v_cache);
+  a.ko = mview(k_out);
+  a.vo = mview(v_out);
+  a.scores = scores;
+  a.scores_out = scores_out;
+  a.slots = slots;
+  a.lengths = p->lengths;
+  a.lengths_out = lengths_out;
+  a.B = p->batch;
+  a.H = p->heads_kv;
+  a.C = p->cache_rows;
+  a.D = p->head_dim;
+  a.keep = p->keep;
+  a.recent = p->recent;
+  a.sinks = p->sinks;
+  a.out_rows = p->out_rows;
+  a.fill = p->fill;
+  a.es = (int)elt_size(p->dtype);
+  return (int)evict_run(a, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -79,6 +79,64 @@ struct BwdSplitArgs {
   int nrt;      // 32-row tiles of packed query rows per (b, hkv) (set by the launcher)
 };
 
+// Rotary positions, out of place or into a cache (rotary.hip).
+struct RotaryArgs {
+  View q, k, v;        // k with Hkv > 0, v with the append
+  MutView qo, ko, vo;  // ko, vo: the cache with cache_rows > 0
+  const double* inv_freq;
+  const void* positions;  // int32 or int64 (pos_bytes), or pos_bytes 0: the token's slot
+  int64_t pos_sb, pos_ss;
+  const int* lengths;     // [B], the append
+  int B, Hq, Hkv, S, D, rotary, inter, pos_bytes, cache_rows;
+  int heads;  // q, k and v heads walked in all
+  int hpt;    // heads per thread (set by the launcher)
+  float mag, sign;
+};
+
+// Attention of a tree of drafted tokens over a cache (tree_attn.hip).
+struct TreeArgs {
+  View q, k, v;
+  MutView o;
+  float* lse;
+  float* part_o;    // [B * Hq * T][nsplit][D], O of each partial / its row sums
+  float* part_lse;  // [B * Hq * T][nsplit], LSE of each partial in log2 units
+  const int* lengths;          // [B]
+  const unsigned char* mask;   // [1 or B][T][T], or nullptr: a chain
+  int64_t mask_sb;
+  const int* depths;           // [B][T] with a window, or nullptr: t
+  Shape p;  // Sq: T, Skv: rows of the cache
+  int nsplit;  // most workgroups per row tile
+  int nrt;     // row tiles of packed query rows per (b, hkv) (set by the launcher)
+};
+
+// Attention weight received by each key (weight_sums.hip).
+struct WeightArgs {
+  View q, k;
+  const float* lse;   // [B][Hq][Sq]
+  float* sums;        // [B][Hkv][Skv]
+  const int* lengths;  // [B] or nullptr: Skv
+  const int* starts;   // [B] or nullptr: start
+  Shape p;
+  int start;  // position of the first query row
+  int add;    // 1: added to what sums holds
+};
+
+// Eviction (evict.hip).
+struct EvictArgs {
+  View k, v;
+  MutView ko, vo;
+  const float* scores;  // [B][H][C]
+  float* scores_out;    // [B][H][out_rows]
+  int* slots;           // [B][H][keep]
+  const int* lengths;
+  int* lengths_out;
+  int B, H, C, D, keep, recent, sinks, out_rows;
+  int fill;  // 1: rows of ko and vo behind the last kept one, up to keep, are zeroed
+  int es;    // bytes per element
+};
+
+typedef hipError_t (*TreeLauncher)(const TreeArgs&, hipStream_t);
+typedef hipError_t (*WeightLauncher)(const WeightArgs&, hipStream_t);
 typedef hipError_t (*FwdLauncher)(const FwdArgs&, hipStream_t);
 typedef hipError_t (*DecodeLauncher)(const DecodeArgs&, hipStream_t);
 typedef hipError_t (*BwdLauncher)(const BwdArgs&, hipStream_t);
@@ -108,6 +166,24 @@ bool fwd_ws_fits(const Shape& p);  // its LDS (with a block map's lists) fits on
 hipError_t doc_bounds_run(const void* ids, int ids_bytes, int B, int S, int* bounds, hipStream_t);
 
 hipError_t bwd_delta(int dtype, const DeltaArgs&, hipStream_t);
+
+hipError_t rotary_run(int dtype, const RotaryArgs&, hipStream_t);
+hipError_t evict_run(const EvictArgs&, hipStream_t);
+
+// Tree attention (tree_attn.hip) and weight sums (weight_sums.hip), every D.
+#define FLEXATT_DECL_CACHE(D)                              \
+  hipError_t tree_attn_bf16_d##D(const TreeArgs&, hipStream_t); \
+  hipError_t tree_attn_f16_d##D(const TreeArgs&, hipStream_t);  \
+  hipError_t tree_attn_f32_d##D(const TreeArgs&, hipStream_t);  \
+  hipError_t weight_sums_bf16_d##D(const WeightArgs&, hipStream_t); \
+  hipError_t weight_sums_f16_d##D(const WeightArgs&, hipStream_t);  \
+  hipError_t weight_sums_f32_d##D(const WeightArgs&, hipStream_t);
+
+FLEXATT_DECL_CACHE(32)
+FLEXATT_DECL_CACHE(64)
+FLEXATT_DECL_CACHE(128)
+FLEXATT_DECL_CACHE(256)
+#undef FLEXATT_DECL_CACHE
 
 // Split-KV forward (fwd_split.hip).
 hipError_t fwd_split_bf16_d32(const DecodeArgs&, hipStream_t);

@@ -39,10 +39,17 @@ EXPORTS = (
     "flexatt_bwd_ws_parts_bytes",
     "flexatt_bwd_dkdv_ds",
     "flexatt_bwd_dq_ds",
+    "flexatt_rotary_apply",
+    "flexatt_rotary_append",
+    "flexatt_tree_fwd_workspace",
+    "flexatt_tree_fwd",
+    "flexatt_weight_sums_workspace",
+    "flexatt_weight_sums",
+    "flexatt_evict_rows",
     "flexatt_status_string",
     "flexatt_abi_version",
 )
-ABI_VERSION = 8
+ABI_VERSION = 9
 # Fixed scratch of flexatt_fwd_decode_noalloc (FLEXATT_NOALLOC_SCRATCH_BYTES).
 NOALLOC_SCRATCH_BYTES = 16 << 20
 # Work-queue counters at the end of the staged-dS workspace (FLEXATT_BWD_QUEUE_BYTES).
@@ -85,6 +92,63 @@ class Problem(ctypes.Structure):
     ]
 
 
+class Rotary(ctypes.Structure):
+    """``flexatt_rotary``: rotary positions of new tokens."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "batch", "heads_q", "heads_kv", "seqlen", "head_dim",
+                                              "rotary_dim", "interleaved", "inverse")] + [
+        ("magnitude", ctypes.c_float),
+        ("inv_freq", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("position_stride_b", ctypes.c_int64),
+        ("position_stride_s", ctypes.c_int64),
+        ("position_bytes", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class Tree(ctypes.Structure):
+    """``flexatt_tree``: drafted tokens over a K/V cache."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "batch", "heads_q", "heads_kv", "tokens", "cache_rows",
+                                              "head_dim")] + [
+        ("scale", ctypes.c_float),
+        ("soft_cap", ctypes.c_float),
+        ("sliding_window", ctypes.c_int32),
+        ("mask_batch", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("tree_mask", ctypes.c_void_p),
+        ("depths", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+    ]
+
+
+class Weights(ctypes.Structure):
+    """``flexatt_weights``: attention weight received by keys."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "batch", "heads_q", "heads_kv", "seqlen_q", "seqlen_kv",
+                                              "head_dim")] + [
+        ("scale", ctypes.c_float),
+        ("soft_cap", ctypes.c_float),
+        ("causal", ctypes.c_int32),
+        ("sliding_window", ctypes.c_int32),
+        ("query_start", ctypes.c_int32),
+        ("accumulate", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("query_starts", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+    ]
+
+
+class Evict(ctypes.Structure):
+    """``flexatt_evict``: eviction from a K/V cache."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "batch", "heads_kv", "cache_rows", "head_dim", "keep",
+                                              "recent", "sinks", "out_rows", "fill")] + [
+        ("lengths", ctypes.c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -122,6 +186,11 @@ def load() -> ctypes.CDLL:
         "flexatt_bwd_split": [pr, T, T, T, T, T, fp, fp, T, T, T, fp, ctypes.c_size_t, st],
         "flexatt_bwd_dkdv_ds": [pr, T, T, T, T, fp, fp, T, T, fp, ctypes.c_size_t, st],
         "flexatt_bwd_dq_ds": [pr, T, fp, ctypes.c_size_t, T, st],
+        "flexatt_rotary_apply": [P(Rotary), T, T, T, T, st],
+        "flexatt_rotary_append": [P(Rotary), T, T, T, T, T, T, ctypes.c_int32, fp, st],
+        "flexatt_tree_fwd": [P(Tree), T, T, T, T, fp, fp, ctypes.c_size_t, st],
+        "flexatt_weight_sums": [P(Weights), T, T, fp, fp, fp, ctypes.c_size_t, st],
+        "flexatt_evict_rows": [P(Evict), T, T, fp, T, T, fp, fp, fp, st],
     }
     for name, args in sig.items():
         fn = getattr(lib, name)
@@ -130,6 +199,9 @@ def load() -> ctypes.CDLL:
     for name in ("flexatt_fwd_decode_workspace", "flexatt_fwd_split_workspace", "flexatt_bwd_workspace",
                  "flexatt_bwd_split_workspace", "flexatt_bwd_ws_parts_bytes"):
         getattr(lib, name).argtypes = [pr]
+        getattr(lib, name).restype = ctypes.c_size_t
+    for name, arg in (("flexatt_tree_fwd_workspace", P(Tree)), ("flexatt_weight_sums_workspace", P(Weights))):
+        getattr(lib, name).argtypes = [arg]
         getattr(lib, name).restype = ctypes.c_size_t
     lib.flexatt_bwd_workspace_limited.argtypes = [pr, ctypes.c_size_t]
     lib.flexatt_bwd_workspace_limited.restype = ctypes.c_size_t
