@@ -138,6 +138,20 @@ int check_weights(const flexatt_weights* p) {
   if ((p->causal & ~1) || (p->accumulate & ~1) || p->reserved != 0) return FLEXATT_EINVAL;
   return FLEXATT_OK;
 }
+
+// Workgroups that share the query rows of one block of keys: enough for eight per
+// CU in all, of four row tiles at least.
+int weight_parts(const flexatt_weights* p) {
+  const int keys = p->head_dim * elt_size(p->dtype) <= 512 ? 256 : 128;  // (WsCfg)
+  const int64_t wgs = (int64_t)((p->seqlen_kv + keys - 1) / keys) * p->batch * p->heads_kv;
+  int64_t rows = p->seqlen_q;
+  if (p->sliding_window > 0 && rows > (int64_t)p->sliding_window + keys) rows = (int64_t)p->sliding_window + keys;
+  const int64_t tiles = (rows * (p->heads_q / p->heads_kv) + 31) / 32;
+  int64_t n = (8 * cus() + wgs - 1) / wgs;
+  if (n > tiles / 4) n = tiles / 4;
+  if (n > 64) n = 64;
+  return n < 1 ? 1 : (int)n;
+}
 }  // namespace
 
 extern "C" {
@@ -227,7 +241,8 @@ int flexatt_tree_fwd(const flexatt_tree* p, const flexatt_tensor* q, const flexa
 
 size_t flexatt_weight_sums_workspace(const flexatt_weights* p) {
   if (check_weights(p) != FLEXATT_OK) return SIZE_MAX;
-  return 0;
+  const int n = weight_parts(p);
+  return n == 1 ? 0 : (size_t)n * p->batch * p->heads_kv * p->seqlen_kv * sizeof(float);
 }
 
 int flexatt_weight_sums(const flexatt_weights* p, const flexatt_tensor* q, const flexatt_tensor* k, const float* lse,
@@ -250,6 +265,8 @@ int flexatt_weight_sums(const flexatt_weights* p, const flexatt_tensor* q, const
   a.starts = p->query_starts;
   a.start = p->query_start;
   a.add = p->accumulate;
+  a.part = (float*)workspace;
+  a.nparts = weight_parts(p);
   a.p = score_shape(p->batch, p->heads_q, p->heads_kv, p->seqlen_q, p->seqlen_kv, p->scale, p->soft_cap,
                     p->sliding_window);
   a.p.causal = p->causal;

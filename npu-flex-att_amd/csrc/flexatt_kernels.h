@@ -119,6 +119,8 @@ struct WeightArgs {
   Shape p;
   int start;  // position of the first query row
   int add;    // 1: added to what sums holds
+  float* part;  // nparts > 1: [nparts][B][Hkv][Skv]
+  int nparts;   // workgroups that share the query rows of a block of keys
 };
 
 // Eviction (evict.hip).
