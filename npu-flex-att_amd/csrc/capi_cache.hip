@@ -139,18 +139,25 @@ int check_weights(const flexatt_weights* p) {
   return FLEXATT_OK;
 }
 
-// Workgroups that share the query rows of one block of keys: enough for eight per
-// CU in all, of four row tiles at least.
+// Workgroups that share the query rows of one pair of key blocks: the number whose
+// rounds of workgroups (two per CU, one with rows of 512 bytes) take least, with
+// about four row tiles' time to load and add up each block.
 int weight_parts(const flexatt_weights* p) {
-  const int keys = p->head_dim * elt_size(p->dtype) <= 512 ? 256 : 128;  // (WsCfg)
-  const int64_t wgs = (int64_t)((p->seqlen_kv + keys - 1) / keys) * p->batch * p->heads_kv;
+  const int rowb = p->head_dim * (int)elt_size(p->dtype);
+  const int keys = rowb <= 512 ? 256 : 128;  // (WsCfg)
+  const int64_t nkb = (p->seqlen_kv + keys - 1) / keys;
+  const int64_t pairs = (nkb + 1) / 2 * p->batch * p->heads_kv, slots = (rowb >= 512 ? 1 : 2) * cus();
   int64_t rows = p->seqlen_q;
   if (p->sliding_window > 0 && rows > (int64_t)p->sliding_window + keys) rows = (int64_t)p->sliding_window + keys;
-  const int64_t tiles = (rows * (p->heads_q / p->heads_kv) + 31) / 32;
-  int64_t n = (8 * cus() + wgs - 1) / wgs;
-  if (n > tiles / 4) n = tiles / 4;
-  if (n > 64) n = 64;
-  return n < 1 ? 1 : (int)n;
+  int64_t tiles = (rows * (p->heads_q / p->heads_kv) + 31) / 32;  // that a block of keys is seen by at most
+  const bool half = p->causal && p->sliding_window == 0 && p->seqlen_q > p->seqlen_kv / 2;
+  const int64_t work = (nkb > 1 && !half ? 2 : 1) * tiles;
+  int64_t best = 1, best_cost = INT64_MAX;
+  for (int64_t n = 1; n <= 64 && (n == 1 || tiles / n >= 4); ++n) {
+    const int64_t cost = (pairs * n + slots - 1) / slots * ((work + n - 1) / n + 8);
+    if (cost < best_cost) best = n, best_cost = cost;
+  }
+  return (int)best;
 }
 }  // namespace
 

@@ -125,6 +125,14 @@ __device__ __forceinline__ void pin_in(const X& x) {
 __device__ __forceinline__ void load_lds16(const void* gptr, unsigned lds_addr) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gptr), "s"(lds_addr) : "memory");
 }
+// The same from gptr + OFF bytes.  The instruction adds its offset to both addresses,
+// so it is taken off the LDS one.
+template <int OFF>
+__device__ __forceinline__ void load_lds16_at(const void* gptr, unsigned lds_addr) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off offset:%2" ::"v"(gptr), "s"(lds_addr - OFF),
+               "n"(OFF)
+               : "memory");
+}
 // Same for one dword per lane (lane l's 4 bytes land at lds_addr + 4 * l).
 __device__ __forceinline__ void load_lds4(const void* gptr, unsigned lds_addr) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(gptr), "s"(lds_addr) : "memory");

@@ -11,16 +11,14 @@
 //    a workgroup of four waves kWsWaves * NK * 32 keys of one (b, hkv);
 //  * the query rows of the KV head's G heads, packed with the heads innermost (row
 //    r: query row r / G of head r % G), are streamed in tiles of 32, the columns of
-//    an MFMA tile, through a ring of three LDS stages that the four waves share
-//    (direct-to-LDS copies, one barrier per tile; a stage is refilled two tiles
-//    after its last reader passed the barrier);
+//    an MFMA tile, through a ring of LDS stages that the four waves share
+//    (direct-to-LDS copies, one barrier per step of two tiles, two steps ahead);
 //  * a lane adds the weights of its column's rows for 16 keys of each block in fp32;
 //    the 32 columns are added at the end by exchanging halves, so that lane c ends
 //    up with one key's sum, in a fixed order;
 //  * the tiles of a key block are shared by nparts workgroups where key blocks alone
-//    would leave CUs idle (a causal prefill, whose first keys are seen by every row
-//    and whose last by few, also balances by them: longest first); their sums go to
-//    the workspace and a second kernel adds them in order.
+//    would leave CUs idle; their sums go to the workspace and a second kernel adds
+//    them in order.
 // What bounds it: per 32 x 32 pairs and SIMD, one fma, one exponential (a quarter
 // rate instruction) and one add an element are 384 cycles of VALU, the MFMAs 2 D
 // cycles beside them.
@@ -40,13 +38,12 @@ template <class T, int D>
 struct WsCfg {
   static constexpr int ROWB = D * (int)sizeof(T);  // bytes per row
   static constexpr int KC = ROWB / 32;             // 32-byte steps of S = K Q^T
-  static constexpr int CPR = ROWB / 16;            // 16-byte chunks per row
-  static constexpr int TB = 32 * ROWB;             // bytes of a query tile
+  static constexpr int TB = 32 * ROWB;             // bytes of a query tile: KC copies of 1 KB
   static constexpr int NK = ROWB <= 512 ? 2 : 1;   // 32-key blocks per wave (registers)
   static constexpr int KEYS = kWsWaves * NK * 32;  // keys per workgroup
-  static constexpr int E = TB / 1024;              // 1 KB copies per tile
-  static constexpr int EW = (E + kWsWaves - 1) / kWsWaves;  // and per wave
   static constexpr int STAGEB = TB + 256;          // a tile and its 32 rows' LSE (a 64-lane copy)
+  static constexpr int TPS = ROWB <= 512 ? 2 : 1;  // tiles per barrier
+  static constexpr int RING = 3 * TPS;             // stages
 };
 
 template <class T>
@@ -62,21 +59,39 @@ __device__ __forceinline__ f32x16 mma_step(i32x4 k, i32x4 q, f32x16 c) {
   }
 }
 
-// Adds the 32 columns of 16 values per lane half: lane c of each half ends up with
-// the sum of element c % 16 (lanes c and c ^ 16 both have it).
+// A query tile in LDS is a block of 2 KB for each 64 bytes of its rows, 32 rows of 64
+// bytes whose 16-byte chunks are permuted by (row / 4) % 4: the 16 rows that one LDS
+// cycle of a column read takes hit 16 groups of banks, and a step's reads differ from
+// the one two steps on by a constant.  A copy (1 KB) is 16 rows of a block; wave w
+// makes copies w, w + 4, ...
+template <int KC, int X>
+__device__ __forceinline__ void copy_steps(const char* row, unsigned dst) {
+  if constexpr (X < KC) {
+    load_lds16_at<32 * X>(row, dst + X * 1024);
+    copy_steps<KC, X + kWsWaves>(row, dst);
+  }
+}
+
+// Adds the 32 columns of 16 values per lane half, one step per bit of the lane:
+// lanes W apart exchange the halves of the 2 W values left, so that lane c of each
+// half ends up with the sum of element c % 16 (lanes c and c ^ 16 both have it).
+template <int W>
+__device__ __forceinline__ void exchange(float (&x)[16], int l32) {
+  const bool up = l32 & W;
+#pragma unroll
+  for (int e = 0; e < W; ++e) {  // keep the element whose bit W is this lane's
+    const float send = up ? x[e] : x[e + W], keep = up ? x[e + W] : x[e];
+    x[e] = keep + __shfl_xor(send, W);
+  }
+}
 __device__ __forceinline__ float column_sums(const f32x16& a, int l32) {
   float x[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) x[e] = a[e];
-#pragma unroll
-  for (int w = 8; w; w >>= 1) {
-    const bool up = l32 & w;
-#pragma unroll
-    for (int e = 0; e < w; ++e) {  // keep the half whose bit w of the element is this lane's
-      const float send = up ? x[e] : x[e + w], keep = up ? x[e + w] : x[e];
-      x[e] = keep + __shfl_xor(send, w);
-    }
-  }
+  exchange<8>(x, l32);
+  exchange<4>(x, l32);
+  exchange<2>(x, l32);
+  exchange<1>(x, l32);
   return x[0] + __shfl_xor(x[0], 16);
 }
 }  // namespace
@@ -86,179 +101,230 @@ __global__ __launch_bounds__(kWsWaves * 64) __attribute__((amdgpu_waves_per_eu(D
 void weight_sums_kernel(WeightArgs a) {
   using C = WsCfg<T, D>;
   constexpr int KC = C::KC;
-  __shared__ __attribute__((aligned(1024))) char smem[3 * C::STAGEB];
+  __shared__ __attribute__((aligned(1024))) char smem[C::RING * C::STAGEB];
   const Shape& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, l32 = lane & 31;
 
-  // (key block, part, b, hkv): those of one (b, hkv) share an XCD where their number
-  // is a multiple of 8, and under a causal mask the longest walks go first
-  const int nbh = p.B * p.Hkv;
+  // (part, pair of key blocks, b, hkv): block x and block nkb - 1 - x one after the
+  // other, so that under a causal mask, too, workgroups have equal work; those of one
+  // (b, hkv) share an XCD where their number is a multiple of 8
+  const int nbh = p.B * p.Hkv, nkb = (p.Skv + C::KEYS - 1) / C::KEYS, npair = (nkb + 1) / 2;
   const int bh = blockIdx.x % nbh, hk = bh % p.Hkv, b = bh / p.Hkv;
-  const int part = blockIdx.x / nbh % a.nparts, kb = blockIdx.x / nbh / a.nparts;
-  const int j0 = kb * C::KEYS;
+  const int pair = blockIdx.x / nbh % npair, part = blockIdx.x / nbh / npair;
   int n = a.lengths ? min(max(a.lengths[b], 0), p.Skv) : p.Skv;
   n = __builtin_amdgcn_readfirstlane(n);
   const int64_t start = a.starts ? a.starts[b] : a.start;
   float* out = a.nparts > 1 ? a.part + ((int64_t)part * nbh + bh) * p.Skv : a.sums + (int64_t)bh * p.Skv;
   const bool add = a.nparts == 1 && a.add;
-  if (j0 >= n) {  // no key in use
-    if (a.nparts == 1 && !a.add)
-      for (int j = j0 + tid; j < min(j0 + C::KEYS, p.Skv); j += kWsWaves * 64) out[j] = 0.f;
-    return;
-  }
-
-  // The query rows [i_lo, i_hi) that see a key of the workgroup, and those that see
-  // all keys of the workgroup, as tiles of packed rows; this part's tiles.
-  const int R = p.G * p.Sq;
-  const int64_t jl = min(j0 + C::KEYS, n) - 1;
-  int64_t i_lo = 0, i_hi = p.Sq, f_lo = 0, f_hi = p.Sq;
-  if (p.causal) i_lo = j0 - start, f_lo = jl - start;
-  if (p.window > 0) i_hi = min(i_hi, jl + p.window - start + 1), f_hi = min(f_hi, j0 + p.window - start + 1);
-  i_lo = min(max(i_lo, (int64_t)0), (int64_t)p.Sq);
-  i_hi = max(i_hi, i_lo);
-  f_lo = max(f_lo, (int64_t)0);
-  const int t_lo = (int)(i_lo * p.G / 32), t_hi = (int)((i_hi * p.G + 31) / 32);
-  const int64_t r_full_lo = f_lo * p.G, r_full_hi = f_hi * p.G;
-  const int per = (t_hi - t_lo + a.nparts - 1) / a.nparts;
-  const int t0 = __builtin_amdgcn_readfirstlane(t_lo + part * per);
-  const int t1 = __builtin_amdgcn_readfirstlane(min(t_hi, t_lo + (part + 1) * per));
-
-  // this lane's share of a tile's copies: packed rows 32 t + row of copy slot x, kept
-  // as (query row, head) and moved on by 32 rows a tile
-  const T* qp = (const T*)a.q.data + b * a.q.sb + (int64_t)hk * p.G * a.q.sh;
-  const float* lp = a.lse + ((int64_t)b * p.Hq + (int64_t)hk * p.G) * p.Sq;
-  const int dq = 32 / p.G, dg = 32 % p.G;
-  int ci[C::EW], cg[C::EW], li, lg;
-#pragma unroll
-  for (int x = 0; x < C::EW; ++x) {
-    const int r = 32 * t0 + ((x * kWsWaves + wave) * 64 + lane) / C::CPR;
-    ci[x] = r / p.G;
-    cg[x] = r % p.G;
-  }
-  li = (32 * t0 + l32) / p.G;
-  lg = (32 * t0 + l32) % p.G;
   const unsigned lds0 = lds_addr_of(smem);
-  auto issue = [&](int st) {  // the next tile into stage st; rows past the last repeat it
-#pragma unroll
-    for (int x = 0; x < C::EW; ++x) {
-      const int e = x * kWsWaves + wave;
-      if (C::E % kWsWaves == 0 || e < C::E) {
-        const int row = (e * 64 + lane) / C::CPR, pc = (e * 64 + lane) % C::CPR;
-        const bool in = ci[x] < p.Sq;
-        const int i = in ? ci[x] : p.Sq - 1, g = in ? cg[x] : p.G - 1;
-        load_lds16((const char*)(qp + (int64_t)g * a.q.sh + (int64_t)i * a.q.ss) + swz_col<C::CPR>(row, pc) * 16,
-                   lds0 + st * C::STAGEB + e * 1024);
-      }
-      ci[x] += dq;
-      cg[x] += dg;
-      if (cg[x] >= p.G) cg[x] -= p.G, ci[x] += 1;
-    }
-    const bool in = li < p.Sq;
-    load_lds4(lp + (int64_t)(in ? lg : p.G - 1) * p.Sq + (in ? li : p.Sq - 1), lds0 + st * C::STAGEB + C::TB);
-    li += dq;
-    lg += dg;
-    if (lg >= p.G) lg -= p.G, li += 1;
+  float c2 = p.scale_log2;
+  bool flip = false;
+  if constexpr (!CAP) {  // masked scores are -inf: a negative scale moves into K, and 0 becomes a tiny one
+    flip = c2 < 0.f;
+    c2 = c2 == 0.f ? 1e-30f : fabsf(c2);
+  }
+  // A weight from a score: raw, or with a soft-cap already in log2 units.
+  auto weight = [&](float s, float l2) {
+    if constexpr (CAP) return fast_exp2(s - l2);
+    else return fast_exp2(__builtin_fmaf(s, c2, -l2));
   };
-  // copies of one tile this wave has issued
-  constexpr int kCopies = (C::E % kWsWaves == 0 ? C::EW : 0) + 1;
 
-  f32x16 acc[NK];
+  for (int seg = 0; seg < 2; ++seg) {
+    const int kb = seg == 0 ? pair : nkb - 1 - pair;
+    if (seg == 1 && kb == pair) break;
+    const int j0 = kb * C::KEYS;
+    if (j0 >= n) {  // no key in use
+      if (a.nparts == 1 && !a.add)
+        for (int j = j0 + tid; j < min(j0 + C::KEYS, p.Skv); j += kWsWaves * 64) out[j] = 0.f;
+      continue;
+    }
+
+    // The query rows [i_lo, i_hi) that see a key of the workgroup, and those that see
+    // all keys of the workgroup, as tiles of packed rows; this part's tiles.
+    const int R = p.G * p.Sq;
+    const int64_t jl = min(j0 + C::KEYS, n) - 1;
+    int64_t i_lo = 0, i_hi = p.Sq, f_lo = 0, f_hi = p.Sq;
+    if (p.causal) i_lo = j0 - start, f_lo = jl - start;
+    if (p.window > 0) i_hi = min(i_hi, jl + p.window - start + 1), f_hi = min(f_hi, j0 + p.window - start + 1);
+    i_lo = min(max(i_lo, (int64_t)0), (int64_t)p.Sq);
+    i_hi = max(i_hi, i_lo);
+    f_lo = max(f_lo, (int64_t)0);
+    const int t_lo = (int)(i_lo * p.G / 32), t_hi = (int)((i_hi * p.G + 31) / 32);
+    // the tiles all of whose rows see all keys of the workgroup
+    const int full_lo = __builtin_amdgcn_readfirstlane((int)((min(f_lo, (int64_t)p.Sq) * p.G + 31) / 32));
+    const int full_hi = __builtin_amdgcn_readfirstlane((int)(max(f_hi, (int64_t)0) * p.G / 32));
+    // this part's tiles: every nparts-th, so that all have their share of masked ones
+    const int t0 = __builtin_amdgcn_readfirstlane(t_lo + part), dt = a.nparts;
+    const int nt = __builtin_amdgcn_readfirstlane(t0 < t_hi ? (t_hi - t0 + dt - 1) / dt : 0);
+
+    // The row of the next tile that this lane copies 16 bytes of per step, and the one
+    // whose LSE it copies; a step of 32 nparts rows is dq query rows and dg heads.
+    const T* qp = (const T*)a.q.data + b * a.q.sb + (int64_t)hk * p.G * a.q.sh;
+    const float* lp = a.lse + ((int64_t)b * p.Hq + (int64_t)hk * p.G) * p.Sq;
+    const int dq = 32 * dt / p.G, dg = 32 * dt % p.G;
+    const int64_t qstep = ((int64_t)dq * a.q.ss + (int64_t)dg * a.q.sh) * (int)sizeof(T);
+    const int64_t qwrap = (a.q.ss - (int64_t)p.G * a.q.sh) * (int)sizeof(T);
+    const int64_t lstep = ((int64_t)dq + (int64_t)dg * p.Sq) * 4, lwrap = (1 - (int64_t)p.G * p.Sq) * 4;
+    const int crow = (wave & 1) * 16 + (lane >> 2);
+    const int cbyte = (wave >> 1) * 64 + ((lane & 3) ^ ((crow >> 2) & 3)) * 16;
+    const int cr0 = 32 * t0 + crow, lr0 = 32 * t0 + l32;
+    int cg = cr0 % p.G, lg = lr0 % p.G;
+    const char* ca = (const char*)(qp + (int64_t)cg * a.q.sh + (int64_t)(cr0 / p.G) * a.q.ss) + cbyte;
+    const char* la = (const char*)(lp + (int64_t)lg * p.Sq + lr0 / p.G);
+    auto issue = [&](int u) {  // the part's tile u, the one after the last issued
+      const int t = t0 + u * dt;
+      const unsigned dst = lds0 + u % C::RING * C::STAGEB;
+      if (32 * t + 31 >= R) {  // rows past the last repeat it
+        asm volatile("");      // (a branch, not a selection in every tile)
+        if (crow >= R - 32 * t)
+          ca = (const char*)(qp + (int64_t)(p.G - 1) * a.q.sh + (int64_t)(p.Sq - 1) * a.q.ss) + cbyte;
+        if (l32 >= R - 32 * t) la = (const char*)(lp + (int64_t)p.G * p.Sq - 1);
+      }
+      if (KC % kWsWaves == 0 || wave < KC) {
+        copy_steps<KC, 0>(ca, dst + wave * 1024);
+        load_lds4(la, dst + C::TB);
+      }
+      ca += qstep;
+      la += lstep;
+      if (dg) {  // G does not divide 32: the heads of the rows change
+        asm volatile("");
+        cg += dg;
+        lg += dg;
+        if (cg >= p.G) cg -= p.G, ca += qwrap;
+        if (lg >= p.G) lg -= p.G, la += lwrap;
+      }
+    };
+    // copies of one tile that a wave has issued
+    constexpr int kCopies = (KC + kWsWaves - 1) / kWsWaves + 1;
+
+    f32x16 acc[NK];
 #pragma unroll
-  for (int kb2 = 0; kb2 < NK; ++kb2) acc[kb2] = f32x16{};
-  i32x4 kf[NK][KC];
-  if (t0 < t1) {
+    for (int kb2 = 0; kb2 < NK; ++kb2) acc[kb2] = f32x16{};
+    i32x4 kf[NK][KC];
+    if (nt > 0) {
+#pragma unroll
+      for (int x = 0; x < NK; ++x) {
+        const int64_t j = min(j0 + (wave * NK + x) * 32 + l32, n - 1);
+        const char* src = (const char*)((const T*)a.k.data + b * a.k.sb + hk * a.k.sh + j * a.k.ss) + 16 * h;
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) kf[x][kc] = ld_global16(src + 32 * kc);
+      }
+      if (seg == 1) __builtin_amdgcn_s_barrier();  // every wave has read the first block's last tiles
+#pragma unroll
+      for (int u = 0; u < 2 * C::TPS; ++u)
+        if (u < nt) issue(u);
+      // wait for K here, once, with the first tiles: at its first use the compiler's
+      // own wait would drain the copies of later tiles
+#pragma unroll
+      for (int x = 0; x < NK; ++x)
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) pin(kf[x][kc]);
+    }
+
+    // steps 2 i and 2 i + 1 of row l32 in block i
+    const int koff[2] = {l32 * 64 + (h ^ ((l32 >> 2) & 3)) * 16, l32 * 64 + ((2 + h) ^ ((l32 >> 2) & 3)) * 16};
+    if constexpr (!CAP) {
+      if (flip) {
+        constexpr int kSign = sizeof(T) == 4 ? (int)0x80000000 : (int)0x80008000;
+#pragma unroll
+        for (int x = 0; x < NK; ++x)
+#pragma unroll
+          for (int kc = 0; kc < KC; ++kc) kf[x][kc] ^= i32x4{kSign, kSign, kSign, kSign};
+      }
+    }
+    // The last block's scores of a tile wait for the first MFMAs of the next one, and
+    // the others' for those of the block after them, so that the exponentials run
+    // beside MFMAs.  (None waits: scores of 0 of a row with LSE +inf, weights of 0.)
+    f32x16 sw = f32x16{};
+    float lw = kPosInf;
+    for (int u = 0; u < nt; ++u) {
+      if (u % C::TPS == 0) {
+        // this wave's copies of this step's tiles have landed (those of the next step may
+        // be in flight) ...
+        if (u + 2 * C::TPS <= nt) wait_vmcnt<C::TPS * kCopies>();
+        else wait_vmcnt<0>();
+        __builtin_amdgcn_s_barrier();  // ... and every wave's; all are done with the step before
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int x = 0; x < C::TPS; ++x)  // into the stages of the step before
+          if (u + 2 * C::TPS + x < nt) issue(u + 2 * C::TPS + x);
+      }
+      const int t = t0 + u * dt;
+      const char* sQ = smem + u % C::RING * C::STAGEB;
+      // all reads first: one at a time, each would be waited for
+      const float lse = *(const float*)(sQ + C::TB + l32 * 4);
+      i32x4 qf[KC];
+#pragma unroll
+      for (int kc = 0; kc < KC; ++kc) qf[kc] = lds_read16(sQ + koff[kc & 1] + (kc >> 1) * 2048);
+      // a row without keys gives no weight, whatever its scores
+      const bool dead = 32 * t + l32 >= R || lse == kNegInf;
+      const float l2 = dead ? kPosInf : lse * kLog2e;
+      const bool masked = t < full_lo || t >= full_hi || __builtin_amdgcn_ballot_w64(dead);
+      int hi32 = 0, lo32 = 0;  // keys [lo, hi) of the row, relative to the lane half's first of the workgroup
+      if (masked) {
+        asm volatile("");  // a branch: the compiler would compute the mask of every tile
+        const int64_t pos = start + (32 * t + l32) / p.G, base = j0 + 4 * h;
+        const int64_t hi = dead ? -1 : p.causal ? pos + 1 - base : (int64_t)1 << 30;
+        const int64_t lo = p.window > 0 ? pos - p.window - base : -1;
+        hi32 = (int)min(max(hi, (int64_t)-1), (int64_t)1 << 30);
+        lo32 = (int)min(max(lo, (int64_t)-1), (int64_t)1 << 30);
+      }
+#pragma unroll
+      for (int x = 0; x < NK; ++x) {
+        // The MFMAs of this block, and between them the weights of the waiting one, added
+        // a step after their exponential.  The order is held by sched_barrier: left to
+        // itself the compiler puts all weights first and their registers to use again.
+        f32x16 sc = f32x16{};
+        f32x16& to = acc[x == 0 ? NK - 1 : x - 1];
+        f32x16 pe;
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+          sc = mma_step<T>(kf[x][kc], qf[kc], sc);
+#pragma unroll
+          for (int e = 16 * kc / KC; e < 16 * (kc + 1) / KC; ++e) pe[e] = weight(sw[e], x == 0 ? lw : l2);
+#pragma unroll
+          for (int e = kc > 0 ? 16 * (kc - 1) / KC : 16; e < 16 * kc / KC; ++e) to[e] += pe[e];
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int e = 16 * (KC - 1) / KC; e < 16; ++e) to[e] += pe[e];
+        pin(to);  // here, not behind the branch below
+        if constexpr (CAP) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float tv;
+            if constexpr (sizeof(T) == 4) sc[e] = p.cap_log2 * tanhf(sc[e] * p.scale * p.inv_cap);
+            else sc[e] = score_log2<true, false>(sc[e], p, 0.f, 0, 0, tv);
+          }
+        }
+        if (masked) {
+          asm volatile("");
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int jj = (wave * NK + x) * 32 + 8 * (e >> 2) + (e & 3);
+            if (jj >= hi32 || jj < lo32) sc[e] = kNegInf;
+          }
+        }
+        sw = sc;
+      }
+      lw = l2;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[NK - 1][e] += weight(sw[e], lw);
+
 #pragma unroll
     for (int x = 0; x < NK; ++x) {
-      const int64_t j = min(j0 + (wave * NK + x) * 32 + l32, n - 1);
-      const char* src = (const char*)((const T*)a.k.data + b * a.k.sb + hk * a.k.sh + j * a.k.ss) + 16 * h;
-#pragma unroll
-      for (int kc = 0; kc < KC; ++kc) kf[x][kc] = ld_global16(src + 32 * kc);
-    }
-    issue(0);
-    if (t0 + 1 < t1) issue(1);
-    // wait for K here, once, with the first tiles: at its first use the compiler's
-    // own wait would drain the copies of later tiles
-#pragma unroll
-    for (int x = 0; x < NK; ++x)
-#pragma unroll
-      for (int kc = 0; kc < KC; ++kc) pin(kf[x][kc]);
-  }
-
-  int koff[KC];
-#pragma unroll
-  for (int kc = 0; kc < KC; ++kc) koff[kc] = l32 * C::ROWB + swz_col<C::CPR>(l32, 2 * kc + h) * 16;
-  const float c2 = p.scale_log2;
-
-  int st = 0;
-  for (int t = t0; t < t1; ++t) {
-    // this wave's copies of tile t have landed (those of t + 1 may be in flight) ...
-    if (t + 1 < t1 && C::E % kWsWaves == 0) wait_vmcnt<kCopies>();
-    else wait_vmcnt<0>();
-    __builtin_amdgcn_s_barrier();  // ... and every wave's; all are done with tile t - 1
-    asm volatile("" ::: "memory");
-    if (t + 2 < t1) issue(st >= 1 ? st - 1 : 2);  // (t + 2) % 3 stages on: where tile t - 1 was
-    const char* sQ = smem + st * C::STAGEB;
-    const float lse = *(const float*)(sQ + C::TB + l32 * 4);
-
-    f32x16 sc[NK];
-#pragma unroll
-    for (int x = 0; x < NK; ++x) sc[x] = f32x16{};
-#pragma unroll
-    for (int kc = 0; kc < KC; ++kc) {
-      const i32x4 q = lds_read16(sQ + koff[kc]);
-#pragma unroll
-      for (int x = 0; x < NK; ++x) sc[x] = mma_step<T>(kf[x][kc], q, sc[x]);
-    }
-    const int r = 32 * t + l32;
-    const bool live = r < R && lse != kNegInf;  // a row without keys gives no weight
-    const float l2 = lse * kLog2e;
-    const bool full = 32 * t >= r_full_lo && 32 * (int64_t)t + 31 < r_full_hi &&
-                      __builtin_amdgcn_ballot_w64(!live) == 0;
-    auto weight = [&](float s) {
-      float y;
-      if constexpr (!CAP) y = __builtin_fmaf(s, c2, -l2);
-      else if constexpr (sizeof(T) == 4) y = p.cap_log2 * tanhf(s * p.scale * p.inv_cap) - l2;
-      else {
-        float tv;
-        y = score_log2<true, false>(s, p, 0.f, 0, 0, tv) - l2;
-      }
-      return fast_exp2(y);
-    };
-    if (full) {
-#pragma unroll
-      for (int x = 0; x < NK; ++x)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[x][e] += weight(sc[x][e]);
-    } else {
-      const int64_t pos = start + r / p.G;
-      // keys [lo, hi) of the row, relative to the lane half's first
-      const int64_t base = j0 + 4 * h;
-      int64_t hi = p.causal ? pos + 1 - base : (int64_t)1 << 30, lo = p.window > 0 ? pos - p.window - base : -1;
-      if (!live) hi = -1;
-      const int hi32 = (int)min(max(hi, (int64_t)-1), (int64_t)1 << 30), lo32 = (int)min(max(lo, (int64_t)-1), (int64_t)1 << 30);
-#pragma unroll
-      for (int x = 0; x < NK; ++x)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int jj = (wave * NK + x) * 32 + 8 * (e >> 2) + (e & 3);
-          acc[x][e] += (jj < hi32 && jj >= lo32) ? weight(sc[x][e]) : 0.f;
+      const float w = column_sums(acc[x], l32);
+      const int e = l32 & 15;
+      const int j = j0 + (wave * NK + x) * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+      if (l32 < 16 && j < p.Skv) {
+        if (add) {
+          if (j < n) out[j] += w;
+        } else {
+          out[j] = j < n ? w : 0.f;
         }
-    }
-    st = st == 2 ? 0 : st + 1;
-  }
-
-#pragma unroll
-  for (int x = 0; x < NK; ++x) {
-    const float w = column_sums(acc[x], l32);
-    const int e = l32 & 15;
-    const int j = j0 + (wave * NK + x) * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-    if (l32 < 16 && j < p.Skv) {
-      if (add) {
-        if (j < n) out[j] += w;
-      } else {
-        out[j] = j < n ? w : 0.f;
       }
     }
   }
@@ -282,7 +348,7 @@ template <class T, int D>
 hipError_t launch_weights(const WeightArgs& a, hipStream_t st) {
   using C = WsCfg<T, D>;
   const int64_t nkb = (a.p.Skv + C::KEYS - 1) / C::KEYS;
-  const dim3 grid((unsigned)(nkb * a.nparts * a.p.B * a.p.Hkv)), block(kWsWaves * 64);
+  const dim3 grid((unsigned)((nkb + 1) / 2 * a.nparts * a.p.B * a.p.Hkv)), block(kWsWaves * 64);
   if (a.p.cap > 0.f) hipLaunchKernelGGL((weight_sums_kernel<T, D, C::NK, true>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((weight_sums_kernel<T, D, C::NK, false>), grid, block, 0, st, a);
   const hipError_t e = hipGetLastError();
