@@ -1,4 +1,5 @@
-"""Build libflexatt.so (the HIP kernels + C ABI) in-tree for gfx950.
+"""Build libflexatt.so (the HIP kernels + C ABI) and flexatt_native.so (its
+torch binding for the cache and rotary calls) in-tree for gfx950.
 
 Each kernel source is compiled once per head dim (-DFLEXATT_D=...) so the
 template instances compile in parallel; the objects are linked into
@@ -17,6 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libflexatt.so")
+NATIVE = os.path.join(HERE, "flexatt_native.so")  # linked against libflexatt.so beside it
 HEAD_DIMS = (32, 64, 128, 256)
 PER_D_SOURCES = ("fwd_mfma.hip", "fwd_ws.hip", "fwd_split.hip", "bwd_mfma.hip", "bwd_kv.hip", "bwd_q.hip", "bwd_dq_ds.hip",
                   "bwd_split.hip", "f32_mfma.hip", "f32_split.hip", "tree_attn.hip", "weight_sums.hip")
@@ -87,6 +89,35 @@ def _compile(job):
     return obj
 
 
+def native_command(out: str, lib: str) -> list:
+    """The compiler command of the torch binding (host code)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    rocm = os.path.dirname(os.path.dirname(hipcc()))
+    inc = cpp_extension.include_paths() + [os.path.join(rocm, "include"), sysconfig.get_paths()["include"]]
+    return ([shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+            + [x for i in inc for x in ("-isystem", i)]
+            + [os.path.join(CSRC, "torch_binding.cpp"), "-o", out, f"-L{os.path.dirname(lib)}",
+               f"-l:{os.path.basename(lib)}", f"-L{torch_lib}"]
+            + [f"-l{x}" for x in ("torch", "torch_cpu", "torch_hip", "c10", "c10_hip", "torch_python")]
+            + ["-Wl,-rpath,$ORIGIN"])
+
+
+def _build_native() -> None:
+    tmp = NATIVE + ".tmp"
+    cmd = native_command(tmp, LIB)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, NATIVE)
+
+
 def build(njobs: int | None = None, verbose: bool = False) -> str:
     os.makedirs(OUT_DIR, exist_ok=True)
     njobs = njobs or min(16, os.cpu_count() or 4)
@@ -99,8 +130,9 @@ def build(njobs: int | None = None, verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    _build_native()
     if verbose:
-        print(f"built {LIB} from {len(objs)} objects")
+        print(f"built {LIB} from {len(objs)} objects, and {NATIVE}")
     return LIB
 
 

@@ -1,8 +1,9 @@
 """ctypes binding of libflexatt.so, the C ABI declared in include/flexatt.h.
 
-This is the only bridge between the Python API and the HIP kernels.  There is
-no fallback: if the library is missing or fails to load, every entry point
-raises ``RuntimeError``.
+This and flexatt_native.so (csrc/torch_binding.cpp: the cache and rotary calls,
+see :func:`native`) are the only bridges between the Python API and the HIP
+kernels.  There is no fallback: if a library is missing or fails to load, every
+entry point raises ``RuntimeError``.
 """
 from __future__ import annotations
 
@@ -150,6 +151,7 @@ class Evict(ctypes.Structure):
 
 
 _lib = None
+_native = None
 
 
 def load() -> ctypes.CDLL:
@@ -216,6 +218,31 @@ def load() -> ctypes.CDLL:
         raise RuntimeError("libflexatt.so ABI version mismatch; rebuild the library")
     _lib = lib
     return lib
+
+
+def native():
+    """The torch binding of the cache and rotary entry points: an extension module
+    with functions of positional arguments, which checks them, allocates outputs and
+    workspaces and calls the C ABI."""
+    global _native
+    if _native is not None:
+        return _native
+    load()  # the library it is linked against, and torch before it
+    path = os.path.join(HERE, "flexatt_native.so")
+    if not os.path.exists(path):
+        raise RuntimeError(
+            f"flexatt_native.so not found at {path}: build it with "
+            "`python npu-flex-att_amd/build_lib.py` or `python -c 'import __graft_entry__ as g; g.build()'`"
+        )
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location("flexatt_native", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    if mod.ABI_VERSION != ABI_VERSION:
+        raise RuntimeError("flexatt_native.so ABI version mismatch; rebuild the library")
+    _native = mod
+    return mod
 
 
 def check(status: int, what: str) -> None:

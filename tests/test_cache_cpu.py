@@ -130,31 +130,12 @@ def test_cpu_tensors_have_no_fallback():
             f()
 
 
-def test_per_sequence_checks():
-    n = torch.tensor([3, 4], dtype=torch.int32)
-    assert fc._per_sequence("lengths", n, 2, CPU) is n
-    assert fc._per_sequence("lengths", torch.arange(4, dtype=torch.int32)[::2], 2, CPU).is_contiguous()
-    for bad in (n.long(), n[:1], n[None], [3, 4], 3):
-        with pytest.raises(RuntimeError, match="lengths"):
-            fc._per_sequence("lengths", bad, 2, CPU)
-
-
-def test_tree_mask_forms():
-    m = torch.tensor([[1, 0], [1, 1]])
-    for x in (m, m.bool(), m.to(torch.uint8), m.to(torch.int32), m[None], m[None].expand(3, 2, 2), m.t().contiguous().t()):
-        y = fc._tree_mask(x, 3, 2, CPU)
-        assert y.dtype == torch.uint8 and y.is_contiguous() and y.shape[0] in (1, 3)
-        assert torch.equal(y[0] != 0, m != 0)
-    assert int(fc._tree_mask(m * 256, 3, 2, CPU)[0, 0, 0]) == 1  # whole values, not their low byte
-    for bad in (m.float(), m[:, :1], m[None].expand(2, 2, 2), m[None, None], [[1]]):
-        with pytest.raises(RuntimeError, match="tree_mask"):
-            fc._tree_mask(bad, 3, 2, CPU)
-
-
-def test_score_parameters():
-    assert fc._score_params(None, None, None, 64) == (0.125, 0.0, 0)
-    assert fc._score_params(0.5, -1.0, -3, 64) == (0.5, 0.0, 0)
-    assert fc._score_params(0.5, 30.0, 1 << 40, 64) == (0.5, 30.0, 0x7fffffff)
+def test_native_module_counts_its_arguments():
+    c = L.native()
+    assert c.ABI_VERSION == L.ABI_VERSION
+    for f in (c.rotary, c.rotary_append, c.tree_attention, c.weight_sums, c.evict):
+        with pytest.raises(TypeError):
+            f()
 
 
 def test_oracles_agree_with_plain_attention():

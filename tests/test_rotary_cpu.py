@@ -63,26 +63,6 @@ def test_cpu_tensors_have_no_fallback():
         rot.rotary_embedding(q, q, rot.rotary_frequencies(64)[0])
 
 
-def test_frequency_and_position_checks():
-    f = rot.rotary_frequencies(64)[0]
-    cpu = torch.device("cpu")
-    assert rot._check_frequencies(f, 64, cpu) is f
-    for bad in (f.float(), f[None], list(f)):
-        with pytest.raises(RuntimeError, match="float64"):
-            rot._check_frequencies(bad, 64, cpu)
-    with pytest.raises(RuntimeError, match="pairs"):
-        rot._check_frequencies(f, 32, cpu)
-    assert rot._check_frequencies(torch.stack((f, f), 1)[:, 0], 64, cpu).is_contiguous()
-    pos = torch.arange(12)
-    assert rot._check_positions(pos, 3, 12, cpu) == (0, 1)
-    assert rot._check_positions(pos[None], 3, 12, cpu) == (0, 1)
-    assert rot._check_positions(pos[None].expand(3, 12), 3, 12, cpu) == (0, 1)
-    assert rot._check_positions(torch.zeros(3, 24, dtype=torch.int32)[:, ::2], 3, 12, cpu) == (24, 2)
-    for bad in (pos.float(), pos[:5], pos[None].expand(2, 12), pos.to(torch.int16)):
-        with pytest.raises(RuntimeError):
-            rot._check_positions(bad, 3, 12, cpu)
-
-
 def _rotary(**kw):
     r = L.Rotary(L.BF16, 2, 4, 2, 8, 64, 64, 0, 0, 1.0, FAKE, None, 0, 0, 0, 0)
     for k, v in kw.items():
