@@ -121,21 +121,22 @@ __device__ __forceinline__ void pin_in(const X& x) {
 // a full vmcnt(0) wait before every later LDS access; completion is tracked
 // by the caller with wait_vmcnt<N>() followed by a workgroup barrier (vector
 // memory operations retire in order, so the compiler's own waits stay valid,
-// only more conservative).
+// only more conservative).  A copy must be one instruction away from the write
+// of M0, which the compiler sees to in code of its own.
 __device__ __forceinline__ void load_lds16(const void* gptr, unsigned lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gptr), "s"(lds_addr) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gptr), "s"(lds_addr) : "memory");
 }
 // The same from gptr + OFF bytes.  The instruction adds its offset to both addresses,
 // so it is taken off the LDS one.
 template <int OFF>
 __device__ __forceinline__ void load_lds16_at(const void* gptr, unsigned lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off offset:%2" ::"v"(gptr), "s"(lds_addr - OFF),
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2" ::"v"(gptr), "s"(lds_addr - OFF),
                "n"(OFF)
                : "memory");
 }
 // Same for one dword per lane (lane l's 4 bytes land at lds_addr + 4 * l).
 __device__ __forceinline__ void load_lds4(const void* gptr, unsigned lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(gptr), "s"(lds_addr) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(gptr), "s"(lds_addr) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
@@ -269,6 +270,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
+}
+// Between MFMAs and asm that reads their results: the compiler keeps the wait states
+// an MFMA result needs (19 after 16 passes, the longest) before instructions of its
+// own, but does not look into asm, which would read what the registers held before.
+__device__ __forceinline__ void settle(f32x16& a) {
+  asm volatile("s_nop 15\n\ts_nop 2" : "+v"(a));
 }
 // Max of 16 accumulator values as 7 instructions, leaving two partials.
 __device__ __forceinline__ void max16_partial(const f32x16& s, float& f, float& g) {

@@ -243,6 +243,7 @@ void fwd_split_kernel(DecodeArgs a) {
       for (int e = 0; e < 16; ++e)
         if ((unsigned)(8 * (e >> 2) + (e & 3) - a0) >= row_w) sc[e] = kNegInf;
     }
+    if constexpr (RAW) settle(sc);  // (an unmasked tile's scores come straight from the MFMAs)
     float mx, mx2;
     max16_partial(sc, mx, mx2);
     mx = max2(mx, mx2);
