@@ -348,7 +348,7 @@ typedef struct flexatt_tree {
   int32_t batch;
   int32_t heads_q;
   int32_t heads_kv;
-  int32_t tokens;         /* T >= 1 */
+  int32_t tokens;         /* T >= 1; (Hq / Hkv) T at most 2^20 and B Hq T at most 2^28 (else FLEXATT_ERANGE) */
   int32_t cache_rows;     /* >= 1 */
   int32_t head_dim;
   float scale;

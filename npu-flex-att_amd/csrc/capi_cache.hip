@@ -108,6 +108,9 @@ int check_tree(const flexatt_tree* p) {
   FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_q, p->tokens, p->head_dim));
   FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim));
   if (p->heads_q % p->heads_kv != 0) return FLEXATT_ESHAPE;
+  // (workgroups: up to the row tiles times the chunks, of 256 CUs or of (b, hkv) and more)
+  if ((int64_t)(p->heads_q / p->heads_kv) * p->tokens > 1 << 20) return FLEXATT_ERANGE;
+  if ((int64_t)p->batch * p->heads_q * p->tokens > 1 << 28) return FLEXATT_ERANGE;
   FLEXATT_TRY(check_scores(p->scale, p->soft_cap, p->sliding_window));
   if (p->reserved != 0 || !p->lengths) return FLEXATT_EINVAL;
   if (p->tree_mask ? p->mask_batch != 1 && p->mask_batch != p->batch : p->mask_batch != 0) return FLEXATT_EINVAL;
@@ -115,19 +118,34 @@ int check_tree(const flexatt_tree* p) {
   return FLEXATT_OK;
 }
 
-// Workgroups per row tile at most (each sequence takes as many of them as its own
-// length is worth, in the kernel): about two per CU in all, two tiles per wave at
-// least if the cache is full.
-int tree_splits(const flexatt_tree* p) {
-  const int64_t rows = (int64_t)(p->heads_q / p->heads_kv) * p->tokens;
-  const int64_t groups = (int64_t)p->batch * p->heads_kv * ((rows + 31) / 32);
-  const int nw = p->head_dim * elt_size(p->dtype) <= 512 ? 4 : 2;  // (TreeCfg)
-  int64_t ns = (512 + groups - 1) / groups;
-  const int64_t most = (p->cache_rows + 31) / 32 / (2 * nw);
+// How the key tiles are cut (tree_chunk, on the device, where the lengths are): into
+// about as many chunks as workgroups run at once, of eight tiles at least.  Chunks end
+// with their (b, hkv), which makes up to one more for each.  With a full cache a (b,
+// hkv) has its even share of the chunks, and up to twice that where lengths are
+// unequal.
+struct TreePlan {
+  int slots, nchunk, min_tiles, nsplit;
+};
+TreePlan tree_plan(const flexatt_tree* p) {
+  TreePlan t;
+  const int rowb = p->head_dim * (int)elt_size(p->dtype);
+  const int64_t rt = ((int64_t)(p->heads_q / p->heads_kv) * p->tokens + 31) / 32;
+  const int64_t groups = rowb <= 256 && elt_size(p->dtype) == 2 ? (rt + 1) / 2 : rt;  // (launch_tree)
+  const int64_t slots = (rowb >= 256 ? 1 : 2) * cus() / groups;
+  const int64_t bh = (int64_t)p->batch * p->heads_kv, tiles = (p->cache_rows + 31) / 32;
+  t.min_tiles = 8;
+  t.slots = slots < 1 ? 1 : (int)slots;
+  const int64_t most = (tiles + t.min_tiles - 1) / t.min_tiles;  // chunks of one (b, hkv)
+  int64_t ns = 2 * ((t.slots + bh - 1) / bh) + 1;
+  if (2 * bh > t.slots && p->batch > 1) ns = 3;  // (few chunks each: unequal lengths count most)
   if (ns > most) ns = most;
-  if (ns > 256) ns = 256;
-  return ns < 1 ? 1 : (int)ns;
+  t.nsplit = (int)ns;
+  int64_t n = t.slots + bh;
+  if (n > bh * ns) n = bh * ns;
+  t.nchunk = (int)n;
+  return t;
 }
+size_t tree_rows(const flexatt_tree* p) { return (size_t)p->batch * p->heads_q * p->tokens; }
 
 int check_weights(const flexatt_weights* p) {
   if (!p) return FLEXATT_EINVAL;
@@ -209,9 +227,9 @@ int flexatt_rotary_append(const flexatt_rotary* r, const flexatt_tensor* q, cons
 
 size_t flexatt_tree_fwd_workspace(const flexatt_tree* p) {
   if (check_tree(p) != FLEXATT_OK) return SIZE_MAX;
-  const int ns = tree_splits(p);
+  const int ns = tree_plan(p).nsplit;
   if (ns == 1) return 0;
-  return (size_t)p->batch * p->heads_q * p->tokens * ns * (p->head_dim + 1) * sizeof(float);
+  return tree_rows(p) * ns * (p->head_dim + 1) * sizeof(float) + (size_t)p->batch * p->heads_kv * sizeof(int);
 }
 
 int flexatt_tree_fwd(const flexatt_tree* p, const flexatt_tensor* q, const flexatt_tensor* k_cache,
@@ -234,9 +252,16 @@ int flexatt_tree_fwd(const flexatt_tree* p, const flexatt_tensor* q, const flexa
   a.v = view(v_cache);
   a.o = mview(o);
   a.lse = lse;
-  a.nsplit = tree_splits(p);
-  a.part_o = (float*)workspace;
-  a.part_lse = a.nsplit > 1 ? a.part_o + (int64_t)p->batch * p->heads_q * p->tokens * a.nsplit * p->head_dim : nullptr;
+  const TreePlan plan = tree_plan(p);
+  a.slots = plan.slots;
+  a.nchunk = plan.nchunk;
+  a.min_tiles = plan.min_tiles;
+  a.nsplit = plan.nsplit;
+  if (a.nsplit > 1) {
+    a.part_o = (float*)workspace;
+    a.part_lse = a.part_o + tree_rows(p) * a.nsplit * p->head_dim;
+    a.counts = (int*)(a.part_lse + tree_rows(p) * a.nsplit);
+  }
   a.lengths = p->lengths;
   a.mask = p->tree_mask;
   a.mask_sb = p->mask_batch > 1 ? (int64_t)p->tokens * p->tokens : 0;

@@ -105,8 +105,12 @@ struct TreeArgs {
   int64_t mask_sb;
   const int* depths;           // [B][T] with a window, or nullptr: t
   Shape p;  // Sq: T, Skv: rows of the cache
-  int nsplit;  // most workgroups per row tile
-  int nrt;     // row tiles of packed query rows per (b, hkv) (set by the launcher)
+  int* counts;    // [B * Hkv], chunks of each (b, hkv), for the merge; nullptr with nsplit 1
+  int slots;      // workgroups per row tile that run at once
+  int nchunk;     // most chunks of all (b, hkv) together
+  int min_tiles;  // least 32-key tiles of a chunk
+  int nsplit;     // most chunks of one (b, hkv)
+  int nrt;        // groups of packed query row tiles per (b, hkv) (set by the launcher)
 };
 
 // Attention weight received by each key (weight_sums.hip).

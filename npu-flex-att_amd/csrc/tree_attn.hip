@@ -9,18 +9,26 @@
 // (no mask: u <= t).  A row without keys is 0 with LSE -inf; a sequence whose
 // n + T rows do not fit the cache (or n < 0) is NaN.
 //
-// Decomposition (that of fwd_split.hip)
+// Decomposition
 //  * the G * T query rows of one KV head are packed with the heads innermost into
-//    tiles of 32, the columns of an MFMA tile, so heads and tokens share K and V;
-//  * a workgroup has one row tile of one (b, hkv) and a contiguous chunk of 32-key
-//    tiles; wave w takes tiles w, w + NW, ... with its own LDS stages and online
-//    softmax, no barriers; the waves' states are combined through LDS;
-//  * the chunks are cut on the device from the sequence's own length, so that a
-//    cache of large capacity that holds little costs what it holds; the partials
-//    of a row (O over its row sum, LSE) are merged in a fixed order.
+//    tiles of 32, the columns of an MFMA tile, so heads and tokens share K and V; a
+//    wave has NR such tiles (two from 33 rows on, where the registers allow), which
+//    share its LDS reads of K and V too;
+//  * the 32-key tiles of a (b, hkv), as many as the sequence's own length has, are cut
+//    into equal chunks of about `len` tiles, one per workgroup; `len` is found on the
+//    device from all lengths, so that a cache of large capacity that holds little, or a
+//    batch of unequal lengths, fills the chip once; the workgroups of one chunk for
+//    different row tiles share an XCD and with it L2;
+//  * within a chunk, wave w takes tiles w, w + NW, ... with its own LDS stages and
+//    online softmax, no barriers; the waves' states are combined through LDS, and the
+//    chunks' partials (O over its row sum, LSE) by a second kernel in a fixed order;
 //  * rows behind n + T are never read: the copies repeat the last row instead, so
 //    what a cache holds there (NaN too) does not matter.
-// What bounds it: K and V from HBM for long caches.
+// What bounds it: K and V from HBM for long caches and few rows; from some hundred
+// rows per KV head on the softmax's VALU work and the MFMAs; latency for short caches.
+// Of that the instructions are the larger part: a launch finds the instruction cache
+// cold and runs most of this code once, at about one cycle a byte, so what is outside
+// the tile loop is kept short (16-byte LDS accesses in the combine, rolled loops).
 #include "flexatt_device.h"
 #include "flexatt_kernels.h"
 
@@ -44,14 +52,19 @@ struct TreeCfg {
   static constexpr int KC = ROWB / 32;                // 32-byte steps of S^T = K Q^T
   static constexpr int DB = D / 32;                   // 32-row blocks of O^T
   static constexpr int CPR = ROWB / 16;               // 16-byte chunks per row
+  static constexpr int RPC = 64 / CPR;                // rows per 1 KB copy
   static constexpr int TB = BN * ROWB;                // bytes of one K or V tile
-  static constexpr int E = TB / 1024;                 // 1 KB copies per tile
+  static constexpr int E = TB / 1024;                 // copies per tile
+  static constexpr int PK = RPC >= 16 ? 1 : 16 / RPC;  // copies after which K's swizzle repeats (16 rows)
+  static constexpr int VROWS = sizeof(T) == 4 ? (CPR >= 16 ? 8 : 1) : CPR == 4 ? 1 : CPR == 32 ? 8 : 4;
+  static constexpr int PV = RPC >= VROWS ? 1 : VROWS / RPC;  // and V's
   static constexpr int NW = ROWB <= 512 ? 4 : 2;      // waves per workgroup
   static constexpr int ST = ROWB <= 256 ? 2 : 1;      // stages
   static constexpr int WAVEB = ST * 2 * TB;
   static constexpr int COMBB = NW * 64 * 4 * (2 + 16 * DB);
   static constexpr int LDSB = NW * WAVEB > COMBB ? NW * WAVEB : COMBB;
-  static_assert(E * 1024 == TB && LDSB <= 160 * 1024, "LDS");
+  static constexpr int NR = sizeof(T) == 2 && D <= 128 ? 2 : 1;  // most row tiles per wave
+  static_assert(E * 1024 == TB && LDSB <= 160 * 1024 && E % PK == 0 && E % PV == 0, "tiles");
 };
 
 // V tiles of 32-bit elements are read one element per lane, 32 of a row by each
@@ -83,30 +96,119 @@ __device__ __forceinline__ f32x16 mma_step(i32x4 k, i32x4 q, f32x16 c) {
   }
 }
 
-// The key tiles [t0, t1) of sequence b and how they are cut: ns chunks of `chunk`.
-struct TreePlan {
-  int n, t0, t1, ns, chunk;
+// Sequence b: its length, and its key tiles [t0, t1).  `bad`: the tree does not fit.
+struct TreeSeq {
+  int n, t0, t1;
   bool bad;
 };
-template <int NW>
-__device__ __forceinline__ TreePlan tree_plan(const TreeArgs& a, int b) {
-  TreePlan x;
-  x.n = __builtin_amdgcn_readfirstlane(a.lengths[b]);
+__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
+  TreeSeq x;
+  x.n = a.lengths[b];
   x.bad = x.n < 0 || x.n > a.p.Skv - a.p.Sq;
   if (x.bad) x.n = 0;
   x.t0 = a.p.window > 0 ? max(x.n - a.p.window, 0) / 32 : 0;
   x.t1 = (x.n + a.p.Sq + 31) / 32;
-  const int nt = x.t1 - x.t0;
-  int ns = x.bad ? 1 : min(a.nsplit, nt / (2 * NW));  // at least two tiles per wave
-  if (ns < 1) ns = 1;
-  x.chunk = (nt + ns - 1) / ns;
-  x.ns = (nt + x.chunk - 1) / x.chunk;
   return x;
+}
+// Inclusive sum, and maximum over the wave, of non-negative numbers, by lane shifts
+// within rows of 16 and broadcasts between them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+  x += dpp<0x111, 0xf>(x);
+  x += dpp<0x112, 0xf>(x);
+  x += dpp<0x114, 0xf>(x);
+  x += dpp<0x118, 0xf>(x);
+  x += dpp<0x142, 0xa>(x);
+  x += dpp<0x143, 0xc>(x);
+  return x;
+}
+__device__ __forceinline__ int wave_max(int x) {
+  x = max(x, dpp<0x111, 0xf>(x));
+  x = max(x, dpp<0x112, 0xf>(x));
+  x = max(x, dpp<0x114, 0xf>(x));
+  x = max(x, dpp<0x118, 0xf>(x));
+  x = max(x, dpp<0x142, 0xa>(x));
+  x = max(x, dpp<0x143, 0xc>(x));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+// The chunk of workgroup x: which (b, hkv) (b < 0: none, x is past the last chunk),
+// which chunk of how many, its first tile and how many.  Every lane of a wave calls
+// it and gets the same; lane l looks at sequences l, l + 64, ....
+struct TreeChunk {
+  int b, hk, s, ns, first, count;
+};
+__device__ __forceinline__ TreeChunk tree_chunk(const TreeArgs& a, int x, int nw) {
+  const int lane = threadIdx.x & 63;
+  const int B = a.p.B, H = a.p.Hkv;
+  auto tiles_of = [&](int b) {
+    const TreeSeq q = tree_seq(a, min(b, B - 1));
+    return b < B ? q.t1 - q.t0 : 0;
+  };
+  const int mine = tiles_of(lane);
+  int total = 0, most = 0;
+  for (int b0 = 0, v = mine; b0 < B; b0 += 64, v = tiles_of(b0 + lane)) {
+    total += __builtin_amdgcn_readlane(wave_scan(v), 63);
+    most = max(most, wave_max(v));
+  }
+  // The shortest chunks, whole rounds of the waves, with which one round of workgroups
+  // has them all; not looked for where there are many sequences anyway.  Quotients by
+  // reciprocals (a division of integers is some forty instructions): `len` only has to
+  // be as long as the two bounds, and a sequence's chunks at most nsplit and at most
+  // one more than its tiles over len.
+  int len = max((int)((float)total * (float)H * fast_rcp((float)a.slots) * 1.00001f),
+                (int)((float)most * fast_rcp((float)a.nsplit) * 1.00001f)) + 1;
+  len = (max(len, a.min_tiles) + nw - 1) / nw * nw;
+  auto chunks_of = [&](int v) {
+    const int c = (int)((float)(v + len - 1) * fast_rcp((float)len));
+    return v > 0 ? min(max(c, 1), a.nsplit) : 0;
+  };
+  if (2 * B * H <= a.slots && B <= 64) {
+    for (int tries = 0; tries < 8; ++tries) {
+      if (__builtin_amdgcn_readlane(wave_scan(chunks_of(mine)), 63) * H <= a.slots) break;
+      len += nw;
+    }
+  }
+  TreeChunk r;
+  r.b = -1;
+  for (int b0 = 0, v = mine; b0 < B; b0 += 64, v = tiles_of(b0 + lane)) {
+    const int c = chunks_of(v), upto = wave_scan(c);
+    const unsigned long long in = __builtin_amdgcn_ballot_w64(upto * H > x);
+    if (in) {
+      const int l = __builtin_ctzll(in);
+      const int tiles = __builtin_amdgcn_readlane(v, l), n = __builtin_amdgcn_readlane(c, l);
+      x -= (__builtin_amdgcn_readlane(upto, l) - n) * H;
+      r.b = b0 + l;
+      const float inv = fast_rcp((float)n);
+      r.hk = (int)((float)x * inv);
+      r.s = x - r.hk * n;
+      if (r.s < 0) r.s += n, r.hk -= 1;
+      if (r.s >= n) r.s -= n, r.hk += 1;
+      r.ns = n;
+      int each = (int)((float)tiles * inv) + 1;
+      if ((each - 1) * n >= tiles) each -= 1;
+      r.first = r.s * each;
+      r.count = max(min(each, tiles - r.first), 0);
+      return r;
+    }
+    x -= __builtin_amdgcn_readlane(upto, 63) * H;
+  }
+  return r;
+}
+
+// Direct-to-LDS copies of a tile of rows: lane offsets from the tile's first row (the
+// swizzle repeats after PERIOD copies, so there are as many of them) and a scalar
+// base, a copy being RPC rows.
+__device__ __forceinline__ void load_lds16_base(unsigned voff, uint64_t base, unsigned lds_addr) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds_addr) : "memory");
 }
 }  // namespace
 
-template <class T, int D, int NW, bool CAP>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(D * sizeof(T) >= 512 ? 1 : 2)))
+template <class T, int D, int NW, int NR, bool CAP>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(D * sizeof(T) >= 256 ? 1 : 2)))
 void tree_attn_kernel(TreeArgs a) {
   using C = TreeCfg<T, D>;
   constexpr int ST = C::ST;
@@ -117,102 +219,29 @@ void tree_attn_kernel(TreeArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, l32 = lane & 31;
 
-  // (b, hkv, row tile, split): the row tiles of one chunk are neighbours
-  int item = blockIdx.x;
-  const int rt = item % a.nrt;
-  item /= a.nrt;
-  const int s = item % a.nsplit;
-  const int bh = item / a.nsplit;
-  const int hk = bh % p.Hkv, b = bh / p.Hkv;
-  const TreePlan pl = tree_plan<NW>(a, b);
-  if (s >= pl.ns) return;
-
-  // packed query row of this lane
-  const int R = p.G * p.Sq;
-  const int r = min(32 * rt + l32, R - 1);
-  const int g = r % p.G, qi = r / p.G;
-  const int hq = hk * p.G + g;
-  const int64_t row = ((int64_t)b * p.Hq + hq) * p.Sq + qi;
-
-  if (pl.bad) {
-    if (32 * rt + l32 < R) {
-      const float nan = __builtin_nanf("");
-      T* out = (T*)a.o.data + b * a.o.sb + hq * a.o.sh + (int64_t)qi * a.o.ss;
-      for (int d = wave * 2 + h; d < D; d += NW * 2) out[d] = from_f32<T>(nan);
-      if (wave == 0 && h == 0) a.lse[row] = nan;
-    }
-    return;
+  // (chunk, row tiles): the row tiles of one chunk are 8 workgroups apart, on one XCD
+  // and started together (as rows of a two-dimensional grid, started one after the
+  // other, they find the chunk gone from L2: fp16 B=4 Hq=28 Hkv=4 T=64, caches of
+  // 16384 D=64, 58 -> 74 us)
+  int rt0 = 0, x = blockIdx.x;
+  if (a.nrt > 1) {
+    rt0 = blockIdx.x / 8 % a.nrt * NR;
+    x = blockIdx.x / (8 * a.nrt) * 8 + blockIdx.x % 8;
   }
-
-  i32x4 qf[C::KC];
-  {
-    const char* src = (const char*)((const T*)a.q.data + b * a.q.sb + hq * a.q.sh + (int64_t)qi * a.q.ss) + 16 * h;
-#pragma unroll
-    for (int kc = 0; kc < C::KC; ++kc) qf[kc] = ld_global16(src + 32 * kc);
-  }
-
-  // This row sees the cached keys [row_lo, n); the tiles that hold only keys every
-  // row of the tile sees need no mask.
-  const int n = pl.n;
-  int row_lo = 0, full_lo = 0;
-  if (p.window > 0) {
-    const int depth = a.depths ? max(a.depths[(int64_t)b * p.Sq + qi], 0) : qi;
-    // (n + depth - window without leaving 32 bits: depth at most the window counts)
-    row_lo = max(n - (p.window - min(depth, p.window)), 0);
-    full_lo = row_lo;
-#pragma unroll
-    for (int x = 32; x; x >>= 1) full_lo = max(full_lo, __shfl_xor(full_lo, x));
-    full_lo = __builtin_amdgcn_readfirstlane(full_lo);
-  }
-  const unsigned char* mrow = a.mask ? a.mask + b * a.mask_sb + (int64_t)qi * p.Sq : nullptr;
-
-  // this wave's tiles: first + NW * j, j < nt
-  const int t_lo = pl.t0 + s * pl.chunk, t_hi = min(pl.t1, t_lo + pl.chunk);
-  const int first = t_lo + wave;
-  const int nt = __builtin_amdgcn_readfirstlane(max((t_hi - first + NW - 1) / NW, 0));
-
-  const T* kp = (const T*)a.k.data + b * a.k.sb + hk * a.k.sh;
-  const T* vp = (const T*)a.v.data + b * a.v.sb + hk * a.v.sh;
-  const int last = n + p.Sq - 1;
-  const unsigned wbase = lds_addr_of(smem) + wave * C::WAVEB;
-  auto issue_k = [&](int t, int st) {
-#pragma unroll
-    for (int e = 0; e < C::E; ++e) {
-      const int q = e * 64 + lane, kr = q / C::CPR, pc = q % C::CPR;
-      const int64_t j = min(t * C::BN + kr, last);
-      load_lds16((const char*)(kp + j * a.k.ss) + swz_col<C::CPR>(kr, pc) * 16, wbase + st * 2 * C::TB + e * 1024);
-    }
-  };
-  auto issue_v = [&](int t, int st) {
-#pragma unroll
-    for (int e = 0; e < C::E; ++e) {
-      const int q = e * 64 + lane, kr = q / C::CPR, pc = q % C::CPR;
-      const int64_t j = min(t * C::BN + kr, last);
-      load_lds16((const char*)(vp + j * a.v.ss) + swz_v<T, C::CPR>(kr, pc) * 16,
-                 wbase + st * 2 * C::TB + C::TB + e * 1024);
-    }
-  };
-  // this wave's LDS reads have returned: the buffer they read may be refilled
-  auto reads_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
-  if (nt > 0) {
-    issue_k(first, 0);
-    issue_v(first, 0);
-  }
+  const TreeChunk ck = tree_chunk(a, x, NW);
+  if (ck.b < 0) return;
+  const int b = ck.b, hk = ck.hk, s = ck.s, ns = ck.ns;
+  TreeSeq sq = tree_seq(a, b);
+  sq.n = __builtin_amdgcn_readfirstlane(sq.n);
+  sq.t0 = __builtin_amdgcn_readfirstlane(sq.t0);
+  if (rt0 == 0 && s == 0 && tid == 0 && a.counts) a.counts[b * p.Hkv + hk] = sq.bad ? 1 : ns;
 
   float c2 = p.scale_log2;
+  bool flip = false;
   if constexpr (!CAP) {  // as in the forward: a negative scale moves into Q
-    if (c2 < 0.f) {
-      constexpr int kSign = sizeof(T) == 4 ? (int)0x80000000 : (int)0x80008000;
-#pragma unroll
-      for (int kc = 0; kc < C::KC; ++kc) qf[kc] ^= i32x4{kSign, kSign, kSign, kSign};
-      c2 = -c2;
-    }
-    if (c2 == 0.f) c2 = 1e-30f;
+    flip = c2 < 0.f;
+    c2 = c2 == 0.f ? 1e-30f : fabsf(c2);
   }
-  // wait for Q here, once: see fwd_split.hip
-#pragma unroll
-  for (int kc = 0; kc < C::KC; ++kc) pin(qf[kc]);
-
   int koff[C::KC], voff[C::DB];
 #pragma unroll
   for (int kc = 0; kc < C::KC; ++kc) koff[kc] = l32 * C::ROWB + swz_col<C::CPR>(l32, 2 * kc + h) * 16;
@@ -227,11 +256,135 @@ void tree_attn_kernel(TreeArgs a) {
     for (int db = 0; db < C::DB; ++db)
       voff[db] = tr_row * C::ROWB + swz_tr<C::CPR>(tr_row, 4 * db + (tr_col >> 3)) * 16 + (tr_col & 7) * 2;
   }
-
-  f32x16 acc[C::DB];
+  // this lane's offsets in a tile's copies
+  const unsigned kss = (unsigned)(a.k.ss * (int)sizeof(T)), vss = (unsigned)(a.v.ss * (int)sizeof(T));
+  const int crow = lane / C::CPR, cchunk = lane % C::CPR;
+  unsigned kvo[C::PK], vvo[C::PV];
 #pragma unroll
-  for (int db = 0; db < C::DB; ++db) acc[db] = f32x16{};
-  float m_run = kNegInf, l_run = 0.f;
+  for (int e = 0; e < C::PK; ++e)
+    kvo[e] = (e * C::RPC + crow) * kss + swz_col<C::CPR>(e * C::RPC + crow, cchunk) * 16;
+#pragma unroll
+  for (int e = 0; e < C::PV; ++e)
+    vvo[e] = (e * C::RPC + crow) * vss + swz_v<T, C::CPR>(e * C::RPC + crow, cchunk) * 16;
+  const unsigned wbase = lds_addr_of(smem) + wave * C::WAVEB;
+  // this wave's LDS reads have returned: the buffer they read may be refilled
+  auto reads_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
+
+  // packed query rows of this lane
+  const int R = p.G * p.Sq;
+  int hqo[NR], qi[NR];  // head within the group, drafted token
+#pragma unroll
+  for (int nr = 0; nr < NR; ++nr) {
+    const int r = min(32 * (rt0 + nr) + l32, R - 1);
+    hqo[nr] = r % p.G;
+    qi[nr] = r / p.G;
+  }
+
+  if (sq.bad) {
+    if (s == 0) {
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr) {
+        if (32 * (rt0 + nr) + l32 >= R) continue;
+        const int hq = hk * p.G + hqo[nr];
+        T* out = (T*)a.o.data + b * a.o.sb + hq * a.o.sh + (int64_t)qi[nr] * a.o.ss;
+        for (int d = wave * 2 + h; d < D; d += NW * 2) out[d] = from_f32<T>(__builtin_nanf(""));
+        if (wave == 0 && h == 0) a.lse[((int64_t)b * p.Hq + hq) * p.Sq + qi[nr]] = __builtin_nanf("");
+      }
+    }
+    return;
+  }
+
+  i32x4 qf[NR][C::KC];
+#pragma unroll
+  for (int nr = 0; nr < NR; ++nr) {
+    const int hq = hk * p.G + hqo[nr];
+    const char* src = (const char*)((const T*)a.q.data + b * a.q.sb + hq * a.q.sh + (int64_t)qi[nr] * a.q.ss) + 16 * h;
+#pragma unroll
+    for (int kc = 0; kc < C::KC; ++kc) qf[nr][kc] = ld_global16(src + 32 * kc);
+  }
+
+  // this wave's tiles: first + NW * j, j < nt
+  const int n = sq.n, last = n + p.Sq - 1;
+  const int first = sq.t0 + ck.first + wave;
+  const int nt = __builtin_amdgcn_readfirstlane(max((ck.count - wave + NW - 1) / NW, 0));
+  const uint64_t kp = (uint64_t)((const T*)a.k.data + b * a.k.sb + hk * a.k.sh);
+  const uint64_t vp = (uint64_t)((const T*)a.v.data + b * a.v.sb + hk * a.v.sh);
+  auto issue_k = [&](int t, int st) {
+    const unsigned dst = wbase + st * 2 * C::TB;
+    const uint64_t base = kp + (uint64_t)(t * C::BN) * kss;
+    if (t * C::BN + C::BN - 1 <= last) {
+#pragma unroll
+      for (int e = 0; e < C::E; ++e)
+        load_lds16_base(kvo[e % C::PK], base + (uint64_t)(e / C::PK * C::PK * C::RPC) * kss, dst + e * 1024);
+    } else {  // rows behind the last one repeat it
+#pragma unroll 1
+      for (int e = 0; e < C::E; ++e) {
+        const int kr = e * C::RPC + crow;
+        load_lds16_base(min(kr, last - t * C::BN) * kss + swz_col<C::CPR>(kr, cchunk) * 16, base, dst + e * 1024);
+      }
+    }
+  };
+  auto issue_v = [&](int t, int st) {
+    const unsigned dst = wbase + st * 2 * C::TB + C::TB;
+    const uint64_t base = vp + (uint64_t)(t * C::BN) * vss;
+    if (t * C::BN + C::BN - 1 <= last) {
+#pragma unroll
+      for (int e = 0; e < C::E; ++e)
+        load_lds16_base(vvo[e % C::PV], base + (uint64_t)(e / C::PV * C::PV * C::RPC) * vss, dst + e * 1024);
+    } else {
+#pragma unroll 1
+      for (int e = 0; e < C::E; ++e) {
+        const int kr = e * C::RPC + crow;
+        load_lds16_base(min(kr, last - t * C::BN) * vss + swz_v<T, C::CPR>(kr, cchunk) * 16, base, dst + e * 1024);
+      }
+    }
+  };
+  if (nt > 0) {
+    issue_k(first, 0);
+    issue_v(first, 0);
+  }
+
+  // Row qi sees the cached keys [row_lo, n); the tiles that hold only keys every row
+  // sees need no mask.
+  int row_lo[NR], full_lo = 0;
+#pragma unroll
+  for (int nr = 0; nr < NR; ++nr) row_lo[nr] = 0;
+  if (p.window > 0) {
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+      const int depth = a.depths ? max(a.depths[(int64_t)b * p.Sq + qi[nr]], 0) : qi[nr];
+      // (n + depth - window without leaving 32 bits: depth at most the window counts)
+      row_lo[nr] = max(n - (p.window - min(depth, p.window)), 0);
+      full_lo = max(full_lo, row_lo[nr]);
+    }
+#pragma unroll
+    for (int y = 32; y; y >>= 1) full_lo = max(full_lo, __shfl_xor(full_lo, y));
+    full_lo = __builtin_amdgcn_readfirstlane(full_lo);
+  }
+  const unsigned char* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+
+  // wait for Q here, once: see fwd_split.hip
+#pragma unroll
+  for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+    for (int kc = 0; kc < C::KC; ++kc) {
+      if constexpr (!CAP) {
+        constexpr int kSign = sizeof(T) == 4 ? (int)0x80000000 : (int)0x80008000;
+        const int f = flip ? kSign : 0;
+        qf[nr][kc] ^= i32x4{f, f, f, f};
+      }
+      pin(qf[nr][kc]);
+    }
+
+  f32x16 acc[NR][C::DB];
+  float m_run[NR], l_run[NR];
+#pragma unroll
+  for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db) acc[nr][db] = f32x16{};
+    m_run[nr] = kNegInf;
+    l_run[nr] = 0.f;
+  }
 
   for (int j = 0; j < nt; ++j) {
     const int t = first + NW * j;
@@ -252,9 +405,15 @@ void tree_attn_kernel(TreeArgs a) {
     const char* sV = sK + C::TB;
     const int n0 = t * C::BN;
 
-    f32x16 sc = f32x16{};
+    f32x16 sc[NR];
 #pragma unroll
-    for (int kc = 0; kc < C::KC; ++kc) sc = mma_step<T>(lds_read16(sK + koff[kc]), qf[kc], sc);
+    for (int nr = 0; nr < NR; ++nr) sc[nr] = f32x16{};
+#pragma unroll
+    for (int kc = 0; kc < C::KC; ++kc) {
+      const i32x4 kf = lds_read16(sK + koff[kc]);
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr) sc[nr] = mma_step<T>(kf, qf[nr][kc], sc[nr]);
+    }
     if constexpr (ST == 1) {
       reads_done();
       if (more) issue_k(t + NW, 0);
@@ -263,48 +422,63 @@ void tree_attn_kernel(TreeArgs a) {
     // element e is key n0 + 8(e/4) + 4h + e%4
     if constexpr (CAP) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        float tv;
-        if constexpr (sizeof(T) == 4) sc[e] = p.cap_log2 * tanhf(sc[e] * p.scale * p.inv_cap);
-        else sc[e] = score_log2<true, false>(sc[e], p, 0.f, 0, 0, tv);
-      }
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float tv;
+          if constexpr (sizeof(T) == 4) sc[nr][e] = p.cap_log2 * tanhf(sc[nr][e] * p.scale * p.inv_cap);
+          else sc[nr][e] = score_log2<true, false>(sc[nr][e], p, 0.f, 0, 0, tv);
+        }
     }
     if (n0 < full_lo || n0 + C::BN > n) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int jj = n0 + 8 * (e >> 2) + 4 * h + (e & 3), u = jj - n;
-        bool ok;
-        if (u < 0) ok = jj >= row_lo;
-        else if (u >= p.Sq) ok = false;
-        else ok = mrow ? mrow[u] != 0 : u <= qi;
-        if (!ok) sc[e] = kNegInf;
+      for (int nr = 0; nr < NR; ++nr) {
+        // this lane's keys, relative to its first: e, and hidden before lo or from hi on
+        const int lo = row_lo[nr] - n0 - 4 * h, hi = n + (mask ? p.Sq : qi[nr] + 1) - n0 - 4 * h;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if ((unsigned)(8 * (e >> 2) + (e & 3) - lo) >= (unsigned)max(hi - lo, 0)) sc[nr][e] = kNegInf;
+        if (mask && n0 + C::BN > n) {  // all of the tile's mask bytes at once
+          const unsigned char* mrow = mask + (int64_t)qi[nr] * p.Sq;
+          const int u0 = n0 + 4 * h - n;
+          unsigned char m[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) m[e] = mrow[min(max(u0 + 8 * (e >> 2) + (e & 3), 0), p.Sq - 1)];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (u0 + 8 * (e >> 2) + (e & 3) >= 0 && m[e] == 0) sc[nr][e] = kNegInf;
+        }
       }
     }
-    float mx, mx2;
-    max16_partial(sc, mx, mx2);
-    mx = max2(mx, mx2);
-    if constexpr (!CAP) mx *= c2;
-    mx = fmaxf(mx, swap_halves(mx));
-    if (mx != mx) mx = kNegInf;
-    const bool grow = mx > m_run + kTreeRescale;
-    if (__builtin_amdgcn_ballot_w64(grow)) {
-      const float m_new = grow ? mx : m_run;
-      const float alpha = grow ? fast_exp2(m_run - m_new) : 1.f;
-      l_run *= alpha;
+    f32x16 pe[NR];
 #pragma unroll
-      for (int db = 0; db < C::DB; ++db) scale_inplace(acc[db], alpha);
-      m_run = m_new;
-    }
-    const float m_use = (m_run == kNegInf) ? 0.f : m_run;
-    f32x16 pe;
-    float rs[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int nr = 0; nr < NR; ++nr) {
+      if constexpr (!CAP) settle(sc[nr]);  // (an unmasked tile's scores come straight from the MFMAs)
+      float mx, mx2;
+      max16_partial(sc[nr], mx, mx2);
+      mx = max2(mx, mx2);
+      if constexpr (!CAP) mx *= c2;
+      mx = fmaxf(mx, swap_halves(mx));
+      if (mx != mx) mx = kNegInf;
+      const bool grow = mx > m_run[nr] + kTreeRescale;
+      if (__builtin_amdgcn_ballot_w64(grow)) {
+        const float m_new = grow ? mx : m_run[nr];
+        const float alpha = grow ? fast_exp2(m_run[nr] - m_new) : 1.f;
+        l_run[nr] *= alpha;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      if constexpr (!CAP) pe[e] = fast_exp2(__builtin_fmaf(sc[e], c2, -m_use));
-      else pe[e] = fast_exp2(sc[e] - m_use);
-      rs[e & 3] += pe[e];
+        for (int db = 0; db < C::DB; ++db) scale_inplace(acc[nr][db], alpha);
+        m_run[nr] = m_new;
+      }
+      const float m_use = (m_run[nr] == kNegInf) ? 0.f : m_run[nr];
+      float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if constexpr (!CAP) pe[nr][e] = fast_exp2(__builtin_fmaf(sc[nr][e], c2, -m_use));
+        else pe[nr][e] = fast_exp2(sc[nr][e] - m_use);
+        rs[e & 3] += pe[nr][e];
+      }
+      l_run[nr] += (rs[0] + rs[1]) + (rs[2] + rs[3]);
     }
-    l_run += (rs[0] + rs[1]) + (rs[2] + rs[3]);
     if constexpr (ST == 1) {  // V of tile j landed (the next K may be in flight)
       if (more) wait_vmcnt<C::E>();
       else wait_vmcnt<0>();
@@ -317,20 +491,25 @@ void tree_attn_kernel(TreeArgs a) {
 #pragma unroll
         for (int db = 0; db < C::DB; ++db) {
           const float v = *(const float*)(vr + voff[db]);
-          acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, pe[i], acc[db], 0, 0, 0);
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr)
+            acc[nr][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, pe[nr][i], acc[nr][db], 0, 0, 0);
         }
       }
     } else {
       typedef typename Mfma<T>::v8 V8;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const V8 pb = pack8<T>(pe, 8 * c);
+        V8 pb[NR];
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) pb[nr] = pack8<T>(pe[nr], 8 * c);
         const char* vr = sV + 16 * c * C::ROWB;
 #pragma unroll
         for (int db = 0; db < C::DB; ++db) {
           const i16x4 lo = lds_read_tr4(vr + voff[db]);
           const i16x4 hi = lds_read_tr4(vr + 8 * C::ROWB + voff[db]);
-          acc[db] = Mfma<T>::mma(cat_tr<V8>(lo, hi), pb, acc[db]);
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr) acc[nr][db] = Mfma<T>::mma(cat_tr<V8>(lo, hi), pb[nr], acc[nr][db]);
         }
       }
     }
@@ -340,106 +519,151 @@ void tree_attn_kernel(TreeArgs a) {
     }
   }
 
-  // The NW waves' (m, l, acc) combined in wave order through LDS (every wave's
-  // copies have landed: its last tile waited for vmcnt 0), then O / l and LSE.
-  const float l_tot = l_run + swap_halves(l_run);
-  __syncthreads();
-  float* xm = (float*)smem;  // [NW][64]
-  float* xl = xm + NW * 64;  // [NW][64]
-  float* xa = xl + NW * 64;  // [NW][DB][16][64]
-  xm[wave * 64 + lane] = m_run;
-  xl[wave * 64 + lane] = l_tot;
+  // The NW waves' (m, l, acc) combined in wave order through LDS, one row tile after
+  // the other (every wave's copies have landed: its last tile waited for vmcnt 0),
+  // then O / l and LSE.
+  float* xm = (float*)smem;            // [NW][64]
+  float* xl = xm + NW * 64;            // [NW][64]
+  f32x4* xa = (f32x4*)(xl + NW * 64);  // [NW][4 DB][64]: columns 8 y + 4 h .. + 3 of row l32
 #pragma unroll
-  for (int db = 0; db < C::DB; ++db)
+  for (int nr = 0; nr < NR; ++nr) {
+    const float l_tot = l_run[nr] + swap_halves(l_run[nr]);
+    __syncthreads();
+    xm[wave * 64 + lane] = m_run[nr];
+    xl[wave * 64 + lane] = l_tot;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) xa[((wave * C::DB + db) * 16 + e) * 64 + lane] = acc[db][e];
-  __syncthreads();
-  float mw[NW], mall = kNegInf;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    mw[w] = xm[w * 64 + lane];
-    mall = fmaxf(mall, mw[w]);
-  }
-  float al[NW], L = 0.f;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    // a wave whose maximum stayed -inf has weights of 0, or NaN scores
-    al[w] = mw[w] == kNegInf ? (xl[w * 64 + lane] == 0.f ? 0.f : 1.f) : fast_exp2(mw[w] - mall);
-    L = __builtin_fmaf(al[w], xl[w * 64 + lane], L);
-  }
-  const bool empty = L == 0.f;  // no key; NaN (a NaN query row or key) is not
-  const float inv = empty ? 0.f : 1.0f / L;
-  if (32 * rt + l32 < R) {
-    float* po = a.part_o + (row * a.nsplit + s) * D + 4 * h;
-    T* out = (T*)a.o.data + b * a.o.sb + hq * a.o.sh + (int64_t)qi * a.o.ss + 4 * h;
-    for (int x = wave; x < 4 * C::DB; x += NW) {  // 4 columns of this row per half wave
-      f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < NW; ++w)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = __builtin_fmaf(al[w], xa[(w * C::DB * 16 + 4 * x + j) * 64 + lane], o[j]);
-      o *= inv;
-      if (pl.ns > 1) *(f32x4*)(po + 8 * x) = o;
-      else if constexpr (sizeof(T) == 4) *(f32x4*)(out + 8 * x) = o;
-      else st_global8(out + 8 * x, pack4<T>(o[0], o[1], o[2], o[3]));
+    for (int y = 0; y < 4 * C::DB; ++y) {
+      const f32x16& v = acc[nr][y / 4];
+      const int e = y % 4 * 4;
+      xa[(wave * 4 * C::DB + y) * 64 + lane] = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
     }
-    if (wave == 0 && h == 0) {
-      const float lse = empty ? kNegInf : mall + log2f(L);
-      if (pl.ns > 1) a.part_lse[row * a.nsplit + s] = lse;
-      else a.lse[row] = lse * kLn2;
+    __syncthreads();
+    float mw[NW], mall = kNegInf;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      mw[w] = xm[w * 64 + lane];
+      mall = fmaxf(mall, mw[w]);
+    }
+    float al[NW], L = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      // a wave whose maximum stayed -inf has weights of 0, or NaN scores
+      const float lw = xl[w * 64 + lane];
+      al[w] = mw[w] == kNegInf ? (lw == 0.f ? 0.f : 1.f) : fast_exp2(mw[w] - mall);
+      L = __builtin_fmaf(al[w], lw, L);
+    }
+    const bool empty = L == 0.f;  // no key; NaN (a NaN query row or key) is not
+    const float inv = empty ? 0.f : 1.0f / L;
+    if (32 * (rt0 + nr) + l32 < R) {
+      const int hq = hk * p.G + hqo[nr];
+      const int64_t row = ((int64_t)b * p.Hq + hq) * p.Sq + qi[nr];
+      float* po = a.part_o + (row * a.nsplit + s) * D + 4 * h;
+      T* out = (T*)a.o.data + b * a.o.sb + hq * a.o.sh + (int64_t)qi[nr] * a.o.ss + 4 * h;
+#pragma unroll 2
+      for (int y = wave; y < 4 * C::DB; y += NW) {
+        f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const f32x4 v = xa[(w * 4 * C::DB + y) * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(al[w], v[e], o[e]);
+        }
+        o *= inv;
+        if (ns > 1) *(f32x4*)(po + 8 * y) = o;
+        else if constexpr (sizeof(T) == 4) *(f32x4*)(out + 8 * y) = o;
+        else st_global8(out + 8 * y, pack4<T>(o[0], o[1], o[2], o[3]));
+      }
+      if (wave == 0 && h == 0) {
+        const float lse = empty ? kNegInf : mall + log2f(L);
+        if (ns > 1) a.part_lse[row * a.nsplit + s] = lse;
+        else a.lse[row] = lse * kLn2;
+      }
     }
   }
 }
 
-// Merge of a row's partials, one workgroup per row, four columns per thread:
-// M = max LSE_s, O = sum 2^(LSE_s - M) O_s / sum 2^(LSE_s - M).  A partial without
-// keys has LSE -inf and is left out; one with a NaN score makes the row NaN.
+// Merge of a row's partials, one wave per row, four columns per lane and D / 4 lanes
+// for every NG-th partial: M = max LSE_s, O = sum 2^(LSE_s - M) O_s /
+// sum 2^(LSE_s - M).  A partial without keys has LSE -inf and is left out; one with a
+// NaN score makes the row NaN.  Latency-bound: all LSEs at once, one per lane.
 template <class T, int D>
-__global__ __launch_bounds__(64) void tree_merge_kernel(TreeArgs a) {
-  constexpr int TPR = D / 4;
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
+  constexpr int TPR = D / 4, NG = TPR < 64 ? 64 / TPR : 1;
   const Shape& p = a.p;
-  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (int64_t)p.B * p.Hq * p.Sq) return;
   const int i = (int)(row % p.Sq);
   const int64_t bh = row / p.Sq;
-  const int hq = (int)(bh % p.Hq), b = (int)(bh / p.Hq);
-  const int ns = tree_plan<TreeCfg<T, D>::NW>(a, b).ns;
+  const int hq = (int)(bh % p.Hq), b = (int)(bh / p.Hq), hk = hq / p.G;
+  const int ns = a.counts[b * p.Hkv + hk];
   if (ns == 1) return;  // (and a sequence that does not fit) written by its workgroup
   const float* pl = a.part_lse + row * a.nsplit;
   float mx = kNegInf;
-  for (int s = 0; s < ns; ++s) mx = fmaxf(mx, pl[s]);
-  const float m0 = mx == kNegInf ? 0.f : mx;
-  float ws = 0.f;
-  for (int s = 0; s < ns; ++s) ws += fast_exp2(pl[s] - m0);
-  const bool none = ws == 0.f;
-  const int c = threadIdx.x;
-  if (c < TPR) {
-    const f32x4* po = (const f32x4*)(a.part_o + row * a.nsplit * D) + c;
-    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < ns; ++s) {
-      const float lw = pl[s], w = fast_exp2(lw - m0);
-      const f32x4 v = po[(int64_t)s * TPR];
+  for (int s0 = 0; s0 < ns; s0 += 64) mx = fmaxf(mx, s0 + lane < ns ? pl[s0 + lane] : kNegInf);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = lw != kNegInf ? __builtin_fmaf(w, v[j], acc[j]) : acc[j];
+  for (int x = 32; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
+  const float m0 = mx == kNegInf ? 0.f : mx;
+  const int c = lane % TPR, g = lane / TPR;
+  const f32x4* po = (const f32x4*)(a.part_o + row * a.nsplit * D) + c;
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  float ws = 0.f;
+  constexpr int U = 4;
+  for (int s0 = g; s0 < ns; s0 += NG * U) {
+    f32x4 v[U];
+    float lw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // (a partial past the last: the last again, without a weight)
+      const int s = s0 + NG * u, t = min(s, ns - 1);
+      v[u] = po[(int64_t)t * TPR];
+      lw[u] = s < ns ? pl[t] : kNegInf;
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float w = fast_exp2(lw[u] - m0);
+      const bool keys = lw[u] != kNegInf;  // without keys the values do not count, not even an inf
+      ws += w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = keys ? __builtin_fmaf(w, v[u][j], acc[j]) : acc[j];
+    }
+  }
+#pragma unroll
+  for (int x = TPR; x < 64; x *= 2) {
+    ws += __shfl_xor(ws, x);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], x);
+  }
+  const bool none = ws == 0.f;  // no key for this row
+  if (g == 0) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[j] = none ? 0.f : acc[j] / ws;
     T* out = (T*)a.o.data + b * a.o.sb + hq * a.o.sh + (int64_t)i * a.o.ss + 4 * c;
     if constexpr (sizeof(T) == 4) *(f32x4*)out = acc;
     else st_global8(out, pack4<T>(acc[0], acc[1], acc[2], acc[3]));
   }
-  if (c == 0) a.lse[row] = none ? kNegInf : (mx + log2f(ws)) * kLn2;
+  if (lane == 0) a.lse[row] = none ? kNegInf : (mx + log2f(ws)) * kLn2;
+}
+
+template <class T, int D, int NR>
+void launch_tree_nr(const TreeArgs& a, hipStream_t st) {
+  using C = TreeCfg<T, D>;
+  const dim3 grid((unsigned)((a.nchunk + 7) / 8 * 8 * a.nrt)), block(C::NW * 64);
+  if (a.p.cap > 0.f) hipLaunchKernelGGL((tree_attn_kernel<T, D, C::NW, NR, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((tree_attn_kernel<T, D, C::NW, NR, false>), grid, block, 0, st, a);
 }
 
 template <class T, int D>
 hipError_t launch_tree(TreeArgs a, hipStream_t st) {
   using C = TreeCfg<T, D>;
-  a.nrt = (int)(((int64_t)a.p.G * a.p.Sq + 31) / 32);
-  const dim3 grid((unsigned)((int64_t)a.nsplit * a.nrt * a.p.B * a.p.Hkv)), block(C::NW * 64);
-  if (a.p.cap > 0.f) hipLaunchKernelGGL((tree_attn_kernel<T, D, C::NW, true>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((tree_attn_kernel<T, D, C::NW, false>), grid, block, 0, st, a);
+  const int64_t tiles = ((int64_t)a.p.G * a.p.Sq + 31) / 32;
+  const bool two = C::NR == 2 && tiles > 1;
+  a.nrt = (int)(two ? (tiles + 1) / 2 : tiles);
+  if (two) launch_tree_nr<T, D, C::NR>(a, st);
+  else launch_tree_nr<T, D, 1>(a, st);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.nsplit == 1) return e;
-  hipLaunchKernelGGL((tree_merge_kernel<T, D>), dim3((unsigned)((int64_t)a.p.B * a.p.Hq * a.p.Sq)), dim3(64), 0, st, a);
+  const int64_t rows = (int64_t)a.p.B * a.p.Hq * a.p.Sq;
+  hipLaunchKernelGGL((tree_merge_kernel<T, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
