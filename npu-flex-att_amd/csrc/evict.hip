@@ -4,12 +4,16 @@
 // in the reference, which has no cache.
 //
 //  * evict_select_kernel: one workgroup per (sequence, head).  A score becomes an
-//    unsigned key of the same order (NaN above everything, -0 as 0), and the
-//    smallest kept key is found digit by digit, 8 bits a pass: a histogram of the
-//    keys that match the digits so far, and the digit at which the count from
-//    above reaches the number wanted.  Keys above it stay; of those equal to it
-//    the lowest slots.  A scan over the slots then gives each kept row its place.
-//    Counts are integers, so the order of the atomics does not matter.
+//    unsigned key of the same order (NaN above everything, -0 as 0).  The keys are
+//    narrowed to those that share their leading bits with the last kept one, a digit a
+//    pass from the highest bit in which any two differ: a histogram, and the digit at
+//    which the count from above reaches the number wanted.  Once at most 64 are left,
+//    each lane of a wave counts the larger ones of one (of equal ones the lower slot is
+//    the larger), and the one with the right rank is the last kept; where more than
+//    that have the same key, their slots are counted in order instead.  A scan over the slots then gives each kept row its place.  Counts are
+//    integers and ranks follow from keys and slots, so the order of the atomics does
+//    not matter.  Latency: a chain of passes over keys that stay in registers up to
+//    eight slots a thread; 256 threads up to 2048 slots, for cheaper barriers.
 //  * evict_gather_kernel: copies the rows, 16 bytes per lane; bound by memory
 //    (each kept row read and written once).
 #include "flexatt_device.h"
@@ -18,126 +22,206 @@
 namespace flexatt {
 
 namespace {
-constexpr int kSel = 1024;  // threads of a selection
-constexpr int kSelWaves = kSel / 64;
+constexpr int kPer = 8;  // consecutive slots per thread and block
 
 // Larger float <-> larger unsigned; NaN is the largest, and -0 equals 0.
 __device__ __forceinline__ unsigned order_key(float x) {
-  if (x != x) return 0xffffffffu;
   const unsigned u = __float_as_uint(x + 0.0f);  // -0 + 0 = 0
-  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  const unsigned k = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  return x != x ? 0xffffffffu : k;
 }
 
-// Exclusive sum over the workgroup; `total` gets the whole sum.
+// Exclusive sum over a workgroup of NT threads; `total` gets the whole sum.  Every
+// thread calls it.
+template <int NT>
 __device__ __forceinline__ int scan_sum(int v, int* tot, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
+  const int x = wave_scan(v);
   __syncthreads();  // the previous use of tot is over
   if (lane == 63) tot[wave] = x;
   __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kSelWaves; ++w) {
-    if (w < wave) before += tot[w];
-    all += tot[w];
-  }
-  total = all;
-  return before + x - v;
+  const int mine = lane < NT / 64 ? tot[lane] : 0;
+  const int upto = wave_scan(mine);
+  total = __builtin_amdgcn_readlane(upto, 63);
+  return __builtin_amdgcn_readlane(upto - mine, __builtin_amdgcn_readfirstlane(wave)) + x - v;
 }
 
-__global__ __launch_bounds__(kSel) void evict_select_kernel(EvictArgs a) {
-  __shared__ int hist[256];
-  __shared__ int tot[kSelWaves];
-  __shared__ unsigned s_digit;
-  __shared__ int s_above;
-  const int tid = threadIdx.x;
+template <int NT>
+__global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
+  constexpr int kBins = 2 * NT, kDigit = NT == 1024 ? 11 : 9;
+  static_assert(kBins == 1 << kDigit, "two bins per thread");
+  __shared__ int hist[kBins];
+  __shared__ int tot[NT / 64];
+  __shared__ unsigned lows[NT / 64], highs[NT / 64];
+  __shared__ unsigned ckey[64];
+  __shared__ int cslot[64];
+  __shared__ int s_digit, s_above, s_count, s_slot;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int bh = blockIdx.x, b = bh / a.H;
   const int n = min(max(a.lengths[b], 0), a.C);
   const float* sc = a.scores + (int64_t)bh * a.C;
   float* so = a.scores_out + (int64_t)bh * a.out_rows;
   int* slots = a.slots + (int64_t)bh * a.keep;
   const int kept = min(n, a.keep);
-  if (bh % a.H == 0 && tid == 0) a.lengths_out[b] = kept;
-  for (int i = kept + tid; i < a.out_rows; i += kSel) so[i] = 0.f;
-  for (int i = kept + tid; i < a.keep; i += kSel) slots[i] = -1;
+  if (bh - b * a.H == 0 && tid == 0) a.lengths_out[b] = kept;
+  for (int i = kept + tid; i < a.out_rows; i += NT) so[i] = 0.f;
+  for (int i = kept + tid; i < a.keep; i += NT) slots[i] = -1;
   if (n <= a.keep) {
-    for (int i = tid; i < n; i += kSel) {
+    for (int i = tid; i < n; i += NT) {
       slots[i] = i;
       so[i] = sc[i];
     }
     return;
   }
 
-  // the slots that go by their score: [lo, hi), `want` of them stay
-  const int lo = a.sinks, hi = n - a.recent, want = a.keep - a.sinks - a.recent;
-  unsigned prefix = 0, mask = 0;
-  int need = want;  // still wanted among the keys that match the digits so far
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    for (int i = lo + tid; i < hi; i += kSel) {
-      const unsigned k = order_key(sc[i]);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+  // the slots that go by their score: [lo, hi), `need` of them stay
+  const int lo = a.sinks, hi = n - a.recent;
+  int need = a.keep - a.sinks - a.recent;
+  constexpr int kBlock = NT * kPer;
+  const int nb = (n - 1) / kBlock + 1;
+  float x[kPer];  // this thread's slots of block `blk`: kBlock blk + kPer tid + e
+  auto load = [&](int blk) {
+    const int i0 = blk * kBlock + tid * kPer;
+    if (i0 + kPer <= n) {
+      struct __attribute__((packed, aligned(4))) Quad {
+        float v[4];
+      };
+      const Quad* q = (const Quad*)(sc + i0);
+      const Quad q0 = q[0], q1 = q[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = q0.v[e], x[4 + e] = q1.v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) x[e] = sc[min(i0 + e, n - 1)];
     }
+  };
+  auto each = [&](auto f) {  // f(slot, key) for the slots that go by their score
+    for (int blk = 0; blk < nb; ++blk) {
+      if (nb > 1) load(blk);  // (a single block stays in registers)
+      const int i0 = blk * kBlock + tid * kPer;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        if (i0 + e >= lo && i0 + e < hi) f(i0 + e, order_key(x[e]));
+    }
+  };
+  if (nb == 1) load(0);
+
+  // A slot stays by its score where its key is above last_key, or is last_key and the
+  // slot is at most last_slot.
+  unsigned last_key = 0xffffffffu;
+  int last_slot = -1;
+  if (need > 0) {
+    hist[tid] = 0;
+    hist[tid + NT] = 0;
+    // the bits that all keys share
+    unsigned low = 0, high = 0;  // of the complements, and of the keys, the largest
+    each([&](int, unsigned k) {
+      low = max(low, ~k);
+      high = max(high, k);
+    });
+    low = wave_max(low);
+    high = wave_max(high);
+    if (lane == 0) lows[wave] = low, highs[wave] = high;
     __syncthreads();
-    // the digit d with (keys above d) < need <= (keys at or above d)
-    if (tid < 64) {
-      int c[4], sum = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        c[e] = hist[255 - (4 * tid + e)];
-        sum += c[e];
+    low = ~wave_max(lane < NT / 64 ? lows[lane] : 0);
+    high = wave_max(lane < NT / 64 ? highs[lane] : 0);
+    // keys whose bits from `top` on equal `prefix`'s are left: `count` of them
+    int top = low == high ? 0 : 32 - __builtin_clz(low ^ high);
+    unsigned prefix = top >= 32 ? 0 : high >> top << top;
+    int count = hi - lo;
+    while (count > 64 && top > 0) {
+      const int shift = max(top - kDigit, 0);
+      const unsigned width = (1u << (top - shift)) - 1u;
+      each([&](int, unsigned k) {
+        if (((uint64_t)(k ^ prefix) >> top) == 0) atomicAdd(&hist[(k >> shift) & width], 1);
+      });
+      __syncthreads();
+      // thread t has the bins 2 t and 2 t + 1 from above
+      const int h0 = hist[kBins - 1 - 2 * tid], h1 = hist[kBins - 2 - 2 * tid];
+      int all;
+      const int above = scan_sum<NT>(h0 + h1, tot, all);
+      if (above < need && above + h0 + h1 >= need) {
+        const bool first = above + h0 >= need;
+        s_digit = kBins - 1 - 2 * tid - (first ? 0 : 1);
+        s_above = above + (first ? 0 : h0);
+        s_count = first ? h0 : h1;
       }
-      int x = sum;
+      hist[kBins - 1 - 2 * tid] = 0;
+      hist[kBins - 2 - 2 * tid] = 0;
+      __syncthreads();
+      prefix |= (unsigned)s_digit << shift;
+      need -= s_above;
+      count = s_count;
+      top = shift;
+    }
+    if (count > 64) {  // equal keys: the slot of the need-th of them
+      last_key = prefix;
+      int seen = 0;
+      for (int blk = 0; blk < nb; ++blk) {
+        if (nb > 1) load(blk);
+        const int i0 = blk * kBlock + tid * kPer;
+        int eq = 0;
 #pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const int y = __shfl_up(x, d);
-        if (tid >= d) x += y;
-      }
-      int above = x - sum;
+        for (int e = 0; e < kPer; ++e) eq += i0 + e >= lo && i0 + e < hi && order_key(x[e]) == prefix;
+        int all, at = seen + scan_sum<NT>(eq, tot, all);
+        seen += all;
+        if (at < need && at + eq >= need) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (above < need && above + c[e] >= need) {
-          s_digit = 255 - (4 * tid + e);
-          s_above = above;
+          for (int e = 0; e < kPer; ++e)
+            if (i0 + e >= lo && i0 + e < hi && order_key(x[e]) == prefix && ++at == need) s_slot = i0 + e;
         }
-        above += c[e];
       }
-      if (need <= 0 && tid == 0) {  // nothing goes by score: a threshold no key passes
-        s_digit = 255;
-        s_above = 0;
+      __syncthreads();
+      last_slot = s_slot;
+    } else {
+      // the candidates, in any order, and the one with need - 1 larger ones
+      __syncthreads();
+      if (tid == 0) s_count = 0;
+      __syncthreads();
+      each([&](int i, unsigned k) {
+        if (((uint64_t)(k ^ prefix) >> top) == 0) {
+          const int c = atomicAdd(&s_count, 1);
+          ckey[c] = k;
+          cslot[c] = i;
+        }
+      });
+      __syncthreads();
+      const unsigned k = lane < count ? ckey[lane] : 0;
+      const int i = lane < count ? cslot[lane] : 0x7fffffff;
+      int larger = 0;
+      for (int c = 0; c < count; ++c) {
+        const unsigned kc = (unsigned)__builtin_amdgcn_readlane((int)k, c);
+        larger += kc > k || (kc == k && __builtin_amdgcn_readlane(i, c) < i);
       }
+      const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < count && larger == need - 1) | 1ull << 63);
+      last_key = (unsigned)__builtin_amdgcn_readlane((int)k, l);
+      last_slot = __builtin_amdgcn_readlane(i, l);
     }
-    __syncthreads();
-    prefix |= s_digit << shift;
-    mask |= 255u << shift;
-    need -= s_above;
-    __syncthreads();
   }
 
-  // prefix: the smallest kept key; `need` of its equals stay, the lowest slots
-  int ties = 0, place = 0;  // before this chunk
-  for (int i0 = 0; i0 < n; i0 += kSel) {
-    const int i = i0 + tid;
-    const bool in = i < n, free = in && i >= lo && i < hi;
-    const float x = in ? sc[i] : 0.f;
-    const unsigned k = order_key(x);
-    const int eq = free && k == prefix;
-    int all;
-    const int tie = ties + scan_sum(eq, tot, all);
-    ties += all;
-    const int stay = in && (!free || (want > 0 && (k > prefix || (eq && tie < need))));
-    const int at = place + scan_sum(stay, tot, all);
-    place += all;
-    if (stay) {
-      slots[at] = i;
-      so[at] = x;
+  // places, in slot order
+  int place = 0;
+  for (int blk = 0; blk < nb; ++blk) {
+    if (nb > 1) load(blk);
+    const int i0 = blk * kBlock + tid * kPer;
+    unsigned stay = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int i = i0 + e;
+      const unsigned k = order_key(x[e]);
+      const bool by_score = k > last_key || (k == last_key && i <= last_slot);
+      if (i < n && (i < lo || i >= hi || by_score)) stay |= 1u << e;
     }
+    int all;
+    int at = place + scan_sum<NT>(__builtin_popcount(stay), tot, all);
+    place += all;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (stay & (1u << e)) {
+        slots[at] = i0 + e;
+        so[at] = x[e];
+        at += 1;
+      }
   }
 }
 
@@ -185,7 +269,8 @@ void gather(const EvictArgs& a, hipStream_t st) {
 }  // namespace
 
 hipError_t evict_run(const EvictArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(evict_select_kernel, dim3(a.B * a.H), dim3(kSel), 0, st, a);
+  if (a.C <= 256 * kPer) hipLaunchKernelGGL(evict_select_kernel<256>, dim3(a.B * a.H), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(evict_select_kernel<1024>, dim3(a.B * a.H), dim3(1024), 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   switch (a.D * a.es / 16) {

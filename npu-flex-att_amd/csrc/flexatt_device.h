@@ -229,6 +229,32 @@ __device__ __forceinline__ float swap_halves(float x) {
   return __uint_as_float(lo ? r[1] : r[0]);
 }
 
+// Inclusive sum over the lanes of a wave, and the maximum of all of them, of
+// numbers for which 0 changes nothing: by lane shifts within rows of 16 and
+// broadcasts between them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or0(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+  x += dpp_or0<0x111, 0xf>(x);
+  x += dpp_or0<0x112, 0xf>(x);
+  x += dpp_or0<0x114, 0xf>(x);
+  x += dpp_or0<0x118, 0xf>(x);
+  x += dpp_or0<0x142, 0xa>(x);
+  x += dpp_or0<0x143, 0xc>(x);
+  return x;
+}
+__device__ __forceinline__ unsigned wave_max(unsigned x) {
+  x = max(x, (unsigned)dpp_or0<0x111, 0xf>((int)x));
+  x = max(x, (unsigned)dpp_or0<0x112, 0xf>((int)x));
+  x = max(x, (unsigned)dpp_or0<0x114, 0xf>((int)x));
+  x = max(x, (unsigned)dpp_or0<0x118, 0xf>((int)x));
+  x = max(x, (unsigned)dpp_or0<0x142, 0xa>((int)x));
+  x = max(x, (unsigned)dpp_or0<0x143, 0xc>((int)x));
+  return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
+}
+
 __device__ __forceinline__ i32x4 ld_global16(const void* p) { return *(const i32x4*)p; }
 __device__ __forceinline__ void st_global8(void* p, i32x2 v) { *(i32x2*)p = v; }
 

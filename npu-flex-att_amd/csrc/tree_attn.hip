@@ -110,31 +110,6 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
   x.t1 = (x.n + a.p.Sq + 31) / 32;
   return x;
 }
-// Inclusive sum, and maximum over the wave, of non-negative numbers, by lane shifts
-// within rows of 16 and broadcasts between them.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp(int x) {
-  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ int wave_scan(int x) {
-  x += dpp<0x111, 0xf>(x);
-  x += dpp<0x112, 0xf>(x);
-  x += dpp<0x114, 0xf>(x);
-  x += dpp<0x118, 0xf>(x);
-  x += dpp<0x142, 0xa>(x);
-  x += dpp<0x143, 0xc>(x);
-  return x;
-}
-__device__ __forceinline__ int wave_max(int x) {
-  x = max(x, dpp<0x111, 0xf>(x));
-  x = max(x, dpp<0x112, 0xf>(x));
-  x = max(x, dpp<0x114, 0xf>(x));
-  x = max(x, dpp<0x118, 0xf>(x));
-  x = max(x, dpp<0x142, 0xa>(x));
-  x = max(x, dpp<0x143, 0xc>(x));
-  return __builtin_amdgcn_readlane(x, 63);
-}
-
 // The chunk of workgroup x: which (b, hkv) (b < 0: none, x is past the last chunk),
 // which chunk of how many, its first tile and how many.  Every lane of a wave calls
 // it and gets the same; lane l looks at sequences l, l + 64, ....
@@ -152,7 +127,7 @@ __device__ __forceinline__ TreeChunk tree_chunk(const TreeArgs& a, int x, int nw
   int total = 0, most = 0;
   for (int b0 = 0, v = mine; b0 < B; b0 += 64, v = tiles_of(b0 + lane)) {
     total += __builtin_amdgcn_readlane(wave_scan(v), 63);
-    most = max(most, wave_max(v));
+    most = max(most, (int)wave_max((unsigned)v));
   }
   // The shortest chunks, whole rounds of the waves, with which one round of workgroups
   // has them all; not looked for where there are many sequences anyway.  Quotients by
@@ -591,40 +566,52 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   constexpr int TPR = D / 4, NG = TPR < 64 ? 64 / TPR : 1;
   const Shape& p = a.p;
   const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)p.B * p.Hq * p.Sq) return;
-  const int i = (int)(row % p.Sq);
-  const int64_t bh = row / p.Sq;
-  const int hq = (int)(bh % p.Hq), b = (int)(bh / p.Hq), hk = hq / p.G;
-  const int ns = a.counts[b * p.Hkv + hk];
+  const int row32 = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row32 >= p.B * p.Hq * p.Sq) return;
+  const int64_t row = row32;
+  const int bh = row32 / p.Sq, i = row32 - bh * p.Sq;
+  const int b = bh / p.Hq, hq = bh - b * p.Hq;
+  const int most = a.nsplit;
+  const float* pl = a.part_lse + row * most;
+  const int c = lane % TPR, g = lane / TPR;
+  const f32x4* po = (const f32x4*)(a.part_o + row * most * D) + c;
+  // The first partials are read before it is known how many the row has: what is
+  // there instead of the others is read (nsplit of them are the row's) and not used.
+  constexpr int U = 4;
+  f32x4 v[U];
+  float lw[U], ll;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int t = min(g + NG * u, most - 1);
+    v[u] = po[(int64_t)t * TPR];
+    lw[u] = pl[t];
+  }
+  ll = pl[min(lane, most - 1)];
+  const int ns = a.counts[b * p.Hkv + hq / p.G];
   if (ns == 1) return;  // (and a sequence that does not fit) written by its workgroup
-  const float* pl = a.part_lse + row * a.nsplit;
-  float mx = kNegInf;
-  for (int s0 = 0; s0 < ns; s0 += 64) mx = fmaxf(mx, s0 + lane < ns ? pl[s0 + lane] : kNegInf);
+  float mx = lane < ns ? ll : kNegInf;
+  for (int s0 = 64; s0 < ns; s0 += 64) mx = fmaxf(mx, s0 + lane < ns ? pl[s0 + lane] : kNegInf);
 #pragma unroll
   for (int x = 32; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
   const float m0 = mx == kNegInf ? 0.f : mx;
-  const int c = lane % TPR, g = lane / TPR;
-  const f32x4* po = (const f32x4*)(a.part_o + row * a.nsplit * D) + c;
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
   float ws = 0.f;
-  constexpr int U = 4;
-  for (int s0 = g; s0 < ns; s0 += NG * U) {
-    f32x4 v[U];
-    float lw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {  // (a partial past the last: the last again, without a weight)
-      const int s = s0 + NG * u, t = min(s, ns - 1);
-      v[u] = po[(int64_t)t * TPR];
-      lw[u] = s < ns ? pl[t] : kNegInf;
-    }
+  for (int s0 = g;;) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float w = fast_exp2(lw[u] - m0);
-      const bool keys = lw[u] != kNegInf;  // without keys the values do not count, not even an inf
+      const bool keys = s0 + NG * u < ns && lw[u] != kNegInf;  // without keys the values do not count, not even an inf
+      const float w = keys ? fast_exp2(lw[u] - m0) : 0.f;
       ws += w;
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[j] = keys ? __builtin_fmaf(w, v[u][j], acc[j]) : acc[j];
+    }
+    s0 += NG * U;
+    if (s0 - g >= ns) break;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = min(s0 + NG * u, most - 1);
+      v[u] = po[(int64_t)t * TPR];
+      lw[u] = pl[t];
     }
   }
 #pragma unroll
