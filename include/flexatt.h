@@ -331,7 +331,8 @@ int flexatt_rotary_apply(const flexatt_rotary* r, const flexatt_tensor* q, const
 
 /* q_out = turned q, and the rows lengths[b] .. lengths[b] + S - 1 of the cache
  * receive turned k and v [B, Hkv, S, D].  A row outside [0, cache_rows) is not
- * written.  `lengths` is not changed.  k and v may not overlap the cache. */
+ * written.  `lengths` is not changed.  k and v may not overlap the cache, nor k_cache be
+ * v_cache. */
 int flexatt_rotary_append(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* k,
                           const flexatt_tensor* v, const flexatt_tensor* q_out, const flexatt_tensor* k_cache,
                           const flexatt_tensor* v_cache, int32_t cache_rows, const int32_t* lengths, void* stream);
@@ -342,13 +343,15 @@ int flexatt_rotary_append(const flexatt_rotary* r, const flexatt_tensor* q, cons
  * drafted tokens themselves, where tree_mask[b][t][u] is not 0 (no mask: u <= t).
  * Scores, soft-cap, softmax and LSE as flexatt_fwd; a row without keys is 0 with
  * LSE -inf.  A sequence with n < 0 or n + T > cache_rows gets NaN (o and lse).
- * Rows of the cache from n + T on are not read. */
+ * Rows of the cache from n + T on are not read.  Values of rows that a token does not see
+ * have weight 0 in its sum, so they must be finite.  Rows of k_cache and v_cache lie less
+ * than 2^26 bytes apart (else FLEXATT_ERANGE). */
 typedef struct flexatt_tree {
   int32_t dtype;
   int32_t batch;
   int32_t heads_q;
   int32_t heads_kv;
-  int32_t tokens;         /* T >= 1; (Hq / Hkv) T at most 2^20 and B Hq T at most 2^28 (else FLEXATT_ERANGE) */
+  int32_t tokens;         /* T >= 1; (Hq / Hkv) T at most 2^20 and B Hq T at most 2^23 (else FLEXATT_ERANGE) */
   int32_t cache_rows;     /* >= 1 */
   int32_t head_dim;
   float scale;
@@ -428,7 +431,7 @@ typedef struct flexatt_evict {
 
 /* scores: contiguous fp32 [B, Hkv, cache_rows]; scores_out [B, Hkv, out_rows];
  * slots int32 [B, Hkv, keep]; lengths_out int32 [B].  No output may
- * overlap an input. */
+ * lie within the span of an input, nor k_out be v_out. */
 int flexatt_evict_rows(const flexatt_evict* p, const flexatt_tensor* k_cache, const flexatt_tensor* v_cache,
                        const float* scores, const flexatt_tensor* k_out, const flexatt_tensor* v_out,
                        float* scores_out, int32_t* slots, int32_t* lengths_out, void* stream);

@@ -25,7 +25,8 @@ int check_sizes(int dtype, int64_t b, int64_t h, int64_t s, int head_dim) {
   if (elt_size(dtype) == 0) return FLEXATT_EDTYPE;
   if (b <= 0 || h <= 0 || s <= 0) return FLEXATT_EINVAL;
   if (head_index(head_dim) < 0) return FLEXATT_EHEADDIM;
-  if (b * h > INT32_MAX || b * h * s > INT32_MAX) return FLEXATT_ESHAPE;
+  // (s: indices of up to a few tiles behind the last row fit 32 bits)
+  if (s > 1 << 30 || b * h > INT32_MAX || b * h * s > INT32_MAX) return FLEXATT_ESHAPE;
   return FLEXATT_OK;
 }
 
@@ -108,9 +109,9 @@ int check_tree(const flexatt_tree* p) {
   FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_q, p->tokens, p->head_dim));
   FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim));
   if (p->heads_q % p->heads_kv != 0) return FLEXATT_ESHAPE;
-  // (workgroups: up to the row tiles times the chunks, of 256 CUs or of (b, hkv) and more)
+  // (2^32 work-items are one launch's most)
   if ((int64_t)(p->heads_q / p->heads_kv) * p->tokens > 1 << 20) return FLEXATT_ERANGE;
-  if ((int64_t)p->batch * p->heads_q * p->tokens > 1 << 28) return FLEXATT_ERANGE;
+  if ((int64_t)p->batch * p->heads_q * p->tokens > 1 << 23) return FLEXATT_ERANGE;
   FLEXATT_TRY(check_scores(p->scale, p->soft_cap, p->sliding_window));
   if (p->reserved != 0 || !p->lengths) return FLEXATT_EINVAL;
   if (p->tree_mask ? p->mask_batch != 1 && p->mask_batch != p->batch : p->mask_batch != 0) return FLEXATT_EINVAL;
@@ -152,6 +153,7 @@ int check_weights(const flexatt_weights* p) {
   FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_q, p->seqlen_q, p->head_dim));
   FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_kv, p->seqlen_kv, p->head_dim));
   if (p->heads_q % p->heads_kv != 0) return FLEXATT_ESHAPE;
+  if ((int64_t)(p->heads_q / p->heads_kv) * p->seqlen_q > 1 << 30) return FLEXATT_ESHAPE;
   FLEXATT_TRY(check_scores(p->scale, p->soft_cap, p->sliding_window));
   if ((p->causal & ~1) || (p->accumulate & ~1) || p->reserved != 0) return FLEXATT_EINVAL;
   return FLEXATT_OK;
@@ -209,6 +211,7 @@ int flexatt_rotary_append(const flexatt_rotary* r, const flexatt_tensor* q, cons
   FLEXATT_TRY(check_out_tensor(q_out, r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
   FLEXATT_TRY(check_out_tensor(k_cache, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim));
   FLEXATT_TRY(check_out_tensor(v_cache, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim));
+  if (k_cache->data == v_cache->data) return FLEXATT_ELAYOUT;
   for (const flexatt_tensor* x : {k, v})
     for (const flexatt_tensor* y : {k_cache, v_cache})
       if (overlap(span_of(x, r->dtype, r->batch, r->heads_kv, r->seqlen, r->head_dim),
@@ -239,6 +242,8 @@ int flexatt_tree_fwd(const flexatt_tree* p, const flexatt_tensor* q, const flexa
   FLEXATT_TRY(check_tensor(q, p->dtype));
   FLEXATT_TRY(check_tensor(k_cache, p->dtype));
   FLEXATT_TRY(check_tensor(v_cache, p->dtype));
+  for (const flexatt_tensor* x : {k_cache, v_cache})  // offsets within a tile of 32 rows are 32 bits
+    if (p->cache_rows > 1 && x->stride_s >= (1 << 26) / (int64_t)elt_size(p->dtype)) return FLEXATT_ERANGE;
   FLEXATT_TRY(check_out_tensor(o, p->dtype, p->batch, p->heads_q, p->tokens, p->head_dim));
   if (!lse) return FLEXATT_EINVAL;
   const size_t need = flexatt_tree_fwd_workspace(p);
@@ -318,6 +323,7 @@ int flexatt_evict_rows(const flexatt_evict* p, const flexatt_tensor* k_cache, co
   FLEXATT_TRY(check_tensor(v_cache, p->dtype));
   FLEXATT_TRY(check_out_tensor(k_out, p->dtype, p->batch, p->heads_kv, p->out_rows, p->head_dim));
   FLEXATT_TRY(check_out_tensor(v_out, p->dtype, p->batch, p->heads_kv, p->out_rows, p->head_dim));
+  if (k_out->data == v_out->data) return FLEXATT_ELAYOUT;
   const int64_t bh = (int64_t)p->batch * p->heads_kv;
   const Span in[] = {span_of(k_cache, p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim),
                      span_of(v_cache, p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim),

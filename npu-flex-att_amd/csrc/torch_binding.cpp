@@ -417,7 +417,9 @@ PyObject* py_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Tensor lse = at::empty({B, Hq, T}, query.options().dtype(at::kFloat).requires_grad(false));
   if (query.numel() > 0) {
     // (the kernels' row offsets within a tile are 32 bits)
-    const auto near = [](const Tensor& t) { return t.stride(2) * t.element_size() < 1 << 26 ? prepare(t) : t.contiguous(); };
+    const auto near = [](const Tensor& t) {
+      return t.size(2) == 1 || t.stride(2) * t.element_size() < 1 << 26 ? prepare(t) : t.contiguous();
+    };
     const Tensor q = prepare(query), k = near(kc), v = near(vc);
     const size_t bytes = flexatt_tree_fwd_workspace(&p);
     const Tensor ws = workspace(bytes, dev);

@@ -160,11 +160,12 @@ __device__ __forceinline__ TreeChunk tree_chunk(const TreeArgs& a, int x, int nw
       const float inv = fast_rcp((float)n);
       r.hk = (int)((float)x * inv);
       r.s = x - r.hk * n;
-      if (r.s < 0) r.s += n, r.hk -= 1;
-      if (r.s >= n) r.s -= n, r.hk += 1;
+      while (r.s < 0) r.s += n, r.hk -= 1;
+      while (r.s >= n) r.s -= n, r.hk += 1;
       r.ns = n;
       int each = (int)((float)tiles * inv) + 1;
-      if ((each - 1) * n >= tiles) each -= 1;
+      while ((each - 1) * n >= tiles) each -= 1;
+      while (each * n < tiles) each += 1;
       r.first = r.s * each;
       r.count = max(min(each, tiles - r.first), 0);
       return r;

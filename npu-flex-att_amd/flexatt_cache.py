@@ -48,7 +48,8 @@ def tree_attention(query, key_cache, value_cache, lengths, tree_mask=None, slidi
     which token ``t`` sees those with ``tree_mask[t][u]`` set: a bool or integer [T, T]
     or [B, T, T], itself and its ancestors for a tree; None is a chain (``u <= t``).
     One token per sequence with no mask is ordinary decoding.  Rows behind those are
-    not read.
+    not read; values of rows a token does not see are multiplied by 0, so they must be
+    finite.
 
     ``sliding_window`` W keeps cached token ``j`` for drafted token ``t`` where
     ``lengths[b] + depths[b][t] - j <= W``; ``depths`` (int32 [T] or [B, T], 0 for a

@@ -27,7 +27,9 @@ TREE_BAD = [
     (dict(heads_kv=3), -4), (dict(heads_kv=0), -1), (dict(scale=float("nan")), -1), (dict(soft_cap=-1.0), -1),
     (dict(soft_cap=float("inf")), -1), (dict(sliding_window=-1), -1), (dict(reserved=1), -1), (dict(lengths=None), -1),
     (dict(mask_batch=1), -1), (dict(tree_mask=FAKE), -1), (dict(tree_mask=FAKE, mask_batch=3), -1),
-    (dict(tree_mask=FAKE, mask_batch=2, sliding_window=5), -1), (dict(batch=1 << 16, cache_rows=1 << 16), -4)]
+    (dict(tree_mask=FAKE, mask_batch=2, sliding_window=5), -1), (dict(batch=1 << 16, cache_rows=1 << 16), -4),
+    (dict(batch=1, heads_kv=1, heads_q=1, cache_rows=(1 << 30) + 1), -4),
+    (dict(heads_q=2, tokens=(1 << 20) + 1), -6), (dict(batch=1 << 12, heads_q=2, tokens=1 << 11), -6)]
 
 
 @pytest.mark.parametrize("kw,code", TREE_BAD)
@@ -48,6 +50,10 @@ def test_tree_capi_refuses_tensors_and_workspace():
     assert lib.flexatt_tree_fwd(p, q, odd, c, q, FAKE, FAKE, n, None) == -5
     assert lib.flexatt_tree_fwd(p, q, c, odd, q, FAKE, FAKE, n, None) == -5
     assert lib.flexatt_tree_fwd(p, q, c, c, L.Tensor(FAKE, 0, 512, 64, 1), FAKE, FAKE, n, None) == -5
+    # rows 2^26 bytes apart: their offsets within a tile would leave 32 bits
+    far = L.Tensor(FAKE, 1 << 40, 64, 1 << 25, 1)
+    assert lib.flexatt_tree_fwd(p, q, far, c, q, FAKE, FAKE, n, None) == -6
+    assert lib.flexatt_tree_fwd(p, q, c, far, q, FAKE, FAKE, n, None) == -6
     assert lib.flexatt_tree_fwd(p, q, c, c, q, None, FAKE, n, None) == -1
     assert lib.flexatt_tree_fwd(p, q, c, c, q, FAKE, None, 0, None) == -1
     assert lib.flexatt_tree_fwd(p, q, c, c, q, FAKE, FAKE, n - 1, None) == -1
@@ -64,7 +70,8 @@ def _weights(**kw):
 @pytest.mark.parametrize("kw,code", [
     (dict(dtype=-1), -2), (dict(seqlen_q=0), -1), (dict(seqlen_kv=0), -1), (dict(head_dim=48), -3),
     (dict(heads_kv=3), -4), (dict(scale=float("inf")), -1), (dict(soft_cap=float("nan")), -1), (dict(causal=2), -1),
-    (dict(accumulate=3), -1), (dict(sliding_window=-4), -1), (dict(reserved=9), -1)])
+    (dict(accumulate=3), -1), (dict(sliding_window=-4), -1), (dict(reserved=9), -1),
+    (dict(batch=1, heads_q=2, heads_kv=1, seqlen_q=(1 << 29) + 1), -4)])
 def test_weights_capi_refuses(kw, code):
     lib = L.load()
     assert lib.flexatt_weight_sums(_weights(**kw), _t(4, 8), _t(), FAKE, FAKE, FAKE, 1 << 40, None) == code
@@ -107,6 +114,7 @@ def test_evict_capi_refuses_overlap():
         bad = list(args)
         bad[i] = inside
         assert lib.flexatt_evict_rows(*bad) == -5
+    assert lib.flexatt_evict_rows(*args) == -5  # k_out is v_out
     for i in (1, 2, 3, 4, 5, 6, 7, 8):
         bad = list(args)
         bad[i] = None

@@ -209,3 +209,57 @@ def test_graph_replays_as_the_cache_grows(gpu_device):
         g2.replay()
         torch.cuda.synchronize()
         assert torch.equal(o1, e1) and torch.equal(o2, e2)
+
+
+@pytest.mark.parametrize("dtype,T,D,window", [(BF, 1, 32, 0), (FH, 3, 128, 90), (FS, 2, 64, 0)])
+def test_many_sequences_of_unequal_lengths(gpu_device, dtype, T, D, window):
+    """More sequences than a wave has lanes, from nothing cached to a full cache, one that does not fit among them."""
+    B, C = 150, 700
+    g = torch.Generator().manual_seed(5)
+    n = torch.randint(0, C - T + 1, (B,), generator=g).int()
+    n[::7], n[3::11], n[70] = 0, C - T, C
+    q, kc, vc = draw(1, B, 2, T, D, dtype), draw(2, B, 1, C, D, dtype, "bsnd"), draw(3, B, 1, C, D, dtype)
+    o, lse = fc.tree_attention(q, kc, vc, n.cuda(), sliding_window=window, return_lse=True)
+    ref = orc.tree_attention(q.cpu(), kc.cpu(), vc.cpu(), n, None, window, dtype=dtype)
+    check("o", o, ref[0], ref[2])
+    check("lse", lse, ref[1], ref[3])
+
+
+def test_caches_of_one_row_and_strides_of_size_one_dimensions(gpu_device):
+    q, k, v = draw(1, 3, 4, 1, 64, BF), draw(2, 3, 2, 1, 64, BF), draw(3, 3, 2, 1, 64, BF)
+    n = torch.zeros(3, dtype=torch.int32, device="cuda")
+    o, lse = fc.tree_attention(q, k, v, n, return_lse=True)
+    ref = orc.tree_attention(q.cpu(), k.cpu(), v.cpu(), n.cpu(), dtype=BF)
+    check("o", o, ref[0], ref[2])
+    check("lse", lse, ref[1], ref[3])
+    far = torch.as_strided(k, k.shape, (128, 64, 1 << 40, 1))  # no second row lies there
+    assert torch.equal(o, fc.tree_attention(q, far, v, n))
+    assert torch.equal(o, fc.tree_attention(torch.as_strided(q, q.shape, (256, 64, 3, 1)), k, v, n))
+
+
+def test_what_a_workspace_holds_does_not_matter(gpu_device):
+    q, kc, vc, n, m, depths, kw, dtype = run_case(13)
+    a = fc.tree_attention(q, kc, vc, n.cuda(), return_lse=True, **kw)
+    torch.cuda.synchronize()
+    for fill in (float("nan"), float("inf")):
+        junk = [torch.full((1 << s,), fill, device="cuda") for s in range(14, 23)]
+        del junk  # what the allocator hands out next
+        b = fc.tree_attention(q, kc, vc, n.cuda(), return_lse=True, **kw)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_two_streams_at_once(gpu_device):
+    q, kc, vc, n, m, depths, kw, dtype = run_case(13)
+    n = n.cuda()
+    want = [fc.tree_attention(q, kc, vc, n, scale=s) for s in (0.05, 0.2)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(fc.tree_attention(q, kc, vc, n, scale=(0.05, 0.2)[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for x in got[i]:
+            assert torch.equal(x, want[i])

@@ -26,6 +26,9 @@ CASES = [
     (FH, 1, 2, 1, 700, 600, 128, True, 0, None, 100, 0.0),            # rows behind every key's window
     (BF, 1, 16, 1, 3, 5000, 128, True, 4997, None, 0, 0.0),
     (BF, 1, 1, 1, 1, 1, 32, True, 0, None, 0, 0.0),
+    (FH, 1, 5, 1, 900, 70, 64, False, 0, None, 0, 0.0),               # few keys, many rows, five heads a key
+    (BF, 2, 11, 1, 401, 300, 128, True, [0, -390], [300, 7], 0, 20.0),
+    (FS, 1, 6, 2, 500, 40, 256, False, 0, [33], 0, 0.0),
 ]
 
 

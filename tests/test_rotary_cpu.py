@@ -113,3 +113,4 @@ def test_capi_append_refuses():
     assert call(vc=L.Tensor(far, 2 * 100 * 64, 0, 64, 1)) == -5          # heads at one place
     assert call(k=L.Tensor(far + 64, 1024, 512, 64, 1)) == -5            # the tokens overlap the cache
     assert call(v=L.Tensor(far + 64, 1024, 512, 64, 1)) == -5
+    assert call() == -5                                                  # one cache for keys and values
