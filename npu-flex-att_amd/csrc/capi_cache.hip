@@ -355,7 +355,7 @@ int flexatt_evict_rows(const flexatt_evict* p, const flexatt_tensor* k_cache, co
   a.out_rows = p->out_rows;
   a.fill = p->fill;
   a.es = (int)elt_size(p->dtype);
-  return (int)evict_run(a, (hipStream_t)stream);
+  return (int)evict_run(a, cus(), (hipStream_t)stream);
 }
 
 }  // extern "C"

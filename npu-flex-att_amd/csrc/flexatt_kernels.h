@@ -139,6 +139,7 @@ struct EvictArgs {
   int B, H, C, D, keep, recent, sinks, out_rows;
   int fill;  // 1: rows of ko and vo behind the last kept one, up to keep, are zeroed
   int es;    // bytes per element
+  int lanes_log2, nparts;  // lanes that copy a row, workgroups per (sequence, head) (set by the launcher)
 };
 
 typedef hipError_t (*TreeLauncher)(const TreeArgs&, hipStream_t);
@@ -174,7 +175,7 @@ hipError_t doc_bounds_run(const void* ids, int ids_bytes, int B, int S, int* bou
 hipError_t bwd_delta(int dtype, const DeltaArgs&, hipStream_t);
 
 hipError_t rotary_run(int dtype, const RotaryArgs&, hipStream_t);
-hipError_t evict_run(const EvictArgs&, hipStream_t);
+hipError_t evict_run(const EvictArgs&, int cus, hipStream_t);
 
 // Tree attention (tree_attn.hip) and weight sums (weight_sums.hip), every D.
 #define FLEXATT_DECL_CACHE(D)                              \

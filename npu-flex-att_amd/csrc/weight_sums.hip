@@ -141,20 +141,16 @@ void weight_sums_kernel(WeightArgs a) {
       continue;
     }
 
-    // The query rows [i_lo, i_hi) that see a key of the workgroup, and those that see
-    // all keys of the workgroup, as tiles of packed rows; this part's tiles.
+    // The query rows [i_lo, i_hi) that see a key of the workgroup, as tiles of packed
+    // rows; this part's tiles.
     const int R = p.G * p.Sq;
     const int64_t jl = min(j0 + C::KEYS, n) - 1;
-    int64_t i_lo = 0, i_hi = p.Sq, f_lo = 0, f_hi = p.Sq;
-    if (p.causal) i_lo = j0 - start, f_lo = jl - start;
-    if (p.window > 0) i_hi = min(i_hi, jl + p.window - start + 1), f_hi = min(f_hi, j0 + p.window - start + 1);
+    int64_t i_lo = 0, i_hi = p.Sq;
+    if (p.causal) i_lo = j0 - start;
+    if (p.window > 0) i_hi = min(i_hi, jl + p.window - start + 1);
     i_lo = min(max(i_lo, (int64_t)0), (int64_t)p.Sq);
     i_hi = max(i_hi, i_lo);
-    f_lo = max(f_lo, (int64_t)0);
     const int t_lo = (int)(i_lo * p.G / 32), t_hi = (int)((i_hi * p.G + 31) / 32);
-    // the tiles all of whose rows see all keys of the workgroup
-    const int full_lo = __builtin_amdgcn_readfirstlane((int)((min(f_lo, (int64_t)p.Sq) * p.G + 31) / 32));
-    const int full_hi = __builtin_amdgcn_readfirstlane((int)(max(f_hi, (int64_t)0) * p.G / 32));
     // this part's tiles: every nparts-th, so that all have their share of masked ones
     const int t0 = __builtin_amdgcn_readfirstlane(t_lo + part), dt = a.nparts;
     const int nt = __builtin_amdgcn_readfirstlane(t0 < t_hi ? (t_hi - t0 + dt - 1) / dt : 0);
@@ -213,7 +209,7 @@ void weight_sums_kernel(WeightArgs a) {
       }
       if (seg == 1) __builtin_amdgcn_s_barrier();  // every wave has read the first block's last tiles
 #pragma unroll
-      for (int u = 0; u < 2 * C::TPS; ++u)
+      for (int u = 0; u < C::RING; ++u)
         if (u < nt) issue(u);
       // wait for K here, once, with the first tiles: at its first use the compiler's
       // own wait would drain the copies of later tiles
@@ -234,45 +230,58 @@ void weight_sums_kernel(WeightArgs a) {
           for (int kc = 0; kc < KC; ++kc) kf[x][kc] ^= i32x4{kSign, kSign, kSign, kSign};
       }
     }
+    // The tiles that need a mask, of each block of 32 keys.
+    int part_lo[NK], part_hi[NK];
+#pragma unroll
+    for (int x = 0; x < NK; ++x) {
+      const int64_t f = j0 + (wave * NK + x) * 32, l = min(f + 31, (int64_t)n - 1);
+      const int64_t lo = p.causal ? max(l - start, (int64_t)0) : 0;
+      const int64_t hi = p.window > 0 ? max(f + p.window - start + 1, (int64_t)0) : p.Sq;
+      part_lo[x] = __builtin_amdgcn_readfirstlane((int)((min(lo, (int64_t)p.Sq) * p.G + 31) / 32));
+      part_hi[x] = __builtin_amdgcn_readfirstlane((int)(min(hi, (int64_t)p.Sq) * p.G / 32));
+    }
     // The last block's scores of a tile wait for the first MFMAs of the next one, and
     // the others' for those of the block after them, so that the exponentials run
     // beside MFMAs.  (None waits: scores of 0 of a row with LSE +inf, weights of 0.)
     f32x16 sw = f32x16{};
     float lw = kPosInf;
+    // A tile's rows are read from LDS while the MFMAs of the tile before last use its
+    // own: as each step is done, its registers are filled again.
+    i32x4 qf[KC];
+    float lse = 0.f;
+    if (nt > 0) {
+      if (nt >= C::RING) wait_vmcnt<2 * C::TPS * kCopies>();
+      else wait_vmcnt<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int kc = 0; kc < KC; ++kc) qf[kc] = lds_read16(smem + koff[kc & 1] + (kc >> 1) * 2048);
+      lse = *(const float*)(smem + C::TB + l32 * 4);
+    }
     for (int u = 0; u < nt; ++u) {
-      if (u % C::TPS == 0) {
-        // this wave's copies of this step's tiles have landed (those of the next step may
-        // be in flight) ...
-        if (u + 2 * C::TPS <= nt) wait_vmcnt<C::TPS * kCopies>();
-        else wait_vmcnt<0>();
-        __builtin_amdgcn_s_barrier();  // ... and every wave's; all are done with the step before
-        asm volatile("" ::: "memory");
-#pragma unroll
-        for (int x = 0; x < C::TPS; ++x)  // into the stages of the step before
-          if (u + 2 * C::TPS + x < nt) issue(u + 2 * C::TPS + x);
-      }
       const int t = t0 + u * dt;
-      const char* sQ = smem + u % C::RING * C::STAGEB;
-      // all reads first: one at a time, each would be waited for
-      const float lse = *(const float*)(sQ + C::TB + l32 * 4);
-      i32x4 qf[KC];
-#pragma unroll
-      for (int kc = 0; kc < KC; ++kc) qf[kc] = lds_read16(sQ + koff[kc & 1] + (kc >> 1) * 2048);
+      const char* sN = smem + (u + 1) % C::RING * C::STAGEB;  // the next tile
       // a row without keys gives no weight, whatever its scores
       const bool dead = 32 * t + l32 >= R || lse == kNegInf;
+      const bool any_dead = __builtin_amdgcn_ballot_w64(dead);
       const float l2 = dead ? kPosInf : lse * kLog2e;
-      const bool masked = t < full_lo || t >= full_hi || __builtin_amdgcn_ballot_w64(dead);
-      int hi32 = 0, lo32 = 0;  // keys [lo, hi) of the row, relative to the lane half's first of the workgroup
-      if (masked) {
-        asm volatile("");  // a branch: the compiler would compute the mask of every tile
-        const int64_t pos = start + (32 * t + l32) / p.G, base = j0 + 4 * h;
-        const int64_t hi = dead ? -1 : p.causal ? pos + 1 - base : (int64_t)1 << 30;
-        const int64_t lo = p.window > 0 ? pos - p.window - base : -1;
-        hi32 = (int)min(max(hi, (int64_t)-1), (int64_t)1 << 30);
-        lo32 = (int)min(max(lo, (int64_t)-1), (int64_t)1 << 30);
-      }
 #pragma unroll
       for (int x = 0; x < NK; ++x) {
+        if (x == NK - 1) {
+          if (u % C::TPS == C::TPS - 1 && u + 1 < nt) {
+            // this wave's copies of the next step have landed (those of the one after may
+            // be in flight), and its reads of this step's last tile have returned ...
+            if (u + 1 + 2 * C::TPS <= nt) wait_vmcnt<C::TPS * kCopies>();
+            else wait_vmcnt<0>();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();  // ... and every wave's
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int y = 1; y <= C::TPS; ++y)  // into the stages of this step
+              if (u + 2 * C::TPS + y < nt) issue(u + 2 * C::TPS + y);
+          }
+          lse = *(const float*)(sN + C::TB + l32 * 4);
+        }
         // The MFMAs of this block, and between them the weights of the waiting one, added
         // a step after their exponential.  The order is held by sched_barrier: left to
         // itself the compiler puts all weights first and their registers to use again.
@@ -282,6 +291,7 @@ void weight_sums_kernel(WeightArgs a) {
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
           sc = mma_step<T>(kf[x][kc], qf[kc], sc);
+          if (x == NK - 1) qf[kc] = lds_read16(sN + koff[kc & 1] + (kc >> 1) * 2048);
 #pragma unroll
           for (int e = 16 * kc / KC; e < 16 * (kc + 1) / KC; ++e) pe[e] = weight(sw[e], x == 0 ? lw : l2);
 #pragma unroll
@@ -299,11 +309,17 @@ void weight_sums_kernel(WeightArgs a) {
             else sc[e] = score_log2<true, false>(sc[e], p, 0.f, 0, 0, tv);
           }
         }
-        if (masked) {
-          asm volatile("");
+        if (t < part_lo[x] || t >= part_hi[x] || any_dead) {
+          asm volatile("");  // a branch: the compiler would compute the mask of every tile
+          // keys [lo, hi) of the row, relative to the lane half's first of this block
+          const int64_t pos = start + (32 * t + l32) / p.G, base = j0 + (wave * NK + x) * 32 + 4 * h;
+          const int64_t hi = dead ? -1 : p.causal ? pos + 1 - base : (int64_t)1 << 30;
+          const int64_t lo = p.window > 0 ? pos - p.window - base : -1;
+          const int hi32 = (int)min(max(hi, (int64_t)-1), (int64_t)1 << 30);
+          const int lo32 = (int)min(max(lo, (int64_t)-1), (int64_t)1 << 30);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int jj = (wave * NK + x) * 32 + 8 * (e >> 2) + (e & 3);
+            const int jj = 8 * (e >> 2) + (e & 3);
             if (jj >= hi32 || jj < lo32) sc[e] = kNegInf;
           }
         }
