@@ -120,7 +120,10 @@ int check_tree(const flexatt_tree* p) {
 }
 
 // How the key tiles are cut (tree_chunk, on the device, where the lengths are): into
-// about as many chunks as workgroups run at once, of eight tiles at least.  Chunks end
+// about as many chunks as workgroups run at once, of eight tiles at least (two per wave;
+// of 4 or 16 changes a short cache's 15 us by less than 0.2).  Rows of 256 bytes and more
+// leave room for one workgroup per CU (LDS; cut for two: bf16 D=256, window 4096, 25 ->
+// 35 us), shorter ones for two (cut for one: fp16 T=64 D=64 56 -> 75 us).  Chunks end
 // with their (b, hkv), which makes up to one more for each.  With a full cache a (b,
 // hkv) has its even share of the chunks, and up to twice that where lengths are
 // unequal.
@@ -161,7 +164,8 @@ int check_weights(const flexatt_weights* p) {
 
 // Workgroups that share the query rows of one pair of key blocks: the number whose
 // rounds of workgroups (two per CU, one with rows of 512 bytes) take least, with
-// about four row tiles' time to load and add up each block.
+// eight row tiles' time to load and add up the blocks.  (bf16 B=2 Hq=32 Hkv=8 S=4096
+// D=128 causal, 128 pairs: 4 parts 162 us, 6 and 8 167, 12 175, 16 177.)
 int weight_parts(const flexatt_weights* p) {
   const int rowb = p->head_dim * (int)elt_size(p->dtype);
   const int keys = rowb <= 512 ? 256 : 128;  // (WsCfg)
