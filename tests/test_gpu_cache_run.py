@@ -81,3 +81,55 @@ def test_prompt_evict_draft_accept(gpu_device, dtype, D, inter):
     kc2, vc2, score2, slots, n2 = fc.evict_cache(kc, vc, score, n, keep, recent=16)
     assert n2.tolist() == [keep, 53] and slots[1, 0, :53].tolist() == list(range(53))
     assert bool((slots[0, :, -16:] == torch.arange(keep + 3 - 16, keep + 3, device="cuda")).all())
+
+
+def test_offsets_past_32_bits(gpu_device):
+    """Caches whose rows lie 2^22 elements apart, so that row 520 starts past 2^31: as from dense ones, bit for bit."""
+    D, C = 64, 600
+    g = torch.Generator().manual_seed(3)
+    new = lambda *s: torch.randn(*s, D, generator=g).bfloat16().cuda()  # noqa: E731
+    wide = torch.zeros(C << 22, dtype=torch.bfloat16, device="cuda").view(1, 1, C, 1 << 22)
+    far = [wide[..., 64 * i:64 * i + 64] for i in range(4)]
+    k, v = new(1, 1, C), new(1, 1, C)
+    far[0].copy_(k), far[1].copy_(v)
+    n = torch.tensor([590], dtype=torch.int32, device="cuda")
+    f, _ = rot.rotary_frequencies(D, device="cuda")
+    q, k1, v1 = new(1, 2, 5), new(1, 1, 5), new(1, 1, 5)
+    a = fc.rotary_append(q, k1, v1, k, v, n, f)
+    b = fc.rotary_append(q, k1, v1, far[0], far[1], n, f)
+    assert torch.equal(a, b) and torch.equal(far[0], k) and torch.equal(far[1], v)
+    o, lse = fc.tree_attention(a, k, v, n, return_lse=True)
+    assert torch.equal(o, fc.tree_attention(a, far[0], far[1], n))
+    w = fc.attention_weight_sums(a, k, lse, causal=True, query_start=n, lengths=n + 5)
+    assert torch.equal(w, fc.attention_weight_sums(a, far[0], lse, causal=True, query_start=n, lengths=n + 5))
+    want = fc.evict_cache(k, v, w, n, 550)
+    got = fc.evict_cache(far[0].clone(), far[1], w, n, 550)
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+    into = (torch.zeros(C << 22, dtype=torch.bfloat16, device="cuda").view(1, 1, C, 1 << 22)[..., :64], new(1, 1, C),
+            torch.empty(1, 1, C, device="cuda"))
+    got = fc.evict_cache(k, v, w, n, 550, out=into)
+    assert torch.equal(got[0][:, :, :550], want[0]) and torch.equal(got[1][:, :, :550], want[1])
+
+
+def test_in_inference_mode_and_what_autograd_knows(gpu_device):
+    """The calls inside inference mode; and a graph that saved a cache which is written to afterwards refuses to run."""
+    g = torch.Generator().manual_seed(4)
+    new = lambda h, s: torch.randn(1, h, s, 64, generator=g).half().cuda()  # noqa: E731
+    n = torch.tensor([20], dtype=torch.int32, device="cuda")
+    f, _ = rot.rotary_frequencies(64, device="cuda")
+    with torch.inference_mode():
+        q, kc, vc = new(4, 3), new(2, 40), new(2, 40)
+        q = fc.rotary_append(q, new(2, 3), new(2, 3), kc, vc, n, f)
+        o, lse = fc.tree_attention(q, kc, vc, n, return_lse=True)
+        w = fc.attention_weight_sums(q, kc, lse, causal=True, query_start=n, lengths=n + 3)
+        fc.attention_weight_sums(q, kc, lse, causal=True, query_start=n, lengths=n + 3, into=w)
+        fc.evict_cache(kc, vc, w, n + 3, 10, out=(new(2, 12), new(2, 12), torch.empty(1, 2, 12, device="cuda")))
+        rot.rotary_embedding(q, None, f)
+        total = w.double().sum(-1).cpu()
+    assert bool(((total - 12).abs() <= 12 * 2.0 ** -9).all())
+    kc, vc, x = new(2, 40), new(2, 40), new(2, 40).requires_grad_()
+    y = (x * kc).sum()
+    with torch.no_grad():
+        fc.rotary_append(new(4, 1), new(2, 1), new(2, 1), kc, vc, n, f)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()

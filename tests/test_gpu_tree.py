@@ -263,3 +263,23 @@ def test_two_streams_at_once(gpu_device):
     for i in range(2):
         for x in got[i]:
             assert torch.equal(x, want[i])
+
+
+def test_more_drafted_tokens_than_workgroups_at_once(gpu_device):
+    """A chain of 2000 tokens behind 900 cached ones: its row tiles alone fill the chip, each takes all keys."""
+    q, kc, vc = draw(1, 1, 8, 2000, 32, FH), draw(2, 1, 1, 3000, 32, FH), draw(3, 1, 1, 3000, 32, FH)
+    n = torch.tensor([900], dtype=torch.int32)
+    o, lse = fc.tree_attention(q, kc, vc, n.cuda(), return_lse=True)
+    ref = orc.tree_attention(q.cpu(), kc.cpu(), vc.cpu(), n, dtype=FH)
+    check("o", o, ref[0], ref[2])
+    check("lse", lse, ref[1], ref[3])
+
+
+def test_a_row_that_is_not_a_number_stays_alone(gpu_device):
+    q, kc, vc, n, m, depths, kw, dtype = run_case(1)
+    a = fc.tree_attention(q, kc, vc, n.cuda(), m.cuda(), return_lse=True)
+    q[1, 3, 5, 7] = float("nan")
+    b = fc.tree_attention(q, kc, vc, n.cuda(), m.cuda(), return_lse=True)
+    assert bool(torch.isnan(b[0][1, 3, 5]).all()) and bool(torch.isnan(b[1][1, 3, 5]))
+    b[0][1, 3, 5], b[1][1, 3, 5] = a[0][1, 3, 5], a[1][1, 3, 5]
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
