@@ -22,7 +22,8 @@
 // eight slots a thread (256 threads up to 2048 slots, for cheaper barriers), and of
 // that a good part the code, which a launch finds out of the instruction cache (at
 // about a byte a cycle; hence one copy of each loop, and the kernel that reads the
-// scores again in every pass, for more slots, apart).
+// scores again in every pass, for more slots, apart).  Times: 64 heads of 8192 slots,
+// 2048 kept, 37 us; of 16384, 4096 of D=64 kept, 49; one head of 131072 97 us.
 #include "flexatt_device.h"
 #include "flexatt_kernels.h"
 
@@ -90,7 +91,9 @@ __device__ __forceinline__ void gather(const EvictArgs& a, int b, int h, const i
   }
 }
 
-// MANY: more than one block of NT * kPer slots.
+// MANY: more than one block of NT * kPer slots.  Each pass reads their scores again, the
+// next block's while it works on this one's, until the candidates are few enough for a
+// few registers of each thread.
 template <int NT, bool MANY>
 __global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
   constexpr int kBins = 2 * NT, kDigit = NT == 1024 ? 11 : 9;
@@ -98,8 +101,9 @@ __global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
   __shared__ int hist[kBins];
   __shared__ int tot[NT / 64];
   __shared__ unsigned lows[NT / 64], highs[NT / 64];
-  __shared__ unsigned ckey[64];
-  __shared__ int cslot[64];
+  constexpr int kFew = MANY ? 4 : 0, kCand = MANY ? kFew * NT : 64;
+  __shared__ unsigned ckey[kCand];
+  __shared__ int cslot[kCand];
   __shared__ int s_digit, s_above, s_count, s_slot;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int nbh = a.B * a.H, part = blockIdx.x / nbh, bh = blockIdx.x % nbh, b = bh / a.H;
@@ -122,9 +126,9 @@ __global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
     // This thread's slots of block `blk`, kBlock blk + kPer tid + e: their scores, the
     // keys of those that go by them (0 for the others), and as bits e those that stay
     // anyway.
-    float x[kPer];
+    float x[kPer], ahead[kPer];
     unsigned key[kPer], sure = 0;
-    auto load = [&](int blk) {
+    auto fetch = [&](int blk) {
       const int i0 = blk * kBlock + tid * kPer;
       if (i0 + kPer <= n) {
         struct __attribute__((packed, aligned(4))) Quad {
@@ -133,28 +137,45 @@ __global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
         const Quad* q = (const Quad*)(sc + i0);
         const Quad q0 = q[0], q1 = q[1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = q0.v[e], x[4 + e] = q1.v[e];
+        for (int e = 0; e < 4; ++e) ahead[e] = q0.v[e], ahead[4 + e] = q1.v[e];
       } else {
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) x[e] = sc[min(i0 + e, n - 1)];
+        for (int e = 0; e < kPer; ++e) ahead[e] = sc[min(i0 + e, n - 1)];
       }
+    };
+    auto take = [&](int blk) {
+      const int i0 = blk * kBlock + tid * kPer;
       sure = 0;
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
+        x[e] = ahead[e];
         const bool by_score = (unsigned)(i0 + e - lo) < (unsigned)(hi - lo);
         key[e] = by_score ? order_key(x[e]) : 0;
         if (!by_score && i0 + e < n) sure |= 1u << e;
       }
     };
-    auto each = [&](auto f) {  // f(slot, key), key 0: not one of them
+    auto blocks = [&](auto f) {  // f(first slot of this thread) for every block
+      if (!MANY) {
+        f(tid * kPer);
+        return;
+      }
+      fetch(0);
       for (int blk = 0; blk < nb; ++blk) {
-        if (MANY) load(blk);
-        const int i0 = blk * kBlock + tid * kPer;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) f(i0 + e, key[e]);
+        take(blk);
+        if (blk + 1 < nb) fetch(blk + 1);
+        f(blk * kBlock + tid * kPer);
       }
     };
-    if (!MANY) load(0);
+    auto each = [&](auto f) {  // f(slot, key), key 0: not one of them
+      blocks([&](int i0) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) f(i0 + e, key[e]);
+      });
+    };
+    if (!MANY) {
+      fetch(0);
+      take(0);
+    }
 
     // A slot stays by its score where its key is above last_key, or is last_key and the
     // slot is at most last_slot.
@@ -180,10 +201,10 @@ __global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
       unsigned mask = top >= 32 ? 0 : ~0u << top;
       unsigned prefix = high & mask;
       int count = hi - lo;
-      while (count > 64 && top > 0) {
+      auto digit = [&](auto all_of) {  // one pass: the bits [shift, top) of the last kept key
         const int shift = max(top - kDigit, 0);
         const unsigned width = (1u << (top - shift)) - 1u;
-        each([&](int, unsigned k) {
+        all_of([&](int, unsigned k) {
           if (((k ^ prefix) & mask) == 0 && k) atomicAdd(&hist[(k >> shift) & width], 1);
         });
         __syncthreads();
@@ -205,12 +226,48 @@ __global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
         count = s_count;
         top = shift;
         mask = ~0u << top;
+      };
+      auto collect = [&](auto all_of) {  // the `count` candidates to ckey and cslot, in any order
+        __syncthreads();
+        if (tid == 0) s_count = 0;
+        __syncthreads();
+        all_of([&](int i, unsigned k) {
+          if (((k ^ prefix) & mask) == 0 && k) {
+            const int c = atomicAdd(&s_count, 1);
+            ckey[c] = k;
+            cslot[c] = i;
+          }
+        });
+        __syncthreads();
+      };
+      while (count > kCand && top > 0) digit(each);
+      if constexpr (MANY) {
+        if (count <= kCand && count > 64 && top > 0) {
+          collect(each);
+          unsigned fk[kFew];
+          int fs[kFew];
+#pragma unroll
+          for (int e = 0; e < kFew; ++e) {
+            const int c = e * NT + tid;
+            fk[e] = c < count ? ckey[c] : 0;
+            fs[e] = c < count ? cslot[c] : 0;
+          }
+          auto few = [&](auto f) {
+#pragma unroll
+            for (int e = 0; e < kFew; ++e) f(fs[e], fk[e]);
+          };
+          while (count > 64 && top > 0) digit(few);
+          if (count <= 64) collect(few);
+        } else if (count <= 64) {
+          collect(each);
+        }
+      } else if (count <= 64) {
+        collect(each);
       }
       if (count > 64) {  // equal keys: the slot of the need-th of them
         last_key = prefix;
         int seen = 0;
-        for (int blk = 0; blk < nb; ++blk) {
-          if (MANY) load(blk);
+        blocks([&](int i0) {
           int eq = 0;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) eq += key[e] == prefix;
@@ -219,24 +276,12 @@ __global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
           if (at < need && at + eq >= need) {
 #pragma unroll
             for (int e = 0; e < kPer; ++e)
-              if (key[e] == prefix && ++at == need) s_slot = blk * kBlock + tid * kPer + e;
-          }
-        }
-        __syncthreads();
-        last_slot = s_slot;
-      } else {
-        // the candidates, in any order, and the one with need - 1 larger ones
-        __syncthreads();
-        if (tid == 0) s_count = 0;
-        __syncthreads();
-        each([&](int i, unsigned k) {
-          if (((k ^ prefix) & mask) == 0 && k) {
-            const int c = atomicAdd(&s_count, 1);
-            ckey[c] = k;
-            cslot[c] = i;
+              if (key[e] == prefix && ++at == need) s_slot = i0 + e;
           }
         });
         __syncthreads();
+        last_slot = s_slot;
+      } else {  // the one with need - 1 larger ones
         const unsigned k = lane < count ? ckey[lane] : 0;
         const int i = lane < count ? cslot[lane] : 0x7fffffff;
         int larger = 0;
@@ -252,9 +297,7 @@ __global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
 
     // places, in slot order
     int place = 0;
-    for (int blk = 0; blk < nb; ++blk) {
-      if (MANY) load(blk);
-      const int i0 = blk * kBlock + tid * kPer;
+    blocks([&](int i0) {
       unsigned stay = sure;
 #pragma unroll
       for (int e = 0; e < kPer; ++e)
@@ -271,7 +314,7 @@ __global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
           }
           at += 1;
         }
-    }
+    });
   } else {
     for (int i = p0 + tid; i < p1; i += NT) {
       slots[i] = i < n ? i : -1;

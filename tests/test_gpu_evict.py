@@ -21,6 +21,10 @@ CASES = [
     (BF, 2, 1, 40, 32, 50, 20, 20, [40, 13], "random"),             # a budget beyond the cache
     (BF, 1, 1, 3000, 64, 1024, 0, 0, [3000], "equal"),
     (BF, 2, 2, 257, 64, 128, 1, 0, [1000000, -5], "special"),       # lengths outside the cache
+    (FH, 2, 1, 20001, 32, 5000, 100, 4, [20001, 8200], "random"),    # several blocks of slots
+    (BF, 1, 2, 9000, 32, 1500, 0, 3, [9000], "special"),
+    (BF, 1, 1, 30000, 32, 12000, 64, 0, [29999], "ties"),
+    (BF, 1, 1, 16500, 32, 100, 20, 70, [16500], "random"),
 ]
 
 
