@@ -135,7 +135,10 @@ TreePlan tree_plan(const flexatt_tree* p) {
   const int rowb = p->head_dim * (int)elt_size(p->dtype);
   const int64_t rt = ((int64_t)(p->heads_q / p->heads_kv) * p->tokens + 31) / 32;
   const int64_t groups = rowb <= 256 && elt_size(p->dtype) == 2 ? (rt + 1) / 2 : rt;  // (launch_tree)
-  const int64_t slots = (rowb >= 256 ? 1 : 2) * cus() / groups;
+  // a chunk's row tiles are on one of the 8 XCDs (tree_attn_kernel): whole chunks of each
+  // (fp32 B=2 Hq=8 Hkv=2 T=53 caches of 22374 D=128, 7 row tiles: 36 chunks, five on some
+  // XCDs for 32 CUs, 192 us, 32 chunks 117)
+  const int64_t fit = (rowb >= 256 ? 1 : 2) * cus(), slots = groups <= fit / 8 ? fit / 8 / groups * 8 : fit / groups;
   const int64_t bh = (int64_t)p->batch * p->heads_kv, tiles = (p->cache_rows + 31) / 32;
   t.min_tiles = 8;
   t.slots = slots < 1 ? 1 : (int)slots;
