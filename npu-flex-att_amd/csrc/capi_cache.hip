@@ -165,26 +165,49 @@ int check_weights(const flexatt_weights* p) {
   return FLEXATT_OK;
 }
 
-// Workgroups that share the query rows of one pair of key blocks: the number whose
-// rounds of workgroups (two per CU, one with rows of 512 bytes) take least, with
-// eight row tiles' time to load and add up the blocks.  (bf16 B=2 Hq=32 Hkv=8 S=4096
-// D=128 causal, 128 pairs: 4 parts 162 us, 6 and 8 167, 12 175, 16 177.)
-int weight_parts(const flexatt_weights* p) {
+// Which blocks of keys a workgroup has, one or a pair (the second from the other end,
+// which under a causal mask evens out the work), and how many workgroups share their
+// query rows: what takes the fewest rounds of workgroups (two per CU, one with rows of
+// 512 bytes) times their row tiles, a block counted as some five more to load and add up.
+// (bf16 B=2 Hq=32 Hkv=8 S=4096 D=128 causal, 128 pairs: 4 parts 162 us, 6 and 8 167, 12
+// 175, 16 177.  Blocks alone where they leave CUs idle: bf16 Hq=32 Hkv=8 D=128, 1 row over
+// 700 keys 11.7 -> 7.4 us, fp32 Hq=8 Hkv=1 D=256, 5 over 2803 30 -> 16; pairs where they
+// do not: bf16 B=3, 32 heads, 1 row over 19106 keys 122 -> 115 us.)
+struct WeightPlan {
+  int pair, parts;
+};
+WeightPlan weight_plan(const flexatt_weights* p) {
   const int rowb = p->head_dim * (int)elt_size(p->dtype);
   const int keys = rowb <= 512 ? 256 : 128;  // (WsCfg)
   const int64_t nkb = (p->seqlen_kv + keys - 1) / keys;
-  const int64_t pairs = (nkb + 1) / 2 * p->batch * p->heads_kv, slots = (rowb >= 512 ? 1 : 2) * cus();
-  int64_t rows = p->seqlen_q;
-  if (p->sliding_window > 0 && rows > (int64_t)p->sliding_window + keys) rows = (int64_t)p->sliding_window + keys;
-  int64_t tiles = (rows * (p->heads_q / p->heads_kv) + 31) / 32;  // that a block of keys is seen by at most
-  const bool half = p->causal && p->sliding_window == 0 && p->seqlen_q > p->seqlen_kv / 2;
-  const int64_t work = (nkb > 1 && !half ? 2 : 1) * tiles;
-  int64_t best = 1, best_cost = INT64_MAX;
-  for (int64_t n = 1; n <= 64 && (n == 1 || tiles / n >= 4); ++n) {
-    const int64_t cost = (pairs * n + slots - 1) / slots * ((work + n - 1) / n + 8);
-    if (cost < best_cost) best = n, best_cost = cost;
+  const int64_t bh = (int64_t)p->batch * p->heads_kv, slots = (rowb >= 512 ? 1 : 2) * cus();
+  // the row tiles that see block x (starts on the device: as if the rows were the last)
+  const int64_t start = p->query_starts ? (int64_t)p->seqlen_kv - p->seqlen_q : p->query_start;
+  const auto tiles_of = [&](int64_t x) {
+    int64_t lo = p->causal ? x * keys - start : 0, hi = p->seqlen_q;
+    if (p->sliding_window > 0 && (x + 1) * keys + p->sliding_window - start < hi)
+      hi = (x + 1) * keys + p->sliding_window - start;
+    if (lo < 0) lo = 0;
+    return hi > lo ? ((hi - lo) * (p->heads_q / p->heads_kv) + 31) / 32 : 0;
+  };
+  // the most of a block and of a pair: of the ends', the quarters' and the middle's
+  int64_t tiles = 0, both = 0;
+  for (int64_t x : {(int64_t)0, nkb / 4, (nkb - 1) / 2}) {
+    const int64_t a = tiles_of(x), b = nkb - 1 - x != x ? tiles_of(nkb - 1 - x) : 0;
+    tiles = a > tiles ? a : tiles;
+    tiles = b > tiles ? b : tiles;
+    both = a + b > both ? a + b : both;
   }
-  return (int)best;
+  WeightPlan best = {0, 1};
+  int64_t best_cost = INT64_MAX;
+  for (int pair = nkb > 1 ? 1 : 0; pair >= 0; --pair) {
+    const int64_t groups = (pair ? (nkb + 1) / 2 : nkb) * bh, work = pair ? both : tiles;
+    for (int64_t n = 1; n <= 64 && (n == 1 || tiles / n >= 4); ++n) {
+      const int64_t cost = (groups * n + slots - 1) / slots * ((work + n - 1) / n + (pair ? 9 : 5));
+      if (cost < best_cost) best = {pair, (int)n}, best_cost = cost;
+    }
+  }
+  return best;
 }
 }  // namespace
 
@@ -285,7 +308,7 @@ int flexatt_tree_fwd(const flexatt_tree* p, const flexatt_tensor* q, const flexa
 
 size_t flexatt_weight_sums_workspace(const flexatt_weights* p) {
   if (check_weights(p) != FLEXATT_OK) return SIZE_MAX;
-  const int n = weight_parts(p);
+  const int n = weight_plan(p).parts;
   return n == 1 ? 0 : (size_t)n * p->batch * p->heads_kv * p->seqlen_kv * sizeof(float);
 }
 
@@ -310,7 +333,9 @@ int flexatt_weight_sums(const flexatt_weights* p, const flexatt_tensor* q, const
   a.start = p->query_start;
   a.add = p->accumulate;
   a.part = (float*)workspace;
-  a.nparts = weight_parts(p);
+  const WeightPlan plan = weight_plan(p);
+  a.nparts = plan.parts;
+  a.pair = plan.pair;
   a.p = score_shape(p->batch, p->heads_q, p->heads_kv, p->seqlen_q, p->seqlen_kv, p->scale, p->soft_cap,
                     p->sliding_window);
   a.p.causal = p->causal;

@@ -125,6 +125,7 @@ struct WeightArgs {
   int add;    // 1: added to what sums holds
   float* part;  // nparts > 1: [nparts][B][Hkv][Skv]
   int nparts;   // workgroups that share the query rows of a block of keys
+  int pair;     // 1: a workgroup has block x and the x-th from the end
 };
 
 // Eviction (evict.hip).

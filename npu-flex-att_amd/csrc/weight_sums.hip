@@ -112,12 +112,12 @@ void weight_sums_kernel(WeightArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, l32 = lane & 31;
 
-  // (part, pair of key blocks, b, hkv): block x and block nkb - 1 - x one after the
-  // other, so that under a causal mask, too, workgroups have equal work; those of one
-  // (b, hkv) share an XCD where their number is a multiple of 8
-  const int nbh = p.B * p.Hkv, nkb = (p.Skv + C::KEYS - 1) / C::KEYS, npair = (nkb + 1) / 2;
+  // (part, key block or pair of them, b, hkv).  A pair is block x and block nkb - 1 - x,
+  // one after the other, so that under a causal mask, too, workgroups have equal work;
+  // those of one (b, hkv) share an XCD where their number is a multiple of 8
+  const int nbh = p.B * p.Hkv, nkb = (p.Skv + C::KEYS - 1) / C::KEYS, nx = a.pair ? (nkb + 1) / 2 : nkb;
   const int bh = blockIdx.x % nbh, hk = bh % p.Hkv, b = bh / p.Hkv;
-  const int pair = blockIdx.x / nbh % npair, part = blockIdx.x / nbh / npair;
+  const int x0 = blockIdx.x / nbh % nx, part = blockIdx.x / nbh / nx;
   int n = a.lengths ? min(max(a.lengths[b], 0), p.Skv) : p.Skv;
   n = __builtin_amdgcn_readfirstlane(n);
   const int64_t start = a.starts ? a.starts[b] : a.start;
@@ -136,9 +136,9 @@ void weight_sums_kernel(WeightArgs a) {
     else return fast_exp2(__builtin_fmaf(s, c2, -l2));
   };
 
-  for (int seg = 0; seg < 2; ++seg) {
-    const int kb = seg == 0 ? pair : nkb - 1 - pair;
-    if (seg == 1 && kb == pair) break;
+  for (int seg = 0; seg <= a.pair; ++seg) {
+    const int kb = seg == 0 ? x0 : nkb - 1 - x0;
+    if (seg == 1 && kb == x0) break;
     const int j0 = kb * C::KEYS;
     if (j0 >= n) {  // no key in use
       if (a.nparts == 1 && !a.add)
@@ -369,7 +369,7 @@ template <class T, int D>
 hipError_t launch_weights(const WeightArgs& a, hipStream_t st) {
   using C = WsCfg<T, D>;
   const int64_t nkb = (a.p.Skv + C::KEYS - 1) / C::KEYS;
-  const dim3 grid((unsigned)((nkb + 1) / 2 * a.nparts * a.p.B * a.p.Hkv)), block(kWsWaves * 64);
+  const dim3 grid((unsigned)((a.pair ? (nkb + 1) / 2 : nkb) * a.nparts * a.p.B * a.p.Hkv)), block(kWsWaves * 64);
   if (a.p.cap > 0.f) hipLaunchKernelGGL((weight_sums_kernel<T, D, C::NK, true>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((weight_sums_kernel<T, D, C::NK, false>), grid, block, 0, st, a);
   const hipError_t e = hipGetLastError();
