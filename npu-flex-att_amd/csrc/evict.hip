@@ -19,18 +19,17 @@
 //    D=128, 2048 kept, 42 -> 39 us; two heads of 2048, fp32 D=64, 1000 kept, 12 -> 8.)
 // What bounds it: the copies memory (134 MB there: 26 us at the rate of a large copy),
 // the selection latency: a chain of passes over keys that stay in registers up to
-// eight slots a thread (256 threads up to 2048 slots, for cheaper barriers), and of
+// sixteen slots a thread (256 threads up to 2048 slots, for cheaper barriers), and of
 // that a good part the code, which a launch finds out of the instruction cache (at
 // about a byte a cycle; hence one copy of each loop, and the kernel that reads the
 // scores again in every pass, for more slots, apart).  Times: 64 heads of 8192 slots,
-// 2048 kept, 37 us; of 16384, 4096 of D=64 kept, 49; one head of 131072 97 us.
+// 2048 kept, 37 us; of 16384, 4096 of D=64 kept, 38; one head of 131072 97 us.
 #include "flexatt_device.h"
 #include "flexatt_kernels.h"
 
 namespace flexatt {
 
 namespace {
-constexpr int kPer = 8;  // consecutive slots per thread and block
 
 // Larger float <-> larger unsigned; NaN is the largest, and -0 equals 0.  Never 0.
 __device__ __forceinline__ unsigned order_key(float x) {
@@ -91,10 +90,10 @@ __device__ __forceinline__ void gather(const EvictArgs& a, int b, int h, const i
   }
 }
 
-// MANY: more than one block of NT * kPer slots.  Each pass reads their scores again, the
+// A thread has kPer consecutive slots of a block.  MANY: more than one block of NT * kPer.  Each pass reads their scores again, the
 // next block's while it works on this one's, until the candidates are few enough for a
 // few registers of each thread.
-template <int NT, bool MANY>
+template <int NT, int kPer, bool MANY>
 __global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
   constexpr int kBins = 2 * NT, kDigit = NT == 1024 ? 11 : 9;
   static_assert(kBins == 1 << kDigit, "two bins per thread");
@@ -135,9 +134,12 @@ __global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
           float v[4];
         };
         const Quad* q = (const Quad*)(sc + i0);
-        const Quad q0 = q[0], q1 = q[1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ahead[e] = q0.v[e], ahead[4 + e] = q1.v[e];
+        for (int y = 0; y < kPer / 4; ++y) {
+          const Quad v = q[y];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ahead[4 * y + e] = v.v[e];
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < kPer; ++e) ahead[e] = sc[min(i0 + e, n - 1)];
@@ -325,21 +327,24 @@ __global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
   gather<NT>(a, b, bh - b * a.H, slots, p0, p1);
 }
 
-template <int NT, bool MANY>
+template <int NT, int kPer, bool MANY>
 void launch(EvictArgs a, int cus, hipStream_t st) {
   // rows by 16-byte lanes, 64 at most (D = 256 of 4 bytes)
   a.lanes_log2 = 31 - __builtin_clz(a.D * a.es / 16);
   const int nbh = a.B * a.H, least = 4 * (NT >> a.lanes_log2);  // places of one pass of the copies
   const int64_t most = (a.keep + least - 1) / least, fill = (int64_t)cus * (NT == 1024 ? 1 : 2) / nbh;
   a.nparts = (int)(fill < 1 ? 1 : fill < most ? fill : most);
-  hipLaunchKernelGGL((evict_kernel<NT, MANY>), dim3((unsigned)(nbh * a.nparts)), dim3(NT), 0, st, a);
+  hipLaunchKernelGGL((evict_kernel<NT, kPer, MANY>), dim3((unsigned)(nbh * a.nparts)), dim3(NT), 0, st, a);
 }
 }  // namespace
 
 hipError_t evict_run(const EvictArgs& a, int cus, hipStream_t st) {
-  if (a.C <= 256 * kPer) launch<256, false>(a, cus, st);
-  else if (a.C <= 1024 * kPer) launch<1024, false>(a, cus, st);
-  else launch<1024, true>(a, cus, st);
+  // scores in registers as long as they fit (eight heads of 10698 slots read again in every
+  // pass 34 us, in registers 23)
+  if (a.C <= 256 * 8) launch<256, 8, false>(a, cus, st);
+  else if (a.C <= 1024 * 8) launch<1024, 8, false>(a, cus, st);
+  else if (a.C <= 1024 * 16) launch<1024, 16, false>(a, cus, st);
+  else launch<1024, 8, true>(a, cus, st);
   return hipGetLastError();
 }
 
