@@ -134,7 +134,8 @@ TreePlan tree_plan(const flexatt_tree* p) {
   TreePlan t;
   const int rowb = p->head_dim * (int)elt_size(p->dtype);
   const int64_t rt = ((int64_t)(p->heads_q / p->heads_kv) * p->tokens + 31) / 32;
-  const int64_t groups = rowb <= 256 && elt_size(p->dtype) == 2 ? (rt + 1) / 2 : rt;  // (launch_tree)
+  const int share = tree_share(rowb, (int)elt_size(p->dtype), rt);
+  const int64_t groups = (rt + share - 1) / share;
   // a chunk's row tiles are on one of the 8 XCDs (tree_attn_kernel): whole chunks of each
   // (fp32 B=2 Hq=8 Hkv=2 T=53 caches of 22374 D=128, 7 row tiles: 36 chunks, five on some
   // XCDs for 32 CUs, 192 us, 32 chunks 117)

@@ -143,6 +143,14 @@ struct EvictArgs {
   int lanes_log2, nparts;  // lanes that copy a row, workgroups per (sequence, head) (set by the launcher)
 };
 
+// Row tiles of 32 that the waves of one tree attention workgroup share a key tile for, of
+// `tiles` in all: four of 256-byte rows, or two where four would pad by more than a sixth
+// (tree_attn.hip).
+inline int tree_share(int row_bytes, int elt_bytes, int64_t tiles) {
+  if (elt_bytes != 2 || row_bytes > 256 || tiles < 2) return 1;
+  return row_bytes > 128 && (tiles + 3) / 4 * 4 * 6 <= (tiles + 1) / 2 * 2 * 7 ? 4 : 2;
+}
+
 typedef hipError_t (*TreeLauncher)(const TreeArgs&, hipStream_t);
 typedef hipError_t (*WeightLauncher)(const WeightArgs&, hipStream_t);
 typedef hipError_t (*FwdLauncher)(const FwdArgs&, hipStream_t);

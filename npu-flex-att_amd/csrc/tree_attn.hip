@@ -11,17 +11,18 @@
 //
 // Decomposition
 //  * the G * T query rows of one KV head are packed with the heads innermost into
-//    tiles of 32, the columns of an MFMA tile, so heads and tokens share K and V; a
-//    wave has NR such tiles (two from 33 rows on, where the registers allow), which
-//    share its LDS reads of K and V too;
+//    tiles of 32, the columns of an MFMA tile, so heads and tokens share K and V; a wave
+//    has one such tile, and of several tiles of 16-bit rows up to 256 bytes two or four
+//    waves share the key tiles in LDS (tree_share);
 //  * the 32-key tiles of a (b, hkv), as many as the sequence's own length has, are cut
 //    into equal chunks of about `len` tiles, one per workgroup; `len` is found on the
 //    device from all lengths, so that a cache of large capacity that holds little, or a
 //    batch of unequal lengths, fills the chip once; the workgroups of one chunk for
 //    different row tiles share an XCD and with it L2;
-//  * within a chunk, wave w takes tiles w, w + NW, ... with its own LDS stages and
-//    online softmax, no barriers; the waves' states are combined through LDS, and the
-//    chunks' partials (O over its row sum, LSE) by a second kernel in a fixed order;
+//  * within a chunk, wave (or group of waves) w takes tiles w, w + NW, ... with its own
+//    LDS stages and online softmax, a wave alone without barriers; the states of a row
+//    tile's waves are combined through LDS, and the chunks' partials (O over its row sum,
+//    LSE) by a second kernel in a fixed order;
 //  * rows behind n + T are never read: the copies repeat the last row instead, so
 //    what a cache holds there (NaN too) does not matter.
 // What bounds it: K and V from HBM for long caches and few rows; from some hundred
@@ -29,10 +30,15 @@
 // Of that the instructions are the larger part: a launch finds the instruction cache
 // cold and runs most of this code once, at about one cycle a byte, so what is outside
 // the tile loop is kept short (16-byte LDS accesses in the combine, rolled loops).
-//   bf16 B=8 Hq=32 Hkv=8 T=16, caches of 24576 to 32768, D=128: 185 us, 5.1 TB/s
+//   bf16 B=8 Hq=32 Hkv=8 T=16, caches of 24576 to 32768, D=128: 181 us, 5.2 TB/s
 //   bf16 B=2 Hq=16 Hkv=8 T=16, window 4096, D=256: 24 us (the merge 4.7), 2.8 TB/s
-//   fp16 B=4 Hq=28 Hkv=4 T=64, caches up to 16384, D=64: 55 us, 0.49 PFLOP/s (loop 33 to 42)
+//   fp16 B=4 Hq=28 Hkv=4 T=64, caches up to 16384, D=64: 55 us, 0.49 PFLOP/s
+//   fp16 B=3 Hq=28 Hkv=4 T=64, caches of 20000, D=128: 87 us, 0.63 PFLOP/s
 //   bf16 B=1 Hq=32 Hkv=8 T=8, a cache of 4097, D=128: 14 us (9.5 and the merge 4.6)
+// Shared key tiles halve or quarter the copies from L2, which many rows wait for.  The
+// alternative, two row tiles per wave of its own key tiles, reads LDS as little but has a
+// SIMD to itself (register file) and copies as much: the D=128 cases above 186 and 193 us.
+// Pairs instead of fours: 147 us for the latter, D=64 55 (fours 56).
 #include "flexatt_device.h"
 #include "flexatt_kernels.h"
 
@@ -65,10 +71,7 @@ struct TreeCfg {
   static constexpr int NW = ROWB <= 512 ? 4 : 2;      // waves per workgroup
   static constexpr int ST = ROWB <= 256 ? 2 : 1;      // stages
   static constexpr int WAVEB = ST * 2 * TB;
-  static constexpr int COMBB = NW * 64 * 4 * (2 + 16 * DB);
-  static constexpr int LDSB = NW * WAVEB > COMBB ? NW * WAVEB : COMBB;
-  static constexpr int NR = sizeof(T) == 2 && D <= 128 ? 2 : 1;  // most row tiles per wave
-  static_assert(E * 1024 == TB && LDSB <= 160 * 1024 && E % PK == 0 && E % PV == 0, "tiles");
+  static_assert(E * 1024 == TB && NW * WAVEB <= 160 * 1024 && E % PK == 0 && E % PV == 0, "tiles");
 };
 
 // V tiles of 32-bit elements are read one element per lane, 32 of a row by each
@@ -187,16 +190,23 @@ __device__ __forceinline__ void load_lds16_base(unsigned voff, uint64_t base, un
 }
 }  // namespace
 
-template <class T, int D, int NW, int NR, bool CAP>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(D * sizeof(T) >= 256 ? 1 : 2)))
+// WPT neighbouring waves, a row tile each, share their key tiles: each copies its share of
+// a tile, and a barrier a tile keeps them in step.
+template <class T, int D, int NW, int WPT, bool CAP>
+__global__ __launch_bounds__(NW * WPT * 64)
+__attribute__((amdgpu_waves_per_eu(D * sizeof(T) >= 256 ? (WPT == 1 ? 1 : 2) : WPT == 1 ? 2 : 4)))
 void tree_attn_kernel(TreeArgs a) {
   using C = TreeCfg<T, D>;
-  constexpr int ST = C::ST;
-  __shared__ __attribute__((aligned(1024))) char smem[C::LDSB];
+  constexpr int ST = C::ST, EC = C::E / WPT;  // copies a wave makes of a tile
+  constexpr int PK = C::PK > WPT ? C::PK / WPT : 1, PV = C::PV > WPT ? C::PV / WPT : 1, CROWS = WPT * C::RPC;
+  static_assert(WPT == 1 || (ST == 2 && C::E % WPT == 0), "shared tiles");
+  constexpr int kCombine = NW * WPT * 64 * 4 * (2 + 16 * C::DB);
+  __shared__ __attribute__((aligned(1024))) char smem[NW * C::WAVEB > kCombine ? NW * C::WAVEB : kCombine];
 
   const Shape& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / (WPT * 64));  // its key tiles
+  const int sub = WPT > 1 ? __builtin_amdgcn_readfirstlane((tid >> 6) % WPT) : 0;
   const int h = lane >> 5, l32 = lane & 31;
 
   // (chunk, row tiles): the row tiles of one chunk are 8 workgroups apart, on one XCD
@@ -205,9 +215,10 @@ void tree_attn_kernel(TreeArgs a) {
   // 16384 D=64, 58 -> 74 us)
   int rt0 = 0, x = blockIdx.x;
   if (a.nrt > 1) {
-    rt0 = blockIdx.x / 8 % a.nrt * NR;
+    rt0 = blockIdx.x / 8 % a.nrt * WPT;
     x = blockIdx.x / (8 * a.nrt) * 8 + blockIdx.x % 8;
   }
+  rt0 += sub;
   const TreeChunk ck = tree_chunk(a, x, NW);
   if (ck.b < 0) return;
   const int b = ck.b, hk = ck.hk, s = ck.s, ns = ck.ns;
@@ -238,50 +249,34 @@ void tree_attn_kernel(TreeArgs a) {
   }
   // this lane's offsets in a tile's copies
   const unsigned kss = (unsigned)(a.k.ss * (int)sizeof(T)), vss = (unsigned)(a.v.ss * (int)sizeof(T));
-  const int crow = lane / C::CPR, cchunk = lane % C::CPR;
-  unsigned kvo[C::PK], vvo[C::PV];
+  const int crow = lane / C::CPR + sub * C::RPC, cchunk = lane % C::CPR;
+  unsigned kvo[PK], vvo[PV];
 #pragma unroll
-  for (int e = 0; e < C::PK; ++e)
-    kvo[e] = (e * C::RPC + crow) * kss + swz_col<C::CPR>(e * C::RPC + crow, cchunk) * 16;
+  for (int e = 0; e < PK; ++e) kvo[e] = (e * CROWS + crow) * kss + swz_col<C::CPR>(e * CROWS + crow, cchunk) * 16;
 #pragma unroll
-  for (int e = 0; e < C::PV; ++e)
-    vvo[e] = (e * C::RPC + crow) * vss + swz_v<T, C::CPR>(e * C::RPC + crow, cchunk) * 16;
+  for (int e = 0; e < PV; ++e) vvo[e] = (e * CROWS + crow) * vss + swz_v<T, C::CPR>(e * CROWS + crow, cchunk) * 16;
   const unsigned wbase = lds_addr_of(smem) + wave * C::WAVEB;
   // this wave's LDS reads have returned: the buffer they read may be refilled
   auto reads_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
 
   // packed query rows of this lane
   const int R = p.G * p.Sq;
-  int hqo[NR], qi[NR];  // head within the group, drafted token
-#pragma unroll
-  for (int nr = 0; nr < NR; ++nr) {
-    const int r = min(32 * (rt0 + nr) + l32, R - 1);
-    hqo[nr] = r % p.G;
-    qi[nr] = r / p.G;
-  }
+  const int r = min(32 * rt0 + l32, R - 1);
+  const int hq = hk * p.G + r % p.G, qi = r / p.G;  // head, drafted token
 
   if (sq.bad) {
-    if (s == 0) {
-#pragma unroll
-      for (int nr = 0; nr < NR; ++nr) {
-        if (32 * (rt0 + nr) + l32 >= R) continue;
-        const int hq = hk * p.G + hqo[nr];
-        T* out = (T*)a.o.data + b * a.o.sb + hq * a.o.sh + (int64_t)qi[nr] * a.o.ss;
-        for (int d = wave * 2 + h; d < D; d += NW * 2) out[d] = from_f32<T>(__builtin_nanf(""));
-        if (wave == 0 && h == 0) a.lse[((int64_t)b * p.Hq + hq) * p.Sq + qi[nr]] = __builtin_nanf("");
-      }
+    if (s == 0 && 32 * rt0 + l32 < R) {
+      T* out = (T*)a.o.data + b * a.o.sb + hq * a.o.sh + (int64_t)qi * a.o.ss;
+      for (int d = wave * 2 + h; d < D; d += NW * 2) out[d] = from_f32<T>(__builtin_nanf(""));
+      if (wave == 0 && h == 0) a.lse[((int64_t)b * p.Hq + hq) * p.Sq + qi] = __builtin_nanf("");
     }
     return;
   }
 
-  i32x4 qf[NR][C::KC];
+  i32x4 qf[C::KC];
+  const char* src = (const char*)((const T*)a.q.data + b * a.q.sb + hq * a.q.sh + (int64_t)qi * a.q.ss) + 16 * h;
 #pragma unroll
-  for (int nr = 0; nr < NR; ++nr) {
-    const int hq = hk * p.G + hqo[nr];
-    const char* src = (const char*)((const T*)a.q.data + b * a.q.sb + hq * a.q.sh + (int64_t)qi[nr] * a.q.ss) + 16 * h;
-#pragma unroll
-    for (int kc = 0; kc < C::KC; ++kc) qf[nr][kc] = ld_global16(src + 32 * kc);
-  }
+  for (int kc = 0; kc < C::KC; ++kc) qf[kc] = ld_global16(src + 32 * kc);
 
   // this wave's tiles: first + NW * j, j < nt
   const int n = sq.n, last = n + p.Sq - 1;
@@ -290,32 +285,32 @@ void tree_attn_kernel(TreeArgs a) {
   const uint64_t kp = (uint64_t)((const T*)a.k.data + b * a.k.sb + hk * a.k.sh);
   const uint64_t vp = (uint64_t)((const T*)a.v.data + b * a.v.sb + hk * a.v.sh);
   auto issue_k = [&](int t, int st) {
-    const unsigned dst = wbase + st * 2 * C::TB;
+    const unsigned dst = wbase + st * 2 * C::TB + sub * 1024;
     const uint64_t base = kp + (uint64_t)(t * C::BN) * kss;
     if (t * C::BN + C::BN - 1 <= last) {
 #pragma unroll
-      for (int e = 0; e < C::E; ++e)
-        load_lds16_base(kvo[e % C::PK], base + (uint64_t)(e / C::PK * C::PK * C::RPC) * kss, dst + e * 1024);
+      for (int e = 0; e < EC; ++e)
+        load_lds16_base(kvo[e % PK], base + (uint64_t)(e / PK * PK * CROWS) * kss, dst + e * WPT * 1024);
     } else {  // rows behind the last one repeat it
 #pragma unroll 1
-      for (int e = 0; e < C::E; ++e) {
-        const int kr = e * C::RPC + crow;
-        load_lds16_base(min(kr, last - t * C::BN) * kss + swz_col<C::CPR>(kr, cchunk) * 16, base, dst + e * 1024);
+      for (int e = 0; e < EC; ++e) {
+        const int kr = e * CROWS + crow;
+        load_lds16_base(min(kr, last - t * C::BN) * kss + swz_col<C::CPR>(kr, cchunk) * 16, base, dst + e * WPT * 1024);
       }
     }
   };
   auto issue_v = [&](int t, int st) {
-    const unsigned dst = wbase + st * 2 * C::TB + C::TB;
+    const unsigned dst = wbase + st * 2 * C::TB + C::TB + sub * 1024;
     const uint64_t base = vp + (uint64_t)(t * C::BN) * vss;
     if (t * C::BN + C::BN - 1 <= last) {
 #pragma unroll
-      for (int e = 0; e < C::E; ++e)
-        load_lds16_base(vvo[e % C::PV], base + (uint64_t)(e / C::PV * C::PV * C::RPC) * vss, dst + e * 1024);
+      for (int e = 0; e < EC; ++e)
+        load_lds16_base(vvo[e % PV], base + (uint64_t)(e / PV * PV * CROWS) * vss, dst + e * WPT * 1024);
     } else {
 #pragma unroll 1
-      for (int e = 0; e < C::E; ++e) {
-        const int kr = e * C::RPC + crow;
-        load_lds16_base(min(kr, last - t * C::BN) * vss + swz_v<T, C::CPR>(kr, cchunk) * 16, base, dst + e * 1024);
+      for (int e = 0; e < EC; ++e) {
+        const int kr = e * CROWS + crow;
+        load_lds16_base(min(kr, last - t * C::BN) * vss + swz_v<T, C::CPR>(kr, cchunk) * 16, base, dst + e * WPT * 1024);
       }
     }
   };
@@ -326,17 +321,11 @@ void tree_attn_kernel(TreeArgs a) {
 
   // Row qi sees the cached keys [row_lo, n); the tiles that hold only keys every row
   // sees need no mask.
-  int row_lo[NR], full_lo = 0;
-#pragma unroll
-  for (int nr = 0; nr < NR; ++nr) row_lo[nr] = 0;
+  int row_lo = 0, full_lo = 0;
   if (p.window > 0) {
-#pragma unroll
-    for (int nr = 0; nr < NR; ++nr) {
-      const int depth = a.depths ? max(a.depths[(int64_t)b * p.Sq + qi[nr]], 0) : qi[nr];
-      // (n + depth - window without leaving 32 bits: depth at most the window counts)
-      row_lo[nr] = max(n - (p.window - min(depth, p.window)), 0);
-      full_lo = max(full_lo, row_lo[nr]);
-    }
+    const int depth = a.depths ? max(a.depths[(int64_t)b * p.Sq + qi], 0) : qi;
+    // (n + depth - window without leaving 32 bits: depth at most the window counts)
+    full_lo = row_lo = max(n - (p.window - min(depth, p.window)), 0);
 #pragma unroll
     for (int y = 32; y; y >>= 1) full_lo = max(full_lo, __shfl_xor(full_lo, y));
     full_lo = __builtin_amdgcn_readfirstlane(full_lo);
@@ -345,54 +334,56 @@ void tree_attn_kernel(TreeArgs a) {
 
   // wait for Q here, once: see fwd_split.hip
 #pragma unroll
-  for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-    for (int kc = 0; kc < C::KC; ++kc) {
-      if constexpr (!CAP) {
-        constexpr int kSign = sizeof(T) == 4 ? (int)0x80000000 : (int)0x80008000;
-        const int f = flip ? kSign : 0;
-        qf[nr][kc] ^= i32x4{f, f, f, f};
-      }
-      pin(qf[nr][kc]);
+  for (int kc = 0; kc < C::KC; ++kc) {
+    if constexpr (!CAP) {
+      constexpr int kSign = sizeof(T) == 4 ? (int)0x80000000 : (int)0x80008000;
+      const int f = flip ? kSign : 0;
+      qf[kc] ^= i32x4{f, f, f, f};
     }
-
-  f32x16 acc[NR][C::DB];
-  float m_run[NR], l_run[NR];
-#pragma unroll
-  for (int nr = 0; nr < NR; ++nr) {
-#pragma unroll
-    for (int db = 0; db < C::DB; ++db) acc[nr][db] = f32x16{};
-    m_run[nr] = kNegInf;
-    l_run[nr] = 0.f;
+    pin(qf[kc]);
   }
 
-  for (int j = 0; j < nt; ++j) {
+  f32x16 acc[C::DB];
+  float m_run = kNegInf, l_run = 0.f;
+#pragma unroll
+  for (int db = 0; db < C::DB; ++db) acc[db] = f32x16{};
+
+  const int steps = WPT == 1 ? nt : __builtin_amdgcn_readfirstlane((ck.count + NW - 1) / NW);
+  for (int j = 0; j < steps; ++j) {
     const int t = first + NW * j;
     const bool more = j + 1 < nt;
-    if constexpr (ST == 2) {
+    if constexpr (WPT > 1) {
+      // this wave's copies of tile j have landed and its reads of tile j - 1 have returned ...
+      wait_vmcnt<0>();
+      reads_done();
+      __builtin_amdgcn_s_barrier();  // ... and every wave's
+      asm volatile("" ::: "memory");
+      if (more) {
+        issue_k(t + NW, (j + 1) & 1);
+        issue_v(t + NW, (j + 1) & 1);
+      }
+      if (j >= nt) continue;  // (the last step of waves with one tile less)
+    } else if constexpr (ST == 2) {
       if (more) {  // into the stage of tile j - 1, read in the previous iteration
         reads_done();
         issue_k(t + NW, (j + 1) & 1);
         issue_v(t + NW, (j + 1) & 1);
-        wait_vmcnt<2 * C::E>();  // tile j landed, the next in flight
+        wait_vmcnt<2 * EC>();  // tile j landed, the next in flight
       } else {
         wait_vmcnt<0>();
       }
     } else {
-      wait_vmcnt<C::E>();  // K of tile j landed (its V, issued later, may be in flight)
+      wait_vmcnt<EC>();  // K of tile j landed (its V, issued later, may be in flight)
     }
     const char* sK = smem + wave * C::WAVEB + (ST == 2 ? (j & 1) * 2 * C::TB : 0);
     const char* sV = sK + C::TB;
     const int n0 = t * C::BN;
 
-    f32x16 sc[NR];
-#pragma unroll
-    for (int nr = 0; nr < NR; ++nr) sc[nr] = f32x16{};
+    f32x16 sc = f32x16{};
 #pragma unroll
     for (int kc = 0; kc < C::KC; ++kc) {
       const i32x4 kf = lds_read16(sK + koff[kc]);
-#pragma unroll
-      for (int nr = 0; nr < NR; ++nr) sc[nr] = mma_step<T>(kf, qf[nr][kc], sc[nr]);
+      sc = mma_step<T>(kf, qf[kc], sc);
     }
     if constexpr (ST == 1) {
       reads_done();
@@ -402,65 +393,57 @@ void tree_attn_kernel(TreeArgs a) {
     // element e is key n0 + 8(e/4) + 4h + e%4
     if constexpr (CAP) {
 #pragma unroll
-      for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float tv;
-          if constexpr (sizeof(T) == 4) sc[nr][e] = p.cap_log2 * tanhf(sc[nr][e] * p.scale * p.inv_cap);
-          else sc[nr][e] = score_log2<true, false>(sc[nr][e], p, 0.f, 0, 0, tv);
-        }
+      for (int e = 0; e < 16; ++e) {
+        float tv;
+        if constexpr (sizeof(T) == 4) sc[e] = p.cap_log2 * tanhf(sc[e] * p.scale * p.inv_cap);
+        else sc[e] = score_log2<true, false>(sc[e], p, 0.f, 0, 0, tv);
+      }
     }
     if (n0 < full_lo || n0 + C::BN > n) {
+      // this lane's keys, relative to its first: e, and hidden before lo or from hi on
+      const int lo = row_lo - n0 - 4 * h, hi = n + (mask ? p.Sq : qi + 1) - n0 - 4 * h;
 #pragma unroll
-      for (int nr = 0; nr < NR; ++nr) {
-        // this lane's keys, relative to its first: e, and hidden before lo or from hi on
-        const int lo = row_lo[nr] - n0 - 4 * h, hi = n + (mask ? p.Sq : qi[nr] + 1) - n0 - 4 * h;
+      for (int e = 0; e < 16; ++e)
+        if ((unsigned)(8 * (e >> 2) + (e & 3) - lo) >= (unsigned)max(hi - lo, 0)) sc[e] = kNegInf;
+      if (mask && n0 + C::BN > n) {  // all of the tile's mask bytes at once
+        const unsigned char* mrow = mask + (int64_t)qi * p.Sq;
+        const int u0 = n0 + 4 * h - n;
+        unsigned char m[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m[e] = mrow[min(max(u0 + 8 * (e >> 2) + (e & 3), 0), p.Sq - 1)];
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if ((unsigned)(8 * (e >> 2) + (e & 3) - lo) >= (unsigned)max(hi - lo, 0)) sc[nr][e] = kNegInf;
-        if (mask && n0 + C::BN > n) {  // all of the tile's mask bytes at once
-          const unsigned char* mrow = mask + (int64_t)qi[nr] * p.Sq;
-          const int u0 = n0 + 4 * h - n;
-          unsigned char m[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) m[e] = mrow[min(max(u0 + 8 * (e >> 2) + (e & 3), 0), p.Sq - 1)];
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (u0 + 8 * (e >> 2) + (e & 3) >= 0 && m[e] == 0) sc[nr][e] = kNegInf;
-        }
+          if (u0 + 8 * (e >> 2) + (e & 3) >= 0 && m[e] == 0) sc[e] = kNegInf;
       }
     }
-    f32x16 pe[NR];
+    f32x16 pe;
+    if constexpr (!CAP) settle(sc);  // (an unmasked tile's scores come straight from the MFMAs)
+    float mx, mx2;
+    max16_partial(sc, mx, mx2);
+    mx = max2(mx, mx2);
+    if constexpr (!CAP) mx *= c2;
+    mx = fmaxf(mx, swap_halves(mx));
+    if (mx != mx) mx = kNegInf;
+    const bool grow = mx > m_run + kTreeRescale;
+    if (__builtin_amdgcn_ballot_w64(grow)) {
+      const float m_new = grow ? mx : m_run;
+      const float alpha = grow ? fast_exp2(m_run - m_new) : 1.f;
+      l_run *= alpha;
 #pragma unroll
-    for (int nr = 0; nr < NR; ++nr) {
-      if constexpr (!CAP) settle(sc[nr]);  // (an unmasked tile's scores come straight from the MFMAs)
-      float mx, mx2;
-      max16_partial(sc[nr], mx, mx2);
-      mx = max2(mx, mx2);
-      if constexpr (!CAP) mx *= c2;
-      mx = fmaxf(mx, swap_halves(mx));
-      if (mx != mx) mx = kNegInf;
-      const bool grow = mx > m_run[nr] + kTreeRescale;
-      if (__builtin_amdgcn_ballot_w64(grow)) {
-        const float m_new = grow ? mx : m_run[nr];
-        const float alpha = grow ? fast_exp2(m_run[nr] - m_new) : 1.f;
-        l_run[nr] *= alpha;
-#pragma unroll
-        for (int db = 0; db < C::DB; ++db) scale_inplace(acc[nr][db], alpha);
-        m_run[nr] = m_new;
-      }
-      const float m_use = (m_run[nr] == kNegInf) ? 0.f : m_run[nr];
-      float rs[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if constexpr (!CAP) pe[nr][e] = fast_exp2(__builtin_fmaf(sc[nr][e], c2, -m_use));
-        else pe[nr][e] = fast_exp2(sc[nr][e] - m_use);
-        rs[e & 3] += pe[nr][e];
-      }
-      l_run[nr] += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+      for (int db = 0; db < C::DB; ++db) scale_inplace(acc[db], alpha);
+      m_run = m_new;
     }
+    const float m_use = (m_run == kNegInf) ? 0.f : m_run;
+    float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      if constexpr (!CAP) pe[e] = fast_exp2(__builtin_fmaf(sc[e], c2, -m_use));
+      else pe[e] = fast_exp2(sc[e] - m_use);
+      rs[e & 3] += pe[e];
+    }
+    l_run += (rs[0] + rs[1]) + (rs[2] + rs[3]);
     if constexpr (ST == 1) {  // V of tile j landed (the next K may be in flight)
-      if (more) wait_vmcnt<C::E>();
+      if (more) wait_vmcnt<EC>();
       else wait_vmcnt<0>();
     }
     if constexpr (sizeof(T) == 4) {
@@ -471,25 +454,20 @@ void tree_attn_kernel(TreeArgs a) {
 #pragma unroll
         for (int db = 0; db < C::DB; ++db) {
           const float v = *(const float*)(vr + voff[db]);
-#pragma unroll
-          for (int nr = 0; nr < NR; ++nr)
-            acc[nr][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, pe[nr][i], acc[nr][db], 0, 0, 0);
+          acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, pe[i], acc[db], 0, 0, 0);
         }
       }
     } else {
       typedef typename Mfma<T>::v8 V8;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        V8 pb[NR];
-#pragma unroll
-        for (int nr = 0; nr < NR; ++nr) pb[nr] = pack8<T>(pe[nr], 8 * c);
+        const V8 pb = pack8<T>(pe, 8 * c);
         const char* vr = sV + 16 * c * C::ROWB;
 #pragma unroll
         for (int db = 0; db < C::DB; ++db) {
           const i16x4 lo = lds_read_tr4(vr + voff[db]);
           const i16x4 hi = lds_read_tr4(vr + 8 * C::ROWB + voff[db]);
-#pragma unroll
-          for (int nr = 0; nr < NR; ++nr) acc[nr][db] = Mfma<T>::mma(cat_tr<V8>(lo, hi), pb[nr], acc[nr][db]);
+          acc[db] = Mfma<T>::mma(cat_tr<V8>(lo, hi), pb, acc[db]);
         }
       }
     }
@@ -499,65 +477,60 @@ void tree_attn_kernel(TreeArgs a) {
     }
   }
 
-  // The NW waves' (m, l, acc) combined in wave order through LDS, one row tile after
-  // the other (every wave's copies have landed: its last tile waited for vmcnt 0),
-  // then O / l and LSE.
-  float* xm = (float*)smem;            // [NW][64]
-  float* xl = xm + NW * 64;            // [NW][64]
+  // The (m, l, acc) of a row tile's NW waves combined in wave order through LDS (every
+  // wave's copies have landed: its last tile waited for vmcnt 0), then O / l and LSE.
+  float* xm = (float*)smem + sub * NW * 64 * (2 + 16 * C::DB);  // [NW][64]
+  float* xl = xm + NW * 64;                                     // [NW][64]
   f32x4* xa = (f32x4*)(xl + NW * 64);  // [NW][4 DB][64]: columns 8 y + 4 h .. + 3 of row l32
+  const float l_tot = l_run + swap_halves(l_run);
+  __syncthreads();
+  xm[wave * 64 + lane] = m_run;
+  xl[wave * 64 + lane] = l_tot;
 #pragma unroll
-  for (int nr = 0; nr < NR; ++nr) {
-    const float l_tot = l_run[nr] + swap_halves(l_run[nr]);
-    __syncthreads();
-    xm[wave * 64 + lane] = m_run[nr];
-    xl[wave * 64 + lane] = l_tot;
+  for (int y = 0; y < 4 * C::DB; ++y) {
+    const f32x16& v = acc[y / 4];
+    const int e = y % 4 * 4;
+    xa[(wave * 4 * C::DB + y) * 64 + lane] = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+  }
+  __syncthreads();
+  float mw[NW], mall = kNegInf;
 #pragma unroll
-    for (int y = 0; y < 4 * C::DB; ++y) {
-      const f32x16& v = acc[nr][y / 4];
-      const int e = y % 4 * 4;
-      xa[(wave * 4 * C::DB + y) * 64 + lane] = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
-    }
-    __syncthreads();
-    float mw[NW], mall = kNegInf;
+  for (int w = 0; w < NW; ++w) {
+    mw[w] = xm[w * 64 + lane];
+    mall = fmaxf(mall, mw[w]);
+  }
+  float al[NW], L = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      mw[w] = xm[w * 64 + lane];
-      mall = fmaxf(mall, mw[w]);
-    }
-    float al[NW], L = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      // a wave whose maximum stayed -inf has weights of 0, or NaN scores
-      const float lw = xl[w * 64 + lane];
-      al[w] = mw[w] == kNegInf ? (lw == 0.f ? 0.f : 1.f) : fast_exp2(mw[w] - mall);
-      L = __builtin_fmaf(al[w], lw, L);
-    }
-    const bool empty = L == 0.f;  // no key; NaN (a NaN query row or key) is not
-    const float inv = empty ? 0.f : 1.0f / L;
-    if (32 * (rt0 + nr) + l32 < R) {
-      const int hq = hk * p.G + hqo[nr];
-      const int64_t row = ((int64_t)b * p.Hq + hq) * p.Sq + qi[nr];
-      float* po = a.part_o + (row * a.nsplit + s) * D + 4 * h;
-      T* out = (T*)a.o.data + b * a.o.sb + hq * a.o.sh + (int64_t)qi[nr] * a.o.ss + 4 * h;
+  for (int w = 0; w < NW; ++w) {
+    // a wave whose maximum stayed -inf has weights of 0, or NaN scores
+    const float lw = xl[w * 64 + lane];
+    al[w] = mw[w] == kNegInf ? (lw == 0.f ? 0.f : 1.f) : fast_exp2(mw[w] - mall);
+    L = __builtin_fmaf(al[w], lw, L);
+  }
+  const bool empty = L == 0.f;  // no key; NaN (a NaN query row or key) is not
+  const float inv = empty ? 0.f : 1.0f / L;
+  if (32 * rt0 + l32 < R) {
+    const int64_t row = ((int64_t)b * p.Hq + hq) * p.Sq + qi;
+    float* po = a.part_o + (row * a.nsplit + s) * D + 4 * h;
+    T* out = (T*)a.o.data + b * a.o.sb + hq * a.o.sh + (int64_t)qi * a.o.ss + 4 * h;
 #pragma unroll 2
-      for (int y = wave; y < 4 * C::DB; y += NW) {
-        f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int y = wave; y < 4 * C::DB; y += NW) {
+      f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          const f32x4 v = xa[(w * 4 * C::DB + y) * 64 + lane];
+      for (int w = 0; w < NW; ++w) {
+        const f32x4 v = xa[(w * 4 * C::DB + y) * 64 + lane];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(al[w], v[e], o[e]);
-        }
-        o *= inv;
-        if (ns > 1) *(f32x4*)(po + 8 * y) = o;
-        else if constexpr (sizeof(T) == 4) *(f32x4*)(out + 8 * y) = o;
-        else st_global8(out + 8 * y, pack4<T>(o[0], o[1], o[2], o[3]));
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(al[w], v[e], o[e]);
       }
-      if (wave == 0 && h == 0) {
-        const float lse = empty ? kNegInf : mall + log2f(L);
-        if (ns > 1) a.part_lse[row * a.nsplit + s] = lse;
-        else a.lse[row] = lse * kLn2;
-      }
+      o *= inv;
+      if (ns > 1) *(f32x4*)(po + 8 * y) = o;
+      else if constexpr (sizeof(T) == 4) *(f32x4*)(out + 8 * y) = o;
+      else st_global8(out + 8 * y, pack4<T>(o[0], o[1], o[2], o[3]));
+    }
+    if (wave == 0 && h == 0) {
+      const float lse = empty ? kNegInf : mall + log2f(L);
+      if (ns > 1) a.part_lse[row * a.nsplit + s] = lse;
+      else a.lse[row] = lse * kLn2;
     }
   }
 }
@@ -636,24 +609,26 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   if (lane == 0) a.lse[row] = none ? kNegInf : (mx + log2f(ws)) * kLn2;
 }
 
-template <class T, int D, int NR>
-void launch_tree_nr(const TreeArgs& a, hipStream_t st) {
-  using C = TreeCfg<T, D>;
-  const dim3 grid((unsigned)((a.nchunk + 7) / 8 * 8 * a.nrt)), block(C::NW * 64);
-  if (a.p.cap > 0.f) hipLaunchKernelGGL((tree_attn_kernel<T, D, C::NW, NR, true>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((tree_attn_kernel<T, D, C::NW, NR, false>), grid, block, 0, st, a);
+template <class T, int D, int WPT>
+void launch_tree_share(TreeArgs a, hipStream_t st) {
+  constexpr int NW = WPT == 4 ? TreeCfg<T, D>::NW / 2 : TreeCfg<T, D>::NW;
+  a.nrt = (int)((((int64_t)a.p.G * a.p.Sq + 31) / 32 + WPT - 1) / WPT);
+  const dim3 grid((unsigned)((a.nchunk + 7) / 8 * 8 * a.nrt)), block(NW * WPT * 64);
+  if (a.p.cap > 0.f) hipLaunchKernelGGL((tree_attn_kernel<T, D, NW, WPT, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((tree_attn_kernel<T, D, NW, WPT, false>), grid, block, 0, st, a);
 }
 
 template <class T, int D>
-hipError_t launch_tree(TreeArgs a, hipStream_t st) {
+hipError_t launch_tree(const TreeArgs& a, hipStream_t st) {
   using C = TreeCfg<T, D>;
-  // two row tiles per wave where there are two (one: bf16 B=8 T=16 caches of 32768 D=128
-  // 187 -> 242 us, fp16 B=4 Hq=28 Hkv=4 T=64 caches of 16384 D=64 56 -> 81 us)
-  const int64_t tiles = ((int64_t)a.p.G * a.p.Sq + 31) / 32;
-  const bool two = C::NR == 2 && tiles > 1;
-  a.nrt = (int)(two ? (tiles + 1) / 2 : tiles);
-  if (two) launch_tree_nr<T, D, C::NR>(a, st);
-  else launch_tree_nr<T, D, 1>(a, st);
+  const int share = tree_share(C::ROWB, sizeof(T), ((int64_t)a.p.G * a.p.Sq + 31) / 32);
+  if constexpr (sizeof(T) == 2 && C::ROWB <= 256) {
+    if constexpr (C::ROWB == 256) {
+      if (share == 4) launch_tree_share<T, D, 4>(a, st);
+    }
+    if (share == 2) launch_tree_share<T, D, 2>(a, st);
+  }
+  if (share == 1) launch_tree_share<T, D, 1>(a, st);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.nsplit == 1) return e;
   const int64_t rows = (int64_t)a.p.B * a.p.Hq * a.p.Sq;

@@ -61,6 +61,14 @@ CASES = [
     (BF, 1, 32, 8, 2, 9000, 128, [8998], None, 0, 0.0, "bnsd"),      # many splits
     (BF, 4, 2, 1, 1, 20000, 128, [19999, 3, 0, 7777], None, 0, 0.0, "bnsd"),  # unequal lengths, many splits
     (FH, 1, 1, 1, 300, 1200, 64, [900], "shared", 0, 0.0, "bnsd"),   # more drafted tokens than a tile
+    # several row tiles, whose waves share key tiles: full fours, padded ones, pairs; more waves than key tiles
+    (BF, 1, 8, 2, 30, 1500, 128, [1470], "batch", 0, 0.0, "bnsd"),
+    (FH, 2, 7, 1, 64, 800, 128, [700, 3], "holes", 50, 30.0, "bsnd"),
+    (BF, 2, 6, 1, 27, 600, 128, [500, 0], "shared", 0, 0.0, "bnsd"),
+    (BF, 3, 5, 1, 13, 300, 128, [287, 1, 100], None, 20, 0.0, "bsnd"),
+    (FH, 1, 9, 1, 20, 2000, 32, [1980], "shared", 0, 0.0, "bnsd"),
+    (BF, 2, 8, 1, 40, 60, 64, [20, 0], "batch", 7, 0.0, "bnsd"),
+    (BF, 1, 4, 1, 70, 9000, 128, [8930], "shared", 0, 0.0, "bsnd"),
 ]
 
 
