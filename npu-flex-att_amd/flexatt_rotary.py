@@ -83,5 +83,7 @@ def rotary_embedding(query, key, inv_freq, positions=None, interleaved=False, ma
     :func:`rotary_frequencies`).  ``positions``: int32 or int64 [S] or [B, S];
     default 0, 1, ....  Differentiable in query and key; a backward pass may be captured
     into a graph, as any of torch's, while no eager graph of the same leaves is alive.
+    Small calls wait for autograd's hand-over to its device thread; inside
+    ``torch.autograd.set_multithreading_enabled(False)`` there is none.
     """
     return _lib.native().rotary(query, key, inv_freq, positions, interleaved, magnitude)
