@@ -166,3 +166,20 @@ def test_graph_replays(gpu_device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(into, eager)
+
+
+@pytest.mark.parametrize("dtype", [BF, FH, FS])
+@pytest.mark.parametrize("top", [8.0, 40.0])
+def test_soft_cap_to_the_last_bits(gpu_device, dtype, top):
+    """One query row and keys along one element, so that the scores s are exact, and LSE 0: weights exp(cap tanh(s / cap)).
+    The capped score is off by 9 half steps of itself (scale / cap, the quotient, the series, cap log2 e) up to |s| = cap / 4,
+    and by another 4 of the cap above (1 - 2 / (1 + e^2y): exponential, sum, reciprocal, difference); exp2 by a step."""
+    s = torch.linspace(-top, top, 301).to(dtype)
+    q, k = torch.zeros(1, 1, 1, 64, dtype=dtype), torch.zeros(1, 1, 301, 64, dtype=dtype)
+    q[..., 0], k[0, 0, :, 0] = 1.0, s
+    w = fc.attention_weight_sums(q.cuda(), k.cuda(), torch.zeros(1, 1, 1, device="cuda"), scale=1.0, soft_cap=30.0)
+    x = 30.0 * torch.tanh(s.double() / 30.0)
+    h = 2.0 ** -24
+    tol = 9 * h * x.abs() + torch.where(s.double().abs() > 7.4, 4 * h * 30.0, 0.0) + 2 * h
+    worst = ((w[0, 0].cpu().double() / torch.exp(x) - 1.0).abs() / tol).max().item()
+    assert worst <= 1.0, f"{worst:.2f} tolerances"
