@@ -202,11 +202,15 @@ WeightPlan weight_plan(const flexatt_weights* p) {
     tiles = b > tiles ? b : tiles;
     both = a + b > both ? a + b : both;
   }
+  // row tiles of a part, at least: the second launch adds parts up (bf16 Hq=28 Hkv=4 D=128,
+  // 49 rows over 2123 keys, 11 tiles: of four 14.8 us, two 12.0, one 14.5; fp32, whose
+  // tiles take four times as long, 32 heads, 200 rows, D=128: 40, 24 and 16)
+  const int64_t least = elt_size(p->dtype) == 2 ? 2 : 1;
   WeightPlan best = {0, 1};
   int64_t best_cost = INT64_MAX;
   for (int pair = nkb > 1 ? 1 : 0; pair >= 0; --pair) {
     const int64_t groups = (pair ? (nkb + 1) / 2 : nkb) * bh, work = pair ? both : tiles;
-    for (int64_t n = 1; n <= 64 && (n == 1 || tiles / n >= 4); ++n) {
+    for (int64_t n = 1; n <= 64 && (n == 1 || tiles / n >= least); ++n) {
       const int64_t cost = (groups * n + slots - 1) / slots * ((work + n - 1) / n + (pair ? 9 : 5));
       if (cost < best_cost) best = {pair, (int)n}, best_cost = cost;
     }
