@@ -16,7 +16,7 @@
 //  * Copies, 16 bytes per lane, of the rows of a share of the places: as many
 //    workgroups as fill the chip make the same selection, each for its share.  (The
 //    copies as a kernel of their own behind one selection: 64 heads of 8192 slots, bf16
-//    D=128, 2048 kept, 42 -> 39 us; two heads of 2048, fp32 D=64, 1000 kept, 12 -> 8.)
+//    D=128, 2048 kept, 42 -> 39 us; two heads of 2048, fp32 D=64, 1000 kept, 12 -> 9.)
 // What bounds it: the copies memory (134 MB there: 26 us at the rate of a large copy),
 // the selection latency: a chain of passes over keys that stay in registers up to
 // sixteen slots a thread (256 threads up to 2048 slots, for cheaper barriers), and of
