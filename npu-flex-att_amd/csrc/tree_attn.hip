@@ -25,6 +25,13 @@
 //    LSE) by a second kernel in a fixed order;
 //  * rows behind n + T are never read: the copies repeat the last row instead, so
 //    what a cache holds there (NaN too) does not matter.
+// Precision: scores, maxima, row sums, accumulators, partials and LSE are fp32.  P
+// alone is rounded to the type, as in the forward: it is an operand of the 16-bit MFMAs
+// of P V (a second one for what the rounding leaves out would double them).  A weight
+// is off by half a step at most (2^-8 of it in bf16, 2^-11 in fp16; the row sum has the
+// unrounded ones), which over many keys averages out to about what O's own rounding is: the rms error of bf16 outputs is 1.8e-3 to 2.3e-3 of their
+// rms, 1.7e-3 the output's rounding alone, of fp16 ones 2.9e-4 and 2.1e-4; the same
+// rounding in a plain fp32 computation gives the same errors to three digits.
 // What bounds it: K and V from HBM for long caches and few rows; from some hundred
 // rows per KV head on the softmax's VALU work and the MFMAs; latency for short caches.
 // Of that the instructions are the larger part: a launch finds the instruction cache
