@@ -85,10 +85,24 @@ struct Named {
   const char* name;
   const Tensor* t;
 };
+// The kernels read and write through pointers: a derivative that an argument brings
+// along would be dropped without a word.
+void no_tangents(std::initializer_list<Named> all) {
+  for (const Named& x : all)
+    TORCH_CHECK(!x.t->_fw_grad(/*level=*/0).defined(), x.name,
+                " carries a tangent: the rotary and cache operators have no forward-mode derivatives");
+}
+void no_derivatives(std::initializer_list<Named> all) {
+  no_tangents(all);
+  if (!at::GradMode::is_enabled()) return;
+  for (const Named& x : all)
+    TORCH_CHECK(!x.t->requires_grad(), x.name,
+                " requires a gradient, which the call does not have: detach it, or call under torch.no_grad()");
+}
+
 // Four dimensions, the first one's type and device, a head dim with kernels.
-void check_tensors(std::initializer_list<Named> all, bool no_grad) {
+void check_tensors(std::initializer_list<Named> all) {
   const Tensor& first = *all.begin()->t;
-  const bool grad = no_grad && at::GradMode::is_enabled();
   for (const Named& x : all) {
     const Tensor& t = *x.t;
     TORCH_CHECK(t.is_cuda(), x.name, " must be on a ROCm GPU device (got ", t.device(), ")");
@@ -97,8 +111,6 @@ void check_tensors(std::initializer_list<Named> all, bool no_grad) {
     TORCH_CHECK(t.device() == first.device(), x.name, " must be on ", first.device(), " (got ", t.device(), ")");
     TORCH_CHECK(t.dim() == 4, x.name, " must have four dimensions, got ", t.sizes());
     TORCH_CHECK(t.layout() == at::kStrided, x.name, " must be a strided tensor");
-    TORCH_CHECK(!(grad && t.requires_grad()), x.name,
-                " requires a gradient, which the cache operators do not have: call them under torch.no_grad()");
   }
   dtype_of(first);
   const int64_t d = first.size(3);
@@ -276,13 +288,16 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const OptTensor pos = opt_tensor_arg(a[3], "positions");
   const bool interleaved = bool_arg(a[4]);
   const double magnitude = double_arg(a[5]);
+  no_tangents({{"inv_freq", &freq}});
   if (key) {
-    check_tensors({{"query", &query}, {"key", &*key}}, false);
+    no_tangents({{"query", &query}, {"key", &*key}});
+    check_tensors({{"query", &query}, {"key", &*key}});
     FLEXATT_ASSERT(key->size(0) == query.size(0) && key->size(2) == query.size(2) && key->size(3) == query.size(3),
                    "query and key must have the same batch, length and head dim");
     FLEXATT_ASSERT(key->size(1) > 0, "key must have a head");
   } else {
-    check_tensors({{"query", &query}}, false);
+    no_tangents({{"query", &query}});
+    check_tensors({{"query", &query}});
   }
   freq = check_frequencies(freq, query.size(3), query.device());
   Tensor qo, ko;
@@ -317,7 +332,9 @@ PyObject* py_rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const OptTensor freq = opt_tensor_arg(a[6], "inv_freq"), pos = opt_tensor_arg(a[7], "positions");
   const bool interleaved = bool_arg(a[8]);
   const double magnitude = double_arg(a[9]);
-  check_tensors({{"query", &query}, {"key", &key}, {"value", &value}, {"key_cache", &kc}, {"value_cache", &vc}}, true);
+  if (freq) no_tangents({{"inv_freq", &*freq}});
+  no_derivatives({{"query", &query}, {"key", &key}, {"value", &value}, {"key_cache", &kc}, {"value_cache", &vc}});
+  check_tensors({{"query", &query}, {"key", &key}, {"value", &value}, {"key_cache", &kc}, {"value_cache", &vc}});
   check_cache(query, kc, vc);
   const int64_t B = query.size(0), S = query.size(2), D = query.size(3), hkv = kc.size(1), C = kc.size(2);
   const c10::Device dev = query.device();
@@ -368,7 +385,8 @@ PyObject* py_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor kc = tensor_arg(a[1], "key_cache"), vc = tensor_arg(a[2], "value_cache");
   Tensor lengths = tensor_arg(a[3], "lengths");
   const OptTensor mask = opt_tensor_arg(a[4], "tree_mask"), depth = opt_tensor_arg(a[6], "depths");
-  check_tensors({{"query", &query}, {"key_cache", &kc}, {"value_cache", &vc}}, true);
+  no_derivatives({{"query", &query}, {"key_cache", &kc}, {"value_cache", &vc}});
+  check_tensors({{"query", &query}, {"key_cache", &kc}, {"value_cache", &vc}});
   check_cache(query, kc, vc);
   const int64_t B = query.size(0), Hq = query.size(1), T = query.size(2), D = query.size(3), C = kc.size(2);
   const c10::Device dev = query.device();
@@ -437,7 +455,13 @@ PyObject* py_weight_sums(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want(n, 10, "weight_sums");
   const Tensor query = tensor_arg(a[0], "query"), key = tensor_arg(a[1], "key");
-  check_tensors({{"query", &query}, {"key", &key}}, true);
+  FLEXATT_ASSERT(THPVariable_Check(a[2]), "lse must be [B, Hq, Sq]");
+  Tensor lse = THPVariable_Unpack(a[2]);
+  const OptTensor into = opt_tensor_arg(a[9], "into");
+  no_derivatives({{"query", &query}, {"key", &key}});
+  no_tangents({{"lse", &lse}});
+  if (into) no_derivatives({{"into", &*into}});
+  check_tensors({{"query", &query}, {"key", &key}});
   const int64_t B = query.size(0), Hq = query.size(1), Sq = query.size(2), D = query.size(3);
   const int64_t Hkv = key.size(1), Sk = key.size(2);
   const c10::Device dev = query.device();
@@ -445,8 +469,6 @@ PyObject* py_weight_sums(PyObject*, PyObject* const* a, Py_ssize_t n) {
   FLEXATT_ASSERT(key.size(0) == B, "query and key batch sizes must match");
   FLEXATT_ASSERT(key.size(3) == D, "query and key head dims must match");
   FLEXATT_ASSERT(Hkv > 0 && Hq % Hkv == 0, "Hq must be divisible by Hkv");
-  FLEXATT_ASSERT(THPVariable_Check(a[2]), "lse must be [B, Hq, Sq]");
-  Tensor lse = THPVariable_Unpack(a[2]);
   FLEXATT_ASSERT(lse.dim() == 3 && lse.size(0) == B && lse.size(1) == Hq && lse.size(2) == Sq, "lse must be [B, Hq, Sq]");
   TORCH_CHECK(lse.device() == dev, "lse must be on ", dev, " (got ", lse.device(), ")");
   lse = lse.to(at::kFloat).contiguous();
@@ -476,13 +498,11 @@ PyObject* py_weight_sums(PyObject*, PyObject* const* a, Py_ssize_t n) {
     lengths = per_sequence(*x, "lengths", B, dev);
     p.lengths = lengths.const_data_ptr<int32_t>();
   }
-  const OptTensor into = opt_tensor_arg(a[9], "into");
   if (into) {
     sums = *into;
     TORCH_CHECK(sums.scalar_type() == at::kFloat && sums.dim() == 3 && sums.size(0) == B && sums.size(1) == Hkv &&
                     sums.size(2) == Sk && sums.device() == dev && sums.is_contiguous(),
                 "into must be a contiguous fp32 [B, Hkv, Skv] = [", B, ", ", Hkv, ", ", Sk, "] tensor on ", dev);
-    TORCH_CHECK(!(at::GradMode::is_enabled() && sums.requires_grad()), "into requires a gradient");
     p.accumulate = 1;
   } else {
     sums = at::empty({B, Hkv, Sk}, query.options().dtype(at::kFloat).requires_grad(false));
@@ -512,7 +532,17 @@ PyObject* py_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   want(n, 10, "evict");
   const Tensor kc = tensor_arg(a[0], "key_cache"), vc = tensor_arg(a[1], "value_cache");
   Tensor scores = tensor_arg(a[2], "scores"), lengths = tensor_arg(a[3], "lengths");
-  check_tensors({{"key_cache", &kc}, {"value_cache", &vc}}, true);
+  const bool fresh = a[7] == Py_None;
+  Tensor ko, vo, so;
+  no_derivatives({{"key_cache", &kc}, {"value_cache", &vc}});
+  no_tangents({{"scores", &scores}});
+  if (!fresh) {
+    ko = tensor_arg(a[7], "out key");
+    vo = tensor_arg(a[8], "out value");
+    so = tensor_arg(a[9], "out scores");
+    no_derivatives({{"out key", &ko}, {"out value", &vo}, {"out scores", &so}});
+  }
+  check_tensors({{"key_cache", &kc}, {"value_cache", &vc}});
   FLEXATT_ASSERT(kc.sizes() == vc.sizes(), "key and value cache shapes must match");
   const int64_t B = kc.size(0), H = kc.size(1), C = kc.size(2), D = kc.size(3);
   const c10::Device dev = kc.device();
@@ -526,17 +556,12 @@ PyObject* py_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t keep = int_arg(a[4]), recent = int_arg(a[5]), sinks = int_arg(a[6]);
   TORCH_CHECK(keep >= 1 && keep <= INT32_MAX && recent >= 0 && sinks >= 0 && recent <= keep && sinks <= keep - recent,
               "keep must be at least 1, recent and sinks at least 0 and together at most keep");
-  const bool fresh = a[7] == Py_None;
-  Tensor ko, vo, so;
   if (fresh) {
     ko = at::empty({B, H, keep, D}, kc.options().requires_grad(false));
     vo = at::empty({B, H, keep, D}, kc.options().requires_grad(false));
     so = at::empty({B, H, keep}, scores.options().requires_grad(false));
   } else {
-    ko = tensor_arg(a[7], "out key");
-    vo = tensor_arg(a[8], "out value");
-    so = tensor_arg(a[9], "out scores");
-    check_tensors({{"key_cache", &kc}, {"out key", &ko}, {"out value", &vo}}, true);
+    check_tensors({{"key_cache", &kc}, {"out key", &ko}, {"out value", &vo}});
     TORCH_CHECK(ko.size(0) == B && ko.size(1) == H && ko.size(3) == D && ko.sizes() == vo.sizes() && ko.size(2) >= keep,
                 "out key and value must be [B, Hkv, at least keep, D] = [", B, ", ", H, ", ", keep, ", ", D, "]");
     in_place(ko, "out key");
@@ -544,7 +569,6 @@ PyObject* py_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK(so.scalar_type() == at::kFloat && so.dim() == 3 && so.size(0) == B && so.size(1) == H &&
                     so.size(2) == ko.size(2) && so.device() == dev && so.is_contiguous(),
                 "out scores must be a contiguous fp32 [", B, ", ", H, ", ", ko.size(2), "] tensor on ", dev);
-    TORCH_CHECK(!(at::GradMode::is_enabled() && so.requires_grad()), "out scores requires a gradient");
   }
   const auto ints = lengths.options();
   Tensor slots = at::empty({B, H, keep}, ints), fewer = at::empty({B}, ints);

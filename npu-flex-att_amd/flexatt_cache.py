@@ -12,7 +12,8 @@ device, so every call can be captured into a graph and replayed as the cache gro
   attention_weight_sums(...)  sum over the query rows of the softmax weights, per key
   evict_cache(...)            the rows worth keeping, copied to a smaller cache
 
-None of them is differentiable.
+None of them is differentiable: a tensor that carries a tangent, or with gradients
+on one that requires them, is refused.
 """
 from __future__ import annotations
 
