@@ -288,7 +288,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const OptTensor pos = opt_tensor_arg(a[3], "positions");
   const bool interleaved = bool_arg(a[4]);
   const double magnitude = double_arg(a[5]);
-  no_tangents({{"inv_freq", &freq}});
+  no_derivatives({{"inv_freq", &freq}});
   if (key) {
     no_tangents({{"query", &query}, {"key", &*key}});
     check_tensors({{"query", &query}, {"key", &*key}});
@@ -332,7 +332,7 @@ PyObject* py_rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const OptTensor freq = opt_tensor_arg(a[6], "inv_freq"), pos = opt_tensor_arg(a[7], "positions");
   const bool interleaved = bool_arg(a[8]);
   const double magnitude = double_arg(a[9]);
-  if (freq) no_tangents({{"inv_freq", &*freq}});
+  if (freq) no_derivatives({{"inv_freq", &*freq}});
   no_derivatives({{"query", &query}, {"key", &key}, {"value", &value}, {"key_cache", &kc}, {"value_cache", &vc}});
   check_tensors({{"query", &query}, {"key", &key}, {"value", &value}, {"key_cache", &kc}, {"value_cache", &vc}});
   check_cache(query, kc, vc);
@@ -458,8 +458,7 @@ PyObject* py_weight_sums(PyObject*, PyObject* const* a, Py_ssize_t n) {
   FLEXATT_ASSERT(THPVariable_Check(a[2]), "lse must be [B, Hq, Sq]");
   Tensor lse = THPVariable_Unpack(a[2]);
   const OptTensor into = opt_tensor_arg(a[9], "into");
-  no_derivatives({{"query", &query}, {"key", &key}});
-  no_tangents({{"lse", &lse}});
+  no_derivatives({{"query", &query}, {"key", &key}, {"lse", &lse}});
   if (into) no_derivatives({{"into", &*into}});
   check_tensors({{"query", &query}, {"key", &key}});
   const int64_t B = query.size(0), Hq = query.size(1), Sq = query.size(2), D = query.size(3);
@@ -534,8 +533,7 @@ PyObject* py_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Tensor scores = tensor_arg(a[2], "scores"), lengths = tensor_arg(a[3], "lengths");
   const bool fresh = a[7] == Py_None;
   Tensor ko, vo, so;
-  no_derivatives({{"key_cache", &kc}, {"value_cache", &vc}});
-  no_tangents({{"scores", &scores}});
+  no_derivatives({{"key_cache", &kc}, {"value_cache", &vc}, {"scores", &scores}});
   if (!fresh) {
     ko = tensor_arg(a[7], "out key");
     vo = tensor_arg(a[8], "out value");

@@ -81,10 +81,12 @@ def rotary_embedding(query, key, inv_freq, positions=None, interleaved=False, ma
     ``(2 i, 2 i + 1)`` with ``interleaved``; its angle is ``positions * inv_freq[i]``,
     formed in 64 bits, and ``magnitude`` scales both of its elements (see
     :func:`rotary_frequencies`).  ``positions``: int32 or int64 [S] or [B, S];
-    default 0, 1, ....  Differentiable in query and key, in reverse mode (an argument that
-    carries a tangent is refused); a backward pass may be captured into a graph,
-    as any of torch's, while no eager graph of the same leaves is alive.
-    Small calls wait for autograd's hand-over to its device thread; inside
-    ``torch.autograd.set_multithreading_enabled(False)`` there is none.
+    default 0, 1, ....
+
+    Differentiable in query and key, in reverse mode; an argument that carries a tangent
+    is refused, and so is, with gradients on, an ``inv_freq`` that requires them.  A
+    backward pass may be captured into a graph, as any of torch's, while no eager graph
+    of the same leaves is alive.  Small calls wait for autograd's hand-over to its device
+    thread; inside ``torch.autograd.set_multithreading_enabled(False)`` there is none.
     """
     return _lib.native().rotary(query, key, inv_freq, positions, interleaved, magnitude)

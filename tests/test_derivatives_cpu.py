@@ -44,3 +44,13 @@ def test_tangents_are_refused(op, name, grad):
         given[name] = fwd.unpack_dual(given[name]).primal
         with pytest.raises(RuntimeError, match="ROCm GPU"):  # past the refusal
             call(given)
+
+
+@pytest.mark.parametrize("op,name", [x for x in EVERY if x[0] != "rotary" or x[1] == "inv_freq"])
+def test_gradients_are_refused(op, name):
+    call, given = arguments()[op]
+    given[name] = given[name].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match=f"{name} requires a gradient"):
+        call(given)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="ROCm GPU"):  # past the refusal
+        call(given)
