@@ -306,7 +306,7 @@ int flexatt_bwd_dq_ds(const flexatt_problem* p, const flexatt_tensor* k, const v
 typedef struct flexatt_rotary {
   int32_t dtype;        /* enum flexatt_dtype */
   int32_t batch;        /* B */
-  int32_t heads_q;      /* Hq >= 1 */
+  int32_t heads_q;      /* Hq >= 1; in flexatt_rotary_append also 0: no q */
   int32_t heads_kv;     /* Hkv >= 0; 0: no k */
   int32_t seqlen;       /* S, new tokens per sequence */
   int32_t head_dim;     /* D in {32, 64, 128, 256} */
@@ -330,9 +330,9 @@ int flexatt_rotary_apply(const flexatt_rotary* r, const flexatt_tensor* q, const
                          const flexatt_tensor* q_out, const flexatt_tensor* k_out, void* stream);
 
 /* q_out = turned q, and the rows lengths[b] .. lengths[b] + S - 1 of the cache
- * receive turned k and v [B, Hkv, S, D].  A row outside [0, cache_rows) is not
- * written.  `lengths` is not changed.  k and v may not overlap the cache, nor k_cache be
- * v_cache. */
+ * receive turned k and v [B, Hkv, S, D] (q and q_out NULL when heads_q is 0).  A row
+ * outside [0, cache_rows) is not written.  `lengths` is not changed.  k and v may not
+ * overlap the cache, nor k_cache be v_cache. */
 int flexatt_rotary_append(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* k,
                           const flexatt_tensor* v, const flexatt_tensor* q_out, const flexatt_tensor* k_cache,
                           const flexatt_tensor* v_cache, int32_t cache_rows, const int32_t* lengths, void* stream);

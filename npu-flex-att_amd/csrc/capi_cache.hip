@@ -30,9 +30,9 @@ int check_sizes(int dtype, int64_t b, int64_t h, int64_t s, int head_dim) {
   return FLEXATT_OK;
 }
 
-int check_rotary(const flexatt_rotary* r) {
+int check_rotary(const flexatt_rotary* r, bool append) {
   if (!r) return FLEXATT_EINVAL;
-  FLEXATT_TRY(check_sizes(r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
+  if (r->heads_q != 0 || !append) FLEXATT_TRY(check_sizes(r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
   if (r->heads_kv < 0) return FLEXATT_EINVAL;
   if (r->heads_kv > 0) FLEXATT_TRY(check_sizes(r->dtype, r->batch, r->heads_kv, r->seqlen, r->head_dim));
   if (r->rotary_dim < 0 || r->rotary_dim > r->head_dim || r->rotary_dim % 2) return FLEXATT_EINVAL;
@@ -47,8 +47,10 @@ int check_rotary(const flexatt_rotary* r) {
 
 RotaryArgs rotary_args(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* qo) {
   RotaryArgs a = {};
-  a.q = view(q);
-  a.qo = mview(qo);
+  if (r->heads_q > 0) {
+    a.q = view(q);
+    a.qo = mview(qo);
+  }
   a.inv_freq = r->inv_freq;
   a.positions = r->positions;
   a.pos_sb = r->position_stride_b;
@@ -223,7 +225,7 @@ extern "C" {
 
 int flexatt_rotary_apply(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* k,
                          const flexatt_tensor* q_out, const flexatt_tensor* k_out, void* stream) {
-  FLEXATT_TRY(check_rotary(r));
+  FLEXATT_TRY(check_rotary(r, false));
   FLEXATT_TRY(check_tensor(q, r->dtype));
   FLEXATT_TRY(check_out_tensor(q_out, r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
   if (r->heads_kv == 0 && (k || k_out)) return FLEXATT_EINVAL;
@@ -240,13 +242,17 @@ int flexatt_rotary_apply(const flexatt_rotary* r, const flexatt_tensor* q, const
 int flexatt_rotary_append(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* k,
                           const flexatt_tensor* v, const flexatt_tensor* q_out, const flexatt_tensor* k_cache,
                           const flexatt_tensor* v_cache, int32_t cache_rows, const int32_t* lengths, void* stream) {
-  FLEXATT_TRY(check_rotary(r));
+  FLEXATT_TRY(check_rotary(r, true));
   if (r->heads_kv == 0 || cache_rows <= 0 || !lengths) return FLEXATT_EINVAL;
   if ((int64_t)r->batch * r->heads_kv * cache_rows > INT32_MAX) return FLEXATT_ESHAPE;
-  FLEXATT_TRY(check_tensor(q, r->dtype));
   FLEXATT_TRY(check_tensor(k, r->dtype));
   FLEXATT_TRY(check_tensor(v, r->dtype));
-  FLEXATT_TRY(check_out_tensor(q_out, r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
+  if (r->heads_q > 0) {
+    FLEXATT_TRY(check_tensor(q, r->dtype));
+    FLEXATT_TRY(check_out_tensor(q_out, r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
+  } else if (q || q_out) {
+    return FLEXATT_EINVAL;
+  }
   FLEXATT_TRY(check_out_tensor(k_cache, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim));
   FLEXATT_TRY(check_out_tensor(v_cache, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim));
   if (k_cache->data == v_cache->data) return FLEXATT_ELAYOUT;

@@ -349,11 +349,12 @@ PyObject* py_rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   in_place(vc, "value_cache");
   TORCH_CHECK(C > 0, "the cache has no rows");
   Tensor qo = out_like(query);
-  if (query.numel() > 0) {
+  if (key.numel() > 0) {
+    const bool queried = query.size(1) > 0;
     const Tensor q = prepare(query), k = prepare(key), v = prepare(value);
     const flexatt_tensor tq = view(q), tk = view(k), tv = view(v), to = view(qo), tkc = view(kc), tvc = view(vc);
-    check_status(flexatt_rotary_append(&r, &tq, &tk, &tv, &to, &tkc, &tvc, size32(C, "the cache's rows"),
-                                       lengths.const_data_ptr<int32_t>(), stream_of(dev)),
+    check_status(flexatt_rotary_append(&r, queried ? &tq : nullptr, &tk, &tv, queried ? &to : nullptr, &tkc, &tvc,
+                                       size32(C, "the cache's rows"), lengths.const_data_ptr<int32_t>(), stream_of(dev)),
                  "flexatt_rotary_append");
     written(kc);
     written(vc);

@@ -31,7 +31,8 @@ def rotary_append(query, key, value, key_cache, value_cache, lengths, inv_freq, 
     rotated key and the value of token ``s``, and ``query'`` is the rotated query, as
     :func:`flexatt_rotary.rotary_embedding` gives them; ``positions`` (int32 or int64
     [S] or [B, S]) defaults to the rows' numbers.  ``inv_freq=None`` rotates nothing
-    and returns a copy of the query.  A row outside the cache is not written.
+    and returns a copy of the query.  A row outside the cache is not written.  A query
+    without heads puts keys and values into the cache alone.
     ``lengths`` is read, not changed.
     """
     return _lib.native().rotary_append(query, key, value, key_cache, value_cache, lengths, inv_freq, positions,
