@@ -412,6 +412,41 @@ __device__ __forceinline__ bool xcd_lpt_item(int i, int nk, int ng, int& k, int&
   return true;
 }
 
+// tanh(scale s / cap) of raw scores s, for results in 32 bits.  1 - 2 / (1 + e^2y), as
+// in score_log2 below, is off by eps whatever tanh y is: a score by eps * cap, which
+// 16-bit outputs do not show, but sums of weights and an LSE of few keys do.  Up to |y| =
+// 1/4 (scores of cap / 4) the Taylor series has an error relative to y (first term left
+// out: 1382/155925 y^11), at about the cost of the other; that one is computed in tiles
+// with larger scores only.
+__device__ __forceinline__ void soft_cap(f32x16& sc, const Shape& p) {
+  const float k = p.scale * p.inv_cap;
+  float most = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    sc[e] *= k;
+    most = fmaxf(most, fabsf(sc[e]));
+  }
+  const bool large = __builtin_amdgcn_ballot_w64(most > 0.25f);
+  f32x16 t;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const float y = sc[e], z = y * y;
+    float c = __builtin_fmaf(z, 62.f / 2835.f, -17.f / 315.f);
+    c = __builtin_fmaf(z, c, 2.f / 15.f);
+    c = __builtin_fmaf(z, c, -1.f / 3.f);
+    t[e] = __builtin_fmaf(y * z, c, y);
+  }
+  if (large) {
+    asm volatile("");  // a branch
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float far = 1.f - 2.f * fast_rcp(1.f + fast_exp2(sc[e] * (2.f * kLog2e)));
+      t[e] = fabsf(sc[e]) > 0.25f ? far : t[e];
+    }
+  }
+  sc = t;
+}
+
 // Score transform in the log2 domain for one element: scale, soft-cap, ALiBi
 // (dij = i - j as a float; exact for |i - j| < 2^24).
 template <bool SOFTCAP, bool ALIBI>

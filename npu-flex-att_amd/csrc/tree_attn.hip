@@ -29,9 +29,10 @@
 // alone is rounded to the type, as in the forward: it is an operand of the 16-bit MFMAs
 // of P V (a second one for what the rounding leaves out would double them).  A weight
 // is off by half a step at most (2^-8 of it in bf16, 2^-11 in fp16; the row sum has the
-// unrounded ones), which over many keys averages out to about what O's own rounding is: the rms error of bf16 outputs is 1.8e-3 to 2.3e-3 of their
-// rms, 1.7e-3 the output's rounding alone, of fp16 ones 2.9e-4 and 2.1e-4; the same
-// rounding in a plain fp32 computation gives the same errors to three digits.
+// unrounded ones), which over many keys averages out to about what O's own rounding is:
+// the rms error of bf16 outputs is 1.8e-3 to 2.3e-3 of their rms, 1.7e-3 the output's
+// rounding alone, of fp16 ones 2.9e-4 and 2.1e-4; the same rounding in a plain fp32
+// computation gives the same errors to three digits.
 // What bounds it: K and V from HBM for long caches and few rows; from some hundred
 // rows per KV head on the softmax's VALU work and the MFMAs; latency for short caches.
 // Of that the instructions are the larger part: a launch finds the instruction cache
@@ -399,12 +400,14 @@ void tree_attn_kernel(TreeArgs a) {
 
     // element e is key n0 + 8(e/4) + 4h + e%4
     if constexpr (CAP) {
+      if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        float tv;
-        if constexpr (sizeof(T) == 4) sc[e] = p.cap_log2 * tanhf(sc[e] * p.scale * p.inv_cap);
-        else sc[e] = score_log2<true, false>(sc[e], p, 0.f, 0, 0, tv);
+        for (int e = 0; e < 16; ++e) sc[e] = tanhf(sc[e] * p.scale * p.inv_cap);
+      } else {
+        soft_cap(sc, p);
       }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] *= p.cap_log2;
     }
     if (n0 < full_lo || n0 + C::BN > n) {
       // this lane's keys, relative to its first: e, and hidden before lo or from hi on

@@ -77,40 +77,6 @@ __device__ __forceinline__ void copy_steps(const char* row, unsigned dst) {
   }
 }
 
-// tanh(scale s / cap) of raw scores s.  1 - 2 / (1 + e^2y), which the attention kernels
-// use, is off by eps whatever tanh y is: a weight by eps * cap, which 16-bit outputs do
-// not show but a sum in 32 bits does.  Up to |y| = 1/4 (scores of cap / 4) the Taylor
-// series has an error relative to y (first term left out: 1382/155925 y^11), at about the
-// cost of the other; that one is computed in tiles with larger scores only.
-__device__ __forceinline__ void soft_cap(f32x16& sc, const Shape& p) {
-  const float k = p.scale * p.inv_cap;
-  float most = 0.f;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    sc[e] *= k;
-    most = fmaxf(most, fabsf(sc[e]));
-  }
-  const bool large = __builtin_amdgcn_ballot_w64(most > 0.25f);
-  f32x16 t;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const float y = sc[e], z = y * y;
-    float c = __builtin_fmaf(z, 62.f / 2835.f, -17.f / 315.f);
-    c = __builtin_fmaf(z, c, 2.f / 15.f);
-    c = __builtin_fmaf(z, c, -1.f / 3.f);
-    t[e] = __builtin_fmaf(y * z, c, y);
-  }
-  if (large) {
-    asm volatile("");  // a branch
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float far = 1.f - 2.f * fast_rcp(1.f + fast_exp2(sc[e] * (2.f * kLog2e)));
-      t[e] = fabsf(sc[e]) > 0.25f ? far : t[e];
-    }
-  }
-  sc = t;
-}
-
 // Adds the 32 columns of 16 values per lane half, one step per bit of the lane:
 // lanes W apart exchange the halves of the 2 W values left, so that lane c of each
 // half ends up with the sum of element c % 16 (lanes c and c ^ 16 both have it).
