@@ -151,6 +151,11 @@ TreePlan tree_plan(const flexatt_tree* p) {
   const int64_t most = (tiles + t.min_tiles - 1) / t.min_tiles;  // chunks of one (b, hkv)
   int64_t ns = 2 * ((t.slots + bh - 1) / bh) + 1;
   if (2 * bh > t.slots && p->batch > 1) ns = 3;  // (few chunks each: unequal lengths count most)
+  // A chunk is longer than all sequences' tiles times Hkv / slots (tree_chunk), so a single
+  // one that has them all makes slots / Hkv chunks at most, one where Hkv alone fills the
+  // slots: no partials are kept, and no merge launched, for chunks that never are.
+  const int64_t even = (t.slots + p->heads_kv - 1) / p->heads_kv;
+  if (ns > even) ns = even;
   if (ns > most) ns = most;
   t.nsplit = (int)ns;
   int64_t n = t.slots + bh;
