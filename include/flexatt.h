@@ -402,7 +402,8 @@ typedef struct flexatt_weights {
   const int32_t* lengths;      /* device int32 [B], or NULL */
 } flexatt_weights;
 
-/* sums: contiguous fp32 [B, Hkv, seqlen_kv].  `workspace` as in flexatt_tree_fwd. */
+/* sums: contiguous fp32 [B, Hkv, seqlen_kv], not within the span of an input.
+ * `workspace` as in flexatt_tree_fwd. */
 size_t flexatt_weight_sums_workspace(const flexatt_weights* p);
 int flexatt_weight_sums(const flexatt_weights* p, const flexatt_tensor* q, const flexatt_tensor* k, const float* lse,
                         float* sums, void* workspace, size_t workspace_bytes, void* stream);

@@ -337,6 +337,14 @@ int flexatt_weight_sums(const flexatt_weights* p, const flexatt_tensor* q, const
   FLEXATT_TRY(check_tensor(q, p->dtype));
   FLEXATT_TRY(check_tensor(k, p->dtype));
   if (!lse || !sums) return FLEXATT_EINVAL;
+  // (other workgroups still read the inputs while the sums are written)
+  const Span out = span_of(sums, (size_t)p->batch * p->heads_kv * p->seqlen_kv * 4);
+  for (const Span& in : {span_of(q, p->dtype, p->batch, p->heads_q, p->seqlen_q, p->head_dim),
+                         span_of(k, p->dtype, p->batch, p->heads_kv, p->seqlen_kv, p->head_dim),
+                         span_of(lse, (size_t)p->batch * p->heads_q * p->seqlen_q * 4),
+                         span_of(p->lengths, p->lengths ? (size_t)p->batch * 4 : 0),
+                         span_of(p->query_starts, p->query_starts ? (size_t)p->batch * 4 : 0)})
+    if (overlap(in, out)) return FLEXATT_ELAYOUT;
   const size_t need = flexatt_weight_sums_workspace(p);
   if (need > 0) {
     if (!workspace || workspace_bytes < need) return FLEXATT_EINVAL;

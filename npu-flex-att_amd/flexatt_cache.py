@@ -79,8 +79,9 @@ def attention_weight_sums(query, key, lse, causal=False, query_start=0, lengths=
     ``sliding_window`` W those up to W before it.  With ``lengths`` (int32 [B]) keys
     from ``lengths[b]`` on are left out.  A row with ``lse`` -inf gives no weight.
 
-    ``into`` (fp32 [B, Hkv, Skv], contiguous): the sums are added to it in place, and
-    it is returned; otherwise a new tensor, 0 for keys left out.  Deterministic.
+    ``into`` (fp32 [B, Hkv, Skv], contiguous, apart from the inputs): the sums are added
+    to it in place, and it is returned; otherwise a new tensor, 0 for keys left out.
+    Deterministic.
     """
     return _lib.native().weight_sums(query, key, lse, causal, query_start, lengths, sliding_window, scale, soft_cap, into)
 
