@@ -331,8 +331,8 @@ int flexatt_rotary_apply(const flexatt_rotary* r, const flexatt_tensor* q, const
 
 /* q_out = turned q, and the rows lengths[b] .. lengths[b] + S - 1 of the cache
  * receive turned k and v [B, Hkv, S, D] (q and q_out NULL when heads_q is 0).  A row
- * outside [0, cache_rows) is not written.  `lengths` is not changed.  k and v may not
- * overlap the cache, nor k_cache be v_cache. */
+ * outside [0, cache_rows) is not written.  `lengths` is not changed.  q, q_out, k, v
+ * and lengths may not lie within the span of the cache, nor k_cache be v_cache. */
 int flexatt_rotary_append(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* k,
                           const flexatt_tensor* v, const flexatt_tensor* q_out, const flexatt_tensor* k_cache,
                           const flexatt_tensor* v_cache, int32_t cache_rows, const int32_t* lengths, void* stream);

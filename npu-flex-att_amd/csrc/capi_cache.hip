@@ -261,11 +261,14 @@ int flexatt_rotary_append(const flexatt_rotary* r, const flexatt_tensor* q, cons
   FLEXATT_TRY(check_out_tensor(k_cache, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim));
   FLEXATT_TRY(check_out_tensor(v_cache, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim));
   if (k_cache->data == v_cache->data) return FLEXATT_ELAYOUT;
-  for (const flexatt_tensor* x : {k, v})
+  const auto span = [&](const flexatt_tensor* t, int heads, int rows) {
+    return t ? span_of(t, r->dtype, r->batch, heads, rows, r->head_dim) : Span{};
+  };
+  for (const Span& x : {span(q, r->heads_q, r->seqlen), span(q_out, r->heads_q, r->seqlen),
+                        span(k, r->heads_kv, r->seqlen), span(v, r->heads_kv, r->seqlen),
+                        span_of(lengths, (size_t)r->batch * 4)})
     for (const flexatt_tensor* y : {k_cache, v_cache})
-      if (overlap(span_of(x, r->dtype, r->batch, r->heads_kv, r->seqlen, r->head_dim),
-                  span_of(y, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim)))
-        return FLEXATT_ELAYOUT;
+      if (overlap(x, span(y, r->heads_kv, cache_rows))) return FLEXATT_ELAYOUT;
   RotaryArgs a = rotary_args(r, q, q_out);
   a.k = view(k);
   a.v = view(v);
