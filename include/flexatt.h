@@ -332,7 +332,8 @@ int flexatt_rotary_apply(const flexatt_rotary* r, const flexatt_tensor* q, const
 /* q_out = turned q, and the rows lengths[b] .. lengths[b] + S - 1 of the cache
  * receive turned k and v [B, Hkv, S, D] (q and q_out NULL when heads_q is 0).  A row
  * outside [0, cache_rows) is not written.  `lengths` is not changed.  q, q_out, k, v
- * and lengths may not lie within the span of the cache, nor k_cache be v_cache. */
+ * and lengths may not lie within the span of the cache; k_cache and v_cache may share a
+ * buffer side by side (the same strides), not memory. */
 int flexatt_rotary_append(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* k,
                           const flexatt_tensor* v, const flexatt_tensor* q_out, const flexatt_tensor* k_cache,
                           const flexatt_tensor* v_cache, int32_t cache_rows, const int32_t* lengths, void* stream);
@@ -432,7 +433,8 @@ typedef struct flexatt_evict {
 
 /* scores: contiguous fp32 [B, Hkv, cache_rows]; scores_out [B, Hkv, out_rows];
  * slots int32 [B, Hkv, keep]; lengths_out int32 [B].  No output may
- * lie within the span of an input, nor k_out be v_out. */
+ * lie within the span of an input or of another output; k_out and v_out may share a
+ * buffer side by side (the same strides), not memory. */
 int flexatt_evict_rows(const flexatt_evict* p, const flexatt_tensor* k_cache, const flexatt_tensor* v_cache,
                        const float* scores, const flexatt_tensor* k_out, const flexatt_tensor* v_out,
                        float* scores_out, int32_t* slots, int32_t* lengths_out, void* stream);

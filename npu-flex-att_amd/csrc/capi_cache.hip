@@ -260,7 +260,7 @@ int flexatt_rotary_append(const flexatt_rotary* r, const flexatt_tensor* q, cons
   }
   FLEXATT_TRY(check_out_tensor(k_cache, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim));
   FLEXATT_TRY(check_out_tensor(v_cache, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim));
-  if (k_cache->data == v_cache->data) return FLEXATT_ELAYOUT;
+  FLEXATT_TRY(check_out_pair(k_cache, v_cache, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim));
   const auto span = [&](const flexatt_tensor* t, int heads, int rows) {
     return t ? span_of(t, r->dtype, r->batch, heads, rows, r->head_dim) : Span{};
   };
@@ -385,7 +385,7 @@ int flexatt_evict_rows(const flexatt_evict* p, const flexatt_tensor* k_cache, co
   FLEXATT_TRY(check_tensor(v_cache, p->dtype));
   FLEXATT_TRY(check_out_tensor(k_out, p->dtype, p->batch, p->heads_kv, p->out_rows, p->head_dim));
   FLEXATT_TRY(check_out_tensor(v_out, p->dtype, p->batch, p->heads_kv, p->out_rows, p->head_dim));
-  if (k_out->data == v_out->data) return FLEXATT_ELAYOUT;
+  FLEXATT_TRY(check_out_pair(k_out, v_out, p->dtype, p->batch, p->heads_kv, p->out_rows, p->head_dim));
   const int64_t bh = (int64_t)p->batch * p->heads_kv;
   const Span in[] = {span_of(k_cache, p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim),
                      span_of(v_cache, p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim),
@@ -397,6 +397,9 @@ int flexatt_evict_rows(const flexatt_evict* p, const flexatt_tensor* k_cache, co
   for (const Span& x : in)
     for (const Span& y : out)
       if (overlap(x, y)) return FLEXATT_ELAYOUT;
+  for (int i = 2; i < 5; ++i)
+    for (int j = 0; j < i; ++j)
+      if (overlap(out[i], out[j])) return FLEXATT_ELAYOUT;
   EvictArgs a = {};
   a.k = view(k_cache);
   a.v = view(v_cache);

@@ -47,17 +47,12 @@ inline int check_tensor(const flexatt_tensor* t, int dt) {
   return FLEXATT_OK;
 }
 
-// Output tensors: the input rules, and no two elements of the [b, h, s, d]
-// index space may share an address (several workgroups would store to it,
-// and the results would depend on their order).  Sufficient test: over the
-// dimensions of extent > 1 sorted by stride, each stride exceeds the span of
-// the smaller ones.
-inline int check_out_tensor(const flexatt_tensor* t, int dt, int64_t n_b, int64_t n_h, int64_t n_s, int64_t n_d) {
-  FLEXATT_TRY(check_tensor(t, dt));
-  int64_t st[4] = {t->stride_b, t->stride_h, t->stride_s, 1};
-  int64_t ext[4] = {n_b, n_h, n_s, n_d};
-  int order[4], n = 0;
-  for (int i = 0; i < 4; ++i)
+// No two elements of an index space of up to five dimensions share an address.
+// Sufficient test: over the dimensions of extent > 1 sorted by stride, each stride
+// exceeds the span of the smaller ones.
+inline int check_nested(const int64_t* st, const int64_t* ext, int n_dims) {
+  int order[5], n = 0;
+  for (int i = 0; i < n_dims; ++i)
     if (ext[i] > 1) order[n++] = i;
   for (int i = 1; i < n; ++i)  // insertion sort by stride
     for (int j = i; j > 0 && st[order[j]] < st[order[j - 1]]; --j) {
@@ -72,6 +67,35 @@ inline int check_out_tensor(const flexatt_tensor* t, int dt, int64_t n_b, int64_
     span += (ext[d] - 1) * st[d];
   }
   return FLEXATT_OK;
+}
+
+// Output tensors: the input rules, and no two elements may share an address (several
+// workgroups would store to it, and the results would depend on their order).
+inline int check_out_tensor(const flexatt_tensor* t, int dt, int64_t n_b, int64_t n_h, int64_t n_s, int64_t n_d) {
+  FLEXATT_TRY(check_tensor(t, dt));
+  const int64_t st[4] = {t->stride_b, t->stride_h, t->stride_s, 1}, ext[4] = {n_b, n_h, n_s, n_d};
+  return check_nested(st, ext, 4);
+}
+
+// Two output tensors of one shape that pass check_out_tensor: apart, or, with the same
+// strides, one layout in which the step from one to the other is a dimension of extent 2
+// (keys and values side by side in one buffer).
+inline int check_out_pair(const flexatt_tensor* x, const flexatt_tensor* y, int dt, int64_t n_b, int64_t n_h, int64_t n_s,
+                          int64_t n_d) {
+  const int64_t es = (int64_t)elt_size(dt), ext[5] = {n_b, n_h, n_s, n_d, 2};
+  if ((uintptr_t)x->data > (uintptr_t)y->data) {
+    const flexatt_tensor* z = x;
+    x = y;
+    y = z;
+  }
+  const uintptr_t step = (uintptr_t)y->data - (uintptr_t)x->data;
+  const int64_t last = (n_b - 1) * x->stride_b + (n_h - 1) * x->stride_h + (n_s - 1) * x->stride_s + n_d;
+  if (step >= (uintptr_t)(last * es)) return FLEXATT_OK;
+  const int64_t st[5] = {x->stride_b, x->stride_h, x->stride_s, 1, (int64_t)step / es};
+  const int64_t other[3] = {y->stride_b, y->stride_h, y->stride_s};
+  for (int i = 0; i < 3; ++i)
+    if (ext[i] > 1 && st[i] != other[i]) return FLEXATT_ELAYOUT;
+  return check_nested(st, ext, 5);
 }
 
 inline View view(const flexatt_tensor* t) { return View{t->data, t->stride_b, t->stride_h, t->stride_s}; }

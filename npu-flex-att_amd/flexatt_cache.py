@@ -32,7 +32,8 @@ def rotary_append(query, key, value, key_cache, value_cache, lengths, inv_freq, 
     :func:`flexatt_rotary.rotary_embedding` gives them; ``positions`` (int32 or int64
     [S] or [B, S]) defaults to the rows' numbers.  ``inv_freq=None`` rotates nothing
     and returns a copy of the query.  A row outside the cache is not written.  A query
-    without heads puts keys and values into the cache alone.
+    without heads puts keys and values into the cache alone.  The new tokens, the key
+    cache and the value cache share no memory.
     ``lengths`` is read, not changed.
     """
     return _lib.native().rotary_append(query, key, value, key_cache, value_cache, lengths, inv_freq, positions,
@@ -100,7 +101,7 @@ def evict_cache(key_cache, value_cache, scores, lengths, keep, recent=0, sinks=0
     The new cache has ``keep`` rows, zero behind the last kept one; or ``out=(key,
     value, scores)`` receives it, tensors of one and the same number of rows (at least
     ``keep``, so that the cache can grow again) that share no memory with the old
-    cache.  Rows of ``out``'s key and value behind the last kept one are left as they
+    cache or each other.  Rows of ``out``'s key and value behind the last kept one are left as they
     were; its scores (contiguous fp32) are 0 there.  Lengths outside [0, C] count as
     the nearer end.
     """

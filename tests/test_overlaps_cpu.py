@@ -37,3 +37,36 @@ def test_appended_tokens_lie_apart_from_the_cache(which, cache, end):
     t = {n: tensor(at[n], heads[n], 8) for n in heads}
     c = [tensor(at[n], 2, 100) for n in ("k_cache", "v_cache")]
     assert L.load().flexatt_rotary_append(r, t["q"], t["k"], t["v"], t["q_out"], *c, 100, at["lengths"], None) == -5
+
+
+PAIRS = [
+    # offset of the second tensor in bytes, its strides over the first one's: memory in common
+    (64, (1, 1, 1)), (128, (1, 1, 1)), (16, (1, 1, 1)), (100 * 128 - 128, (1, 1, 1)), (100 * 128, (1, 1, 1)),
+    (2 * 2 * 100 * 128 - 16, (1, 1, 1)), (256, (1, 1, 2)), (3 * 100 * 128, (2, 1, 1)),
+]
+
+
+@pytest.mark.parametrize("offset,times", PAIRS)
+@pytest.mark.parametrize("turn", [False, True])
+def test_keys_and_values_share_no_memory(offset, times, turn):
+    """Two tensors of 2 x 2 x 100 rows of 128 bytes that lie partly on each other, as the append's cache and as eviction's."""
+    a = tensor(1 << 30, 2, 100)
+    b = L.Tensor((1 << 30) + offset, 2 * 6400 * times[0], 6400 * times[1], 64 * times[2], 1)
+    kc, vc = (b, a) if turn else (a, b)
+    r = L.Rotary(L.BF16, 2, 4, 2, 8, 64, 0, 0, 0, 1.0, None, None, 0, 0, 0, 0)
+    q, k = tensor(1 << 24, 4, 8), tensor(1 << 25, 2, 8)
+    assert L.load().flexatt_rotary_append(r, q, k, k, q, kc, vc, 100, 1 << 26, None) == -5
+    e = L.Evict(L.BF16, 2, 2, 300, 64, 100, 8, 4, 100, 0, 1 << 26)
+    c, far = tensor(1 << 24, 2, 300), [1 << 32, 1 << 33, 1 << 34]
+    assert L.load().flexatt_evict_rows(e, c, c, 1 << 27, kc, vc, *far, None) == -5
+
+
+@pytest.mark.parametrize("which,on", [("scores", "key"), ("scores", "value"), ("slots", "scores"), ("slots", "key"),
+                                      ("lengths", "slots"), ("lengths", "scores"), ("lengths", "value")])
+def test_eviction_outputs_share_no_memory(which, on):
+    at = dict(key=1 << 30, value=1 << 31, scores=1 << 32, slots=1 << 33, lengths=1 << 34)
+    at[which] = at[on] + 4 * 100
+    e = L.Evict(L.BF16, 2, 2, 300, 64, 100, 8, 4, 100, 0, 1 << 26)
+    c = tensor(1 << 24, 2, 300)
+    assert L.load().flexatt_evict_rows(e, c, c, 1 << 27, tensor(at["key"], 2, 100), tensor(at["value"], 2, 100),
+                                       at["scores"], at["slots"], at["lengths"], None) == -5
