@@ -11,10 +11,12 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <string>
@@ -79,6 +81,18 @@ int dtype_of(const Tensor& t) {
     case at::kBFloat16: return FLEXATT_BF16;
     default: TORCH_CHECK(false, "unsupported dtype ", t.scalar_type(), " (expected float32, float16 or bfloat16)");
   }
+}
+
+// A trace would record the outputs' allocation but not the kernel that fills them.
+// (torch.compile breaks its graph at these calls and runs them as they are.)
+void no_trace() {
+  bool traced = torch::jit::tracer::isTracing();
+  if (c10::impl::TorchDispatchModeTLS::any_modes_set())
+    for (const auto key : {c10::impl::TorchDispatchModeKey::FAKE, c10::impl::TorchDispatchModeKey::PROXY,
+                           c10::impl::TorchDispatchModeKey::FUNCTIONAL})
+      traced = traced || c10::impl::TorchDispatchModeTLS::get_mode(key).has_value();
+  TORCH_CHECK(!traced, "the rotary and cache calls cannot be traced (make_fx, export, jit.trace, fake tensors): "
+                       "put the call into a torch.library.custom_op");
 }
 
 struct Named {
@@ -213,6 +227,7 @@ flexatt_rotary rotary_struct(const Tensor& q, int64_t hkv, const Tensor& freq, c
 // (query', key'), key' undefined without a key.
 std::pair<Tensor, Tensor> rotate(const Tensor& query, const Tensor& key, const Tensor& freq, const OptTensor& pos,
                                  bool interleaved, double magnitude, bool inverse) {
+  no_trace();  // (a backward pass gets here too)
   const c10::Device dev = query.device();
   const c10::OptionalDeviceGuard guard(dev);
   const bool keyed = key.defined();
@@ -282,6 +297,7 @@ PyObject* pair_of(const Tensor& a, const Tensor& b) {
 PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want(n, 6, "rotary");
+  no_trace();
   const Tensor query = tensor_arg(a[0], "query");
   const OptTensor key = opt_tensor_arg(a[1], "key");
   Tensor freq = tensor_arg(a[2], "inv_freq");
@@ -326,6 +342,7 @@ void check_cache(const Tensor& query, const Tensor& kc, const Tensor& vc) {
 PyObject* py_rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want(n, 10, "rotary_append");
+  no_trace();
   const Tensor query = tensor_arg(a[0], "query"), key = tensor_arg(a[1], "key"), value = tensor_arg(a[2], "value");
   const Tensor kc = tensor_arg(a[3], "key_cache"), vc = tensor_arg(a[4], "value_cache");
   Tensor lengths = tensor_arg(a[5], "lengths");
@@ -382,6 +399,7 @@ ScoreParams score_params(PyObject* scale, PyObject* cap, PyObject* window, int64
 PyObject* py_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want(n, 10, "tree_attention");
+  no_trace();
   const Tensor query = tensor_arg(a[0], "query");
   const Tensor kc = tensor_arg(a[1], "key_cache"), vc = tensor_arg(a[2], "value_cache");
   Tensor lengths = tensor_arg(a[3], "lengths");
@@ -455,6 +473,7 @@ PyObject* py_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_weight_sums(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want(n, 10, "weight_sums");
+  no_trace();
   const Tensor query = tensor_arg(a[0], "query"), key = tensor_arg(a[1], "key");
   FLEXATT_ASSERT(THPVariable_Check(a[2]), "lse must be [B, Hq, Sq]");
   Tensor lse = THPVariable_Unpack(a[2]);
@@ -530,6 +549,7 @@ PyObject* py_weight_sums(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want(n, 10, "evict");
+  no_trace();
   const Tensor kc = tensor_arg(a[0], "key_cache"), vc = tensor_arg(a[1], "value_cache");
   Tensor scores = tensor_arg(a[2], "scores"), lengths = tensor_arg(a[3], "lengths");
   const bool fresh = a[7] == Py_None;

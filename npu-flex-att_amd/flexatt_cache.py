@@ -13,7 +13,8 @@ device, so every call can be captured into a graph and replayed as the cache gro
   evict_cache(...)            the rows worth keeping, copied to a smaller cache
 
 None of them is differentiable: a tensor that carries a tangent, or with gradients
-on one that requires them, is refused.
+on one that requires them, is refused.  Nor can they be traced (``make_fx``, export,
+fake tensors); ``torch.compile`` breaks its graph at them.
 """
 from __future__ import annotations
 

@@ -88,5 +88,7 @@ def rotary_embedding(query, key, inv_freq, positions=None, interleaved=False, ma
     backward pass may be captured into a graph, as any of torch's, while no eager graph
     of the same leaves is alive.  Small calls wait for autograd's hand-over to its device
     thread; inside ``torch.autograd.set_multithreading_enabled(False)`` there is none.
+    Not traceable (``make_fx``, export, fake tensors); ``torch.compile`` breaks its graph
+    here.
     """
     return _lib.native().rotary(query, key, inv_freq, positions, interleaved, magnitude)
