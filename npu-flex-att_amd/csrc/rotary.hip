@@ -10,9 +10,9 @@
 //
 // The angle is formed in 64 bits and reduced to quarter turns there: at position
 // 100000 an fp32 product is off by up to 2^-24 * 100000 = 0.006 radians.  What is
-// left of it, within an eighth of a turn, goes through the Taylor series of sine
-// and cosine in 32 bits (first terms left out: x^11/11! and x^10/10!, under 3e-8
-// at pi/4).
+// left of it, within an eighth of a turn, is rounded to 32 bits and goes through the
+// Taylor series of sine and cosine there (first terms left out: x^11/11! and x^12/12!,
+// under 2e-9 at pi/4, where a half step is 3e-8).
 //
 // Bound by memory: each element is read and written once.  A thread keeps the
 // sines of its 2 x 16 bytes of one token and walks over heads, so the angles cost
@@ -34,12 +34,13 @@ constexpr int kRows = 4;  // heads loaded before the first is stored
 __device__ __forceinline__ void turn_of(double pos, double freq, float mag, float sgn, float& c, float& s) {
   const double q = pos * (freq * 0.63661977236758134308);  // quarter turns: freq / (pi / 2)
   const double n = __builtin_rint(q);
-  const float x = (float)(q - n) * 1.57079632679489662f;  // |x| <= pi/4
+  // |x| <= pi/4 (pi / 2 in 32 bits is off by 3e-8 of itself)
+  const float x = (float)((q - n) * 1.57079632679489661923);
   // n mod 4 without leaving 64 bits, for any n a double holds
   const int k = (int)(n - 4.0 * __builtin_floor(n * 0.25));
   const float z = x * x;
   const float sp = x + x * z * (-1.0f / 6 + z * (1.0f / 120 + z * (-1.0f / 5040 + z * (1.0f / 362880))));
-  const float cp = 1.0f + z * (-0.5f + z * (1.0f / 24 + z * (-1.0f / 720 + z * (1.0f / 40320))));
+  const float cp = 1.0f + z * (-0.5f + z * (1.0f / 24 + z * (-1.0f / 720 + z * (1.0f / 40320 + z * (-1.0f / 3628800)))));
   const float a = (k & 1) ? sp : cp, b = (k & 1) ? cp : sp;
   c = ((k == 1 || k == 2) ? -a : a) * mag;
   s = ((k & 2) ? -b : b) * (mag * sgn);
