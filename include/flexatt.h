@@ -308,7 +308,8 @@ typedef struct flexatt_rotary {
   int32_t batch;        /* B */
   int32_t heads_q;      /* Hq >= 1; in flexatt_rotary_append also 0: no q */
   int32_t heads_kv;     /* Hkv >= 0; 0: no k */
-  int32_t seqlen;       /* S, new tokens per sequence */
+  int32_t seqlen;       /* S, new tokens per sequence (FLEXATT_ERANGE: more than a launch has work-items,
+                         * 2^32 - 1, of which B S D / 2 are taken at most) */
   int32_t head_dim;     /* D in {32, 64, 128, 256} */
   int32_t rotary_dim;   /* even, 0 .. D; 0: nothing is turned and inv_freq may be NULL */
   int32_t interleaved;  /* 1: neighbouring elements are pairs */
@@ -383,7 +384,8 @@ int flexatt_tree_fwd(const flexatt_tree* p, const flexatt_tensor* q, const flexa
  * of sequence b is at position start + i, start = query_starts[b] (NULL:
  * query_start); causal keeps j <= start + i, a window start + i - j <= W.  Keys
  * from lengths[b] on (NULL: seqlen_kv; values outside [0, seqlen_kv] count as the
- * nearer end) get 0, with `accumulate` nothing. */
+ * nearer end) get 0, with `accumulate` nothing.  FLEXATT_ERANGE: more blocks of 256 keys
+ * (of 128 with rows of 1 KB), B Hkv of each, than a launch has workgroups, 2^24 - 1. */
 typedef struct flexatt_weights {
   int32_t dtype;
   int32_t batch;
@@ -416,7 +418,7 @@ int flexatt_weight_sums(const flexatt_weights* p, const flexatt_tensor* q, const
  * first rows of k_out and v_out, their scores to scores_out, their rows' numbers
  * to slots (-1 behind), and min(n, keep) to lengths_out.  Rows of k_out and v_out
  * behind them are left as they were, or with `fill` zeroed up to row keep - 1;
- * scores_out is 0 behind them. */
+ * scores_out is 0 behind them.  FLEXATT_ERANGE: B Hkv of 2^24 or more. */
 typedef struct flexatt_evict {
   int32_t dtype;
   int32_t batch;

@@ -42,7 +42,9 @@ int check_rotary(const flexatt_rotary* r, bool append) {
   if (r->positions ? r->position_bytes != 4 && r->position_bytes != 8 : r->position_bytes != 0) return FLEXATT_EINVAL;
   if (((uintptr_t)r->inv_freq) % 8 || (r->positions && ((uintptr_t)r->positions) % r->position_bytes))
     return FLEXATT_ELAYOUT;
-  return FLEXATT_OK;
+  // (a thread has 16 bytes of each half of a token's pairs, or one pair of them; rotary.hip)
+  const int es = (int)elt_size(r->dtype), units = r->rotary_dim * es % 32 == 0 ? r->head_dim * es / 32 : r->head_dim / 2;
+  return check_launch(((int64_t)r->batch * r->seqlen * units + 255) / 256, 256);
 }
 
 RotaryArgs rotary_args(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* qo) {
@@ -165,6 +167,9 @@ TreePlan tree_plan(const flexatt_tree* p) {
 }
 size_t tree_rows(const flexatt_tree* p) { return (size_t)p->batch * p->heads_q * p->tokens; }
 
+// Keys of a workgroup of the weight sums (WsCfg).
+int weight_keys(const flexatt_weights* p) { return p->head_dim * (int)elt_size(p->dtype) <= 512 ? 256 : 128; }
+
 int check_weights(const flexatt_weights* p) {
   if (!p) return FLEXATT_EINVAL;
   FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_q, p->seqlen_q, p->head_dim));
@@ -173,7 +178,9 @@ int check_weights(const flexatt_weights* p) {
   if ((int64_t)(p->heads_q / p->heads_kv) * p->seqlen_q > 1 << 30) return FLEXATT_ESHAPE;
   FLEXATT_TRY(check_scores(p->scale, p->soft_cap, p->sliding_window));
   if ((p->causal & ~1) || (p->accumulate & ~1) || p->reserved != 0) return FLEXATT_EINVAL;
-  return FLEXATT_OK;
+  // (a workgroup per block of keys; where there are that many its rows are not shared)
+  const int keys = weight_keys(p);
+  return check_launch((int64_t)p->batch * p->heads_kv * ((p->seqlen_kv + keys - 1) / keys), 256);
 }
 
 // Which blocks of keys a workgroup has, one or a pair (the second from the other end,
@@ -189,7 +196,7 @@ struct WeightPlan {
 };
 WeightPlan weight_plan(const flexatt_weights* p) {
   const int rowb = p->head_dim * (int)elt_size(p->dtype);
-  const int keys = rowb <= 512 ? 256 : 128;  // (WsCfg)
+  const int keys = weight_keys(p);
   const int64_t nkb = (p->seqlen_kv + keys - 1) / keys;
   const int64_t bh = (int64_t)p->batch * p->heads_kv, slots = (rowb >= 512 ? 1 : 2) * cus();
   // the row tiles that see block x (starts on the device: as if the rows were the last)
@@ -380,6 +387,7 @@ int flexatt_evict_rows(const flexatt_evict* p, const flexatt_tensor* k_cache, co
   if (p->keep < 1 || p->recent < 0 || p->sinks < 0 || p->out_rows < p->keep || (p->fill & ~1)) return FLEXATT_EINVAL;
   if ((int64_t)p->recent + p->sinks > p->keep) return FLEXATT_EINVAL;
   FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_kv, p->out_rows, p->head_dim));
+  FLEXATT_TRY(check_launch((int64_t)p->batch * p->heads_kv, p->cache_rows <= 2048 ? 256 : 1024));  // (evict_run)
   if (!p->lengths || !scores || !scores_out || !slots || !lengths_out) return FLEXATT_EINVAL;
   FLEXATT_TRY(check_tensor(k_cache, p->dtype));
   FLEXATT_TRY(check_tensor(v_cache, p->dtype));

@@ -98,6 +98,11 @@ inline int check_out_pair(const flexatt_tensor* x, const flexatt_tensor* y, int 
   return check_nested(st, ext, 5);
 }
 
+// A launch has at most 2^32 - 1 work-items.
+inline int check_launch(int64_t workgroups, int threads) {
+  return workgroups <= (((int64_t)1 << 32) - 1) / threads ? FLEXATT_OK : FLEXATT_ERANGE;
+}
+
 inline View view(const flexatt_tensor* t) { return View{t->data, t->stride_b, t->stride_h, t->stride_s}; }
 inline MutView mview(const flexatt_tensor* t) { return MutView{t->data, t->stride_b, t->stride_h, t->stride_s}; }
 
