@@ -187,8 +187,8 @@ int check_weights(const flexatt_weights* p) {
 // which under a causal mask evens out the work), and how many workgroups share their
 // query rows: what takes the fewest rounds of workgroups (two per CU, one with rows of
 // 512 bytes) times their row tiles, a block counted as some five more to load and add up.
-// (bf16 B=2 Hq=32 Hkv=8 S=4096 D=128 causal, 128 pairs: 4 parts 162 us, 6 and 8 167, 12
-// 175, 16 177.  Blocks alone where they leave CUs idle: bf16 Hq=32 Hkv=8 D=128, 1 row over
+// (In one run, bf16 B=2 Hq=32 Hkv=8 S=4096 D=128 causal, 128 pairs: 4 parts 162 us, 6 and
+// 8 167, 12 175, 16 177.  Blocks alone where they leave CUs idle: bf16 Hq=32 Hkv=8 D=128, 1 row over
 // 700 keys 11.7 -> 7.4 us, fp32 Hq=8 Hkv=1 D=256, 5 over 2803 30 -> 16; pairs where they
 // do not: bf16 B=3, 32 heads, 1 row over 19106 keys 122 -> 115 us.)
 struct WeightPlan {

@@ -39,7 +39,7 @@
 // cold and runs most of this code once, at about one cycle a byte, so what is outside
 // the tile loop is kept short (16-byte LDS accesses in the combine, rolled loops).
 //   bf16 B=8 Hq=32 Hkv=8 T=16, caches of 24576 to 32768, D=128: 181 us, 5.2 TB/s
-//   bf16 B=2 Hq=16 Hkv=8 T=16, window 4096, D=256: 24 us (the merge 4.7), 2.8 TB/s
+//   bf16 B=2 Hq=16 Hkv=8 T=16, window 4096, soft-cap 50, D=256: 25 us (the merge 4.8), 2.7 TB/s
 //   fp16 B=4 Hq=28 Hkv=4 T=64, caches up to 16384, D=64: 52 us, 0.52 PFLOP/s
 //   fp16 B=3 Hq=28 Hkv=4 T=64, caches of 20000, D=128: 87 us, 0.63 PFLOP/s
 //   bf16 B=1 Hq=32 Hkv=8 T=8, a cache of 4097, D=128: 14 us (9.5 and the merge 4.6)

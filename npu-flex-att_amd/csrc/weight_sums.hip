@@ -23,7 +23,7 @@
 // What bounds it: per 32 x 32 pairs and SIMD the MFMAs are 2 D cycles (16-bit types),
 // one fma, one exponential (half the rate) and one add an element 256 cycles of VALU, at
 // the clock that the MFMAs' power leaves (1.9 GHz; zeros instead of numbers are 15%
-// faster).  bf16 B=2 Hq=32 Hkv=8 S=4096 D=128 causal: 162 us, 0.85 PFLOP/s beside 3.3e12
+// faster).  bf16 B=2 Hq=32 Hkv=8 S=4096 D=128 causal: 161 us, 0.85 PFLOP/s beside 3.3e12
 // exponentials a second; without the exponentials it would be 142, without masks 151,
 // without the copies of new tiles 150, without the LDS reads 158.  fp16 B=4 Hq=28 Hkv=4,
 // 32 rows over 16383 keys, D=64: 22 us.

@@ -6,6 +6,9 @@ A cache is a pair of [B, Hkv, C, D] tensors (any strides a kernel can read in
 place: innermost stride 1, rows on 16-byte boundaries) with ``lengths``, int32 [B]
 on the device: the rows of each sequence that are in use.  ``lengths`` stays on the
 device, so every call can be captured into a graph and replayed as the cache grows.
+A cache of other strides is refused where it is written; where it is only read, the
+call copies it whole, every time (tree_attention also one with rows 64 MB or more
+apart).
 
   rotary_append(...)          query' and the cache rows of new tokens, in one kernel
   tree_attention(...)         drafted tokens (or one new token) over cache and tree
@@ -102,8 +105,8 @@ def evict_cache(key_cache, value_cache, scores, lengths, keep, recent=0, sinks=0
     The new cache has ``keep`` rows, zero behind the last kept one; or ``out=(key,
     value, scores)`` receives it, tensors of one and the same number of rows (at least
     ``keep``, so that the cache can grow again) that share no memory with the old
-    cache or each other.  Rows of ``out``'s key and value behind the last kept one are left as they
-    were; its scores (contiguous fp32) are 0 there.  Lengths outside [0, C] count as
+    cache or each other.  Rows of ``out``'s key and value behind the last kept one are
+    left as they were; its scores (contiguous fp32) are 0 there.  Lengths outside [0, C] count as
     the nearer end.
     """
     key, value, kept = (None, None, None) if out is None else out
