@@ -441,13 +441,89 @@ int flexatt_evict_rows(const flexatt_evict* p, const flexatt_tensor* k_cache, co
                        const float* scores, const flexatt_tensor* k_out, const flexatt_tensor* v_out,
                        float* scores_out, int32_t* slots, int32_t* lengths_out, void* stream);
 
+/* Queries and keys normalised for each head, then turned: y = R (x w / sqrt(mean x^2 +
+ * eps)), the mean over the head's D elements in 32 bits, R the rotation of
+ * flexatt_rotary (inverse 0).  Rounded once. */
+typedef struct flexatt_norm {
+  int32_t weight_dtype; /* FLEXATT_F32, or the call's dtype */
+  float eps;            /* a normal number above 0 */
+  const void* q_weight; /* device [D]; NULL when heads_q is 0 */
+  const void* k_weight; /* device [D]; NULL when heads_kv is 0 */
+} flexatt_norm;
+
+/* As flexatt_rotary_apply.  An output may be its own input. */
+int flexatt_norm_rotary_apply(const flexatt_rotary* r, const flexatt_norm* n, const flexatt_tensor* q,
+                              const flexatt_tensor* k, const flexatt_tensor* q_out, const flexatt_tensor* k_out,
+                              void* stream);
+
+/* Its gradients: dq, dk and the weights' (device [D] of weight_dtype, sums over all rows
+ * in 32 bits) from q, k and the gradients of q_out and k_out.  k, k_grad, dk and dk_weight
+ * are NULL when heads_kv is 0.  `workspace` as in flexatt_tree_fwd. */
+size_t flexatt_norm_rotary_grad_workspace(const flexatt_rotary* r);
+int flexatt_norm_rotary_grad(const flexatt_rotary* r, const flexatt_norm* n, const flexatt_tensor* q,
+                             const flexatt_tensor* k, const flexatt_tensor* q_grad, const flexatt_tensor* k_grad,
+                             const flexatt_tensor* dq, const flexatt_tensor* dk, void* dq_weight, void* dk_weight,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* As flexatt_rotary_append. */
+int flexatt_norm_rotary_append(const flexatt_rotary* r, const flexatt_norm* n, const flexatt_tensor* q,
+                               const flexatt_tensor* k, const flexatt_tensor* v, const flexatt_tensor* q_out,
+                               const flexatt_tensor* k_cache, const flexatt_tensor* v_cache, int32_t cache_rows,
+                               const int32_t* lengths, void* stream);
+
+/* Caches of 8 bits.  A row (one position of one head) is D codes and one fp32 scale s =
+ * max(amax, 2^-100) / top, of its values' largest size amax and the largest code top:
+ * codes are y / s to the nearest, of two the even one, and stand for code * s.  The values
+ * are rounded nowhere before.  A row with an infinity or NaN has codes 0 and scale NaN.
+ * Code tensors are [B, Hkv, cache_rows, D] views of bytes (strides in bytes, multiples of
+ * 16), scales contiguous fp32 [B, Hkv, cache_rows]. */
+enum flexatt_code {
+  FLEXATT_E4M3 = 1, /* fp8, 4 bits of exponent, 3 of mantissa, no infinity; top 448 */
+  FLEXATT_INT8 = 2  /* top 127 */
+};
+
+/* flexatt_rotary_append, or with a norm (n, may be NULL) flexatt_norm_rotary_append, into
+ * such a cache; q_out is of the call's dtype.  The cache and its scales lie apart from
+ * each other (k_cache and v_cache may share a buffer side by side) and from the rest. */
+int flexatt_quant_append(const flexatt_rotary* r, const flexatt_norm* n, int32_t code, const flexatt_tensor* q,
+                         const flexatt_tensor* k, const flexatt_tensor* v, const flexatt_tensor* q_out,
+                         const flexatt_tensor* k_cache, const flexatt_tensor* v_cache, float* k_scales,
+                         float* v_scales, int32_t cache_rows, const int32_t* lengths, void* stream);
+
+/* The values of the first lengths[b] rows (clamped to [0, cache_rows]) of such a cache,
+ * rounded to dtype, into k_out and v_out [B, Hkv, cache_rows, D]; the rows behind them are
+ * left as they were, or with `fill` zeroed.  FLEXATT_ERANGE: more than a launch has
+ * work-items. */
+typedef struct flexatt_dequant {
+  int32_t dtype;
+  int32_t code;       /* enum flexatt_code */
+  int32_t batch;
+  int32_t heads_kv;
+  int32_t cache_rows;
+  int32_t head_dim;
+  int32_t fill;
+  int32_t reserved;   /* 0 */
+  const int32_t* lengths; /* device int32 [B] */
+} flexatt_dequant;
+int flexatt_dequant_rows(const flexatt_dequant* p, const flexatt_tensor* k_cache, const flexatt_tensor* v_cache,
+                         const float* k_scales, const float* v_scales, const flexatt_tensor* k_out,
+                         const flexatt_tensor* v_out, void* stream);
+
+/* flexatt_tree_fwd over such a cache, for dtype fp16 and bf16 (else FLEXATT_EDTYPE).  The
+ * scores are q . code times the key's scale; weights times the values' scales are rounded
+ * to dtype for the second product. */
+size_t flexatt_quant_tree_fwd_workspace(const flexatt_tree* p);
+int flexatt_quant_tree_fwd(const flexatt_tree* p, int32_t code, const flexatt_tensor* q, const flexatt_tensor* k_cache,
+                           const flexatt_tensor* v_cache, const float* k_scales, const float* v_scales,
+                           const flexatt_tensor* o, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Human-readable text for a status code (static storage). */
 const char* flexatt_status_string(int status);
 
 /* ABI version of this header (bumped on any signature change). */
 int flexatt_abi_version(void);
 
-#define FLEXATT_ABI_VERSION 9
+#define FLEXATT_ABI_VERSION 10
 
 #ifdef __cplusplus
 }

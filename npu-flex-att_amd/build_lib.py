@@ -21,8 +21,9 @@ LIB = os.path.join(HERE, "libflexatt.so")
 NATIVE = os.path.join(HERE, "flexatt_native.so")  # linked against libflexatt.so beside it
 HEAD_DIMS = (32, 64, 128, 256)
 PER_D_SOURCES = ("fwd_mfma.hip", "fwd_ws.hip", "fwd_split.hip", "bwd_mfma.hip", "bwd_kv.hip", "bwd_q.hip", "bwd_dq_ds.hip",
-                  "bwd_split.hip", "f32_mfma.hip", "f32_split.hip", "tree_attn.hip", "weight_sums.hip")
-SINGLE_SOURCES = ("delta.hip", "doc_bounds.hip", "rotary.hip", "evict.hip", "capi.hip", "capi_cache.hip")
+                  "bwd_split.hip", "f32_mfma.hip", "f32_split.hip", "tree_attn.hip", "weight_sums.hip",
+                  "norm_rotary.hip", "quant_attn.hip")
+SINGLE_SOURCES = ("delta.hip", "doc_bounds.hip", "rotary.hip", "evict.hip", "dequant.hip", "capi.hip", "capi_cache.hip")
 # Sources whose kernels load into registers through asm that the compiler
 # does not know is in flight (load16_async): a VGPR spill could store or
 # reuse such a register before its load lands, so their kernels must build

@@ -1,5 +1,6 @@
 // extern "C" entry points around positions and the K/V cache (declared in
 // include/flexatt.h): argument checks, then the kernel launchers.
+#include <float.h>
 #include <math.h>
 #include <stdint.h>
 
@@ -14,9 +15,12 @@ using namespace flexatt;
 struct Span {
   uintptr_t lo, hi;
 };
-Span span_of(const flexatt_tensor* t, int dt, int64_t n_b, int64_t n_h, int64_t n_s, int64_t n_d) {
+Span span_bytes(const flexatt_tensor* t, int64_t es, int64_t n_b, int64_t n_h, int64_t n_s, int64_t n_d) {
   const int64_t last = (n_b - 1) * t->stride_b + (n_h - 1) * t->stride_h + (n_s - 1) * t->stride_s + n_d;
-  return Span{(uintptr_t)t->data, (uintptr_t)t->data + (uintptr_t)(last * (int64_t)elt_size(dt))};
+  return Span{(uintptr_t)t->data, (uintptr_t)t->data + (uintptr_t)(last * es)};
+}
+Span span_of(const flexatt_tensor* t, int dt, int64_t n_b, int64_t n_h, int64_t n_s, int64_t n_d) {
+  return span_bytes(t, (int64_t)elt_size(dt), n_b, n_h, n_s, n_d);
 }
 Span span_of(const void* p, size_t bytes) { return Span{(uintptr_t)p, (uintptr_t)p + bytes}; }
 bool overlap(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
@@ -68,6 +72,78 @@ RotaryArgs rotary_args(const flexatt_rotary* r, const flexatt_tensor* q, const f
   a.mag = r->magnitude;
   a.sign = r->inverse ? -1.0f : 1.0f;
   a.heads = r->heads_q + r->heads_kv;
+  return a;
+}
+
+int check_norm(const flexatt_rotary* r, const flexatt_norm* n) {
+  if (!n) return FLEXATT_EINVAL;
+  if (n->weight_dtype != FLEXATT_F32 && n->weight_dtype != r->dtype) return FLEXATT_EDTYPE;
+  if (!(n->eps >= FLT_MIN) || !isfinite(n->eps) || r->inverse) return FLEXATT_EINVAL;
+  if ((r->heads_q > 0) != (n->q_weight != nullptr) || (r->heads_kv > 0) != (n->k_weight != nullptr)) return FLEXATT_EINVAL;
+  for (const void* w : {n->q_weight, n->k_weight})
+    if ((uintptr_t)w % elt_size(n->weight_dtype)) return FLEXATT_ELAYOUT;
+  return FLEXATT_OK;
+}
+
+NormRotaryArgs norm_args(const RotaryArgs& r, const flexatt_norm* n) {
+  NormRotaryArgs a = {};
+  a.r = r;
+  if (n) {
+    a.norm = 1;
+    a.wq = n->q_weight;
+    a.wk = n->k_weight;
+    a.w_wide = n->weight_dtype == FLEXATT_F32;
+    a.eps = n->eps;
+  }
+  return a;
+}
+
+// [head index]
+const NormRotaryLauncher kNorm[4] = {norm_rotary_d32, norm_rotary_d64, norm_rotary_d128, norm_rotary_d256};
+const NormRotaryLauncher kNormGrad[4] = {norm_rotary_grad_d32, norm_rotary_grad_d64, norm_rotary_grad_d128,
+                                         norm_rotary_grad_d256};
+
+bool is_code(int32_t code) { return code == FLEXATT_E4M3 || code == FLEXATT_INT8; }
+
+// The new tokens' tensors of an append, apart from the cache: `row`: bytes of an element
+// of the cache's.
+int check_append(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* k, const flexatt_tensor* v,
+                 const flexatt_tensor* q_out, const flexatt_tensor* k_cache, const flexatt_tensor* v_cache, int64_t row,
+                 int32_t cache_rows, const int32_t* lengths) {
+  if (r->heads_kv == 0 || cache_rows <= 0 || !lengths) return FLEXATT_EINVAL;
+  if ((int64_t)r->batch * r->heads_kv * cache_rows > INT32_MAX) return FLEXATT_ESHAPE;
+  FLEXATT_TRY(check_tensor(k, r->dtype));
+  FLEXATT_TRY(check_tensor(v, r->dtype));
+  if (r->heads_q > 0) {
+    FLEXATT_TRY(check_tensor(q, r->dtype));
+    FLEXATT_TRY(check_out_tensor(q_out, r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
+  } else if (q || q_out) {
+    return FLEXATT_EINVAL;
+  }
+  FLEXATT_TRY(check_out_view(k_cache, row, r->batch, r->heads_kv, cache_rows, r->head_dim));
+  FLEXATT_TRY(check_out_view(v_cache, row, r->batch, r->heads_kv, cache_rows, r->head_dim));
+  FLEXATT_TRY(check_out_views(k_cache, v_cache, row, r->batch, r->heads_kv, cache_rows, r->head_dim));
+  const auto span = [&](const flexatt_tensor* t, int heads) {
+    return t ? span_of(t, r->dtype, r->batch, heads, r->seqlen, r->head_dim) : Span{};
+  };
+  for (const Span& x : {span(q, r->heads_q), span(q_out, r->heads_q), span(k, r->heads_kv), span(v, r->heads_kv),
+                        span_of(lengths, (size_t)r->batch * 4)})
+    for (const flexatt_tensor* y : {k_cache, v_cache})
+      if (overlap(x, span_bytes(y, row, r->batch, r->heads_kv, cache_rows, r->head_dim))) return FLEXATT_ELAYOUT;
+  return FLEXATT_OK;
+}
+
+RotaryArgs append_args(const flexatt_rotary* r, const flexatt_tensor* q, const flexatt_tensor* k, const flexatt_tensor* v,
+                       const flexatt_tensor* q_out, const flexatt_tensor* k_cache, const flexatt_tensor* v_cache,
+                       int32_t cache_rows, const int32_t* lengths) {
+  RotaryArgs a = rotary_args(r, q, q_out);
+  a.k = view(k);
+  a.v = view(v);
+  a.ko = mview(k_cache);
+  a.vo = mview(v_cache);
+  a.cache_rows = cache_rows;
+  a.lengths = lengths;
+  a.heads += r->heads_kv;
   return a;
 }
 
@@ -123,6 +199,17 @@ int check_tree(const flexatt_tree* p) {
   return FLEXATT_OK;
 }
 
+int check_quant_tree(const flexatt_tree* p) {
+  FLEXATT_TRY(check_tree(p));
+  return p->dtype == FLEXATT_F32 ? FLEXATT_EDTYPE : FLEXATT_OK;
+}
+
+// [fp16, bf16][head index]
+const QuantTreeLauncher kQuantTree[2][4] = {
+    {quant_attn_f16_d32, quant_attn_f16_d64, quant_attn_f16_d128, quant_attn_f16_d256},
+    {quant_attn_bf16_d32, quant_attn_bf16_d64, quant_attn_bf16_d128, quant_attn_bf16_d256},
+};
+
 // How the key tiles are cut (tree_chunk, on the device, where the lengths are): into
 // about as many chunks as workgroups run at once, of eight tiles at least (two per wave;
 // of 4 or 16 changes a short cache's 15 us by less than 0.2).  Rows of 256 bytes and more
@@ -134,16 +221,15 @@ int check_tree(const flexatt_tree* p) {
 struct TreePlan {
   int slots, nchunk, min_tiles, nsplit;
 };
-TreePlan tree_plan(const flexatt_tree* p) {
+int64_t row_tiles(const flexatt_tree* p) { return ((int64_t)(p->heads_q / p->heads_kv) * p->tokens + 31) / 32; }
+// `share`: row tiles of a workgroup; `per_cu`: workgroups that fit a CU.
+TreePlan plan_of(const flexatt_tree* p, int share, int per_cu) {
   TreePlan t;
-  const int rowb = p->head_dim * (int)elt_size(p->dtype);
-  const int64_t rt = ((int64_t)(p->heads_q / p->heads_kv) * p->tokens + 31) / 32;
-  const int share = tree_share(rowb, (int)elt_size(p->dtype), rt);
-  const int64_t groups = (rt + share - 1) / share;
+  const int64_t groups = (row_tiles(p) + share - 1) / share;
   // a chunk's row tiles are on one of the 8 XCDs (tree_attn_kernel): whole chunks of each
   // (fp32 B=2 Hq=8 Hkv=2 T=53 caches of 22374 D=128, 7 row tiles: 36 chunks, five on some
   // XCDs for 32 CUs, 192 us, 32 chunks 117)
-  const int64_t fit = (rowb >= 256 ? 1 : 2) * cus(), slots = groups <= fit / 8 ? fit / 8 / groups * 8 : fit / groups;
+  const int64_t fit = per_cu * cus(), slots = groups <= fit / 8 ? fit / 8 / groups * 8 : fit / groups;
   const int64_t bh = (int64_t)p->batch * p->heads_kv, tiles = (p->cache_rows + 31) / 32;
   // a cache of up to 512 rows whole: what the chunks save the merge costs (bf16 B=1 Hq=32
   // Hkv=8 T=8 D=128, 500 rows 13.4 -> 11.3 us, 1000 rows 14.0 -> 14.9; fp32 D=64, 500 rows
@@ -165,7 +251,54 @@ TreePlan tree_plan(const flexatt_tree* p) {
   t.nchunk = (int)n;
   return t;
 }
+TreePlan tree_plan(const flexatt_tree* p) {
+  const int rowb = p->head_dim * (int)elt_size(p->dtype);
+  return plan_of(p, tree_share(rowb, (int)elt_size(p->dtype), row_tiles(p)), rowb >= 256 ? 1 : 2);
+}
+TreePlan quant_plan(const flexatt_tree* p) {
+  const int share = quant_row_tiles(p->head_dim, row_tiles(p));
+  return plan_of(p, share, p->head_dim >= 128 || share > 1 ? 1 : 2);
+}
 size_t tree_rows(const flexatt_tree* p) { return (size_t)p->batch * p->heads_q * p->tokens; }
+
+size_t plan_bytes(const flexatt_tree* p, const TreePlan& plan) {
+  const int ns = plan.nsplit;
+  if (ns == 1) return 0;
+  return tree_rows(p) * ns * (p->head_dim + 1) * sizeof(float) + (size_t)p->batch * p->heads_kv * sizeof(int);
+}
+
+// The workspace and score parameters of a call whose tensors are set.
+TreeArgs tree_args(const flexatt_tree* p, const TreePlan& plan, const flexatt_tensor* q, const flexatt_tensor* k_cache,
+                   const flexatt_tensor* v_cache, const flexatt_tensor* o, float* lse, void* workspace) {
+  TreeArgs a = {};
+  a.q = view(q);
+  a.k = view(k_cache);
+  a.v = view(v_cache);
+  a.o = mview(o);
+  a.lse = lse;
+  a.slots = plan.slots;
+  a.nchunk = plan.nchunk;
+  a.min_tiles = plan.min_tiles;
+  a.nsplit = plan.nsplit;
+  if (a.nsplit > 1) {
+    a.part_o = (float*)workspace;
+    a.part_lse = a.part_o + tree_rows(p) * a.nsplit * p->head_dim;
+    a.counts = (int*)(a.part_lse + tree_rows(p) * a.nsplit);
+  }
+  a.lengths = p->lengths;
+  a.mask = p->tree_mask;
+  a.mask_sb = p->mask_batch > 1 ? (int64_t)p->tokens * p->tokens : 0;
+  a.depths = p->depths;
+  a.p = score_shape(p->batch, p->heads_q, p->heads_kv, p->tokens, p->cache_rows, p->scale, p->soft_cap,
+                    p->sliding_window);
+  return a;
+}
+
+int check_workspace(size_t need, const void* workspace, size_t bytes) {
+  if (need == 0) return FLEXATT_OK;
+  if (!workspace || bytes < need) return FLEXATT_EINVAL;
+  return (uintptr_t)workspace % 16 != 0 ? FLEXATT_ELAYOUT : FLEXATT_OK;
+}
 
 // Keys of a workgroup of the weight sums (WsCfg).
 int weight_keys(const flexatt_weights* p) { return p->head_dim * (int)elt_size(p->dtype) <= 512 ? 256 : 128; }
@@ -255,43 +388,147 @@ int flexatt_rotary_append(const flexatt_rotary* r, const flexatt_tensor* q, cons
                           const flexatt_tensor* v, const flexatt_tensor* q_out, const flexatt_tensor* k_cache,
                           const flexatt_tensor* v_cache, int32_t cache_rows, const int32_t* lengths, void* stream) {
   FLEXATT_TRY(check_rotary(r, true));
-  if (r->heads_kv == 0 || cache_rows <= 0 || !lengths) return FLEXATT_EINVAL;
-  if ((int64_t)r->batch * r->heads_kv * cache_rows > INT32_MAX) return FLEXATT_ESHAPE;
-  FLEXATT_TRY(check_tensor(k, r->dtype));
-  FLEXATT_TRY(check_tensor(v, r->dtype));
-  if (r->heads_q > 0) {
-    FLEXATT_TRY(check_tensor(q, r->dtype));
-    FLEXATT_TRY(check_out_tensor(q_out, r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
-  } else if (q || q_out) {
-    return FLEXATT_EINVAL;
-  }
-  FLEXATT_TRY(check_out_tensor(k_cache, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim));
-  FLEXATT_TRY(check_out_tensor(v_cache, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim));
-  FLEXATT_TRY(check_out_pair(k_cache, v_cache, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim));
-  const auto span = [&](const flexatt_tensor* t, int heads, int rows) {
-    return t ? span_of(t, r->dtype, r->batch, heads, rows, r->head_dim) : Span{};
-  };
-  for (const Span& x : {span(q, r->heads_q, r->seqlen), span(q_out, r->heads_q, r->seqlen),
-                        span(k, r->heads_kv, r->seqlen), span(v, r->heads_kv, r->seqlen),
-                        span_of(lengths, (size_t)r->batch * 4)})
-    for (const flexatt_tensor* y : {k_cache, v_cache})
-      if (overlap(x, span(y, r->heads_kv, cache_rows))) return FLEXATT_ELAYOUT;
+  FLEXATT_TRY(check_append(r, q, k, v, q_out, k_cache, v_cache, (int64_t)elt_size(r->dtype), cache_rows, lengths));
+  return (int)rotary_run(r->dtype, append_args(r, q, k, v, q_out, k_cache, v_cache, cache_rows, lengths),
+                         (hipStream_t)stream);
+}
+
+int flexatt_norm_rotary_apply(const flexatt_rotary* r, const flexatt_norm* n, const flexatt_tensor* q,
+                              const flexatt_tensor* k, const flexatt_tensor* q_out, const flexatt_tensor* k_out,
+                              void* stream) {
+  FLEXATT_TRY(check_rotary(r, false));
+  FLEXATT_TRY(check_norm(r, n));
+  FLEXATT_TRY(check_tensor(q, r->dtype));
+  FLEXATT_TRY(check_out_tensor(q_out, r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
+  if (r->heads_kv == 0 && (k || k_out)) return FLEXATT_EINVAL;
   RotaryArgs a = rotary_args(r, q, q_out);
-  a.k = view(k);
-  a.v = view(v);
-  a.ko = mview(k_cache);
-  a.vo = mview(v_cache);
-  a.cache_rows = cache_rows;
-  a.lengths = lengths;
-  a.heads += r->heads_kv;
-  return (int)rotary_run(r->dtype, a, (hipStream_t)stream);
+  if (r->heads_kv > 0) {
+    FLEXATT_TRY(check_tensor(k, r->dtype));
+    FLEXATT_TRY(check_out_tensor(k_out, r->dtype, r->batch, r->heads_kv, r->seqlen, r->head_dim));
+    a.k = view(k);
+    a.ko = mview(k_out);
+  }
+  return (int)kNorm[head_index(r->head_dim)](r->dtype, norm_args(a, n), (hipStream_t)stream);
+}
+
+size_t flexatt_norm_rotary_grad_workspace(const flexatt_rotary* r) {
+  if (check_rotary(r, false) != FLEXATT_OK) return SIZE_MAX;
+  const NormGradPlan p = norm_grad_plan(r->batch, r->seqlen, r->heads_q, r->heads_kv, r->head_dim, (int)elt_size(r->dtype));
+  return (size_t)p.columns * (p.q_groups + p.k_groups) * r->head_dim * sizeof(float);
+}
+
+int flexatt_norm_rotary_grad(const flexatt_rotary* r, const flexatt_norm* n, const flexatt_tensor* q,
+                             const flexatt_tensor* k, const flexatt_tensor* q_grad, const flexatt_tensor* k_grad,
+                             const flexatt_tensor* dq, const flexatt_tensor* dk, void* dq_weight, void* dk_weight,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  FLEXATT_TRY(check_rotary(r, false));
+  FLEXATT_TRY(check_norm(r, n));
+  FLEXATT_TRY(check_tensor(q, r->dtype));
+  FLEXATT_TRY(check_tensor(q_grad, r->dtype));
+  FLEXATT_TRY(check_out_tensor(dq, r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
+  if (r->heads_kv == 0 && (k || k_grad || dk || dk_weight)) return FLEXATT_EINVAL;
+  RotaryArgs a = rotary_args(r, q, dq);
+  if (r->heads_kv > 0) {
+    FLEXATT_TRY(check_tensor(k, r->dtype));
+    FLEXATT_TRY(check_tensor(k_grad, r->dtype));
+    FLEXATT_TRY(check_out_tensor(dk, r->dtype, r->batch, r->heads_kv, r->seqlen, r->head_dim));
+    if (!dk_weight) return FLEXATT_EINVAL;
+    a.k = view(k);
+    a.ko = mview(dk);
+  }
+  if (!dq_weight || !workspace || workspace_bytes < flexatt_norm_rotary_grad_workspace(r)) return FLEXATT_EINVAL;
+  if ((uintptr_t)workspace % 16) return FLEXATT_ELAYOUT;
+  for (const void* w : {dq_weight, dk_weight})
+    if ((uintptr_t)w % elt_size(n->weight_dtype)) return FLEXATT_ELAYOUT;
+  NormRotaryArgs g = norm_args(a, n);
+  g.gq = view(q_grad);
+  if (r->heads_kv > 0) g.gk = view(k_grad);
+  g.dwq = dq_weight;
+  g.dwk = dk_weight;
+  g.part = (float*)workspace;
+  return (int)kNormGrad[head_index(r->head_dim)](r->dtype, g, (hipStream_t)stream);
+}
+
+int flexatt_norm_rotary_append(const flexatt_rotary* r, const flexatt_norm* n, const flexatt_tensor* q,
+                               const flexatt_tensor* k, const flexatt_tensor* v, const flexatt_tensor* q_out,
+                               const flexatt_tensor* k_cache, const flexatt_tensor* v_cache, int32_t cache_rows,
+                               const int32_t* lengths, void* stream) {
+  FLEXATT_TRY(check_rotary(r, true));
+  FLEXATT_TRY(check_norm(r, n));
+  FLEXATT_TRY(check_append(r, q, k, v, q_out, k_cache, v_cache, (int64_t)elt_size(r->dtype), cache_rows, lengths));
+  const RotaryArgs a = append_args(r, q, k, v, q_out, k_cache, v_cache, cache_rows, lengths);
+  return (int)kNorm[head_index(r->head_dim)](r->dtype, norm_args(a, n), (hipStream_t)stream);
+}
+
+int flexatt_quant_append(const flexatt_rotary* r, const flexatt_norm* n, int32_t code, const flexatt_tensor* q,
+                         const flexatt_tensor* k, const flexatt_tensor* v, const flexatt_tensor* q_out,
+                         const flexatt_tensor* k_cache, const flexatt_tensor* v_cache, float* k_scales,
+                         float* v_scales, int32_t cache_rows, const int32_t* lengths, void* stream) {
+  FLEXATT_TRY(check_rotary(r, true));
+  if (!is_code(code) || r->inverse) return FLEXATT_EINVAL;
+  if (n) FLEXATT_TRY(check_norm(r, n));
+  FLEXATT_TRY(check_append(r, q, k, v, q_out, k_cache, v_cache, 1, cache_rows, lengths));
+  if (!k_scales || !v_scales) return FLEXATT_EINVAL;
+  if ((uintptr_t)k_scales % 4 || (uintptr_t)v_scales % 4) return FLEXATT_ELAYOUT;
+  const size_t bytes = (size_t)r->batch * r->heads_kv * cache_rows * 4;
+  const Span ks = span_of(k_scales, bytes), vs = span_of(v_scales, bytes);
+  if (overlap(ks, vs)) return FLEXATT_ELAYOUT;
+  const auto span = [&](const flexatt_tensor* t, int heads) {
+    return t ? span_of(t, r->dtype, r->batch, heads, r->seqlen, r->head_dim) : Span{};
+  };
+  for (const Span& x : {span(q, r->heads_q), span(q_out, r->heads_q), span(k, r->heads_kv), span(v, r->heads_kv),
+                        span_of(lengths, (size_t)r->batch * 4),
+                        span_bytes(k_cache, 1, r->batch, r->heads_kv, cache_rows, r->head_dim),
+                        span_bytes(v_cache, 1, r->batch, r->heads_kv, cache_rows, r->head_dim)})
+    if (overlap(x, ks) || overlap(x, vs)) return FLEXATT_ELAYOUT;
+  NormRotaryArgs a = norm_args(append_args(r, q, k, v, q_out, k_cache, v_cache, cache_rows, lengths), n);
+  a.kind = code;
+  a.k_scales = k_scales;
+  a.v_scales = v_scales;
+  return (int)kNorm[head_index(r->head_dim)](r->dtype, a, (hipStream_t)stream);
+}
+
+int flexatt_dequant_rows(const flexatt_dequant* p, const flexatt_tensor* k_cache, const flexatt_tensor* v_cache,
+                         const float* k_scales, const float* v_scales, const flexatt_tensor* k_out,
+                         const flexatt_tensor* v_out, void* stream) {
+  if (!p) return FLEXATT_EINVAL;
+  FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim));
+  if (!is_code(p->code) || (p->fill & ~1) || p->reserved != 0 || !p->lengths) return FLEXATT_EINVAL;
+  // (rows of a workgroup: dequant.hip)
+  const int64_t rows = 256 / (p->head_dim * (int)elt_size(p->dtype) / 16);
+  FLEXATT_TRY(check_launch((int64_t)p->batch * p->heads_kv * ((p->cache_rows + rows - 1) / rows), 256));
+  FLEXATT_TRY(check_view(k_cache, 1));
+  FLEXATT_TRY(check_view(v_cache, 1));
+  FLEXATT_TRY(check_out_tensor(k_out, p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim));
+  FLEXATT_TRY(check_out_tensor(v_out, p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim));
+  FLEXATT_TRY(check_out_pair(k_out, v_out, p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim));
+  if (!k_scales || !v_scales) return FLEXATT_EINVAL;
+  if ((uintptr_t)k_scales % 4 || (uintptr_t)v_scales % 4) return FLEXATT_ELAYOUT;
+  const size_t bytes = (size_t)p->batch * p->heads_kv * p->cache_rows * 4;
+  for (const Span& x : {span_bytes(k_cache, 1, p->batch, p->heads_kv, p->cache_rows, p->head_dim),
+                        span_bytes(v_cache, 1, p->batch, p->heads_kv, p->cache_rows, p->head_dim),
+                        span_of(k_scales, bytes), span_of(v_scales, bytes), span_of(p->lengths, (size_t)p->batch * 4)})
+    for (const flexatt_tensor* y : {k_out, v_out})
+      if (overlap(x, span_of(y, p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim))) return FLEXATT_ELAYOUT;
+  DequantArgs a = {};
+  a.k = view(k_cache);
+  a.v = view(v_cache);
+  a.ko = mview(k_out);
+  a.vo = mview(v_out);
+  a.k_scales = k_scales;
+  a.v_scales = v_scales;
+  a.lengths = p->lengths;
+  a.B = p->batch;
+  a.H = p->heads_kv;
+  a.C = p->cache_rows;
+  a.D = p->head_dim;
+  a.kind = p->code;
+  a.fill = p->fill;
+  return (int)dequant_run(p->dtype, a, (hipStream_t)stream);
 }
 
 size_t flexatt_tree_fwd_workspace(const flexatt_tree* p) {
-  if (check_tree(p) != FLEXATT_OK) return SIZE_MAX;
-  const int ns = tree_plan(p).nsplit;
-  if (ns == 1) return 0;
-  return tree_rows(p) * ns * (p->head_dim + 1) * sizeof(float) + (size_t)p->batch * p->heads_kv * sizeof(int);
+  return check_tree(p) != FLEXATT_OK ? SIZE_MAX : plan_bytes(p, tree_plan(p));
 }
 
 int flexatt_tree_fwd(const flexatt_tree* p, const flexatt_tensor* q, const flexatt_tensor* k_cache,
@@ -305,34 +542,37 @@ int flexatt_tree_fwd(const flexatt_tree* p, const flexatt_tensor* q, const flexa
     if (p->cache_rows > 1 && x->stride_s >= (1 << 26) / (int64_t)elt_size(p->dtype)) return FLEXATT_ERANGE;
   FLEXATT_TRY(check_out_tensor(o, p->dtype, p->batch, p->heads_q, p->tokens, p->head_dim));
   if (!lse) return FLEXATT_EINVAL;
-  const size_t need = flexatt_tree_fwd_workspace(p);
-  if (need > 0) {
-    if (!workspace || workspace_bytes < need) return FLEXATT_EINVAL;
-    if (((uintptr_t)workspace) % 16 != 0) return FLEXATT_ELAYOUT;
-  }
-  TreeArgs a = {};
-  a.q = view(q);
-  a.k = view(k_cache);
-  a.v = view(v_cache);
-  a.o = mview(o);
-  a.lse = lse;
   const TreePlan plan = tree_plan(p);
-  a.slots = plan.slots;
-  a.nchunk = plan.nchunk;
-  a.min_tiles = plan.min_tiles;
-  a.nsplit = plan.nsplit;
-  if (a.nsplit > 1) {
-    a.part_o = (float*)workspace;
-    a.part_lse = a.part_o + tree_rows(p) * a.nsplit * p->head_dim;
-    a.counts = (int*)(a.part_lse + tree_rows(p) * a.nsplit);
+  FLEXATT_TRY(check_workspace(plan_bytes(p, plan), workspace, workspace_bytes));
+  return (int)kTree[p->dtype][head_index(p->head_dim)](tree_args(p, plan, q, k_cache, v_cache, o, lse, workspace),
+                                                       (hipStream_t)stream);
+}
+
+size_t flexatt_quant_tree_fwd_workspace(const flexatt_tree* p) {
+  return check_quant_tree(p) != FLEXATT_OK ? SIZE_MAX : plan_bytes(p, quant_plan(p));
+}
+
+int flexatt_quant_tree_fwd(const flexatt_tree* p, int32_t code, const flexatt_tensor* q, const flexatt_tensor* k_cache,
+                           const flexatt_tensor* v_cache, const float* k_scales, const float* v_scales,
+                           const flexatt_tensor* o, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  FLEXATT_TRY(check_quant_tree(p));
+  if (!is_code(code)) return FLEXATT_EINVAL;
+  FLEXATT_TRY(check_tensor(q, p->dtype));
+  for (const flexatt_tensor* x : {k_cache, v_cache}) {
+    FLEXATT_TRY(check_view(x, 1));
+    if (p->cache_rows > 1 && x->stride_s >= 1 << 26) return FLEXATT_ERANGE;  // (as flexatt_tree_fwd)
   }
-  a.lengths = p->lengths;
-  a.mask = p->tree_mask;
-  a.mask_sb = p->mask_batch > 1 ? (int64_t)p->tokens * p->tokens : 0;
-  a.depths = p->depths;
-  a.p = score_shape(p->batch, p->heads_q, p->heads_kv, p->tokens, p->cache_rows, p->scale, p->soft_cap,
-                    p->sliding_window);
-  return (int)kTree[p->dtype][head_index(p->head_dim)](a, (hipStream_t)stream);
+  FLEXATT_TRY(check_out_tensor(o, p->dtype, p->batch, p->heads_q, p->tokens, p->head_dim));
+  if (!lse || !k_scales || !v_scales) return FLEXATT_EINVAL;
+  if ((uintptr_t)k_scales % 4 || (uintptr_t)v_scales % 4) return FLEXATT_ELAYOUT;
+  const TreePlan plan = quant_plan(p);
+  FLEXATT_TRY(check_workspace(plan_bytes(p, plan), workspace, workspace_bytes));
+  QuantTreeArgs a = {};
+  a.t = tree_args(p, plan, q, k_cache, v_cache, o, lse, workspace);
+  a.k_scales = k_scales;
+  a.v_scales = v_scales;
+  a.kind = code;
+  return (int)kQuantTree[p->dtype == FLEXATT_BF16][head_index(p->head_dim)](a, (hipStream_t)stream);
 }
 
 size_t flexatt_weight_sums_workspace(const flexatt_weights* p) {

@@ -37,15 +37,15 @@ inline int head_index(int d) {
   }
 }
 
-inline int check_tensor(const flexatt_tensor* t, int dt) {
+inline int check_view(const flexatt_tensor* t, int64_t es) {
   if (!t || !t->data) return FLEXATT_EINVAL;
-  const int64_t es = (int64_t)elt_size(dt);
   if (t->stride_d != 1) return FLEXATT_ELAYOUT;
   if (t->stride_b < 0 || t->stride_h < 0 || t->stride_s < 0) return FLEXATT_ELAYOUT;
   if (((uintptr_t)t->data) % 16 != 0) return FLEXATT_ELAYOUT;
   if ((t->stride_b * es) % 16 || (t->stride_h * es) % 16 || (t->stride_s * es) % 16) return FLEXATT_ELAYOUT;
   return FLEXATT_OK;
 }
+inline int check_tensor(const flexatt_tensor* t, int dt) { return check_view(t, (int64_t)elt_size(dt)); }
 
 // No two elements of an index space of up to five dimensions share an address.
 // Sufficient test: over the dimensions of extent > 1 sorted by stride, each stride
@@ -71,18 +71,21 @@ inline int check_nested(const int64_t* st, const int64_t* ext, int n_dims) {
 
 // Output tensors: the input rules, and no two elements may share an address (several
 // workgroups would store to it, and the results would depend on their order).
-inline int check_out_tensor(const flexatt_tensor* t, int dt, int64_t n_b, int64_t n_h, int64_t n_s, int64_t n_d) {
-  FLEXATT_TRY(check_tensor(t, dt));
+inline int check_out_view(const flexatt_tensor* t, int64_t es, int64_t n_b, int64_t n_h, int64_t n_s, int64_t n_d) {
+  FLEXATT_TRY(check_view(t, es));
   const int64_t st[4] = {t->stride_b, t->stride_h, t->stride_s, 1}, ext[4] = {n_b, n_h, n_s, n_d};
   return check_nested(st, ext, 4);
+}
+inline int check_out_tensor(const flexatt_tensor* t, int dt, int64_t n_b, int64_t n_h, int64_t n_s, int64_t n_d) {
+  return check_out_view(t, (int64_t)elt_size(dt), n_b, n_h, n_s, n_d);
 }
 
 // Two output tensors of one shape that pass check_out_tensor: apart, or, with the same
 // strides, one layout in which the step from one to the other is a dimension of extent 2
 // (keys and values side by side in one buffer).
-inline int check_out_pair(const flexatt_tensor* x, const flexatt_tensor* y, int dt, int64_t n_b, int64_t n_h, int64_t n_s,
-                          int64_t n_d) {
-  const int64_t es = (int64_t)elt_size(dt), ext[5] = {n_b, n_h, n_s, n_d, 2};
+inline int check_out_views(const flexatt_tensor* x, const flexatt_tensor* y, int64_t es, int64_t n_b, int64_t n_h,
+                           int64_t n_s, int64_t n_d) {
+  const int64_t ext[5] = {n_b, n_h, n_s, n_d, 2};
   if ((uintptr_t)x->data > (uintptr_t)y->data) {
     const flexatt_tensor* z = x;
     x = y;
@@ -96,6 +99,10 @@ inline int check_out_pair(const flexatt_tensor* x, const flexatt_tensor* y, int 
   for (int i = 0; i < 3; ++i)
     if (ext[i] > 1 && st[i] != other[i]) return FLEXATT_ELAYOUT;
   return check_nested(st, ext, 5);
+}
+inline int check_out_pair(const flexatt_tensor* x, const flexatt_tensor* y, int dt, int64_t n_b, int64_t n_h, int64_t n_s,
+                          int64_t n_d) {
+  return check_out_views(x, y, (int64_t)elt_size(dt), n_b, n_h, n_s, n_d);
 }
 
 // A launch has at most 2^32 - 1 work-items.

@@ -93,6 +93,52 @@ struct RotaryArgs {
   float mag, sign;
 };
 
+// The same with a norm of each head before the rotation, and into a cache of 8 bits
+// (norm_rotary.hip).
+struct NormRotaryArgs {
+  RotaryArgs r;  // the gradient: q, k what went in, qo, ko their gradients
+  View gq, gk;   // the gradient: of what came out
+  const void *wq, *wk;  // [D], 4 bytes each with w_wide, else of the call's type
+  void *dwq, *dwk;
+  float* part;   // the gradient: [groups of heads][columns][D]
+  float *k_scales, *v_scales;  // [B][Hkv][cache_rows] with kind
+  float eps;
+  int norm, w_wide;
+  int kind;      // 0, or enum flexatt_code: the cache's rows are bytes
+  int q_groups;  // groups of q heads (set by the launcher)
+};
+
+// The gradient's workgroups: `columns` of tokens times the groups of hpt heads, q's and
+// k's apart, about 1024 workgroups (four a CU) where there are tokens for them.
+struct NormGradPlan {
+  int columns, hpt, q_groups, k_groups;
+};
+inline NormGradPlan norm_grad_plan(int B, int S, int Hq, int Hkv, int D, int es) {
+  NormGradPlan p;
+  const int64_t per = 256 / (D * es / 32), nb = ((int64_t)B * S + per - 1) / per;
+  const int heads = Hq + Hkv;
+  int64_t groups = (1024 + nb - 1) / nb;
+  if (groups > heads) groups = heads;
+  p.hpt = 1;
+  while (2 * p.hpt * groups <= heads) p.hpt *= 2;
+  p.q_groups = (Hq + p.hpt - 1) / p.hpt;
+  p.k_groups = (Hkv + p.hpt - 1) / p.hpt;
+  int64_t most = 2048 / (p.q_groups + p.k_groups);
+  if (most < 1) most = 1;
+  p.columns = (int)(nb < most ? nb : most);
+  return p;
+}
+
+// A cache of 8 bits read back (dequant.hip).
+struct DequantArgs {
+  View k, v;  // bytes
+  MutView ko, vo;
+  const float *k_scales, *v_scales;  // [B][H][C]
+  const int* lengths;
+  int B, H, C, D, kind;
+  int fill;  // 1: rows behind the length are zeroed
+};
+
 // Attention of a tree of drafted tokens over a cache (tree_attn.hip).
 struct TreeArgs {
   View q, k, v;
@@ -111,6 +157,13 @@ struct TreeArgs {
   int min_tiles;  // least 32-key tiles of a chunk
   int nsplit;     // most chunks of one (b, hkv)
   int nrt;        // groups of packed query row tiles per (b, hkv) (set by the launcher)
+};
+
+// The same over a cache of 8 bits (quant_attn.hip): t.k and t.v are bytes.
+struct QuantTreeArgs {
+  TreeArgs t;
+  const float *k_scales, *v_scales;  // [B][Hkv][Skv]
+  int kind;
 };
 
 // Attention weight received by each key (weight_sums.hip).
@@ -152,6 +205,12 @@ inline int tree_share(int row_bytes, int elt_bytes, int64_t tiles) {
 }
 
 typedef hipError_t (*TreeLauncher)(const TreeArgs&, hipStream_t);
+// Row tiles of one wave of the attention over a cache of 8 bits: two share what a tile's
+// conversion costs, where registers hold them (quant_attn.hip).
+inline int quant_row_tiles(int head_dim, int64_t tiles) { return head_dim <= 128 && tiles > 1 ? 2 : 1; }
+
+typedef hipError_t (*QuantTreeLauncher)(const QuantTreeArgs&, hipStream_t);
+typedef hipError_t (*NormRotaryLauncher)(int dtype, const NormRotaryArgs&, hipStream_t);
 typedef hipError_t (*WeightLauncher)(const WeightArgs&, hipStream_t);
 typedef hipError_t (*FwdLauncher)(const FwdArgs&, hipStream_t);
 typedef hipError_t (*DecodeLauncher)(const DecodeArgs&, hipStream_t);
@@ -185,15 +244,21 @@ hipError_t bwd_delta(int dtype, const DeltaArgs&, hipStream_t);
 
 hipError_t rotary_run(int dtype, const RotaryArgs&, hipStream_t);
 hipError_t evict_run(const EvictArgs&, int cus, hipStream_t);
+hipError_t dequant_run(int dtype, const DequantArgs&, hipStream_t);
 
-// Tree attention (tree_attn.hip) and weight sums (weight_sums.hip), every D.
+// Tree attention (tree_attn.hip, quant_attn.hip), weight sums (weight_sums.hip), norm and
+// rotation (norm_rotary.hip), every D.
 #define FLEXATT_DECL_CACHE(D)                              \
   hipError_t tree_attn_bf16_d##D(const TreeArgs&, hipStream_t); \
   hipError_t tree_attn_f16_d##D(const TreeArgs&, hipStream_t);  \
   hipError_t tree_attn_f32_d##D(const TreeArgs&, hipStream_t);  \
   hipError_t weight_sums_bf16_d##D(const WeightArgs&, hipStream_t); \
   hipError_t weight_sums_f16_d##D(const WeightArgs&, hipStream_t);  \
-  hipError_t weight_sums_f32_d##D(const WeightArgs&, hipStream_t);
+  hipError_t weight_sums_f32_d##D(const WeightArgs&, hipStream_t);  \
+  hipError_t quant_attn_bf16_d##D(const QuantTreeArgs&, hipStream_t); \
+  hipError_t quant_attn_f16_d##D(const QuantTreeArgs&, hipStream_t);  \
+  hipError_t norm_rotary_d##D(int, const NormRotaryArgs&, hipStream_t); \
+  hipError_t norm_rotary_grad_d##D(int, const NormRotaryArgs&, hipStream_t);
 
 FLEXATT_DECL_CACHE(32)
 FLEXATT_DECL_CACHE(64)

@@ -1,0 +1,490 @@
+// Attention of a tree of drafted tokens over a K/V cache of 8 bits (norm_rotary.hip writes
+// it): the semantics, the chunks of key tiles and their merge are those of tree_attn.hip.
+// No counterpart in the reference, which has no cache.
+//
+// With codes c_j, c'_j and scales s_j, s'_j of key j's row of K and V,
+//   x_ij = scale s_j (q_i . c_j),   o_i = sum_j (p_ij s'_j) c'_j / sum_j p_ij,
+// so a scale meets a score and a weight, never an element.  Codes of either kind are exact
+// in bf16 and fp16, the types of the MFMAs, and are converted on the way to them:
+//  * K: a lane has 16 codes of its key in one LDS read, the operands of two MFMAs; which
+//    k of the products they are is the same for Q's fragments, which are loaded to match;
+//  * V: the transpose read of 8-bit elements gives a lane eight keys of its column, those
+//    whose weights the scores' accumulators hold.
+// p s' is rounded to the type, as P is elsewhere.  fp16 has a narrow range: there the
+// scales are taken relative to a power of two that is at least the largest one a wave has
+// met, and the accumulators follow it as they follow the running maximum.
+//
+// A wave has one row tile of 32 packed query rows, or two (MT) that share the tile's LDS
+// reads and conversions, and every NW-th 32-key tile of its workgroup's chunk, copied to
+// its own LDS stages without barriers, the scales with one copy more.
+//
+// Bound by HBM for long caches and few rows, by the softmax's VALU work for many.
+#include "flexatt_device.h"
+#include "flexatt_kernels.h"
+#include "tree_device.h"
+
+#ifndef FLEXATT_D
+#error "FLEXATT_D (head dim) must be defined"
+#endif
+
+namespace flexatt {
+
+namespace {
+template <int D>
+struct QuantCfg {
+  static constexpr int BN = 32;              // keys per tile
+  static constexpr int KC = D / 32;          // 32-byte steps of S^T = K Q^T, two MFMAs each
+  static constexpr int DB = D / 32;          // 32-row blocks of O^T
+  static constexpr int CPR = D / 16;         // 16-byte chunks per row
+  static constexpr int RPC = 64 / CPR;       // rows per 1 KB copy
+  static constexpr int TB = BN * D;          // bytes of one K or V tile
+  static constexpr int E = TB / 1024;        // copies of one
+  static constexpr int PK = RPC >= 16 ? 1 : 16 / RPC;  // copies after which K's swizzle repeats
+  static constexpr int PV = RPC >= 8 ? 1 : 8 / RPC;    // and V's
+  static constexpr int EC = 2 * E + 1;       // copies of a stage: K, V, both scales
+  static constexpr int STB = 2 * TB + 256;   // bytes of a stage
+  static constexpr int NW = 4;               // waves per workgroup
+  static constexpr int ST = D >= 256 ? 2 : 4;  // stages
+  static_assert(E * 1024 == TB && NW * ST * STB <= 160 * 1024 && E % PK == 0 && E % PV == 0, "tiles");
+};
+
+// K is read 16 bytes a lane from 32 rows, V by transpose reads of 32 bytes of 16 rows
+// (rows 16 c + 0..15 of a block of 32 columns); both spread evenly over the banks.
+template <int CPR>
+__device__ __forceinline__ int swz_k8(int r, int c) {
+  if constexpr (CPR == 2) return c ^ ((r >> 3) & 1);
+  else return swz_col<CPR>(r, c);
+}
+template <int CPR>
+__device__ __forceinline__ int swz_v8(int r, int c) {
+  if constexpr (CPR == 2) return c;
+  else if constexpr (CPR == 4) return c ^ (((r >> 2) & 1) << 1);
+  else if constexpr (CPR == 8) return c ^ (((r >> 1) & 3) << 1);
+  else return c ^ ((r & 7) << 1);
+}
+
+// Eight codes as an MFMA operand.
+template <class T, int CODE>
+__device__ __forceinline__ typename Mfma<T>::v8 operand8(int lo, int hi) {
+  typedef T x2 __attribute__((ext_vector_type(2)));
+  x2 p[4];
+  if constexpr (CODE == FLEXATT_E4M3) {
+    if constexpr (__is_same(T, __bf16)) {
+      p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
+      p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+      p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
+      p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+    } else {
+      p[0] = __builtin_bit_cast(x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false));
+      p[1] = __builtin_bit_cast(x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true));
+      p[2] = __builtin_bit_cast(x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false));
+      p[3] = __builtin_bit_cast(x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true));
+    }
+  } else if constexpr (__is_same(T, __bf16)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int w = i < 2 ? lo : hi;
+      p[i] = x2{(T)(float)(signed char)(w >> (16 * (i & 1))), (T)(float)(signed char)(w >> (16 * (i & 1) + 8))};
+    }
+  } else {
+    // 0x6400 + u is 1024 + u in fp16, u = code + 128
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned u = (unsigned)(i < 2 ? lo : hi) ^ 0x80808080u;
+      const unsigned w = __builtin_amdgcn_perm(0x64646464u, u, i & 1 ? 0x04030402u : 0x04010400u);
+      p[i] = __builtin_bit_cast(x2, w) - x2{(T)1152.f, (T)1152.f};
+    }
+  }
+  const i32x4 v = {__builtin_bit_cast(int, p[0]), __builtin_bit_cast(int, p[1]), __builtin_bit_cast(int, p[2]),
+                   __builtin_bit_cast(int, p[3])};
+  return as_v8<typename Mfma<T>::v8>(v);
+}
+
+// Transposed 8 x 8-bit read: lane i of 16 gets byte i % 8 at the addresses of lanes
+// 2 t + i / 8, t = 0 .. 7.
+__device__ __forceinline__ i32x2 lds_read_tr8(const void* p) {
+  return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+      (__attribute__((address_space(3))) i32x2*)((__attribute__((address_space(3))) char*)p));
+}
+
+template <class T, int CODE, int D, int MT, bool CAP>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D >= 128 || MT > 1 ? 1 : 2)))
+void quant_attn_kernel(QuantTreeArgs qa) {
+  using C = QuantCfg<D>;
+  typedef typename Mfma<T>::v8 V8;
+  constexpr int ST = C::ST, NW = C::NW, EC = C::EC, PK = C::PK, PV = C::PV;
+  constexpr bool NARROW = __is_same(T, _Float16);
+  constexpr int kCombine = NW * 64 * 4 * (3 + 16 * C::DB);
+  __shared__ __attribute__((aligned(1024))) char smem[NW * ST * C::STB > kCombine ? NW * ST * C::STB : kCombine];
+
+  const TreeArgs& a = qa.t;
+  const Shape& p = a.p;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = lane >> 5, l32 = lane & 31;
+
+  // (chunk, row tiles): as in tree_attn.hip
+  int rt0 = 0, x = blockIdx.x;
+  if (a.nrt > 1) {
+    rt0 = blockIdx.x / 8 % a.nrt * MT;
+    x = blockIdx.x / (8 * a.nrt) * 8 + blockIdx.x % 8;
+  }
+  const TreeChunk ck = tree_chunk(a, x, NW);
+  if (ck.b < 0) return;
+  const int b = ck.b, hk = ck.hk, s = ck.s, ns = ck.ns;
+  TreeSeq sq = tree_seq(a, b);
+  sq.n = __builtin_amdgcn_readfirstlane(sq.n);
+  sq.t0 = __builtin_amdgcn_readfirstlane(sq.t0);
+  if (rt0 == 0 && s == 0 && tid == 0 && a.counts) a.counts[b * p.Hkv + hk] = sq.bad ? 1 : ns;
+
+  // packed query rows of this lane: head, drafted token
+  const int R = p.G * p.Sq;
+  int hq[MT], qi[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int r = min(32 * (rt0 + m) + l32, R - 1);
+    hq[m] = hk * p.G + r % p.G;
+    qi[m] = r / p.G;
+  }
+  if (sq.bad) {
+    if (s == 0) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if (32 * (rt0 + m) + l32 >= R) continue;
+        T* out = (T*)a.o.data + b * a.o.sb + hq[m] * a.o.sh + (int64_t)qi[m] * a.o.ss;
+        for (int d = wave * 2 + h; d < D; d += NW * 2) out[d] = from_f32<T>(__builtin_nanf(""));
+        if (wave == 0 && h == 0) a.lse[((int64_t)b * p.Hq + hq[m]) * p.Sq + qi[m]] = __builtin_nanf("");
+      }
+    }
+    return;
+  }
+
+  int koff[C::KC], voff[C::DB];
+#pragma unroll
+  for (int kc = 0; kc < C::KC; ++kc) koff[kc] = l32 * D + swz_k8<C::CPR>(l32, 2 * kc + h) * 16;
+  {
+    const int t = (lane & 15) >> 1, row = 4 * h + (t & 3) + 2 * (t & 4);  // keys 4 h + 0..3, 8 + 4 h + 0..3
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db)
+      voff[db] = row * D + swz_v8<C::CPR>(row, 2 * db + ((lane >> 4) & 1)) * 16 + (lane & 1) * 8;
+  }
+  // this lane's offsets in a tile's copies
+  const unsigned kss = (unsigned)a.k.ss, vss = (unsigned)a.v.ss;
+  const int crow = lane / C::CPR, cchunk = lane % C::CPR;
+  unsigned kvo[PK], vvo[PV];
+#pragma unroll
+  for (int e = 0; e < PK; ++e) kvo[e] = (e * C::RPC + crow) * kss + swz_k8<C::CPR>(e * C::RPC + crow, cchunk) * 16;
+#pragma unroll
+  for (int e = 0; e < PV; ++e) vvo[e] = (e * C::RPC + crow) * vss + swz_v8<C::CPR>(e * C::RPC + crow, cchunk) * 16;
+  const unsigned wbase = lds_addr_of(smem) + wave * (ST * C::STB);
+  auto reads_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
+
+  // this wave's tiles: first + NW * j, j < nt
+  const int n = sq.n, last = n + p.Sq - 1;
+  const int first = sq.t0 + ck.first + wave;
+  const int nt = __builtin_amdgcn_readfirstlane(max((ck.count - wave + NW - 1) / NW, 0));
+  const uint64_t kp = (uint64_t)((const char*)a.k.data + b * a.k.sb + hk * a.k.sh);
+  const uint64_t vp = (uint64_t)((const char*)a.v.data + b * a.v.sb + hk * a.v.sh);
+  const float* scales = (h ? qa.v_scales : qa.k_scales) + ((int64_t)b * p.Hkv + hk) * p.Skv;
+  auto issue = [&](int j) {  // tile j of this wave into its stage
+    const int t = first + NW * j;
+    const unsigned dst = wbase + j % ST * C::STB;
+    const uint64_t kb = kp + (uint64_t)(t * C::BN) * kss, vb = vp + (uint64_t)(t * C::BN) * vss;
+    if (t * C::BN + C::BN - 1 <= last) {
+#pragma unroll
+      for (int e = 0; e < C::E; ++e)
+        load_lds16_base(kvo[e % PK], kb + (uint64_t)(e / PK * PK * C::RPC) * kss, dst + e * 1024);
+#pragma unroll
+      for (int e = 0; e < C::E; ++e)
+        load_lds16_base(vvo[e % PV], vb + (uint64_t)(e / PV * PV * C::RPC) * vss, dst + C::TB + e * 1024);
+    } else {  // rows behind the last one repeat it
+#pragma unroll 1
+      for (int e = 0; e < C::E; ++e) {
+        const int kr = e * C::RPC + crow;
+        load_lds16_base(min(kr, last - t * C::BN) * kss + swz_k8<C::CPR>(kr, cchunk) * 16, kb, dst + e * 1024);
+      }
+#pragma unroll 1
+      for (int e = 0; e < C::E; ++e) {
+        const int kr = e * C::RPC + crow;
+        load_lds16_base(min(kr, last - t * C::BN) * vss + swz_v8<C::CPR>(kr, cchunk) * 16, vb, dst + C::TB + e * 1024);
+      }
+    }
+    load_lds4(scales + min(t * C::BN + l32, last), dst + 2 * C::TB);
+  };
+  if (nt > 0) issue(0);
+
+  // Q: lane half h has elements 32 kc + 16 h .. + 15 of its row, the codes' order
+  i32x4 qf[MT][2 * C::KC];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const char* src = (const char*)((const T*)a.q.data + b * a.q.sb + hq[m] * a.q.sh + (int64_t)qi[m] * a.q.ss) + 32 * h;
+#pragma unroll
+    for (int kc = 0; kc < 2 * C::KC; ++kc) qf[m][kc] = ld_global16(src + 64 * (kc >> 1) + 16 * (kc & 1));
+  }
+  // Row qi sees the cached keys [row_lo, n); the tiles that hold only keys every row
+  // sees need no mask.
+  int row_lo[MT], full_lo = 0;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) row_lo[m] = 0;
+  if (p.window > 0) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int depth = a.depths ? max(a.depths[(int64_t)b * p.Sq + qi[m]], 0) : qi[m];
+      row_lo[m] = max(n - (p.window - min(depth, p.window)), 0);
+      full_lo = max(full_lo, row_lo[m]);
+    }
+#pragma unroll
+    for (int y = 32; y; y >>= 1) full_lo = max(full_lo, __shfl_xor(full_lo, y));
+    full_lo = __builtin_amdgcn_readfirstlane(full_lo);
+  }
+  const unsigned char* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+  // wait for Q here, once: see fwd_split.hip
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int kc = 0; kc < 2 * C::KC; ++kc) pin(qf[m][kc]);
+#pragma unroll
+  for (int j = 1; j < ST - 1; ++j)
+    if (j < nt) issue(j);
+
+  f32x16 acc[MT][C::DB];
+  float m_run[MT], l_run[MT];
+  float rel = 0x1p126f;  // fp16: acc has values times rel, and rel times a scale is at most 1
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    m_run[m] = kNegInf, l_run[m] = 0.f;
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db) acc[m][db] = f32x16{};
+  }
+
+  for (int j = 0; j < nt; ++j) {
+    const int n0 = (first + NW * j) * C::BN;
+    if (j + ST - 1 < nt) {  // into the stage of tile j - 1, read in the previous iteration
+      reads_done();
+      issue(j + ST - 1);
+      wait_vmcnt<(ST - 1) * EC>();  // tile j landed, the next ones in flight
+    } else if (ST > 2 && j + 2 < nt) {
+      wait_vmcnt<(ST > 2 ? 2 : 0) * EC>();
+    } else if (ST > 2 && j + 1 < nt) {
+      wait_vmcnt<(ST > 2 ? 1 : 0) * EC>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    const char* sK = smem + wave * (ST * C::STB) + j % ST * C::STB;
+    const char* sV = sK + C::TB;
+    const char* sS = sV + C::TB + 16 * h;
+
+    f32x16 sc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) sc[m] = f32x16{};
+#pragma unroll
+    for (int kc = 0; kc < C::KC; ++kc) {
+      const i32x4 kf = lds_read16(sK + koff[kc]);
+      const V8 k0 = operand8<T, CODE>(kf[0], kf[1]), k1 = operand8<T, CODE>(kf[2], kf[3]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        sc[m] = Mfma<T>::mma(k0, as_v8<V8>(qf[m][2 * kc]), sc[m]);
+        sc[m] = Mfma<T>::mma(k1, as_v8<V8>(qf[m][2 * kc + 1]), sc[m]);
+      }
+    }
+    // scales of this lane's keys: element e is key n0 + 8(e/4) + 4h + e%4
+    float ks[16], vs[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const i32x4 k4 = lds_read16(sS + 32 * i), v4 = lds_read16(sS + 128 + 32 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ks[4 * i + e] = __int_as_float(k4[e]), vs[4 * i + e] = __int_as_float(v4[e]);
+    }
+    if constexpr (!CAP) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ks[e] *= p.scale_log2;
+    }
+    if constexpr (NARROW) {
+      float top = vs[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, vs[e]);
+      top = fmaxf(top, swap_halves(top));
+      if (__builtin_amdgcn_readfirstlane(top * rel > 1.f)) {
+        // the power of two above the largest scale, as far as there is one
+        const int expo = (int)(__float_as_uint(top) >> 23) & 255;
+        const float now = __int_as_float(max(253 - expo, 1) << 23), turn = now / rel;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int db = 0; db < C::DB; ++db) scale_inplace(acc[m][db], turn);
+        rel = now;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) vs[e] *= rel;
+    }
+
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[m][e] *= ks[e];
+      if constexpr (CAP) {
+        soft_cap(sc[m], p);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[m][e] *= p.cap_log2;
+      }
+      if (n0 < full_lo || n0 + C::BN > n) {
+        // this lane's keys, relative to its first: e, and hidden before lo or from hi on
+        const int lo = row_lo[m] - n0 - 4 * h, hi = n + (mask ? p.Sq : qi[m] + 1) - n0 - 4 * h;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if ((unsigned)(8 * (e >> 2) + (e & 3) - lo) >= (unsigned)max(hi - lo, 0)) sc[m][e] = kNegInf;
+        if (mask && n0 + C::BN > n) {  // all of the tile's mask bytes at once
+          const unsigned char* mrow = mask + (int64_t)qi[m] * p.Sq;
+          const int u0 = n0 + 4 * h - n;
+          unsigned char mb[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mb[e] = mrow[min(max(u0 + 8 * (e >> 2) + (e & 3), 0), p.Sq - 1)];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (u0 + 8 * (e >> 2) + (e & 3) >= 0 && mb[e] == 0) sc[m][e] = kNegInf;
+        }
+      }
+      float mx, mx2;
+      max16_partial(sc[m], mx, mx2);
+      mx = max2(mx, mx2);
+      mx = fmaxf(mx, swap_halves(mx));
+      if (mx != mx) mx = kNegInf;
+      const bool grow = mx > m_run[m] + kTreeRescale;
+      if (__builtin_amdgcn_ballot_w64(grow)) {
+        const float m_new = grow ? mx : m_run[m];
+        const float alpha = grow ? fast_exp2(m_run[m] - m_new) : 1.f;
+        l_run[m] *= alpha;
+#pragma unroll
+        for (int db = 0; db < C::DB; ++db) scale_inplace(acc[m][db], alpha);
+        m_run[m] = m_new;
+      }
+      const float m_use = (m_run[m] == kNegInf) ? 0.f : m_run[m];
+      float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float pe = fast_exp2(sc[m][e] - m_use);
+        rs[e & 3] += pe;
+        sc[m][e] = pe * vs[e];
+      }
+      l_run[m] += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      V8 pb[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) pb[m] = pack8<T>(sc[m], 8 * c);
+      const char* vr = sV + 16 * c * D;
+#pragma unroll
+      for (int db = 0; db < C::DB; ++db) {
+        const i32x2 w = lds_read_tr8(vr + voff[db]);
+        const V8 v = operand8<T, CODE>(w[0], w[1]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[m][db] = Mfma<T>::mma(v, pb[m], acc[m][db]);
+      }
+    }
+  }
+
+  // The (m, l, acc) of a row tile's NW waves combined in wave order through LDS (every
+  // wave's copies have landed: its last tile waited for vmcnt 0), then O / l and LSE.
+  float* xm = (float*)smem;       // [NW][64]
+  float* xl = xm + NW * 64;       // [NW][64]
+  float* xr = xl + NW * 64;       // [NW][64]: 1 / rel
+  f32x4* xa = (f32x4*)(xr + NW * 64);  // [NW][4 DB][64]: columns 8 y + 4 h .. + 3 of row l32
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    if (32 * (rt0 + m) >= R) break;  // (every wave)
+    const float l_tot = l_run[m] + swap_halves(l_run[m]);
+    __syncthreads();
+    xm[wave * 64 + lane] = m_run[m];
+    xl[wave * 64 + lane] = l_tot;
+    xr[wave * 64 + lane] = NARROW ? 1.0f / rel : 1.f;
+#pragma unroll
+    for (int y = 0; y < 4 * C::DB; ++y) {
+      const f32x16& v = acc[m][y / 4];
+      const int e = y % 4 * 4;
+      xa[(wave * 4 * C::DB + y) * 64 + lane] = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+    }
+    __syncthreads();
+    float mw[NW], mall = kNegInf;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      mw[w] = xm[w * 64 + lane];
+      mall = fmaxf(mall, mw[w]);
+    }
+    float al[NW], L = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      // a wave whose maximum stayed -inf has weights of 0, or NaN scores
+      const float lw = xl[w * 64 + lane];
+      al[w] = mw[w] == kNegInf ? (lw == 0.f ? 0.f : 1.f) : fast_exp2(mw[w] - mall);
+      L = __builtin_fmaf(al[w], lw, L);
+      al[w] *= xr[w * 64 + lane];
+    }
+    const bool empty = L == 0.f;  // no key; NaN (a NaN query row or key) is not
+    const float inv = empty ? 0.f : 1.0f / L;
+    if (32 * (rt0 + m) + l32 < R) {
+      const int64_t row = ((int64_t)b * p.Hq + hq[m]) * p.Sq + qi[m];
+      float* po = a.part_o + (row * a.nsplit + s) * D + 4 * h;
+      T* out = (T*)a.o.data + b * a.o.sb + hq[m] * a.o.sh + (int64_t)qi[m] * a.o.ss + 4 * h;
+#pragma unroll 2
+      for (int y = wave; y < 4 * C::DB; y += NW) {
+        f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const f32x4 v = xa[(w * 4 * C::DB + y) * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(al[w], v[e], o[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= inv;
+        if (ns > 1) *(f32x4*)(po + 8 * y) = o;
+        else st_global8(out + 8 * y, pack4<T>(o[0], o[1], o[2], o[3]));
+      }
+      if (wave == 0 && h == 0) {
+        const float lse = empty ? kNegInf : mall + log2f(L);
+        if (ns > 1) a.part_lse[row * a.nsplit + s] = lse;
+        else a.lse[row] = lse * kLn2;
+      }
+    }
+  }
+}
+
+template <class T, int CODE, int D, int MT>
+void launch_rows(QuantTreeArgs a, hipStream_t st) {
+  a.t.nrt = (int)((((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32 + MT - 1) / MT);
+  const dim3 grid((unsigned)((a.t.nchunk + 7) / 8 * 8 * a.t.nrt)), block(256);
+  if (a.t.p.cap > 0.f) hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, MT, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, MT, false>), grid, block, 0, st, a);
+}
+
+template <class T, int CODE, int D>
+void launch_code(const QuantTreeArgs& a, hipStream_t st) {
+  const int mt = quant_row_tiles(D, ((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32);
+  if constexpr (D <= 128) {
+    if (mt == 2) launch_rows<T, CODE, D, 2>(a, st);
+  }
+  if (mt == 1) launch_rows<T, CODE, D, 1>(a, st);
+}
+
+template <class T, int D>
+hipError_t launch_quant(const QuantTreeArgs& a, hipStream_t st) {
+  if (a.kind == FLEXATT_E4M3) launch_code<T, FLEXATT_E4M3, D>(a, st);
+  else launch_code<T, FLEXATT_INT8, D>(a, st);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.t.nsplit == 1) return e;
+  const int64_t rows = (int64_t)a.t.p.B * a.t.p.Hq * a.t.p.Sq;
+  hipLaunchKernelGGL((tree_merge_kernel<T, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a.t);
+  return hipGetLastError();
+}
+}  // namespace
+
+#define FLEXATT_CAT2(a, b) a##b
+#define FLEXATT_CAT(a, b) FLEXATT_CAT2(a, b)
+hipError_t FLEXATT_CAT(quant_attn_bf16_d, FLEXATT_D)(const QuantTreeArgs& a, hipStream_t st) {
+  return launch_quant<__bf16, FLEXATT_D>(a, st);
+}
+hipError_t FLEXATT_CAT(quant_attn_f16_d, FLEXATT_D)(const QuantTreeArgs& a, hipStream_t st) {
+  return launch_quant<_Float16, FLEXATT_D>(a, st);
+}
+
+}  // namespace flexatt

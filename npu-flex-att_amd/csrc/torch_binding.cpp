@@ -19,6 +19,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
+#include <limits>
 #include <string>
 
 #include "../../include/flexatt.h"
@@ -281,6 +282,128 @@ struct Rotary : torch::autograd::Function<Rotary> {
   }
 };
 
+// ---------------------------------------------------- norm of each head, rotation --
+// A weight [D] of the call's dtype or fp32, on its device.
+Tensor check_weight(const Tensor& w, const char* name, const Tensor& x) {
+  TORCH_CHECK(w.device() == x.device(), name, " must be on ", x.device(), " (got ", w.device(), ")");
+  TORCH_CHECK(w.scalar_type() == at::kFloat || w.scalar_type() == x.scalar_type(), name, " has dtype ", w.scalar_type(),
+              ", expected ", x.scalar_type(), " or float32");
+  TORCH_CHECK(w.layout() == at::kStrided && w.dim() == 1 && w.size(0) == x.size(3), name, " must be [D] = [", x.size(3), "]");
+  return w.contiguous();
+}
+void check_eps(double eps) {
+  TORCH_CHECK((float)eps >= std::numeric_limits<float>::min() && std::isfinite((float)eps),
+              "eps must be a positive number that 32 bits hold");
+}
+flexatt_norm norm_struct(const Tensor& wq, const Tensor& wk, double eps) {
+  flexatt_norm n = {};
+  const Tensor& any = wq.defined() ? wq : wk;
+  n.weight_dtype = dtype_of(any);
+  TORCH_CHECK(!wq.defined() || !wk.defined() || wq.scalar_type() == wk.scalar_type(),
+              "query_weight and key_weight must have one dtype");
+  n.eps = (float)eps;
+  n.q_weight = data_or_null(wq);
+  n.k_weight = data_or_null(wk);
+  return n;
+}
+
+// (query', key'), key' undefined without a key.
+std::pair<Tensor, Tensor> norm_rotate(const Tensor& query, const Tensor& key, const Tensor& wq, const Tensor& wk,
+                                      const Tensor& freq, const OptTensor& pos, bool interleaved, double magnitude,
+                                      double eps) {
+  const c10::Device dev = query.device();
+  const c10::OptionalDeviceGuard guard(dev);
+  const bool keyed = key.defined();
+  const flexatt_rotary r = rotary_struct(query, keyed ? key.size(1) : 0, freq, pos, interleaved, magnitude, false);
+  const flexatt_norm n = norm_struct(wq, wk, eps);
+  Tensor qo = out_like(query), ko = keyed ? out_like(key) : Tensor();
+  if (query.numel() == 0 && (!keyed || key.numel() == 0)) return {qo, ko};
+  const Tensor q = prepare(query), k = keyed ? prepare(key) : Tensor();
+  const flexatt_tensor tq = view(q), tqo = view(qo);
+  flexatt_tensor tk = {}, tko = {};
+  if (keyed) tk = view(k), tko = view(ko);
+  check_status(flexatt_norm_rotary_apply(&r, &n, &tq, keyed ? &tk : nullptr, &tqo, keyed ? &tko : nullptr, stream_of(dev)),
+               "flexatt_norm_rotary_apply");
+  return {qo, ko};
+}
+
+// The gradients of x and its weight, and of y and its own if there is one.
+struct NormGrads {
+  Tensor dx, dw, dy, dv;
+};
+NormGrads norm_rotate_grad(const Tensor& x, const Tensor& w, const Tensor& gx, const Tensor& y, const Tensor& v,
+                           const Tensor& gy, const Tensor& freq, const OptTensor& pos, bool interleaved, double magnitude,
+                           double eps) {
+  no_trace();
+  const c10::Device dev = x.device();
+  const c10::OptionalDeviceGuard guard(dev);
+  const bool two = y.defined();
+  const flexatt_rotary r = rotary_struct(x, two ? y.size(1) : 0, freq, pos, interleaved, magnitude, false);
+  const flexatt_norm n = norm_struct(w, v, eps);
+  NormGrads g;
+  g.dx = out_like(x);
+  g.dw = at::empty(w.sizes(), w.options().requires_grad(false));
+  if (two) g.dy = out_like(y), g.dv = at::empty(v.sizes(), v.options().requires_grad(false));
+  if (x.numel() == 0) {
+    g.dw.zero_();
+    if (two) g.dv.zero_();
+    return g;
+  }
+  const Tensor px = prepare(x), pg = prepare(gx), py = two ? prepare(y) : Tensor(), ph = two ? prepare(gy) : Tensor();
+  const flexatt_tensor tx = view(px), tg = view(pg), td = view(g.dx);
+  flexatt_tensor ty = {}, th = {}, te = {};
+  if (two) ty = view(py), th = view(ph), te = view(g.dy);
+  const size_t bytes = flexatt_norm_rotary_grad_workspace(&r);
+  const Tensor ws = workspace(bytes, dev);
+  check_status(flexatt_norm_rotary_grad(&r, &n, &tx, two ? &ty : nullptr, &tg, two ? &th : nullptr, &td,
+                                        two ? &te : nullptr, g.dw.data_ptr(), data_or_null(g.dv), data_or_null(ws),
+                                        ws.defined() ? bytes : 0, stream_of(dev)),
+               "flexatt_norm_rotary_grad");
+  return g;
+}
+
+struct NormRotary : torch::autograd::Function<NormRotary> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& query,
+                                                const OptTensor& key, const Tensor& wq, const OptTensor& wk,
+                                                const Tensor& freq, const OptTensor& pos, bool interleaved,
+                                                double magnitude, double eps) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({query, key ? *key : Tensor(), wq, wk ? *wk : Tensor(), freq, pos ? *pos : Tensor()});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["magnitude"] = magnitude;
+    ctx->saved_data["eps"] = eps;
+    auto [q, k] = norm_rotate(query, key ? *key : Tensor(), wq, wk ? *wk : Tensor(), freq, pos, interleaved, magnitude, eps);
+    if (k.defined()) return {q, k};
+    return {q};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool interleaved = ctx->saved_data["interleaved"].toBool();
+    const double magnitude = ctx->saved_data["magnitude"].toDouble(), eps = ctx->saved_data["eps"].toDouble();
+    const Tensor gq = grads[0], gk = grads.size() > 1 ? grads[1] : Tensor();
+    const OptTensor pos = saved[5].defined() ? OptTensor(saved[5]) : std::nullopt;
+    // (a graph of this pass would end here without a word)
+    TORCH_CHECK(!at::GradMode::is_enabled(), "norm_rotary_embedding has no gradients of its gradients (create_graph)");
+    torch::autograd::variable_list out(9);
+    const auto run = [&](const Tensor& x, const Tensor& w, const Tensor& g, const Tensor& y, const Tensor& v,
+                         const Tensor& h) {
+      return norm_rotate_grad(x, w, g, y, v, h, saved[4], pos, interleaved, magnitude, eps);
+    };
+    if (gq.defined() && gk.defined()) {
+      const NormGrads r = run(saved[0], saved[2], gq, saved[1], saved[3], gk);
+      out[0] = r.dx, out[2] = r.dw, out[1] = r.dy, out[3] = r.dv;
+    } else if (gq.defined()) {
+      const NormGrads r = run(saved[0], saved[2], gq, Tensor(), Tensor(), Tensor());
+      out[0] = r.dx, out[2] = r.dw;
+    } else if (gk.defined()) {
+      const NormGrads r = run(saved[1], saved[3], gk, Tensor(), Tensor(), Tensor());
+      out[1] = r.dx, out[3] = r.dw;
+    }
+    return out;
+  }
+};
+
 PyObject* pair_of(const Tensor& a, const Tensor& b) {
   PyObject* t = PyTuple_New(2);
   if (!t) throw python_error();
@@ -331,6 +454,52 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* py_norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  want(n, 9, "norm_rotary");
+  no_trace();
+  const Tensor query = tensor_arg(a[0], "query");
+  const OptTensor key = opt_tensor_arg(a[1], "key");
+  Tensor wq = tensor_arg(a[2], "query_weight");
+  OptTensor wk = opt_tensor_arg(a[3], "key_weight");
+  Tensor freq = tensor_arg(a[4], "inv_freq");
+  const OptTensor pos = opt_tensor_arg(a[5], "positions");
+  const bool interleaved = bool_arg(a[6]);
+  const double magnitude = double_arg(a[7]), eps = double_arg(a[8]);
+  no_derivatives({{"inv_freq", &freq}});
+  no_tangents({{"query", &query}, {"query_weight", &wq}});
+  TORCH_CHECK(key.has_value() == wk.has_value(), "key and key_weight go together");
+  if (key) {
+    no_tangents({{"key", &*key}, {"key_weight", &*wk}});
+    check_tensors({{"query", &query}, {"key", &*key}});
+    FLEXATT_ASSERT(key->size(0) == query.size(0) && key->size(2) == query.size(2) && key->size(3) == query.size(3),
+                   "query and key must have the same batch, length and head dim");
+    FLEXATT_ASSERT(key->size(1) > 0, "key must have a head");
+    wk = check_weight(*wk, "key_weight", query);
+  } else {
+    check_tensors({{"query", &query}});
+  }
+  FLEXATT_ASSERT(query.size(1) > 0, "query must have a head");
+  wq = check_weight(wq, "query_weight", query);
+  check_eps(eps);
+  freq = check_frequencies(freq, query.size(3), query.device());
+  Tensor qo, ko;
+  {
+    pybind11::gil_scoped_release no_gil;
+    if (at::GradMode::is_enabled() && (query.requires_grad() || wq.requires_grad() || (key && key->requires_grad()) ||
+                                       (wk && wk->requires_grad()))) {
+      const auto out = NormRotary::apply(query, key, wq, wk, freq, pos, interleaved, magnitude, eps);
+      qo = out[0];
+      if (key) ko = out[1];
+    } else {
+      std::tie(qo, ko) = norm_rotate(query, key ? *key : Tensor(), wq, wk ? *wk : Tensor(), freq, pos, interleaved,
+                                     magnitude, eps);
+    }
+  }
+  return pair_of(qo, ko);
+  END_HANDLE_TH_ERRORS
+}
+
 // ----------------------------------------------------------------------- cache --
 void check_cache(const Tensor& query, const Tensor& kc, const Tensor& vc) {
   FLEXATT_ASSERT(kc.sizes() == vc.sizes(), "key and value cache shapes must match");
@@ -339,13 +508,55 @@ void check_cache(const Tensor& query, const Tensor& kc, const Tensor& vc) {
   FLEXATT_ASSERT(kc.size(1) > 0 && query.size(1) % kc.size(1) == 0, "Hq must be divisible by Hkv");
 }
 
+// New tokens for a cache: what the appends check, and hand over.
+struct Append {
+  flexatt_rotary r;
+  flexatt_norm n;
+  bool normed = false, queried;
+  Tensor q, k, v, qo, lengths, freq, wq, wk;
+  flexatt_tensor tq, tk, tv, to, tkc, tvc;
+  int32_t rows;
+};
+// False: there is nothing to write.
+bool check_append(Append& x, const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& kc,
+                  const Tensor& vc, const Tensor& lengths, const OptTensor& freq, const OptTensor& pos, bool interleaved,
+                  double magnitude) {
+  const int64_t B = query.size(0), S = query.size(2), D = query.size(3), hkv = kc.size(1), C = kc.size(2);
+  const c10::Device dev = query.device();
+  const std::array<int64_t, 4> shape = {B, hkv, S, D};
+  FLEXATT_ASSERT(key.sizes() == at::IntArrayRef(shape) && value.sizes() == at::IntArrayRef(shape),
+                 "key and value must be [B, Hkv, S, D]");
+  x.lengths = per_sequence(lengths, "lengths", B, dev);
+  x.freq = freq ? check_frequencies(*freq, D, dev) : Tensor();
+  x.r = rotary_struct(query, hkv, x.freq, pos, interleaved, magnitude, false);
+  in_place(kc, "key_cache");
+  in_place(vc, "value_cache");
+  TORCH_CHECK(C > 0, "the cache has no rows");
+  x.rows = size32(C, "the cache's rows");
+  x.qo = out_like(query);
+  if (key.numel() == 0) return false;
+  x.queried = query.size(1) > 0;
+  x.q = prepare(query), x.k = prepare(key), x.v = prepare(value);
+  x.tq = view(x.q), x.tk = view(x.k), x.tv = view(x.v), x.to = view(x.qo), x.tkc = view(kc), x.tvc = view(vc);
+  return true;
+}
+// The norms' weights of an append (key's without a query head).
+void check_append_norm(Append& x, const Tensor& query, const Tensor& wq, const Tensor& wk, double eps) {
+  no_derivatives({{"query_weight", &wq}, {"key_weight", &wk}});
+  x.wq = check_weight(wq, "query_weight", query);
+  x.wk = check_weight(wk, "key_weight", query);
+  check_eps(eps);
+  x.n = norm_struct(query.size(1) > 0 ? x.wq : Tensor(), x.wk, eps);
+  x.normed = true;
+}
+
 PyObject* py_rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want(n, 10, "rotary_append");
   no_trace();
   const Tensor query = tensor_arg(a[0], "query"), key = tensor_arg(a[1], "key"), value = tensor_arg(a[2], "value");
   const Tensor kc = tensor_arg(a[3], "key_cache"), vc = tensor_arg(a[4], "value_cache");
-  Tensor lengths = tensor_arg(a[5], "lengths");
+  const Tensor lengths = tensor_arg(a[5], "lengths");
   const OptTensor freq = opt_tensor_arg(a[6], "inv_freq"), pos = opt_tensor_arg(a[7], "positions");
   const bool interleaved = bool_arg(a[8]);
   const double magnitude = double_arg(a[9]);
@@ -353,30 +564,170 @@ PyObject* py_rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   no_derivatives({{"query", &query}, {"key", &key}, {"value", &value}, {"key_cache", &kc}, {"value_cache", &vc}});
   check_tensors({{"query", &query}, {"key", &key}, {"value", &value}, {"key_cache", &kc}, {"value_cache", &vc}});
   check_cache(query, kc, vc);
-  const int64_t B = query.size(0), S = query.size(2), D = query.size(3), hkv = kc.size(1), C = kc.size(2);
   const c10::Device dev = query.device();
-  const std::array<int64_t, 4> shape = {B, hkv, S, D};
-  FLEXATT_ASSERT(key.sizes() == at::IntArrayRef(shape) && value.sizes() == at::IntArrayRef(shape),
-                 "key and value must be [B, Hkv, S, D]");
-  lengths = per_sequence(lengths, "lengths", B, dev);
   const c10::OptionalDeviceGuard guard(dev);
-  const Tensor f = freq ? check_frequencies(*freq, D, dev) : Tensor();
-  const flexatt_rotary r = rotary_struct(query, hkv, f, pos, interleaved, magnitude, false);
-  in_place(kc, "key_cache");
-  in_place(vc, "value_cache");
-  TORCH_CHECK(C > 0, "the cache has no rows");
-  Tensor qo = out_like(query);
-  if (key.numel() > 0) {
-    const bool queried = query.size(1) > 0;
-    const Tensor q = prepare(query), k = prepare(key), v = prepare(value);
-    const flexatt_tensor tq = view(q), tk = view(k), tv = view(v), to = view(qo), tkc = view(kc), tvc = view(vc);
-    check_status(flexatt_rotary_append(&r, queried ? &tq : nullptr, &tk, &tv, queried ? &to : nullptr, &tkc, &tvc,
-                                       size32(C, "the cache's rows"), lengths.const_data_ptr<int32_t>(), stream_of(dev)),
+  Append x;
+  if (check_append(x, query, key, value, kc, vc, lengths, freq, pos, interleaved, magnitude)) {
+    check_status(flexatt_rotary_append(&x.r, x.queried ? &x.tq : nullptr, &x.tk, &x.tv, x.queried ? &x.to : nullptr,
+                                       &x.tkc, &x.tvc, x.rows, x.lengths.const_data_ptr<int32_t>(), stream_of(dev)),
                  "flexatt_rotary_append");
     written(kc);
     written(vc);
   }
-  return THPVariable_Wrap(qo);
+  return THPVariable_Wrap(x.qo);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_norm_rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  want(n, 13, "norm_rotary_append");
+  no_trace();
+  const Tensor query = tensor_arg(a[0], "query"), key = tensor_arg(a[1], "key"), value = tensor_arg(a[2], "value");
+  const Tensor kc = tensor_arg(a[3], "key_cache"), vc = tensor_arg(a[4], "value_cache");
+  const Tensor lengths = tensor_arg(a[5], "lengths");
+  const Tensor wq = tensor_arg(a[6], "query_weight"), wk = tensor_arg(a[7], "key_weight");
+  const OptTensor freq = opt_tensor_arg(a[8], "inv_freq"), pos = opt_tensor_arg(a[9], "positions");
+  const bool interleaved = bool_arg(a[10]);
+  const double magnitude = double_arg(a[11]), eps = double_arg(a[12]);
+  if (freq) no_derivatives({{"inv_freq", &*freq}});
+  no_derivatives({{"query", &query}, {"key", &key}, {"value", &value}, {"key_cache", &kc}, {"value_cache", &vc}});
+  check_tensors({{"query", &query}, {"key", &key}, {"value", &value}, {"key_cache", &kc}, {"value_cache", &vc}});
+  check_cache(query, kc, vc);
+  const c10::Device dev = query.device();
+  const c10::OptionalDeviceGuard guard(dev);
+  Append x;
+  check_append_norm(x, query, wq, wk, eps);
+  if (check_append(x, query, key, value, kc, vc, lengths, freq, pos, interleaved, magnitude)) {
+    check_status(flexatt_norm_rotary_append(&x.r, &x.n, x.queried ? &x.tq : nullptr, &x.tk, &x.tv,
+                                            x.queried ? &x.to : nullptr, &x.tkc, &x.tvc, x.rows,
+                                            x.lengths.const_data_ptr<int32_t>(), stream_of(dev)),
+                 "flexatt_norm_rotary_append");
+    written(kc);
+    written(vc);
+  }
+  return THPVariable_Wrap(x.qo);
+  END_HANDLE_TH_ERRORS
+}
+
+// ------------------------------------------------------------- a cache of 8 bits --
+int32_t code_of(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat8_e4m3fn: return FLEXATT_E4M3;
+    case at::kChar: return FLEXATT_INT8;
+    default:
+      TORCH_CHECK(false, "unsupported cache dtype ", t.scalar_type(), " (expected float8_e4m3fn or int8)");
+  }
+}
+// Caches of one 8-bit dtype on `dev`, and their scales; `write`: they are written in place.
+int32_t check_codes(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, c10::Device dev, bool write) {
+  no_derivatives({{"key_cache", &kc}, {"value_cache", &vc}, {"key_scales", &ks}, {"value_scales", &vs}});
+  for (const Named& x : {Named{"key_cache", &kc}, Named{"value_cache", &vc}}) {
+    TORCH_CHECK(x.t->device() == dev, x.name, " must be on ", dev, " (got ", x.t->device(), ")");
+    TORCH_CHECK(x.t->dim() == 4 && x.t->layout() == at::kStrided, x.name, " must be a strided tensor of four dimensions");
+  }
+  const int32_t code = code_of(kc);
+  TORCH_CHECK(vc.scalar_type() == kc.scalar_type(), "value_cache has dtype ", vc.scalar_type(), ", expected ",
+              kc.scalar_type());
+  FLEXATT_ASSERT(kc.sizes() == vc.sizes(), "key and value cache shapes must match");
+  for (const Named& x : {Named{"key_scales", &ks}, Named{"value_scales", &vs}}) {
+    const Tensor& t = *x.t;
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.dim() == 3 && t.size(0) == kc.size(0) && t.size(1) == kc.size(1) &&
+                    t.size(2) == kc.size(2) && t.device() == dev,
+                x.name, " must be an fp32 [B, Hkv, C] = [", kc.size(0), ", ", kc.size(1), ", ", kc.size(2),
+                "] tensor on ", dev);
+    TORCH_CHECK(!write || t.is_contiguous(), x.name, " is written in place: it must be contiguous");
+  }
+  return code;
+}
+
+PyObject* py_quant_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  want(n, 15, "quant_append");
+  no_trace();
+  const Tensor query = tensor_arg(a[0], "query"), key = tensor_arg(a[1], "key"), value = tensor_arg(a[2], "value");
+  const Tensor kc = tensor_arg(a[3], "key_cache"), vc = tensor_arg(a[4], "value_cache");
+  const Tensor ks = tensor_arg(a[5], "key_scales"), vs = tensor_arg(a[6], "value_scales");
+  const Tensor lengths = tensor_arg(a[7], "lengths");
+  const OptTensor freq = opt_tensor_arg(a[8], "inv_freq"), pos = opt_tensor_arg(a[9], "positions");
+  const bool interleaved = bool_arg(a[10]);
+  const double magnitude = double_arg(a[11]);
+  const OptTensor wq = opt_tensor_arg(a[12], "query_weight"), wk = opt_tensor_arg(a[13], "key_weight");
+  if (freq) no_derivatives({{"inv_freq", &*freq}});
+  no_derivatives({{"query", &query}, {"key", &key}, {"value", &value}});
+  check_tensors({{"query", &query}, {"key", &key}, {"value", &value}});
+  const c10::Device dev = query.device();
+  const int32_t code = check_codes(kc, vc, ks, vs, dev, true);
+  check_cache(query, kc, vc);
+  const c10::OptionalDeviceGuard guard(dev);
+  Append x;
+  TORCH_CHECK(wq.has_value() == wk.has_value(), "query_weight and key_weight go together");
+  if (wk) check_append_norm(x, query, *wq, *wk, double_arg(a[14]));
+  if (check_append(x, query, key, value, kc, vc, lengths, freq, pos, interleaved, magnitude)) {
+    check_status(flexatt_quant_append(&x.r, x.normed ? &x.n : nullptr, code, x.queried ? &x.tq : nullptr, &x.tk, &x.tv,
+                                      x.queried ? &x.to : nullptr, &x.tkc, &x.tvc, ks.mutable_data_ptr<float>(),
+                                      vs.mutable_data_ptr<float>(), x.rows, x.lengths.const_data_ptr<int32_t>(),
+                                      stream_of(dev)),
+                 "flexatt_quant_append");
+    for (const Tensor* t : {&kc, &vc, &ks, &vs}) written(*t);
+  }
+  return THPVariable_Wrap(x.qo);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_dequant(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  want(n, 8, "dequant");
+  no_trace();
+  const Tensor kc = tensor_arg(a[0], "key_cache"), vc = tensor_arg(a[1], "value_cache");
+  const Tensor ks = tensor_arg(a[2], "key_scales"), vs = tensor_arg(a[3], "value_scales");
+  Tensor lengths = tensor_arg(a[4], "lengths");
+  const bool fresh = a[6] == Py_None;
+  TORCH_CHECK(kc.is_cuda(), "key_cache must be on a ROCm GPU device (got ", kc.device(), ")");
+  const c10::Device dev = kc.device();
+  const int32_t code = check_codes(kc, vc, ks, vs, dev, false);
+  const c10::OptionalDeviceGuard guard(dev);
+  const int64_t B = kc.size(0), H = kc.size(1), C = kc.size(2), D = kc.size(3);
+  TORCH_CHECK(D == 32 || D == 64 || D == 128 || D == 256, "unsupported head dim ", D, " (expected one of 32, 64, 128, 256)");
+  lengths = per_sequence(lengths, "lengths", B, dev);
+  Tensor ko, vo;
+  if (fresh) {
+    TORCH_CHECK(THPDtype_Check(a[5]), "dtype must be a torch.dtype");
+    const auto options = kc.options().dtype(((THPDtype*)a[5])->scalar_type);
+    ko = at::empty({B, H, C, D}, options);
+    vo = at::empty({B, H, C, D}, options);
+    check_tensors({{"key", &ko}});
+  } else {
+    ko = tensor_arg(a[6], "out key");
+    vo = tensor_arg(a[7], "out value");
+    no_derivatives({{"out key", &ko}, {"out value", &vo}});
+    check_tensors({{"out key", &ko}, {"out value", &vo}});
+    TORCH_CHECK(ko.device() == dev && ko.sizes() == kc.sizes() && vo.sizes() == kc.sizes(),
+                "out key and value must be [B, Hkv, C, D] = ", kc.sizes(), " on ", dev);
+    in_place(ko, "out key");
+    in_place(vo, "out value");
+  }
+  if (kc.numel() > 0) {
+    flexatt_dequant p = {};
+    p.dtype = dtype_of(ko);
+    p.code = code;
+    p.batch = size32(B, "batch");
+    p.heads_kv = size32(H, "Hkv");
+    p.cache_rows = size32(C, "the cache's rows");
+    p.head_dim = (int32_t)D;
+    p.fill = fresh;
+    p.lengths = lengths.const_data_ptr<int32_t>();
+    const Tensor k = prepare(kc), v = prepare(vc), sk = ks.contiguous(), sv = vs.contiguous();
+    const flexatt_tensor tk = view(k), tv = view(v), tko = view(ko), tvo = view(vo);
+    check_status(flexatt_dequant_rows(&p, &tk, &tv, sk.const_data_ptr<float>(), sv.const_data_ptr<float>(), &tko, &tvo,
+                                      stream_of(dev)),
+                 "flexatt_dequant_rows");
+    if (!fresh) {
+      written(ko);
+      written(vo);
+    }
+  }
+  if (fresh) return pair_of(ko, vo);
+  return PyTuple_Pack(2, a[6], a[7]);
   END_HANDLE_TH_ERRORS
 }
 
@@ -396,38 +747,34 @@ ScoreParams score_params(PyObject* scale, PyObject* cap, PyObject* window, int64
   return s;
 }
 
-PyObject* py_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  want(n, 10, "tree_attention");
-  no_trace();
-  const Tensor query = tensor_arg(a[0], "query");
-  const Tensor kc = tensor_arg(a[1], "key_cache"), vc = tensor_arg(a[2], "value_cache");
-  Tensor lengths = tensor_arg(a[3], "lengths");
-  const OptTensor mask = opt_tensor_arg(a[4], "tree_mask"), depth = opt_tensor_arg(a[6], "depths");
-  no_derivatives({{"query", &query}, {"key_cache", &kc}, {"value_cache", &vc}});
-  check_tensors({{"query", &query}, {"key_cache", &kc}, {"value_cache", &vc}});
-  check_cache(query, kc, vc);
-  const int64_t B = query.size(0), Hq = query.size(1), T = query.size(2), D = query.size(3), C = kc.size(2);
+// Drafted tokens over a cache of C rows: what the attention calls over one check, and
+// hand over (m and d hold what p points to).
+struct Drafted {
+  flexatt_tree p;
+  Tensor lengths, m, d, O, lse;
+};
+Drafted check_drafted(const Tensor& query, int64_t Hkv, int64_t C, const Tensor& lengths, const OptTensor& mask,
+                      PyObject* window, const OptTensor& depth, PyObject* scale, PyObject* cap) {
+  const int64_t B = query.size(0), Hq = query.size(1), T = query.size(2), D = query.size(3);
   const c10::Device dev = query.device();
-  const c10::OptionalDeviceGuard guard(dev);
+  Drafted x = {};
   TORCH_CHECK(T <= C, T, " drafted tokens do not fit a cache of ", C, " rows");
-  lengths = per_sequence(lengths, "lengths", B, dev);
-  const ScoreParams s = score_params(a[7], a[8], a[5], D);
-  const bool return_lse = bool_arg(a[9]);
-  flexatt_tree p = {};
+  x.lengths = per_sequence(lengths, "lengths", B, dev);
+  const ScoreParams s = score_params(scale, cap, window, D);
+  flexatt_tree& p = x.p;
   p.dtype = dtype_of(query);
   p.batch = size32(B, "batch");
   p.heads_q = size32(Hq, "Hq");
-  p.heads_kv = size32(kc.size(1), "Hkv");
+  p.heads_kv = size32(Hkv, "Hkv");
   p.tokens = size32(T, "T");
   p.cache_rows = size32(C, "the cache's rows");
   p.head_dim = (int32_t)D;
   p.scale = s.scale;
   p.soft_cap = s.cap;
   p.sliding_window = s.window;
-  p.lengths = lengths.const_data_ptr<int32_t>();
-  Tensor m, d;
+  p.lengths = x.lengths.const_data_ptr<int32_t>();
   if (mask) {
+    Tensor& m = x.m;
     m = *mask;
     TORCH_CHECK(at::isIntegralType(m.scalar_type(), true), "tree_mask must be a bool or integer tensor");
     TORCH_CHECK((m.dim() == 2 || (m.dim() == 3 && (m.size(0) == 1 || m.size(0) == B))) && m.size(-1) == T &&
@@ -442,6 +789,7 @@ PyObject* py_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (s.window > 0) {
     TORCH_CHECK(depth || !mask, "sliding_window with a tree_mask needs depths");
     if (depth) {
+      Tensor& d = x.d;
       d = *depth;
       TORCH_CHECK(d.scalar_type() == at::kInt && d.device() == dev, "depths must be an int32 tensor on ", dev);
       TORCH_CHECK((d.dim() == 1 || (d.dim() == 2 && (d.size(0) == 1 || d.size(0) == B))) && d.size(-1) == T,
@@ -450,23 +798,77 @@ PyObject* py_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       p.depths = d.const_data_ptr<int32_t>();
     }
   }
-  Tensor O = out_like(query);
-  Tensor lse = at::empty({B, Hq, T}, query.options().dtype(at::kFloat).requires_grad(false));
+  x.O = out_like(query);
+  x.lse = at::empty({B, Hq, T}, query.options().dtype(at::kFloat).requires_grad(false));
+  return x;
+}
+// (the kernels' row offsets within a tile are 32 bits)
+Tensor near_rows(const Tensor& t) {
+  return t.size(2) == 1 || t.stride(2) * t.element_size() < 1 << 26 ? prepare(t) : t.contiguous();
+}
+PyObject* attended(const Drafted& x, bool return_lse) {
+  if (return_lse) return pair_of(x.O, x.lse);
+  return THPVariable_Wrap(x.O);
+}
+
+PyObject* py_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  want(n, 10, "tree_attention");
+  no_trace();
+  const Tensor query = tensor_arg(a[0], "query");
+  const Tensor kc = tensor_arg(a[1], "key_cache"), vc = tensor_arg(a[2], "value_cache");
+  const Tensor lengths = tensor_arg(a[3], "lengths");
+  const OptTensor mask = opt_tensor_arg(a[4], "tree_mask"), depth = opt_tensor_arg(a[6], "depths");
+  no_derivatives({{"query", &query}, {"key_cache", &kc}, {"value_cache", &vc}});
+  check_tensors({{"query", &query}, {"key_cache", &kc}, {"value_cache", &vc}});
+  check_cache(query, kc, vc);
+  const c10::Device dev = query.device();
+  const c10::OptionalDeviceGuard guard(dev);
+  const Drafted x = check_drafted(query, kc.size(1), kc.size(2), lengths, mask, a[5], depth, a[7], a[8]);
+  const bool return_lse = bool_arg(a[9]);
   if (query.numel() > 0) {
-    // (the kernels' row offsets within a tile are 32 bits)
-    const auto near = [](const Tensor& t) {
-      return t.size(2) == 1 || t.stride(2) * t.element_size() < 1 << 26 ? prepare(t) : t.contiguous();
-    };
-    const Tensor q = prepare(query), k = near(kc), v = near(vc);
-    const size_t bytes = flexatt_tree_fwd_workspace(&p);
+    const Tensor q = prepare(query), k = near_rows(kc), v = near_rows(vc);
+    const size_t bytes = flexatt_tree_fwd_workspace(&x.p);
     const Tensor ws = workspace(bytes, dev);
-    const flexatt_tensor tq = view(q), tk = view(k), tv = view(v), to = view(O);
-    check_status(flexatt_tree_fwd(&p, &tq, &tk, &tv, &to, lse.mutable_data_ptr<float>(), data_or_null(ws),
+    const flexatt_tensor tq = view(q), tk = view(k), tv = view(v), to = view(x.O);
+    check_status(flexatt_tree_fwd(&x.p, &tq, &tk, &tv, &to, x.lse.mutable_data_ptr<float>(), data_or_null(ws),
                                   ws.defined() ? bytes : 0, stream_of(dev)),
                  "flexatt_tree_fwd");
   }
-  if (return_lse) return pair_of(O, lse);
-  return THPVariable_Wrap(O);
+  return attended(x, return_lse);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_quant_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  want(n, 12, "quant_tree_attention");
+  no_trace();
+  const Tensor query = tensor_arg(a[0], "query");
+  const Tensor kc = tensor_arg(a[1], "key_cache"), vc = tensor_arg(a[2], "value_cache");
+  const Tensor ks = tensor_arg(a[3], "key_scales"), vs = tensor_arg(a[4], "value_scales");
+  const Tensor lengths = tensor_arg(a[5], "lengths");
+  const OptTensor mask = opt_tensor_arg(a[6], "tree_mask"), depth = opt_tensor_arg(a[8], "depths");
+  no_derivatives({{"query", &query}});
+  check_tensors({{"query", &query}});
+  const c10::Device dev = query.device();
+  TORCH_CHECK(query.scalar_type() != at::kFloat, "a cache of 8 bits is attended by float16 or bfloat16 queries (for float32, "
+              "read it back with dequantize_cache)");
+  const int32_t code = check_codes(kc, vc, ks, vs, dev, false);
+  check_cache(query, kc, vc);
+  const c10::OptionalDeviceGuard guard(dev);
+  const Drafted x = check_drafted(query, kc.size(1), kc.size(2), lengths, mask, a[7], depth, a[9], a[10]);
+  const bool return_lse = bool_arg(a[11]);
+  if (query.numel() > 0) {
+    const Tensor q = prepare(query), k = near_rows(kc), v = near_rows(vc), sk = ks.contiguous(), sv = vs.contiguous();
+    const size_t bytes = flexatt_quant_tree_fwd_workspace(&x.p);
+    const Tensor ws = workspace(bytes, dev);
+    const flexatt_tensor tq = view(q), tk = view(k), tv = view(v), to = view(x.O);
+    check_status(flexatt_quant_tree_fwd(&x.p, code, &tq, &tk, &tv, sk.const_data_ptr<float>(), sv.const_data_ptr<float>(),
+                                        &to, x.lse.mutable_data_ptr<float>(), data_or_null(ws), ws.defined() ? bytes : 0,
+                                        stream_of(dev)),
+                 "flexatt_quant_tree_fwd");
+  }
+  return attended(x, return_lse);
   END_HANDLE_TH_ERRORS
 }
 
@@ -630,6 +1032,11 @@ PyMethodDef kMethods[] = {
     {"rotary", (PyCFunction)(void (*)())py_rotary, METH_FASTCALL, nullptr},
     {"rotary_append", (PyCFunction)(void (*)())py_rotary_append, METH_FASTCALL, nullptr},
     {"tree_attention", (PyCFunction)(void (*)())py_tree_attention, METH_FASTCALL, nullptr},
+    {"norm_rotary", (PyCFunction)(void (*)())py_norm_rotary, METH_FASTCALL, nullptr},
+    {"norm_rotary_append", (PyCFunction)(void (*)())py_norm_rotary_append, METH_FASTCALL, nullptr},
+    {"quant_append", (PyCFunction)(void (*)())py_quant_append, METH_FASTCALL, nullptr},
+    {"dequant", (PyCFunction)(void (*)())py_dequant, METH_FASTCALL, nullptr},
+    {"quant_tree_attention", (PyCFunction)(void (*)())py_quant_tree_attention, METH_FASTCALL, nullptr},
     {"weight_sums", (PyCFunction)(void (*)())py_weight_sums, METH_FASTCALL, nullptr},
     {"evict", (PyCFunction)(void (*)())py_evict, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -14,6 +14,15 @@ apart).
   tree_attention(...)         drafted tokens (or one new token) over cache and tree
   attention_weight_sums(...)  sum over the query rows of the softmax weights, per key
   evict_cache(...)            the rows worth keeping, copied to a smaller cache
+  norm_rotary_append(...)     rotary_append behind a norm of each head of query and key
+
+A cache may hold 8 bits an element: ``key_cache`` / ``value_cache`` of float8_e4m3fn or
+int8 and ``key_scales`` / ``value_scales``, float32 [B, Hkv, C] (contiguous where they
+are written), one scale for each row of each head; a row stands for codes * scale.
+
+  quantized_append(...)          the appends, into such a cache
+  dequantize_cache(...)          such a cache in a wider type again
+  quantized_tree_attention(...)  tree_attention over such a cache
 
 None of them is differentiable: a tensor that carries a tangent, or with gradients
 on one that requires them, is refused.  Nor can they be traced (``make_fx``, export,
@@ -21,9 +30,12 @@ fake tensors); ``torch.compile`` breaks its graph at them.
 """
 from __future__ import annotations
 
+import torch
+
 import flexatt_lib as _lib
 
-__all__ = ["rotary_append", "tree_attention", "attention_weight_sums", "evict_cache"]
+__all__ = ["rotary_append", "tree_attention", "attention_weight_sums", "evict_cache", "norm_rotary_append",
+           "quantized_append", "dequantize_cache", "quantized_tree_attention"]
 
 
 def rotary_append(query, key, value, key_cache, value_cache, lengths, inv_freq, positions=None, interleaved=False,
@@ -113,3 +125,56 @@ def evict_cache(key_cache, value_cache, scores, lengths, keep, recent=0, sinks=0
     if out is not None and key is None:
         raise RuntimeError("out must be (key, value, scores)")
     return _lib.native().evict(key_cache, value_cache, scores, lengths, keep, recent, sinks, key, value, kept)
+
+
+def norm_rotary_append(query, key, value, key_cache, value_cache, lengths, query_weight, key_weight, inv_freq,
+                       positions=None, interleaved=False, magnitude=1.0, eps=1e-6):
+    """:func:`rotary_append` with each head of query and key normalised before its rotation,
+    as :func:`flexatt_rotary.norm_rotary_embedding` does it.  ``inv_freq=None`` rotates
+    nothing.
+    """
+    return _lib.native().norm_rotary_append(query, key, value, key_cache, value_cache, lengths, query_weight, key_weight,
+                                            inv_freq, positions, interleaved, magnitude, eps)
+
+
+def quantized_append(query, key, value, key_cache, value_cache, key_scales, value_scales, lengths, inv_freq,
+                     positions=None, interleaved=False, magnitude=1.0, query_weight=None, key_weight=None, eps=1e-6):
+    """:func:`rotary_append`, with both weights :func:`norm_rotary_append`, into a cache of 8
+    bits; returns ``query'``, in query's dtype.
+
+    A row's scale is its largest size (at least 2 ** -100) over the largest code, 448
+    (float8_e4m3fn) or 127 (int8), and its codes are the values over the scale, rounded to
+    the nearest, of two the even one; keys are rounded nowhere before.  A row with an
+    infinity or NaN gets codes of 0 and a scale of NaN.  Rows of the cache and its scales
+    that no token goes to are left as they were; the new tokens, both caches and both
+    scales share no memory.
+    """
+    return _lib.native().quant_append(query, key, value, key_cache, value_cache, key_scales, value_scales, lengths, inv_freq,
+                                      positions, interleaved, magnitude, query_weight, key_weight, eps)
+
+
+def dequantize_cache(key_cache, value_cache, key_scales, value_scales, lengths, dtype=torch.bfloat16, out=None):
+    """``(key, value)`` [B, Hkv, C, D] of ``dtype`` (float32, float16, bfloat16): codes times
+    scales, rounded once, of the first ``lengths[b]`` rows of each sequence (outside [0, C]
+    the nearer end) and zeros behind them.
+
+    ``out=(key, value)`` receives them instead, in its own dtype, tensors that share no
+    memory with the cache or each other; rows behind the lengths are left as they were.
+    """
+    key, value = (None, None) if out is None else out
+    if out is not None and (key is None or value is None):
+        raise RuntimeError("out must be (key, value)")
+    return _lib.native().dequant(key_cache, value_cache, key_scales, value_scales, lengths, dtype, key, value)
+
+
+def quantized_tree_attention(query, key_cache, value_cache, key_scales, value_scales, lengths, tree_mask=None,
+                             sliding_window=0, depths=None, scale=None, soft_cap=0.0, return_lse=False):
+    """:func:`tree_attention` over a cache of 8 bits, for float16 and bfloat16 queries; the
+    other arguments and results are the same.
+
+    Scores are products with the codes times the key's scale, in 32 bits.  A weight times
+    its value's scale is rounded to the query's dtype.  Scales of rows that a token does
+    not see must be finite, as their values.
+    """
+    return _lib.native().quant_tree_attention(query, key_cache, value_cache, key_scales, value_scales, lengths, tree_mask,
+                                              sliding_window, depths, scale, soft_cap, return_lse)

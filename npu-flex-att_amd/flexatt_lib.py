@@ -14,6 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libflexatt.so")
 
 F32, F16, BF16 = 0, 1, 2
+E4M3, INT8 = 1, 2  # enum flexatt_code
 
 # Entry points declared in include/flexatt.h.
 EXPORTS = (
@@ -47,10 +48,18 @@ EXPORTS = (
     "flexatt_weight_sums_workspace",
     "flexatt_weight_sums",
     "flexatt_evict_rows",
+    "flexatt_norm_rotary_apply",
+    "flexatt_norm_rotary_grad_workspace",
+    "flexatt_norm_rotary_grad",
+    "flexatt_norm_rotary_append",
+    "flexatt_quant_append",
+    "flexatt_dequant_rows",
+    "flexatt_quant_tree_fwd_workspace",
+    "flexatt_quant_tree_fwd",
     "flexatt_status_string",
     "flexatt_abi_version",
 )
-ABI_VERSION = 9
+ABI_VERSION = 10
 # Fixed scratch of flexatt_fwd_decode_noalloc (FLEXATT_NOALLOC_SCRATCH_BYTES).
 NOALLOC_SCRATCH_BYTES = 16 << 20
 # Work-queue counters at the end of the staged-dS workspace (FLEXATT_BWD_QUEUE_BYTES).
@@ -150,6 +159,26 @@ class Evict(ctypes.Structure):
     ]
 
 
+class Norm(ctypes.Structure):
+    """``flexatt_norm``: norm of each head before the rotation."""
+
+    _fields_ = [
+        ("weight_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+    ]
+
+
+class Dequant(ctypes.Structure):
+    """``flexatt_dequant``: a cache of 8 bits read back."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "code", "batch", "heads_kv", "cache_rows", "head_dim", "fill",
+                                              "reserved")] + [
+        ("lengths", ctypes.c_void_p),
+    ]
+
+
 _lib = None
 _native = None
 
@@ -193,6 +222,12 @@ def load() -> ctypes.CDLL:
         "flexatt_tree_fwd": [P(Tree), T, T, T, T, fp, fp, ctypes.c_size_t, st],
         "flexatt_weight_sums": [P(Weights), T, T, fp, fp, fp, ctypes.c_size_t, st],
         "flexatt_evict_rows": [P(Evict), T, T, fp, T, T, fp, fp, fp, st],
+        "flexatt_norm_rotary_apply": [P(Rotary), P(Norm), T, T, T, T, st],
+        "flexatt_norm_rotary_grad": [P(Rotary), P(Norm), T, T, T, T, T, T, fp, fp, fp, ctypes.c_size_t, st],
+        "flexatt_norm_rotary_append": [P(Rotary), P(Norm), T, T, T, T, T, T, ctypes.c_int32, fp, st],
+        "flexatt_quant_append": [P(Rotary), P(Norm), ctypes.c_int32, T, T, T, T, T, T, fp, fp, ctypes.c_int32, fp, st],
+        "flexatt_dequant_rows": [P(Dequant), T, T, fp, fp, T, T, st],
+        "flexatt_quant_tree_fwd": [P(Tree), ctypes.c_int32, T, T, T, fp, fp, T, fp, fp, ctypes.c_size_t, st],
     }
     for name, args in sig.items():
         fn = getattr(lib, name)
@@ -202,7 +237,8 @@ def load() -> ctypes.CDLL:
                  "flexatt_bwd_split_workspace", "flexatt_bwd_ws_parts_bytes"):
         getattr(lib, name).argtypes = [pr]
         getattr(lib, name).restype = ctypes.c_size_t
-    for name, arg in (("flexatt_tree_fwd_workspace", P(Tree)), ("flexatt_weight_sums_workspace", P(Weights))):
+    for name, arg in (("flexatt_tree_fwd_workspace", P(Tree)), ("flexatt_weight_sums_workspace", P(Weights)),
+                      ("flexatt_quant_tree_fwd_workspace", P(Tree)), ("flexatt_norm_rotary_grad_workspace", P(Rotary))):
         getattr(lib, name).argtypes = [arg]
         getattr(lib, name).restype = ctypes.c_size_t
     lib.flexatt_bwd_workspace_limited.argtypes = [pr, ctypes.c_size_t]

@@ -8,6 +8,7 @@ also writes new tokens into a K/V cache.
 
   rotary_frequencies(...)  angles per position of each pair, scaled for long contexts
   rotary_embedding(...)    differentiable rotation of query and key
+  norm_rotary_embedding(...)  the same behind a norm of each head, in one pass
 """
 from __future__ import annotations
 
@@ -18,7 +19,7 @@ import torch
 
 import flexatt_lib as _lib
 
-__all__ = ["rotary_frequencies", "rotary_embedding"]
+__all__ = ["rotary_frequencies", "rotary_embedding", "norm_rotary_embedding"]
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
@@ -92,3 +93,21 @@ def rotary_embedding(query, key, inv_freq, positions=None, interleaved=False, ma
     here.
     """
     return _lib.native().rotary(query, key, inv_freq, positions, interleaved, magnitude)
+
+
+def norm_rotary_embedding(query, key, query_weight, key_weight, inv_freq, positions=None, interleaved=False, magnitude=1.0,
+                          eps=1e-6):
+    """Each head of query and key normalised, then turned: ``(query', key')``.
+
+    A head's row ``x`` becomes the rotation (as :func:`rotary_embedding` gives it, with its
+    arguments) of ``x * weight / sqrt(mean(x ** 2) + eps)``, rounded once: squares, sums and
+    the norm are in 32 bits.  ``query_weight`` and ``key_weight``: [D], both of query's
+    dtype or both float32 (a model whose weights are offsets passes ``1 + w``).  Without a
+    key, key and key_weight are None.
+
+    Differentiable in query, key and both weights, in reverse mode and once: a backward pass
+    with ``create_graph`` is refused.  The weights' gradients are sums over all rows in 32
+    bits, in a fixed order.  What :func:`rotary_embedding` says of tangents, ``inv_freq``,
+    graphs and traces holds here.
+    """
+    return _lib.native().norm_rotary(query, key, query_weight, key_weight, inv_freq, positions, interleaved, magnitude, eps)

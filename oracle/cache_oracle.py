@@ -128,3 +128,75 @@ def evict(scores, n, keep, recent, sinks):
     free = range(sinks, n - recent)
     rank = sorted(free, key=lambda j: (0 if math.isnan(scores[j]) else 1, 0.0 if math.isnan(scores[j]) else -scores[j], j))
     return sorted(list(range(sinks)) + list(range(n - recent, n)) + rank[:keep - sinks - recent])
+
+
+def norm_rotary(x, w, inv_freq, positions, interleaved=False, magnitude=1.0, eps=1e-6):
+    """x [B, H, S, D], w [D] (float64): each head normalised and turned, and how far a kernel may be off per element.
+
+    A row's sum of squares has at most 16 fused steps a lane and 5 joins, 21 2^-24 of itself, the mean, eps and the
+    reciprocal root three more: 2^-20 of r in all.  Weight times sine and the product with r round twice more than the
+    rotation alone: 2^-19 (|x1 w1| + |x2 w2|) r."""
+    r = 1.0 / (x.square().mean(dim=-1, keepdim=True) + eps).sqrt()
+    y, slack = rotary(x * r * w, inv_freq, positions, interleaved, magnitude)
+    return y, slack * 4 + (x * r * w).abs() * 2.0 ** -19
+
+
+def norm_rotary_grad(x, w, gy, inv_freq, positions, interleaved=False, magnitude=1.0, eps=1e-6):
+    """The gradients of x and w, with their bounds: ((dx, slack), (dw, slack)).
+
+    g, the gradient turned back, is off by the rotation's bound; r by 2^-20 of itself; the row's sum of g w x by 24 2^-24
+    of its magnitudes.  dw adds up B S H products: a lane's heads one after the other, then at most 40 joins."""
+    D = x.shape[-1]
+    r = 1.0 / (x.square().mean(dim=-1, keepdim=True) + eps).sqrt()
+    g, eg = rotary(gy, inv_freq, positions, interleaved, magnitude, inverse=True)
+    gw = g * w
+    dot = (gw * x).sum(dim=-1, keepdim=True)
+    dx = r * (gw - x * (r * r / D) * dot)
+    off = (eg * (w * x).abs()).sum(dim=-1, keepdim=True) + (gw * x).abs().sum(dim=-1, keepdim=True) * 2.0 ** -18
+    sx = r * (eg * w.abs() + gw.abs() * 2.0 ** -19 + x.abs() * (r * r / D) * off)
+    terms = g * x * r
+    dw = terms.sum(dim=(0, 1, 2))
+    sw = (eg * (x * r).abs() + terms.abs() * (2.0 ** -19 + (x.shape[1] + 40) * 2.0 ** -24)).sum(dim=(0, 1, 2))
+    return (dx, sx), (dw, sw)
+
+
+TOP = {torch.float8_e4m3fn: 448.0, torch.int8: 127.0}
+
+
+def scale_of(y, code):
+    """The scales of rows y [..., D] (float64)."""
+    return y.abs().amax(dim=-1).clamp(min=2.0 ** -100) / TOP[code]
+
+
+def code_tolerance(y, slack, scale, code):
+    """How far code * scale may be from y, which the kernel has to `slack`: half a code's step (int8: half a scale; e4m3:
+    2^-4 of the value, at least half of its smallest step 2^-9), 2^-22 of the value for the scale's and quotient's
+    roundings."""
+    half = scale[..., None] / 2 if code == torch.int8 else torch.maximum(y.abs() * 2.0 ** -4, scale[..., None] * 2.0 ** -10)
+    return half + slack * (1 + 2.0 ** -4) + y.abs() * 2.0 ** -21
+
+
+def quantized_tree_attention(q, kc, vc, ks, vs, lengths, mask=None, window=0, depths=None, scale=None, cap=0.0,
+                             dtype=torch.bfloat16):
+    """O, LSE and their tolerances: those of :func:`tree_attention` over codes * scales.
+
+    The scales add two roundings to a score, 2^-23 of it, and one to a weight.  A weight times its value's scale is
+    rounded where p was; in fp16, relative to a power of two at most twice the largest scale, the numbers under 2^-14
+    have the step 2^-24: (n + T) 2^-24 times the largest scale and code."""
+    k, v = kc.double() * ks.double()[..., None], vc.double() * vs.double()[..., None]
+    O, LSE, tO, tL = tree_attention(q, k, v, lengths, mask, window, depths, scale, cap, dtype)
+    G, T = q.shape[1] // kc.shape[1], q.shape[2]
+    top = TOP[kc.dtype]
+    for b in range(q.shape[0]):
+        n = int(lengths[b])
+        if n < 0 or n + T > kc.shape[2]:
+            continue
+        for h in range(q.shape[1]):
+            x = (q[b, h].double().abs() @ k[b, h // G, :n + T].abs().T).amax() * (abs(scale) if scale is not None else
+                                                                                 1.0 / math.sqrt(q.shape[3]))
+            vmax = v[b, h // G, :n + T].abs().max()
+            tO[b, h] += 2 * x * 2.0 ** -23 * vmax + vmax * 2.0 ** -22
+            if dtype == torch.float16:
+                tO[b, h] += (n + T) * 2.0 ** -24 * vs[b, h // G, :n + T].double().max() * top
+            tL[b, h] += x * 2.0 ** -23
+    return O, LSE, tO, tL
