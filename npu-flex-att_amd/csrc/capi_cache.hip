@@ -153,6 +153,11 @@ const TreeLauncher kTree[3][4] = {
     {tree_attn_f16_d32, tree_attn_f16_d64, tree_attn_f16_d128, tree_attn_f16_d256},
     {tree_attn_bf16_d32, tree_attn_bf16_d64, tree_attn_bf16_d128, tree_attn_bf16_d256},
 };
+const PrefixLauncher kPrefix[3][4] = {
+    {prefix_attn_f32_d32, prefix_attn_f32_d64, prefix_attn_f32_d128, prefix_attn_f32_d256},
+    {prefix_attn_f16_d32, prefix_attn_f16_d64, prefix_attn_f16_d128, prefix_attn_f16_d256},
+    {prefix_attn_bf16_d32, prefix_attn_bf16_d64, prefix_attn_bf16_d128, prefix_attn_bf16_d256},
+};
 const WeightLauncher kWeights[3][4] = {
     {weight_sums_f32_d32, weight_sums_f32_d64, weight_sums_f32_d128, weight_sums_f32_d256},
     {weight_sums_f16_d32, weight_sums_f16_d64, weight_sums_f16_d128, weight_sums_f16_d256},
@@ -259,6 +264,28 @@ TreePlan quant_plan(const flexatt_tree* p) {
   const int share = quant_row_tiles(p->head_dim, row_tiles(p));
   return plan_of(p, share, p->head_dim >= 128 || share > 1 ? 1 : 2);
 }
+// The launch behind a shared prefix: its rows are those of all sequences, and its chunks
+// get their share of the workgroups that run at once, by key tiles times row tiles.
+struct PrefixPlan {
+  TreePlan own;
+  int np;
+};
+PrefixPlan prefix_plan(const flexatt_tree* p, int prefix_rows) {
+  const int rowb = p->head_dim * (int)elt_size(p->dtype);
+  const int64_t rows = (int64_t)(p->heads_q / p->heads_kv) * p->tokens, all = (rows * p->batch + 31) / 32;
+  const int share = tree_share(rowb, (int)elt_size(p->dtype), all), per_cu = rowb >= 256 ? 1 : 2;
+  PrefixPlan t;
+  t.own = plan_of(p, share, per_cu);
+  const int64_t groups = (all + share - 1) / share, tiles = (prefix_rows + 31) / 32;
+  const int64_t mine = groups * tiles, others = ((rows + 31) / 32 + share - 1) / share * p->batch * ((p->cache_rows + 31) / 32);
+  const int64_t slots = per_cu * cus();
+  int64_t np = (slots * mine / (mine + others) + groups * p->heads_kv / 2) / (groups * p->heads_kv);
+  const int64_t most = (tiles + 7) / 8;
+  if (np > most) np = most;
+  if (np > 64) np = 64;
+  t.np = np < 1 ? 1 : (int)np;
+  return t;
+}
 size_t tree_rows(const flexatt_tree* p) { return (size_t)p->batch * p->heads_q * p->tokens; }
 
 size_t plan_bytes(const flexatt_tree* p, const TreePlan& plan) {
@@ -292,6 +319,17 @@ TreeArgs tree_args(const flexatt_tree* p, const TreePlan& plan, const flexatt_te
   a.p = score_shape(p->batch, p->heads_q, p->heads_kv, p->tokens, p->cache_rows, p->scale, p->soft_cap,
                     p->sliding_window);
   return a;
+}
+
+size_t prefix_bytes(const flexatt_tree* p, const PrefixPlan& plan) {
+  return tree_rows(p) * (plan.np + plan.own.nsplit) * (p->head_dim + 1) * sizeof(float) +
+         (size_t)p->batch * p->heads_kv * sizeof(int);
+}
+int check_prefix(const flexatt_tree* p, int32_t prefix_rows) {
+  FLEXATT_TRY(check_tree(p));
+  if (prefix_rows < 1) return FLEXATT_EINVAL;
+  if ((int64_t)prefix_rows + p->cache_rows > 1 << 30) return FLEXATT_ESHAPE;
+  return FLEXATT_OK;
 }
 
 int check_workspace(size_t need, const void* workspace, size_t bytes) {
@@ -573,6 +611,38 @@ int flexatt_quant_tree_fwd(const flexatt_tree* p, int32_t code, const flexatt_te
   a.v_scales = v_scales;
   a.kind = code;
   return (int)kQuantTree[p->dtype == FLEXATT_BF16][head_index(p->head_dim)](a, (hipStream_t)stream);
+}
+
+size_t flexatt_prefix_fwd_workspace(const flexatt_tree* p, int32_t prefix_rows) {
+  return check_prefix(p, prefix_rows) != FLEXATT_OK ? SIZE_MAX : prefix_bytes(p, prefix_plan(p, prefix_rows));
+}
+
+int flexatt_prefix_fwd(const flexatt_tree* p, int32_t prefix_rows, const flexatt_tensor* q,
+                       const flexatt_tensor* prefix_k, const flexatt_tensor* prefix_v, const flexatt_tensor* k_cache,
+                       const flexatt_tensor* v_cache, const flexatt_tensor* o, float* lse, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  FLEXATT_TRY(check_prefix(p, prefix_rows));
+  FLEXATT_TRY(check_tensor(q, p->dtype));
+  for (const flexatt_tensor* x : {prefix_k, prefix_v, k_cache, v_cache}) {
+    FLEXATT_TRY(check_tensor(x, p->dtype));
+    const int rows = x == prefix_k || x == prefix_v ? prefix_rows : p->cache_rows;  // (as flexatt_tree_fwd)
+    if (rows > 1 && x->stride_s >= (1 << 26) / (int64_t)elt_size(p->dtype)) return FLEXATT_ERANGE;
+  }
+  FLEXATT_TRY(check_out_tensor(o, p->dtype, p->batch, p->heads_q, p->tokens, p->head_dim));
+  if (!lse) return FLEXATT_EINVAL;
+  const PrefixPlan plan = prefix_plan(p, prefix_rows);
+  FLEXATT_TRY(check_workspace(prefix_bytes(p, plan), workspace, workspace_bytes));
+  PrefixArgs a = {};
+  a.t = tree_args(p, plan.own, q, k_cache, v_cache, o, lse, nullptr);
+  a.np = plan.np;
+  a.pitch = plan.np + plan.own.nsplit;
+  a.t.part_o = (float*)workspace;
+  a.t.part_lse = a.t.part_o + tree_rows(p) * a.pitch * p->head_dim;
+  a.t.counts = (int*)(a.t.part_lse + tree_rows(p) * a.pitch);
+  a.k = view(prefix_k);
+  a.v = view(prefix_v);
+  a.P = prefix_rows;
+  return (int)kPrefix[p->dtype][head_index(p->head_dim)](a, (hipStream_t)stream);
 }
 
 size_t flexatt_weight_sums_workspace(const flexatt_weights* p) {

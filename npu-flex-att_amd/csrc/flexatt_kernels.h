@@ -159,6 +159,18 @@ struct TreeArgs {
   int nrt;        // groups of packed query row tiles per (b, hkv) (set by the launcher)
 };
 
+// The same behind a prefix that all sequences share (tree_attn.hip): t.nsplit is the most
+// chunks of a sequence's own cache.
+struct PrefixArgs {
+  TreeArgs t;
+  View k, v;  // [Hkv, P, D]: sh, ss
+  int P;
+  int np;     // chunks of the prefix, the first partials of every row
+  int pitch;  // partials of a row, np + t.nsplit
+  int npre;   // workgroups of the prefix, the first of the launch (set by the launcher)
+  int nrtp;   // groups of the prefix's row tiles, B * G * T rows (set by the launcher)
+};
+
 // The same over a cache of 8 bits (quant_attn.hip): t.k and t.v are bytes.
 struct QuantTreeArgs {
   TreeArgs t;
@@ -209,6 +221,7 @@ typedef hipError_t (*TreeLauncher)(const TreeArgs&, hipStream_t);
 // conversion costs, where registers hold them (quant_attn.hip).
 inline int quant_row_tiles(int head_dim, int64_t tiles) { return head_dim <= 128 && tiles > 1 ? 2 : 1; }
 
+typedef hipError_t (*PrefixLauncher)(const PrefixArgs&, hipStream_t);
 typedef hipError_t (*QuantTreeLauncher)(const QuantTreeArgs&, hipStream_t);
 typedef hipError_t (*NormRotaryLauncher)(int dtype, const NormRotaryArgs&, hipStream_t);
 typedef hipError_t (*WeightLauncher)(const WeightArgs&, hipStream_t);
@@ -252,6 +265,9 @@ hipError_t dequant_run(int dtype, const DequantArgs&, hipStream_t);
   hipError_t tree_attn_bf16_d##D(const TreeArgs&, hipStream_t); \
   hipError_t tree_attn_f16_d##D(const TreeArgs&, hipStream_t);  \
   hipError_t tree_attn_f32_d##D(const TreeArgs&, hipStream_t);  \
+  hipError_t prefix_attn_bf16_d##D(const PrefixArgs&, hipStream_t); \
+  hipError_t prefix_attn_f16_d##D(const PrefixArgs&, hipStream_t);  \
+  hipError_t prefix_attn_f32_d##D(const PrefixArgs&, hipStream_t);  \
   hipError_t weight_sums_bf16_d##D(const WeightArgs&, hipStream_t); \
   hipError_t weight_sums_f16_d##D(const WeightArgs&, hipStream_t);  \
   hipError_t weight_sums_f32_d##D(const WeightArgs&, hipStream_t);  \

@@ -839,6 +839,50 @@ PyObject* py_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* py_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  want(n, 12, "prefix_attention");
+  no_trace();
+  const Tensor query = tensor_arg(a[0], "query");
+  const Tensor pk3 = tensor_arg(a[1], "prefix_key"), pv3 = tensor_arg(a[2], "prefix_value");
+  const Tensor kc = tensor_arg(a[3], "key_cache"), vc = tensor_arg(a[4], "value_cache");
+  const Tensor lengths = tensor_arg(a[5], "lengths");
+  const OptTensor mask = opt_tensor_arg(a[6], "tree_mask"), depth = opt_tensor_arg(a[8], "depths");
+  no_derivatives({{"query", &query}, {"prefix_key", &pk3}, {"prefix_value", &pv3}, {"key_cache", &kc}, {"value_cache", &vc}});
+  FLEXATT_ASSERT(pk3.dim() == 3 && pv3.dim() == 3, "the prefix's key and value must be [Hkv, P, D]");
+  const Tensor pk = pk3.unsqueeze(0), pv = pv3.unsqueeze(0);
+  check_tensors({{"query", &query}, {"prefix_key", &pk}, {"prefix_value", &pv}, {"key_cache", &kc}, {"value_cache", &vc}});
+  check_cache(query, kc, vc);
+  FLEXATT_ASSERT(pk.sizes() == pv.sizes() && pk.size(1) == kc.size(1) && pk.size(3) == kc.size(3),
+                 "the prefix's key and value must be [Hkv, P, D] with the cache's Hkv and D");
+  const c10::Device dev = query.device();
+  const c10::OptionalDeviceGuard guard(dev);
+  const Drafted x = check_drafted(query, kc.size(1), kc.size(2), lengths, mask, a[7], depth, a[9], a[10]);
+  const bool return_lse = bool_arg(a[11]);
+  const int32_t rows = size32(pk.size(2), "the prefix's rows");
+  if (query.numel() > 0) {
+    const Tensor q = prepare(query), k = near_rows(kc), v = near_rows(vc);
+    const flexatt_tensor tq = view(q), tk = view(k), tv = view(v), to = view(x.O);
+    if (rows == 0) {  // nothing shared
+      const size_t bytes = flexatt_tree_fwd_workspace(&x.p);
+      const Tensor ws = workspace(bytes, dev);
+      check_status(flexatt_tree_fwd(&x.p, &tq, &tk, &tv, &to, x.lse.mutable_data_ptr<float>(), data_or_null(ws),
+                                    ws.defined() ? bytes : 0, stream_of(dev)),
+                   "flexatt_tree_fwd");
+    } else {
+      const Tensor sk = near_rows(pk), sv = near_rows(pv);
+      const flexatt_tensor tpk = view(sk), tpv = view(sv);
+      const size_t bytes = flexatt_prefix_fwd_workspace(&x.p, rows);
+      const Tensor ws = workspace(bytes, dev);
+      check_status(flexatt_prefix_fwd(&x.p, rows, &tq, &tpk, &tpv, &tk, &tv, &to, x.lse.mutable_data_ptr<float>(),
+                                      data_or_null(ws), ws.defined() ? bytes : 0, stream_of(dev)),
+                   "flexatt_prefix_fwd");
+    }
+  }
+  return attended(x, return_lse);
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* py_quant_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want(n, 12, "quant_tree_attention");
@@ -1036,6 +1080,7 @@ PyMethodDef kMethods[] = {
     {"norm_rotary_append", (PyCFunction)(void (*)())py_norm_rotary_append, METH_FASTCALL, nullptr},
     {"quant_append", (PyCFunction)(void (*)())py_quant_append, METH_FASTCALL, nullptr},
     {"dequant", (PyCFunction)(void (*)())py_dequant, METH_FASTCALL, nullptr},
+    {"prefix_attention", (PyCFunction)(void (*)())py_prefix_attention, METH_FASTCALL, nullptr},
     {"quant_tree_attention", (PyCFunction)(void (*)())py_quant_tree_attention, METH_FASTCALL, nullptr},
     {"weight_sums", (PyCFunction)(void (*)())py_weight_sums, METH_FASTCALL, nullptr},
     {"evict", (PyCFunction)(void (*)())py_evict, METH_FASTCALL, nullptr},

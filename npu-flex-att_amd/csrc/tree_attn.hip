@@ -47,6 +47,8 @@
 // alternative, two row tiles per wave of its own key tiles, reads LDS as little but has a
 // SIMD to itself (register file) and copies as much: the D=128 cases above 186 and 193 us.
 // Pairs instead of fours: 147 us for the latter, D=64 55 (fours 56).
+#include <type_traits>
+
 #include "flexatt_device.h"
 #include "flexatt_kernels.h"
 #include "tree_device.h"
@@ -112,12 +114,24 @@ __device__ __forceinline__ f32x16 mma_step(i32x4 k, i32x4 q, f32x16 c) {
 
 }  // namespace
 
+namespace {
+template <bool PRE>
+using ArgsOf = std::conditional_t<PRE, PrefixArgs, TreeArgs>;
+__device__ __forceinline__ const TreeArgs& tree_of(const TreeArgs& a) { return a; }
+__device__ __forceinline__ const TreeArgs& tree_of(const PrefixArgs& a) { return a.t; }
+}  // namespace
+
 // WPT neighbouring waves, a row tile each, share their key tiles: each copies its share of
 // a tile, and a barrier a tile keeps them in step.
-template <class T, int D, int NW, int WPT, bool CAP>
+//
+// PRE: the sequences share a prefix.  The launch's first workgroups have its chunks, whose
+// rows are those of all sequences (b, token, head, the head innermost), so that a key of
+// it is read once for all of them; the others have the sequences' own caches.
+template <class T, int D, int NW, int WPT, bool CAP, bool PRE>
 __global__ __launch_bounds__(NW * WPT * 64)
 __attribute__((amdgpu_waves_per_eu(D * sizeof(T) >= 256 ? (WPT == 1 ? 1 : 2) : WPT == 1 ? 2 : 4)))
-void tree_attn_kernel(TreeArgs a) {
+void tree_attn_kernel(ArgsOf<PRE> args) {
+  const TreeArgs& a = tree_of(args);
   using C = TreeCfg<T, D>;
   constexpr int ST = C::ST, EC = C::E / WPT;  // copies a wave makes of a tile
   constexpr int PK = C::PK > WPT ? C::PK / WPT : 1, PV = C::PV > WPT ? C::PV / WPT : 1, CROWS = WPT * C::RPC;
@@ -136,18 +150,39 @@ void tree_attn_kernel(TreeArgs a) {
   // other, they find the chunk gone from L2: fp16 B=4 Hq=28 Hkv=4 T=64, caches of
   // 16384 D=64, 58 -> 74 us)
   int rt0 = 0, x = blockIdx.x;
-  if (a.nrt > 1) {
+  bool shared = false;  // a chunk of the prefix
+  if constexpr (PRE) {
+    shared = x < args.npre;
+    if (!shared) x -= args.npre;
+    const int nrt = shared ? args.nrtp : a.nrt, i = x;
+    rt0 = i / 8 % nrt * WPT;
+    x = i / (8 * nrt) * 8 + i % 8;
+  } else if (a.nrt > 1) {
     rt0 = blockIdx.x / 8 % a.nrt * WPT;
     x = blockIdx.x / (8 * a.nrt) * 8 + blockIdx.x % 8;
   }
   rt0 += sub;
-  const TreeChunk ck = tree_chunk(a, x, NW);
-  if (ck.b < 0) return;
+  TreeChunk ck;
+  TreeSeq sq;
+  if (PRE && shared) {
+    if constexpr (PRE) {
+      if (x >= p.Hkv * args.np) return;
+      ck = prefix_chunk(args, x);
+      sq = TreeSeq{args.P, 0, 0, false};
+    }
+  } else {
+    ck = tree_chunk(a, x, NW);
+    if (ck.b < 0) return;
+    sq = tree_seq(a, ck.b);
+    sq.n = __builtin_amdgcn_readfirstlane(sq.n);
+    sq.t0 = __builtin_amdgcn_readfirstlane(sq.t0);
+  }
   const int b = ck.b, hk = ck.hk, s = ck.s, ns = ck.ns;
-  TreeSeq sq = tree_seq(a, b);
-  sq.n = __builtin_amdgcn_readfirstlane(sq.n);
-  sq.t0 = __builtin_amdgcn_readfirstlane(sq.t0);
-  if (rt0 == 0 && s == 0 && tid == 0 && a.counts) a.counts[b * p.Hkv + hk] = sq.bad ? 1 : ns;
+  if constexpr (PRE) {
+    if (!shared && rt0 == 0 && s == 0 && tid == 0) a.counts[b * p.Hkv + hk] = sq.bad ? 1 : args.np + ns;
+  } else {
+    if (rt0 == 0 && s == 0 && tid == 0 && a.counts) a.counts[b * p.Hkv + hk] = sq.bad ? 1 : ns;
+  }
 
   float c2 = p.scale_log2;
   bool flip = false;
@@ -170,7 +205,11 @@ void tree_attn_kernel(TreeArgs a) {
       voff[db] = tr_row * C::ROWB + swz_tr<C::CPR>(tr_row, 4 * db + (tr_col >> 3)) * 16 + (tr_col & 7) * 2;
   }
   // this lane's offsets in a tile's copies
-  const unsigned kss = (unsigned)(a.k.ss * (int)sizeof(T)), vss = (unsigned)(a.v.ss * (int)sizeof(T));
+  View vk = a.k, vv = a.v;
+  if constexpr (PRE) {
+    if (shared) vk = args.k, vv = args.v;
+  }
+  const unsigned kss = (unsigned)(vk.ss * (int)sizeof(T)), vss = (unsigned)(vv.ss * (int)sizeof(T));
   const int crow = lane / C::CPR + sub * C::RPC, cchunk = lane % C::CPR;
   unsigned kvo[PK], vvo[PV];
 #pragma unroll
@@ -182,9 +221,16 @@ void tree_attn_kernel(TreeArgs a) {
   auto reads_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
 
   // packed query rows of this lane
-  const int R = p.G * p.Sq;
+  const int R = PRE && shared ? p.B * p.G * p.Sq : p.G * p.Sq;
   const int r = min(32 * rt0 + l32, R - 1);
-  const int hq = hk * p.G + r % p.G, qi = r / p.G;  // head, drafted token
+  const int hq = hk * p.G + r % p.G;  // head, drafted token, sequence
+  int qi = r / p.G, qb = b;
+  if constexpr (PRE) {
+    if (shared) {
+      qb = qi / p.Sq;
+      qi -= qb * p.Sq;
+    }
+  }
 
   if (sq.bad) {
     if (s == 0 && 32 * rt0 + l32 < R) {
@@ -196,16 +242,16 @@ void tree_attn_kernel(TreeArgs a) {
   }
 
   i32x4 qf[C::KC];
-  const char* src = (const char*)((const T*)a.q.data + b * a.q.sb + hq * a.q.sh + (int64_t)qi * a.q.ss) + 16 * h;
+  const char* src = (const char*)((const T*)a.q.data + qb * a.q.sb + hq * a.q.sh + (int64_t)qi * a.q.ss) + 16 * h;
 #pragma unroll
   for (int kc = 0; kc < C::KC; ++kc) qf[kc] = ld_global16(src + 32 * kc);
 
   // this wave's tiles: first + NW * j, j < nt
-  const int n = sq.n, last = n + p.Sq - 1;
+  const int n = sq.n, last = PRE && shared ? n - 1 : n + p.Sq - 1;
   const int first = sq.t0 + ck.first + wave;
   const int nt = __builtin_amdgcn_readfirstlane(max((ck.count - wave + NW - 1) / NW, 0));
-  const uint64_t kp = (uint64_t)((const T*)a.k.data + b * a.k.sb + hk * a.k.sh);
-  const uint64_t vp = (uint64_t)((const T*)a.v.data + b * a.v.sb + hk * a.v.sh);
+  const uint64_t kp = (uint64_t)((const T*)vk.data + b * vk.sb + hk * vk.sh);
+  const uint64_t vp = (uint64_t)((const T*)vv.data + b * vv.sb + hk * vv.sh);
   auto issue_k = [&](int t, int st) {
     const unsigned dst = wbase + st * 2 * C::TB + sub * 1024;
     const uint64_t base = kp + (uint64_t)(t * C::BN) * kss;
@@ -245,14 +291,19 @@ void tree_attn_kernel(TreeArgs a) {
   // sees need no mask.
   int row_lo = 0, full_lo = 0;
   if (p.window > 0) {
-    const int depth = a.depths ? max(a.depths[(int64_t)b * p.Sq + qi], 0) : qi;
+    const int depth = a.depths ? max(a.depths[(int64_t)qb * p.Sq + qi], 0) : qi;
     // (n + depth - window without leaving 32 bits: depth at most the window counts)
-    full_lo = row_lo = max(n - (p.window - min(depth, p.window)), 0);
+    int past = n;
+    if constexpr (PRE) {
+      if (shared) past += min(max(a.lengths[qb], 0), p.Skv);  // (of a sequence that does not fit: not used)
+    }
+    full_lo = row_lo = max(past - (p.window - min(depth, p.window)), 0);
 #pragma unroll
     for (int y = 32; y; y >>= 1) full_lo = max(full_lo, __shfl_xor(full_lo, y));
     full_lo = __builtin_amdgcn_readfirstlane(full_lo);
   }
-  const unsigned char* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+  const unsigned char* mask = a.mask && !(PRE && shared) ? a.mask + b * a.mask_sb : nullptr;
+  const int reach = PRE && shared ? n : n + (mask ? p.Sq : qi + 1);
 
   // wait for Q here, once: see fwd_split.hip
 #pragma unroll
@@ -285,6 +336,9 @@ void tree_attn_kernel(TreeArgs a) {
         issue_v(t + NW, (j + 1) & 1);
       }
       if (j >= nt) continue;  // (the last step of waves with one tile less)
+      if constexpr (PRE) {
+        if (32 * rt0 >= R) continue;  // (a wave without rows copies only)
+      }
     } else if constexpr (ST == 2) {
       if (more) {  // into the stage of tile j - 1, read in the previous iteration
         reads_done();
@@ -325,7 +379,7 @@ void tree_attn_kernel(TreeArgs a) {
     }
     if (n0 < full_lo || n0 + C::BN > n) {
       // this lane's keys, relative to its first: e, and hidden before lo or from hi on
-      const int lo = row_lo - n0 - 4 * h, hi = n + (mask ? p.Sq : qi + 1) - n0 - 4 * h;
+      const int lo = row_lo - n0 - 4 * h, hi = reach - n0 - 4 * h;
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if ((unsigned)(8 * (e >> 2) + (e & 3) - lo) >= (unsigned)max(hi - lo, 0)) sc[e] = kNegInf;
@@ -434,9 +488,11 @@ void tree_attn_kernel(TreeArgs a) {
   const bool empty = L == 0.f;  // no key; NaN (a NaN query row or key) is not
   const float inv = empty ? 0.f : 1.0f / L;
   if (32 * rt0 + l32 < R) {
-    const int64_t row = ((int64_t)b * p.Hq + hq) * p.Sq + qi;
-    float* po = a.part_o + (row * a.nsplit + s) * D + 4 * h;
-    T* out = (T*)a.o.data + b * a.o.sb + hq * a.o.sh + (int64_t)qi * a.o.ss + 4 * h;
+    const int64_t row = ((int64_t)qb * p.Hq + hq) * p.Sq + qi;
+    int64_t place = row * a.nsplit + s;
+    if constexpr (PRE) place = row * args.pitch + (shared ? s : args.np + s);
+    float* po = a.part_o + place * D + 4 * h;
+    T* out = (T*)a.o.data + qb * a.o.sb + hq * a.o.sh + (int64_t)qi * a.o.ss + 4 * h;
 #pragma unroll 2
     for (int y = wave; y < 4 * C::DB; y += NW) {
       f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -447,13 +503,13 @@ void tree_attn_kernel(TreeArgs a) {
         for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(al[w], v[e], o[e]);
       }
       o *= inv;
-      if (ns > 1) *(f32x4*)(po + 8 * y) = o;
+      if (PRE || ns > 1) *(f32x4*)(po + 8 * y) = o;
       else if constexpr (sizeof(T) == 4) *(f32x4*)(out + 8 * y) = o;
       else st_global8(out + 8 * y, pack4<T>(o[0], o[1], o[2], o[3]));
     }
     if (wave == 0 && h == 0) {
       const float lse = empty ? kNegInf : mall + log2f(L);
-      if (ns > 1) a.part_lse[row * a.nsplit + s] = lse;
+      if (PRE || ns > 1) a.part_lse[place] = lse;
       else a.lse[row] = lse * kLn2;
     }
   }
@@ -464,8 +520,8 @@ void launch_tree_share(TreeArgs a, hipStream_t st) {
   constexpr int NW = WPT == 4 ? TreeCfg<T, D>::NW / 2 : TreeCfg<T, D>::NW;
   a.nrt = (int)((((int64_t)a.p.G * a.p.Sq + 31) / 32 + WPT - 1) / WPT);
   const dim3 grid((unsigned)((a.nchunk + 7) / 8 * 8 * a.nrt)), block(NW * WPT * 64);
-  if (a.p.cap > 0.f) hipLaunchKernelGGL((tree_attn_kernel<T, D, NW, WPT, true>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((tree_attn_kernel<T, D, NW, WPT, false>), grid, block, 0, st, a);
+  if (a.p.cap > 0.f) hipLaunchKernelGGL((tree_attn_kernel<T, D, NW, WPT, true, false>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((tree_attn_kernel<T, D, NW, WPT, false, false>), grid, block, 0, st, a);
 }
 
 template <class T, int D>
@@ -486,6 +542,38 @@ hipError_t launch_tree(const TreeArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+template <class T, int D, int WPT>
+void launch_prefix_share(PrefixArgs a, hipStream_t st) {
+  constexpr int NW = WPT == 4 ? TreeCfg<T, D>::NW / 2 : TreeCfg<T, D>::NW;
+  const int64_t rows = (int64_t)a.t.p.G * a.t.p.Sq;
+  a.t.nrt = (int)(((rows + 31) / 32 + WPT - 1) / WPT);
+  a.nrtp = (int)(((rows * a.t.p.B + 31) / 32 + WPT - 1) / WPT);
+  a.npre = (a.t.p.Hkv * a.np + 7) / 8 * 8 * a.nrtp;
+  const dim3 grid((unsigned)(a.npre + (a.t.nchunk + 7) / 8 * 8 * a.t.nrt)), block(NW * WPT * 64);
+  if (a.t.p.cap > 0.f) hipLaunchKernelGGL((tree_attn_kernel<T, D, NW, WPT, true, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((tree_attn_kernel<T, D, NW, WPT, false, true>), grid, block, 0, st, a);
+}
+
+template <class T, int D>
+hipError_t launch_prefix(const PrefixArgs& a, hipStream_t st) {
+  using C = TreeCfg<T, D>;
+  const int share = tree_share(C::ROWB, sizeof(T), ((int64_t)a.t.p.B * a.t.p.G * a.t.p.Sq + 31) / 32);
+  if constexpr (sizeof(T) == 2 && C::ROWB <= 256) {
+    if constexpr (C::ROWB == 256) {
+      if (share == 4) launch_prefix_share<T, D, 4>(a, st);
+    }
+    if (share == 2) launch_prefix_share<T, D, 2>(a, st);
+  }
+  if (share == 1) launch_prefix_share<T, D, 1>(a, st);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int64_t rows = (int64_t)a.t.p.B * a.t.p.Hq * a.t.p.Sq;
+  TreeArgs m = a.t;
+  m.nsplit = a.pitch;
+  hipLaunchKernelGGL((tree_merge_kernel<T, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, m);
+  return hipGetLastError();
+}
+
 #define FLEXATT_CAT2(a, b) a##b
 #define FLEXATT_CAT(a, b) FLEXATT_CAT2(a, b)
 hipError_t FLEXATT_CAT(tree_attn_bf16_d, FLEXATT_D)(const TreeArgs& a, hipStream_t st) {
@@ -496,6 +584,15 @@ hipError_t FLEXATT_CAT(tree_attn_f16_d, FLEXATT_D)(const TreeArgs& a, hipStream_
 }
 hipError_t FLEXATT_CAT(tree_attn_f32_d, FLEXATT_D)(const TreeArgs& a, hipStream_t st) {
   return launch_tree<float, FLEXATT_D>(a, st);
+}
+hipError_t FLEXATT_CAT(prefix_attn_bf16_d, FLEXATT_D)(const PrefixArgs& a, hipStream_t st) {
+  return launch_prefix<__bf16, FLEXATT_D>(a, st);
+}
+hipError_t FLEXATT_CAT(prefix_attn_f16_d, FLEXATT_D)(const PrefixArgs& a, hipStream_t st) {
+  return launch_prefix<_Float16, FLEXATT_D>(a, st);
+}
+hipError_t FLEXATT_CAT(prefix_attn_f32_d, FLEXATT_D)(const PrefixArgs& a, hipStream_t st) {
+  return launch_prefix<float, FLEXATT_D>(a, st);
 }
 
 }  // namespace flexatt

@@ -88,6 +88,28 @@ __device__ __forceinline__ TreeChunk tree_chunk(const TreeArgs& a, int x, int nw
   return r;
 }
 
+// The chunk x < Hkv np of a shared prefix.  A window leaves its last rows only: as many as
+// the sequence with the fewest cached tokens reaches.
+__device__ __forceinline__ TreeChunk prefix_chunk(const PrefixArgs& a, int x) {
+  const int t1 = (a.P + 31) / 32;
+  int t0 = 0;
+  if (a.t.p.window > 0) {
+    const int lane = threadIdx.x & 63, B = a.t.p.B;
+    unsigned need = 0;
+    for (int b = lane; b < B; b += 64) need = max(need, (unsigned)max(a.t.p.window - tree_seq(a.t, b).n, 0));
+    t0 = (a.P - (int)min(wave_max(need), (unsigned)a.P)) / 32;
+  }
+  TreeChunk r;
+  r.b = 0;
+  r.hk = x / a.np;
+  r.s = x - r.hk * a.np;
+  r.ns = a.np;
+  const int each = (t1 - t0 + a.np - 1) / a.np;
+  r.first = t0 + r.s * each;
+  r.count = max(min(each, t1 - r.first), 0);
+  return r;
+}
+
 // Direct-to-LDS copies of a tile of rows: lane offsets from the tile's first row (the
 // swizzle repeats after PERIOD copies, so there are as many of them) and a scalar
 // base, a copy being RPC rows.

@@ -15,6 +15,7 @@ apart).
   attention_weight_sums(...)  sum over the query rows of the softmax weights, per key
   evict_cache(...)            the rows worth keeping, copied to a smaller cache
   norm_rotary_append(...)     rotary_append behind a norm of each head of query and key
+  shared_prefix_attention(...)  tree_attention behind a prefix that all sequences share
 
 A cache may hold 8 bits an element: ``key_cache`` / ``value_cache`` of float8_e4m3fn or
 int8 and ``key_scales`` / ``value_scales``, float32 [B, Hkv, C] (contiguous where they
@@ -35,7 +36,7 @@ import torch
 import flexatt_lib as _lib
 
 __all__ = ["rotary_append", "tree_attention", "attention_weight_sums", "evict_cache", "norm_rotary_append",
-           "quantized_append", "dequantize_cache", "quantized_tree_attention"]
+           "shared_prefix_attention", "quantized_append", "dequantize_cache", "quantized_tree_attention"]
 
 
 def rotary_append(query, key, value, key_cache, value_cache, lengths, inv_freq, positions=None, interleaved=False,
@@ -135,6 +136,22 @@ def norm_rotary_append(query, key, value, key_cache, value_cache, lengths, query
     """
     return _lib.native().norm_rotary_append(query, key, value, key_cache, value_cache, lengths, query_weight, key_weight,
                                             inv_freq, positions, interleaved, magnitude, eps)
+
+
+def shared_prefix_attention(query, prefix_key, prefix_value, key_cache, value_cache, lengths, tree_mask=None,
+                            sliding_window=0, depths=None, scale=None, soft_cap=0.0, return_lse=False):
+    """:func:`tree_attention` of sequences that share a prefix, whose keys are read once for
+    all of them.
+
+    ``prefix_key`` / ``prefix_value`` [Hkv, P, D], in the cache's dtype: the keys and values
+    of the prefix's positions 0 .. P - 1, of which every drafted token sees all (for a
+    shorter prefix in a larger buffer pass a slice).  Row ``j`` of a sequence's own cache is
+    position ``P + j``: append to it with ``positions`` that say so.  The other arguments
+    and results are those of :func:`tree_attention`; ``sliding_window`` W counts positions,
+    so it keeps row ``j`` of the prefix where ``P + lengths[b] + depths[b][t] - j <= W``.
+    """
+    return _lib.native().prefix_attention(query, prefix_key, prefix_value, key_cache, value_cache, lengths, tree_mask,
+                                          sliding_window, depths, scale, soft_cap, return_lse)
 
 
 def quantized_append(query, key, value, key_cache, value_cache, key_scales, value_scales, lengths, inv_freq,

@@ -56,6 +56,8 @@ EXPORTS = (
     "flexatt_dequant_rows",
     "flexatt_quant_tree_fwd_workspace",
     "flexatt_quant_tree_fwd",
+    "flexatt_prefix_fwd_workspace",
+    "flexatt_prefix_fwd",
     "flexatt_status_string",
     "flexatt_abi_version",
 )
@@ -227,6 +229,7 @@ def load() -> ctypes.CDLL:
         "flexatt_norm_rotary_append": [P(Rotary), P(Norm), T, T, T, T, T, T, ctypes.c_int32, fp, st],
         "flexatt_quant_append": [P(Rotary), P(Norm), ctypes.c_int32, T, T, T, T, T, T, fp, fp, ctypes.c_int32, fp, st],
         "flexatt_dequant_rows": [P(Dequant), T, T, fp, fp, T, T, st],
+        "flexatt_prefix_fwd": [P(Tree), ctypes.c_int32, T, T, T, T, T, T, fp, fp, ctypes.c_size_t, st],
         "flexatt_quant_tree_fwd": [P(Tree), ctypes.c_int32, T, T, T, fp, fp, T, fp, fp, ctypes.c_size_t, st],
     }
     for name, args in sig.items():
@@ -241,6 +244,8 @@ def load() -> ctypes.CDLL:
                       ("flexatt_quant_tree_fwd_workspace", P(Tree)), ("flexatt_norm_rotary_grad_workspace", P(Rotary))):
         getattr(lib, name).argtypes = [arg]
         getattr(lib, name).restype = ctypes.c_size_t
+    lib.flexatt_prefix_fwd_workspace.argtypes = [P(Tree), ctypes.c_int32]
+    lib.flexatt_prefix_fwd_workspace.restype = ctypes.c_size_t
     lib.flexatt_bwd_workspace_limited.argtypes = [pr, ctypes.c_size_t]
     lib.flexatt_bwd_workspace_limited.restype = ctypes.c_size_t
     for name in ("flexatt_bwd_prefers_staging", "flexatt_bwd_prefers_split"):

@@ -200,3 +200,14 @@ def quantized_tree_attention(q, kc, vc, ks, vs, lengths, mask=None, window=0, de
                 tO[b, h] += (n + T) * 2.0 ** -24 * vs[b, h // G, :n + T].double().max() * top
             tL[b, h] += x * 2.0 ** -23
     return O, LSE, tO, tL
+
+
+def prefix_attention(q, pk, pv, kc, vc, lengths, mask=None, window=0, depths=None, scale=None, cap=0.0,
+                     dtype=torch.bfloat16):
+    """O, LSE and their tolerances: those of :func:`tree_attention` over caches that begin with the prefix pk, pv [Hkv, P,
+    D], its P rows among the cached ones."""
+    B, P = q.shape[0], pk.shape[1]
+    k, v = (torch.cat((x[None].expand(B, -1, -1, -1), y), dim=2) for x, y in ((pk, kc), (pv, vc)))
+    fits = [0 <= int(n) <= kc.shape[2] - q.shape[2] for n in lengths]
+    n = torch.tensor([P + int(n) if ok else -1 for n, ok in zip(lengths, fits)])
+    return tree_attention(q, k, v, n, mask, window, depths, scale, cap, dtype)

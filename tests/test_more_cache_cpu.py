@@ -163,12 +163,38 @@ def test_quant_tree_refuses_tensors_and_workspace():
     assert call(o=L.Tensor(FAKE, 0, 512, 64, 1)) == -5
 
 
+@pytest.mark.parametrize("kw,rows,code", [
+    (dict(dtype=9), 50, -2), (dict(batch=0), 50, -1), (dict(tokens=0), 50, -1), (dict(head_dim=80), 50, -3),
+    (dict(heads_kv=3), 50, -4), (dict(scale=float("nan")), 50, -1), (dict(soft_cap=-1.0), 50, -1),
+    (dict(lengths=None), 50, -1), (dict(tree_mask=FAKE, mask_batch=2, sliding_window=5), 50, -1), ({}, 0, -1), ({}, -3, -1),
+    ({}, 1 << 30, -4), (dict(heads_q=2, tokens=(1 << 20) + 1), 50, -6)])
+def test_prefix_refuses(kw, rows, code):
+    lib, c, pre = L.load(), _t(2, 64), _t(2, 50)
+    assert lib.flexatt_prefix_fwd(_tree(**kw), rows, _t(4), pre, pre, c, c, _t(4), FAKE, FAKE, 1 << 40, None) == code
+    assert lib.flexatt_prefix_fwd_workspace(_tree(**kw), rows) == 2 ** 64 - 1
+
+
+def test_prefix_refuses_tensors_and_workspace():
+    lib, p = L.load(), _tree(cache_rows=8192)
+    n = lib.flexatt_prefix_fwd_workspace(p, 5000)
+    assert 0 < n < 1 << 30
+    q, c, pre = _t(4), _t(2, 8192), _t(2, 5000)
+    call = lambda q=q, pk=pre, pv=pre, k=c, v=c, o=q, lse=FAKE, ws=FAKE, size=n: \
+        lib.flexatt_prefix_fwd(p, 5000, q, pk, pv, k, v, o, lse, ws, size, None)  # noqa: E731
+    assert call(pk=None) == call(pv=None) == call(lse=None) == call(ws=None) == call(size=n - 1) == -1
+    far = L.Tensor(FAKE, 1 << 40, 64, 1 << 25, 1)  # rows 2^26 bytes apart
+    assert call(pk=far) == call(pv=far) == call(k=far) == call(v=far) == -6
+    assert call(q=ODD) == call(pk=ODD) == call(pv=ODD) == call(k=ODD) == call(v=ODD) == call(ws=FAKE + 8) == -5
+    assert call(o=L.Tensor(FAKE, 0, 512, 64, 1)) == -5
+
+
 def test_cpu_tensors_have_no_fallback():
     x, w, f = torch.randn(1, 2, 4, 64), torch.ones(64), rot.rotary_frequencies(64)[0]
     c, s, n = torch.zeros(1, 2, 8, 64, dtype=torch.int8), torch.zeros(1, 2, 8), torch.zeros(1, dtype=torch.int32)
     for call in (lambda: rot.norm_rotary_embedding(x, x, w, w, f), lambda: fc.norm_rotary_append(x, x, x, x, x, n, w, w, f),
                  lambda: fc.quantized_append(x, x, x, c, c, s, s, n, f), lambda: fc.dequantize_cache(c, c, s, s, n),
-                 lambda: fc.quantized_tree_attention(x, c, c, s, s, n)):
+                 lambda: fc.quantized_tree_attention(x, c, c, s, s, n),
+                 lambda: fc.shared_prefix_attention(x, x[0], x[0], x, x, n)):
         with pytest.raises(RuntimeError, match="ROCm GPU"):
             call()
     with pytest.raises(RuntimeError, match="out must be"):
