@@ -510,8 +510,8 @@ int flexatt_dequant_rows(const flexatt_dequant* p, const flexatt_tensor* k_cache
                          const flexatt_tensor* v_out, void* stream);
 
 /* flexatt_tree_fwd over such a cache, for dtype fp16 and bf16 (else FLEXATT_EDTYPE).  The
- * scores are q . code times the key's scale; weights times the values' scales are rounded
- * to dtype for the second product. */
+ * scores are q . code times the key's scale; weights times the values' scales, relative to
+ * the largest of these, are rounded to fp16 for the second product. */
 size_t flexatt_quant_tree_fwd_workspace(const flexatt_tree* p);
 int flexatt_quant_tree_fwd(const flexatt_tree* p, int32_t code, const flexatt_tensor* q, const flexatt_tensor* k_cache,
                            const flexatt_tensor* v_cache, const float* k_scales, const float* v_scales,

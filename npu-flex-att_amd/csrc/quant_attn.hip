@@ -10,9 +10,13 @@
 //    k of the products they are is the same for Q's fragments, which are loaded to match;
 //  * V: the transpose read of 8-bit elements gives a lane eight keys of its column, those
 //    whose weights the scores' accumulators hold.
-// p s' is rounded to the type, as P is elsewhere.  fp16 has a narrow range: there the
-// scales are taken relative to a power of two that is at least the largest one a wave has
-// met, and the accumulators follow it as they follow the running maximum.
+// p s' is rounded to fp16 for either type of queries, in which codes are exact: its half
+// step of 2^-11 is far under that of bf16 outputs (bf16 weights: rms errors of 1.3 to 1.6
+// times the output's rounding alone).  For fp16 outputs, where it would be as much as
+// theirs (1.3 to 1.5 times), what the rounding leaves is the operand of MFMAs of its own,
+// which a wave that waits for memory has time for.  The scales are taken relative to a
+// power of two that is at least the largest one a wave has met, and the accumulators
+// follow it as they follow the running maximum, so that fp16's range does.
 //
 // A wave has one row tile of 32 packed query rows, or two (MT) that share the tile's LDS
 // reads and conversions, and every NW-th 32-key tile of its workgroup's chunk, copied to
@@ -63,7 +67,7 @@ __device__ __forceinline__ int swz_v8(int r, int c) {
   else return c ^ ((r & 7) << 1);
 }
 
-// Eight codes as an MFMA operand.
+// Eight codes as an MFMA operand of T.
 template <class T, int CODE>
 __device__ __forceinline__ typename Mfma<T>::v8 operand8(int lo, int hi) {
   typedef T x2 __attribute__((ext_vector_type(2)));
@@ -113,7 +117,8 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   using C = QuantCfg<D>;
   typedef typename Mfma<T>::v8 V8;
   constexpr int ST = C::ST, NW = C::NW, EC = C::EC, PK = C::PK, PV = C::PV;
-  constexpr bool NARROW = __is_same(T, _Float16);
+  typedef _Float16 W;  // the weights' type
+  constexpr bool REST = __is_same(T, _Float16);  // and what their rounding leaves
   constexpr int kCombine = NW * 64 * 4 * (3 + 16 * C::DB);
   __shared__ __attribute__((aligned(1024))) char smem[NW * ST * C::STB > kCombine ? NW * ST * C::STB : kCombine];
 
@@ -249,7 +254,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
 
   f32x16 acc[MT][C::DB];
   float m_run[MT], l_run[MT];
-  float rel = 0x1p126f;  // fp16: acc has values times rel, and rel times a scale is at most 1
+  float rel = 0x1p126f;  // acc has values times rel, and rel times a scale is at most 1
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     m_run[m] = kNegInf, l_run[m] = 0.f;
@@ -299,7 +304,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) ks[e] *= p.scale_log2;
     }
-    if constexpr (NARROW) {
+    {
       float top = vs[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) top = fmaxf(top, vs[e]);
@@ -370,16 +375,25 @@ void quant_attn_kernel(QuantTreeArgs qa) {
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      V8 pb[MT];
+      Mfma<W>::v8 pb[MT], pl[MT];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) pb[m] = pack8<T>(sc[m], 8 * c);
+      for (int m = 0; m < MT; ++m) {
+        pb[m] = pack8<W>(sc[m], 8 * c);
+        if constexpr (REST) {
+#pragma unroll
+          for (int t = 0; t < 8; ++t) pl[m][t] = (W)(sc[m][8 * c + t] - (float)pb[m][t]);
+        }
+      }
       const char* vr = sV + 16 * c * D;
 #pragma unroll
       for (int db = 0; db < C::DB; ++db) {
         const i32x2 w = lds_read_tr8(vr + voff[db]);
-        const V8 v = operand8<T, CODE>(w[0], w[1]);
+        const Mfma<W>::v8 v = operand8<W, CODE>(w[0], w[1]);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[m][db] = Mfma<T>::mma(v, pb[m], acc[m][db]);
+        for (int m = 0; m < MT; ++m) {
+          acc[m][db] = Mfma<W>::mma(v, pb[m], acc[m][db]);
+          if constexpr (REST) acc[m][db] = Mfma<W>::mma(v, pl[m], acc[m][db]);
+        }
       }
     }
   }
@@ -397,7 +411,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
     __syncthreads();
     xm[wave * 64 + lane] = m_run[m];
     xl[wave * 64 + lane] = l_tot;
-    xr[wave * 64 + lane] = NARROW ? 1.0f / rel : 1.f;
+    xr[wave * 64 + lane] = 1.0f / rel;
 #pragma unroll
     for (int y = 0; y < 4 * C::DB; ++y) {
       const f32x16& v = acc[m][y / 4];

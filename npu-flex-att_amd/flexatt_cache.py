@@ -190,7 +190,7 @@ def quantized_tree_attention(query, key_cache, value_cache, key_scales, value_sc
     other arguments and results are the same.
 
     Scores are products with the codes times the key's scale, in 32 bits.  A weight times
-    its value's scale is rounded to the query's dtype.  Scales of rows that a token does
+    its value's scale is rounded to float16, relative to the largest scale.  Scales of rows that a token does
     not see must be finite, as their values.
     """
     return _lib.native().quant_tree_attention(query, key_cache, value_cache, key_scales, value_scales, lengths, tree_mask,

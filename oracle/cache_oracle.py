@@ -54,10 +54,11 @@ def _scores(q, k, scale, cap):
     return x, err + x.abs() * 2.0 ** -22
 
 
-def tree_attention(q, kc, vc, lengths, mask=None, window=0, depths=None, scale=None, cap=0.0, dtype=torch.bfloat16):
+def tree_attention(q, kc, vc, lengths, mask=None, window=0, depths=None, scale=None, cap=0.0, dtype=torch.bfloat16,
+                   weights=None):
     """O, LSE and their tolerances; mask [T, T] or [B, T, T], depths [B, T] or None.
 
-    P is rounded to the type before P V (fp32: not at all): half a step of each weight, and for fp16, whose weights
+    P is rounded to the type, or to ``weights``, before P V (fp32: not at all): half a step of each weight, and for fp16, whose weights
     under 2^-14 have the step 2^-24, n 2^-25 in all beside a largest weight of at least 1.  A score error e scales a
     weight by exp(e) and so the row sum: 2 e max|v|."""
     B, Hq, T, D = q.shape
@@ -67,7 +68,8 @@ def tree_attention(q, kc, vc, lengths, mask=None, window=0, depths=None, scale=N
     O = torch.zeros(B, Hq, T, D, dtype=torch.float64)
     LSE = torch.full((B, Hq, T), float("-inf"), dtype=torch.float64)
     tO, tL = torch.zeros_like(O), torch.zeros_like(LSE)
-    half = 0.0 if dtype == torch.float32 else EPS[dtype] / 2
+    weights = weights or dtype
+    half = 0.0 if weights == torch.float32 else EPS[weights] / 2
     for b in range(B):
         n = int(lengths[b])
         if n < 0 or n + T > C:
@@ -87,7 +89,7 @@ def tree_attention(q, kc, vc, lengths, mask=None, window=0, depths=None, scale=N
             vmax = torch.where(ok[:, :, None], v.abs()[None], torch.zeros(())).amax(dim=(1, 2))
             O[b, h] = o
             LSE[b, h] = lse
-            flat = (n + T) * 2.0 ** -25 if dtype == torch.float16 else 0.0
+            flat = (n + T) * 2.0 ** -25 if weights == torch.float16 else 0.0
             loose = ((half + 2 * e + flat + 2.0 ** -20) * vmax)[:, None].expand_as(o)
             tO[b, h] = rounded(o, loose, dtype)
             tL[b, h] = e + torch.where(some, lse.abs(), torch.zeros_like(lse)) * 2.0 ** -21 + 2.0 ** -20
@@ -181,10 +183,10 @@ def quantized_tree_attention(q, kc, vc, ks, vs, lengths, mask=None, window=0, de
     """O, LSE and their tolerances: those of :func:`tree_attention` over codes * scales.
 
     The scales add two roundings to a score, 2^-23 of it, and one to a weight.  A weight times its value's scale is
-    rounded where p was; in fp16, relative to a power of two at most twice the largest scale, the numbers under 2^-14
-    have the step 2^-24: (n + T) 2^-24 times the largest scale and code."""
+    rounded to fp16 where p was rounded to the type, relative to a power of two at most twice the largest scale; the
+    numbers under 2^-14 have the step 2^-24: (n + T) 2^-24 times the largest scale and code."""
     k, v = kc.double() * ks.double()[..., None], vc.double() * vs.double()[..., None]
-    O, LSE, tO, tL = tree_attention(q, k, v, lengths, mask, window, depths, scale, cap, dtype)
+    O, LSE, tO, tL = tree_attention(q, k, v, lengths, mask, window, depths, scale, cap, dtype, torch.float16)
     G, T = q.shape[1] // kc.shape[1], q.shape[2]
     top = TOP[kc.dtype]
     for b in range(q.shape[0]):
@@ -196,8 +198,7 @@ def quantized_tree_attention(q, kc, vc, ks, vs, lengths, mask=None, window=0, de
                                                                                  1.0 / math.sqrt(q.shape[3]))
             vmax = v[b, h // G, :n + T].abs().max()
             tO[b, h] += 2 * x * 2.0 ** -23 * vmax + vmax * 2.0 ** -22
-            if dtype == torch.float16:
-                tO[b, h] += (n + T) * 2.0 ** -24 * vs[b, h // G, :n + T].double().max() * top
+            tO[b, h] += (n + T) * 2.0 ** -24 * vs[b, h // G, :n + T].double().max() * top
             tL[b, h] += x * 2.0 ** -23
     return O, LSE, tO, tL
 
