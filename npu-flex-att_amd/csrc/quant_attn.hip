@@ -23,6 +23,8 @@
 // its own LDS stages without barriers, the scales with one copy more.
 //
 // Bound by HBM for long caches and few rows, by the softmax's VALU work for many.
+#include <type_traits>
+
 #include "flexatt_device.h"
 #include "flexatt_kernels.h"
 #include "tree_device.h"
@@ -104,11 +106,40 @@ __device__ __forceinline__ typename Mfma<T>::v8 operand8(int lo, int hi) {
   return as_v8<typename Mfma<T>::v8>(v);
 }
 
+// acc *= s where the accumulators stay in their half of the register file: a multiply of
+// its own would have all of them moved back and forth around the branch it is in, in every
+// iteration.  The waits are those between an MFMA and a read of its result, and between
+// the last write and an MFMA.
+__device__ __forceinline__ void scale_acc(f32x16& a, float s) {
+#pragma unroll
+  for (int r = 0; r < 16; r += 4) {
+    float x0, x1, x2, x3, y0 = a[r], y1 = a[r + 1], y2 = a[r + 2], y3 = a[r + 3];
+    asm volatile(
+        "s_nop 15\n\ts_nop 3\n\t"
+        "v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\t"
+        "v_accvgpr_read_b32 %6, %2\n\tv_accvgpr_read_b32 %7, %3\n\ts_nop 1\n\t"
+        "v_mul_f32_e32 %4, %8, %4\n\tv_mul_f32_e32 %5, %8, %5\n\t"
+        "v_mul_f32_e32 %6, %8, %6\n\tv_mul_f32_e32 %7, %8, %7\n\ts_nop 1\n\t"
+        "v_accvgpr_write_b32 %0, %4\n\tv_accvgpr_write_b32 %1, %5\n\t"
+        "v_accvgpr_write_b32 %2, %6\n\tv_accvgpr_write_b32 %3, %7\n\ts_nop 3"
+        : "+a"(y0), "+a"(y1), "+a"(y2), "+a"(y3), "=&v"(x0), "=&v"(x1), "=&v"(x2), "=&v"(x3)
+        : "v"(s));
+    a[r] = y0, a[r + 1] = y1, a[r + 2] = y2, a[r + 3] = y3;
+  }
+}
+
 // Transposed 8 x 8-bit read: lane i of 16 gets byte i % 8 at the addresses of lanes
 // 2 t + i / 8, t = 0 .. 7.
 __device__ __forceinline__ i32x2 lds_read_tr8(const void* p) {
   return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
       (__attribute__((address_space(3))) i32x2*)((__attribute__((address_space(3))) char*)p));
+}
+
+// Accumulators of two row tiles have only that half to be in.
+template <int MT>
+__device__ __forceinline__ void rescale(f32x16& a, float s) {
+  if constexpr (MT > 1) scale_acc(a, s);
+  else scale_inplace(a, s);
 }
 
 template <class T, int CODE, int D, int MT, bool CAP>
@@ -316,15 +347,15 @@ void quant_attn_kernel(QuantTreeArgs qa) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int db = 0; db < C::DB; ++db) scale_inplace(acc[m][db], turn);
+          for (int db = 0; db < C::DB; ++db) rescale<MT>(acc[m][db], turn);
         rel = now;
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e) vs[e] *= rel;
     }
 
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
+    auto softmax = [&](auto which) {  // (a loop over them is not unrolled)
+      constexpr int m = which;
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[m][e] *= ks[e];
       if constexpr (CAP) {
@@ -360,7 +391,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
         const float alpha = grow ? fast_exp2(m_run[m] - m_new) : 1.f;
         l_run[m] *= alpha;
 #pragma unroll
-        for (int db = 0; db < C::DB; ++db) scale_inplace(acc[m][db], alpha);
+        for (int db = 0; db < C::DB; ++db) rescale<MT>(acc[m][db], alpha);
         m_run[m] = m_new;
       }
       const float m_use = (m_run[m] == kNegInf) ? 0.f : m_run[m];
@@ -372,7 +403,9 @@ void quant_attn_kernel(QuantTreeArgs qa) {
         sc[m][e] = pe * vs[e];
       }
       l_run[m] += (rs[0] + rs[1]) + (rs[2] + rs[3]);
-    }
+    };
+    softmax(std::integral_constant<int, 0>{});
+    if constexpr (MT > 1) softmax(std::integral_constant<int, 1>{});
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       Mfma<W>::v8 pb[MT], pl[MT];
