@@ -14,9 +14,9 @@
 // step of 2^-11 is far under that of bf16 outputs (bf16 weights: rms errors of 1.3 to 1.6
 // times the output's rounding alone).  For fp16 outputs, where it would be as much as
 // theirs (1.3 to 1.5 times), what the rounding leaves is the operand of MFMAs of its own,
-// which a wave that waits for memory has time for.  The scales are taken relative to a
-// power of two that is at least the largest one a wave has met, and the accumulators
-// follow it as they follow the running maximum, so that fp16's range does.
+// which a wave that waits for memory has time for.  fp16's range: weights are taken
+// relative to the running maximum less `lift`, so that 2^lift times the largest scale a
+// wave has met is at most 1; sums and accumulators follow both.
 //
 // A wave has one row tile of 32 packed query rows, or two (MT) that share the tile's LDS
 // reads and conversions, and every NW-th 32-key tile of its workgroup's chunk, copied to
@@ -49,8 +49,8 @@ struct QuantCfg {
   static constexpr int PV = RPC >= 8 ? 1 : 8 / RPC;    // and V's
   static constexpr int EC = 2 * E + 1;       // copies of a stage: K, V, both scales
   static constexpr int STB = 2 * TB + 256;   // bytes of a stage
-  static constexpr int NW = 4;               // waves per workgroup
-  static constexpr int ST = D >= 256 ? 2 : 4;  // stages
+  static constexpr int NW = D == 128 ? 8 : 4;  // waves per workgroup
+  static constexpr int ST = D >= 128 ? 2 : 4;  // stages
   static_assert(E * 1024 == TB && NW * ST * STB <= 160 * 1024 && E % PK == 0 && E % PV == 0, "tiles");
 };
 
@@ -143,14 +143,14 @@ __device__ __forceinline__ void rescale(f32x16& a, float s) {
 }
 
 template <class T, int CODE, int D, int MT, bool CAP>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D >= 128 || MT > 1 ? 1 : 2)))
+__global__ __launch_bounds__(QuantCfg<D>::NW * 64) __attribute__((amdgpu_waves_per_eu(D >= 256 || MT > 1 ? 1 : 2)))
 void quant_attn_kernel(QuantTreeArgs qa) {
   using C = QuantCfg<D>;
   typedef typename Mfma<T>::v8 V8;
   constexpr int ST = C::ST, NW = C::NW, EC = C::EC, PK = C::PK, PV = C::PV;
   typedef _Float16 W;  // the weights' type
   constexpr bool REST = __is_same(T, _Float16);  // and what their rounding leaves
-  constexpr int kCombine = NW * 64 * 4 * (3 + 16 * C::DB);
+  constexpr int kCombine = NW * 64 * 4 * (2 + 16 * C::DB);
   __shared__ __attribute__((aligned(1024))) char smem[NW * ST * C::STB > kCombine ? NW * ST * C::STB : kCombine];
 
   const TreeArgs& a = qa.t;
@@ -222,32 +222,44 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   const uint64_t kp = (uint64_t)((const char*)a.k.data + b * a.k.sb + hk * a.k.sh);
   const uint64_t vp = (uint64_t)((const char*)a.v.data + b * a.v.sb + hk * a.v.sh);
   const float* scales = (h ? qa.v_scales : qa.k_scales) + ((int64_t)b * p.Hkv + hk) * p.Skv;
-  auto issue = [&](int j) {  // tile j of this wave into its stage
+  // K, V and scales of tile j of this wave into its stage
+  auto issue_k = [&](int j) {
     const int t = first + NW * j;
     const unsigned dst = wbase + j % ST * C::STB;
-    const uint64_t kb = kp + (uint64_t)(t * C::BN) * kss, vb = vp + (uint64_t)(t * C::BN) * vss;
+    const uint64_t base = kp + (uint64_t)(t * C::BN) * kss;
     if (t * C::BN + C::BN - 1 <= last) {
 #pragma unroll
       for (int e = 0; e < C::E; ++e)
-        load_lds16_base(kvo[e % PK], kb + (uint64_t)(e / PK * PK * C::RPC) * kss, dst + e * 1024);
-#pragma unroll
-      for (int e = 0; e < C::E; ++e)
-        load_lds16_base(vvo[e % PV], vb + (uint64_t)(e / PV * PV * C::RPC) * vss, dst + C::TB + e * 1024);
+        load_lds16_base(kvo[e % PK], base + (uint64_t)(e / PK * PK * C::RPC) * kss, dst + e * 1024);
     } else {  // rows behind the last one repeat it
 #pragma unroll 1
       for (int e = 0; e < C::E; ++e) {
         const int kr = e * C::RPC + crow;
-        load_lds16_base(min(kr, last - t * C::BN) * kss + swz_k8<C::CPR>(kr, cchunk) * 16, kb, dst + e * 1024);
+        load_lds16_base(min(kr, last - t * C::BN) * kss + swz_k8<C::CPR>(kr, cchunk) * 16, base, dst + e * 1024);
       }
+    }
+  };
+  auto issue_v = [&](int j) {
+    const int t = first + NW * j;
+    const unsigned dst = wbase + j % ST * C::STB + C::TB;
+    const uint64_t base = vp + (uint64_t)(t * C::BN) * vss;
+    if (t * C::BN + C::BN - 1 <= last) {
+#pragma unroll
+      for (int e = 0; e < C::E; ++e)
+        load_lds16_base(vvo[e % PV], base + (uint64_t)(e / PV * PV * C::RPC) * vss, dst + e * 1024);
+    } else {
 #pragma unroll 1
       for (int e = 0; e < C::E; ++e) {
         const int kr = e * C::RPC + crow;
-        load_lds16_base(min(kr, last - t * C::BN) * vss + swz_v8<C::CPR>(kr, cchunk) * 16, vb, dst + C::TB + e * 1024);
+        load_lds16_base(min(kr, last - t * C::BN) * vss + swz_v8<C::CPR>(kr, cchunk) * 16, base, dst + e * 1024);
       }
     }
-    load_lds4(scales + min(t * C::BN + l32, last), dst + 2 * C::TB);
+    load_lds4(scales + min(t * C::BN + l32, last), dst + C::TB);
   };
-  if (nt > 0) issue(0);
+  if (nt > 0) {
+    issue_k(0);
+    issue_v(0);
+  }
 
   // Q: lane half h has elements 32 kc + 16 h .. + 15 of its row, the codes' order
   i32x4 qf[MT][2 * C::KC];
@@ -274,18 +286,31 @@ void quant_attn_kernel(QuantTreeArgs qa) {
     full_lo = __builtin_amdgcn_readfirstlane(full_lo);
   }
   const unsigned char* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+  float c2 = p.scale_log2;
+  int flip = 0;
+  if constexpr (!CAP) {  // as in the forward: a negative scale moves into Q
+    if (c2 < 0.f) flip = (int)0x80008000;
+    c2 = c2 == 0.f ? 1e-30f : fabsf(c2);
+  }
   // wait for Q here, once: see fwd_split.hip
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int kc = 0; kc < 2 * C::KC; ++kc) pin(qf[m][kc]);
+    for (int kc = 0; kc < 2 * C::KC; ++kc) {
+      qf[m][kc] ^= i32x4{flip, flip, flip, flip};
+      pin(qf[m][kc]);
+    }
 #pragma unroll
-  for (int j = 1; j < ST - 1; ++j)
-    if (j < nt) issue(j);
+  for (int j = 1; j < ST; ++j)
+    if (j < nt) {
+      issue_k(j);
+      issue_v(j);
+    }
 
   f32x16 acc[MT][C::DB];
   float m_run[MT], l_run[MT];
-  float rel = 0x1p126f;  // acc has values times rel, and rel times a scale is at most 1
+  // weights are 2^(x - m_run + lift), and rel = 2^lift times a scale is at most 1
+  float lift = 90.f, rel = 0x1p90f;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     m_run[m] = kNegInf, l_run[m] = 0.f;
@@ -295,9 +320,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
 
   for (int j = 0; j < nt; ++j) {
     const int n0 = (first + NW * j) * C::BN;
-    if (j + ST - 1 < nt) {  // into the stage of tile j - 1, read in the previous iteration
-      reads_done();
-      issue(j + ST - 1);
+    if (j + ST - 1 < nt) {
       wait_vmcnt<(ST - 1) * EC>();  // tile j landed, the next ones in flight
     } else if (ST > 2 && j + 2 < nt) {
       wait_vmcnt<(ST > 2 ? 2 : 0) * EC>();
@@ -323,35 +346,34 @@ void quant_attn_kernel(QuantTreeArgs qa) {
         sc[m] = Mfma<T>::mma(k1, as_v8<V8>(qf[m][2 * kc + 1]), sc[m]);
       }
     }
+    if (j + ST < nt) {  // K's half of the stage is free
+      reads_done();
+      issue_k(j + ST);
+    }
     // scales of this lane's keys: element e is key n0 + 8(e/4) + 4h + e%4
-    float ks[16], vs[16];
+    f32x16 ks, vs;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const i32x4 k4 = lds_read16(sS + 32 * i), v4 = lds_read16(sS + 128 + 32 * i);
 #pragma unroll
       for (int e = 0; e < 4; ++e) ks[4 * i + e] = __int_as_float(k4[e]), vs[4 * i + e] = __int_as_float(v4[e]);
     }
-    if constexpr (!CAP) {
+    float top, top2;
+    max16_partial(vs, top, top2);
+    top = max2(top, top2);
+    top = fmaxf(top, swap_halves(top));
+    if (__builtin_amdgcn_readfirstlane(top * rel > 1.f)) {
+      // the power of two above the largest scale, as far as there is one
+      const int expo = (int)(__float_as_uint(top) >> 23) & 255, field = min(max(253 - expo, 1), 217);
+      const float now = __int_as_float(field << 23), turn = now / rel;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) ks[e] *= p.scale_log2;
-    }
-    {
-      float top = vs[0];
+      for (int m = 0; m < MT; ++m) {
+        l_run[m] *= turn;
 #pragma unroll
-      for (int e = 1; e < 16; ++e) top = fmaxf(top, vs[e]);
-      top = fmaxf(top, swap_halves(top));
-      if (__builtin_amdgcn_readfirstlane(top * rel > 1.f)) {
-        // the power of two above the largest scale, as far as there is one
-        const int expo = (int)(__float_as_uint(top) >> 23) & 255;
-        const float now = __int_as_float(max(253 - expo, 1) << 23), turn = now / rel;
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int db = 0; db < C::DB; ++db) rescale<MT>(acc[m][db], turn);
-        rel = now;
+        for (int db = 0; db < C::DB; ++db) rescale<MT>(acc[m][db], turn);
       }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) vs[e] *= rel;
+      rel = now;
+      lift = (float)(field - 127);
     }
 
     auto softmax = [&](auto which) {  // (a loop over them is not unrolled)
@@ -383,6 +405,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
       float mx, mx2;
       max16_partial(sc[m], mx, mx2);
       mx = max2(mx, mx2);
+      if constexpr (!CAP) mx *= c2;
       mx = fmaxf(mx, swap_halves(mx));
       if (mx != mx) mx = kNegInf;
       const bool grow = mx > m_run[m] + kTreeRescale;
@@ -394,11 +417,13 @@ void quant_attn_kernel(QuantTreeArgs qa) {
         for (int db = 0; db < C::DB; ++db) rescale<MT>(acc[m][db], alpha);
         m_run[m] = m_new;
       }
-      const float m_use = (m_run[m] == kNegInf) ? 0.f : m_run[m];
+      const float m_use = (m_run[m] == kNegInf ? 0.f : m_run[m]) - lift;
       float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const float pe = fast_exp2(sc[m][e] - m_use);
+        float pe;
+        if constexpr (!CAP) pe = fast_exp2(__builtin_fmaf(sc[m][e], c2, -m_use));
+        else pe = fast_exp2(sc[m][e] - m_use);
         rs[e & 3] += pe;
         sc[m][e] = pe * vs[e];
       }
@@ -429,22 +454,24 @@ void quant_attn_kernel(QuantTreeArgs qa) {
         }
       }
     }
+    if (j + ST < nt) {
+      reads_done();
+      issue_v(j + ST);
+    }
   }
 
   // The (m, l, acc) of a row tile's NW waves combined in wave order through LDS (every
   // wave's copies have landed: its last tile waited for vmcnt 0), then O / l and LSE.
   float* xm = (float*)smem;       // [NW][64]
   float* xl = xm + NW * 64;       // [NW][64]
-  float* xr = xl + NW * 64;       // [NW][64]: 1 / rel
-  f32x4* xa = (f32x4*)(xr + NW * 64);  // [NW][4 DB][64]: columns 8 y + 4 h .. + 3 of row l32
+  f32x4* xa = (f32x4*)(xl + NW * 64);  // [NW][4 DB][64]: columns 8 y + 4 h .. + 3 of row l32
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     if (32 * (rt0 + m) >= R) break;  // (every wave)
     const float l_tot = l_run[m] + swap_halves(l_run[m]);
     __syncthreads();
-    xm[wave * 64 + lane] = m_run[m];
+    xm[wave * 64 + lane] = m_run[m] - lift;  // what l and acc are relative to
     xl[wave * 64 + lane] = l_tot;
-    xr[wave * 64 + lane] = 1.0f / rel;
 #pragma unroll
     for (int y = 0; y < 4 * C::DB; ++y) {
       const f32x16& v = acc[m][y / 4];
@@ -465,7 +492,6 @@ void quant_attn_kernel(QuantTreeArgs qa) {
       const float lw = xl[w * 64 + lane];
       al[w] = mw[w] == kNegInf ? (lw == 0.f ? 0.f : 1.f) : fast_exp2(mw[w] - mall);
       L = __builtin_fmaf(al[w], lw, L);
-      al[w] *= xr[w * 64 + lane];
     }
     const bool empty = L == 0.f;  // no key; NaN (a NaN query row or key) is not
     const float inv = empty ? 0.f : 1.0f / L;
@@ -499,7 +525,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
 template <class T, int CODE, int D, int MT>
 void launch_rows(QuantTreeArgs a, hipStream_t st) {
   a.t.nrt = (int)((((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32 + MT - 1) / MT);
-  const dim3 grid((unsigned)((a.t.nchunk + 7) / 8 * 8 * a.t.nrt)), block(256);
+  const dim3 grid((unsigned)((a.t.nchunk + 7) / 8 * 8 * a.t.nrt)), block(QuantCfg<D>::NW * 64);
   if (a.t.p.cap > 0.f) hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, MT, true>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, MT, false>), grid, block, 0, st, a);
 }
@@ -507,7 +533,7 @@ void launch_rows(QuantTreeArgs a, hipStream_t st) {
 template <class T, int CODE, int D>
 void launch_code(const QuantTreeArgs& a, hipStream_t st) {
   const int mt = quant_row_tiles(D, ((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32);
-  if constexpr (D <= 128) {
+  if constexpr (D <= 64) {
     if (mt == 2) launch_rows<T, CODE, D, 2>(a, st);
   }
   if (mt == 1) launch_rows<T, CODE, D, 1>(a, st);
