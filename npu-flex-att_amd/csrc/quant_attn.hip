@@ -47,11 +47,7 @@ struct QuantCfg {
   static constexpr int E = TB / 1024;        // copies of one
   static constexpr int PK = RPC >= 16 ? 1 : 16 / RPC;  // copies after which K's swizzle repeats
   static constexpr int PV = RPC >= 8 ? 1 : 8 / RPC;    // and V's
-  static constexpr int EC = 2 * E + 1;       // copies of a stage: K, V, both scales
-  static constexpr int STB = 2 * TB + 256;   // bytes of a stage
-  static constexpr int NW = D == 128 ? 8 : 4;  // waves per workgroup
-  static constexpr int ST = D >= 128 ? 2 : 4;  // stages
-  static_assert(E * 1024 == TB && NW * ST * STB <= 160 * 1024 && E % PK == 0 && E % PV == 0, "tiles");
+  static_assert(E * 1024 == TB && E % PK == 0 && E % PV == 0, "tiles");
 };
 
 // K is read 16 bytes a lane from 32 rows, V by transpose reads of 32 bytes of 16 rows
@@ -142,29 +138,37 @@ __device__ __forceinline__ void rescale(f32x16& a, float s) {
   else scale_inplace(a, s);
 }
 
-template <class T, int CODE, int D, int MT, bool CAP>
-__global__ __launch_bounds__(QuantCfg<D>::NW * 64) __attribute__((amdgpu_waves_per_eu(D >= 256 || MT > 1 ? 1 : 2)))
+template <class T, int CODE, int D, int NW, int WPT, int MT, int ST, bool CAP>
+__global__ __launch_bounds__(NW * WPT * 64) __attribute__((amdgpu_waves_per_eu(D >= 256 || MT > 1 ? 1 : 2)))
 void quant_attn_kernel(QuantTreeArgs qa) {
   using C = QuantCfg<D>;
   typedef typename Mfma<T>::v8 V8;
-  constexpr int ST = C::ST, NW = C::NW, EC = C::EC, PK = C::PK, PV = C::PV;
+  constexpr int EW = C::E / WPT;                 // copies a wave makes of a K or V tile
+  constexpr int EC = 2 * EW + 1;                 // and of a stage, with scales
+  constexpr int SCB = WPT > 1 ? 256 : 128;       // bytes from K's scales to V's
+  constexpr int STB = 2 * C::TB + 2 * SCB;       // bytes of a stage
+  constexpr int CROWS = WPT * C::RPC;            // rows of the waves' copies
+  constexpr int PK = C::PK > WPT ? C::PK / WPT : 1, PV = C::PV > WPT ? C::PV / WPT : 1;
+  static_assert(WPT <= 2 && C::E % WPT == 0 && NW * ST * STB <= 160 * 1024, "stages");
   typedef _Float16 W;  // the weights' type
   constexpr bool REST = __is_same(T, _Float16);  // and what their rounding leaves
-  constexpr int kCombine = NW * 64 * 4 * (2 + 16 * C::DB);
-  __shared__ __attribute__((aligned(1024))) char smem[NW * ST * C::STB > kCombine ? NW * ST * C::STB : kCombine];
+  constexpr int kCombine = NW * WPT * 64 * 4 * (2 + 16 * C::DB);
+  __shared__ __attribute__((aligned(1024))) char smem[NW * ST * STB > kCombine ? NW * ST * STB : kCombine];
 
   const TreeArgs& a = qa.t;
   const Shape& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / (WPT * 64));  // its key tiles
+  const int sub = WPT > 1 ? __builtin_amdgcn_readfirstlane((tid >> 6) % WPT) : 0;
   const int h = lane >> 5, l32 = lane & 31;
 
   // (chunk, row tiles): as in tree_attn.hip
   int rt0 = 0, x = blockIdx.x;
   if (a.nrt > 1) {
-    rt0 = blockIdx.x / 8 % a.nrt * MT;
+    rt0 = blockIdx.x / 8 % a.nrt * (WPT * MT);
     x = blockIdx.x / (8 * a.nrt) * 8 + blockIdx.x % 8;
   }
+  rt0 += sub * MT;
   const TreeChunk ck = tree_chunk(a, x, NW);
   if (ck.b < 0) return;
   const int b = ck.b, hk = ck.hk, s = ck.s, ns = ck.ns;
@@ -206,13 +210,13 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   }
   // this lane's offsets in a tile's copies
   const unsigned kss = (unsigned)a.k.ss, vss = (unsigned)a.v.ss;
-  const int crow = lane / C::CPR, cchunk = lane % C::CPR;
+  const int crow = lane / C::CPR + sub * C::RPC, cchunk = lane % C::CPR;
   unsigned kvo[PK], vvo[PV];
 #pragma unroll
-  for (int e = 0; e < PK; ++e) kvo[e] = (e * C::RPC + crow) * kss + swz_k8<C::CPR>(e * C::RPC + crow, cchunk) * 16;
+  for (int e = 0; e < PK; ++e) kvo[e] = (e * CROWS + crow) * kss + swz_k8<C::CPR>(e * CROWS + crow, cchunk) * 16;
 #pragma unroll
-  for (int e = 0; e < PV; ++e) vvo[e] = (e * C::RPC + crow) * vss + swz_v8<C::CPR>(e * C::RPC + crow, cchunk) * 16;
-  const unsigned wbase = lds_addr_of(smem) + wave * (ST * C::STB);
+  for (int e = 0; e < PV; ++e) vvo[e] = (e * CROWS + crow) * vss + swz_v8<C::CPR>(e * CROWS + crow, cchunk) * 16;
+  const unsigned wbase = lds_addr_of(smem) + wave * (ST * STB);
   auto reads_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
 
   // this wave's tiles: first + NW * j, j < nt
@@ -221,40 +225,41 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   const int nt = __builtin_amdgcn_readfirstlane(max((ck.count - wave + NW - 1) / NW, 0));
   const uint64_t kp = (uint64_t)((const char*)a.k.data + b * a.k.sb + hk * a.k.sh);
   const uint64_t vp = (uint64_t)((const char*)a.v.data + b * a.v.sb + hk * a.v.sh);
-  const float* scales = (h ? qa.v_scales : qa.k_scales) + ((int64_t)b * p.Hkv + hk) * p.Skv;
+  // (alone a wave copies both tensors' scales, 32 lanes each, of two waves each one's)
+  const float* scales = ((WPT > 1 ? sub : h) ? qa.v_scales : qa.k_scales) + ((int64_t)b * p.Hkv + hk) * p.Skv;
   // K, V and scales of tile j of this wave into its stage
   auto issue_k = [&](int j) {
     const int t = first + NW * j;
-    const unsigned dst = wbase + j % ST * C::STB;
+    const unsigned dst = wbase + j % ST * STB + sub * 1024;
     const uint64_t base = kp + (uint64_t)(t * C::BN) * kss;
     if (t * C::BN + C::BN - 1 <= last) {
 #pragma unroll
-      for (int e = 0; e < C::E; ++e)
-        load_lds16_base(kvo[e % PK], base + (uint64_t)(e / PK * PK * C::RPC) * kss, dst + e * 1024);
+      for (int e = 0; e < EW; ++e)
+        load_lds16_base(kvo[e % PK], base + (uint64_t)(e / PK * PK * CROWS) * kss, dst + e * (WPT * 1024));
     } else {  // rows behind the last one repeat it
 #pragma unroll 1
-      for (int e = 0; e < C::E; ++e) {
-        const int kr = e * C::RPC + crow;
-        load_lds16_base(min(kr, last - t * C::BN) * kss + swz_k8<C::CPR>(kr, cchunk) * 16, base, dst + e * 1024);
+      for (int e = 0; e < EW; ++e) {
+        const int kr = e * CROWS + crow;
+        load_lds16_base(min(kr, last - t * C::BN) * kss + swz_k8<C::CPR>(kr, cchunk) * 16, base, dst + e * (WPT * 1024));
       }
     }
   };
   auto issue_v = [&](int j) {
     const int t = first + NW * j;
-    const unsigned dst = wbase + j % ST * C::STB + C::TB;
+    const unsigned dst = wbase + j % ST * STB + C::TB + sub * 1024;
     const uint64_t base = vp + (uint64_t)(t * C::BN) * vss;
     if (t * C::BN + C::BN - 1 <= last) {
 #pragma unroll
-      for (int e = 0; e < C::E; ++e)
-        load_lds16_base(vvo[e % PV], base + (uint64_t)(e / PV * PV * C::RPC) * vss, dst + e * 1024);
+      for (int e = 0; e < EW; ++e)
+        load_lds16_base(vvo[e % PV], base + (uint64_t)(e / PV * PV * CROWS) * vss, dst + e * (WPT * 1024));
     } else {
 #pragma unroll 1
-      for (int e = 0; e < C::E; ++e) {
-        const int kr = e * C::RPC + crow;
-        load_lds16_base(min(kr, last - t * C::BN) * vss + swz_v8<C::CPR>(kr, cchunk) * 16, base, dst + e * 1024);
+      for (int e = 0; e < EW; ++e) {
+        const int kr = e * CROWS + crow;
+        load_lds16_base(min(kr, last - t * C::BN) * vss + swz_v8<C::CPR>(kr, cchunk) * 16, base, dst + e * (WPT * 1024));
       }
     }
-    load_lds4(scales + min(t * C::BN + l32, last), dst + C::TB);
+    load_lds4(scales + min(t * C::BN + l32, last), wbase + j % ST * STB + 2 * C::TB + sub * SCB);
   };
   if (nt > 0) {
     issue_k(0);
@@ -301,7 +306,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
       pin(qf[m][kc]);
     }
 #pragma unroll
-  for (int j = 1; j < ST; ++j)
+  for (int j = 1; j < (WPT > 1 ? ST - 1 : ST); ++j)
     if (j < nt) {
       issue_k(j);
       issue_v(j);
@@ -318,18 +323,33 @@ void quant_attn_kernel(QuantTreeArgs qa) {
     for (int db = 0; db < C::DB; ++db) acc[m][db] = f32x16{};
   }
 
-  for (int j = 0; j < nt; ++j) {
+  // tile j landed, later ones in flight (at most `most` of them)
+  auto landed = [&](int j, auto most) {
+    constexpr int N = most;
+    const int left = nt - 1 - j;
+    if (left >= N) wait_vmcnt<N * EC>();
+    else if (N > 2 && left == 2) wait_vmcnt<(N > 2 ? 2 : 0) * EC>();
+    else if (N > 1 && left == 1) wait_vmcnt<(N > 1 ? 1 : 0) * EC>();
+    else wait_vmcnt<0>();
+  };
+  const int steps = WPT == 1 ? nt : __builtin_amdgcn_readfirstlane((ck.count + NW - 1) / NW);
+  for (int j = 0; j < steps; ++j) {
     const int n0 = (first + NW * j) * C::BN;
-    if (j + ST - 1 < nt) {
-      wait_vmcnt<(ST - 1) * EC>();  // tile j landed, the next ones in flight
-    } else if (ST > 2 && j + 2 < nt) {
-      wait_vmcnt<(ST > 2 ? 2 : 0) * EC>();
-    } else if (ST > 2 && j + 1 < nt) {
-      wait_vmcnt<(ST > 2 ? 1 : 0) * EC>();
+    if constexpr (WPT > 1) {
+      // this wave's copies of tile j have landed and its reads of tile j - 1 have returned ...
+      landed(j, std::integral_constant<int, ST - 2>{});
+      reads_done();
+      __builtin_amdgcn_s_barrier();  // ... and every wave's
+      asm volatile("" ::: "memory");
+      if (j + ST - 1 < nt) {
+        issue_k(j + ST - 1);
+        issue_v(j + ST - 1);
+      }
+      if (j >= nt || 32 * rt0 >= R) continue;  // (the last step of waves with one tile less; waves without rows)
     } else {
-      wait_vmcnt<0>();
+      landed(j, std::integral_constant<int, ST - 1>{});
     }
-    const char* sK = smem + wave * (ST * C::STB) + j % ST * C::STB;
+    const char* sK = smem + wave * (ST * STB) + j % ST * STB;
     const char* sV = sK + C::TB;
     const char* sS = sV + C::TB + 16 * h;
 
@@ -346,15 +366,17 @@ void quant_attn_kernel(QuantTreeArgs qa) {
         sc[m] = Mfma<T>::mma(k1, as_v8<V8>(qf[m][2 * kc + 1]), sc[m]);
       }
     }
-    if (j + ST < nt) {  // K's half of the stage is free
-      reads_done();
-      issue_k(j + ST);
+    if constexpr (WPT == 1) {
+      if (j + ST < nt) {  // K's half of the stage is free
+        reads_done();
+        issue_k(j + ST);
+      }
     }
     // scales of this lane's keys: element e is key n0 + 8(e/4) + 4h + e%4
     f32x16 ks, vs;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const i32x4 k4 = lds_read16(sS + 32 * i), v4 = lds_read16(sS + 128 + 32 * i);
+      const i32x4 k4 = lds_read16(sS + 32 * i), v4 = lds_read16(sS + SCB + 32 * i);
 #pragma unroll
       for (int e = 0; e < 4; ++e) ks[4 * i + e] = __int_as_float(k4[e]), vs[4 * i + e] = __int_as_float(v4[e]);
     }
@@ -454,20 +476,22 @@ void quant_attn_kernel(QuantTreeArgs qa) {
         }
       }
     }
-    if (j + ST < nt) {
-      reads_done();
-      issue_v(j + ST);
+    if constexpr (WPT == 1) {
+      if (j + ST < nt) {
+        reads_done();
+        issue_v(j + ST);
+      }
     }
   }
 
   // The (m, l, acc) of a row tile's NW waves combined in wave order through LDS (every
   // wave's copies have landed: its last tile waited for vmcnt 0), then O / l and LSE.
-  float* xm = (float*)smem;       // [NW][64]
-  float* xl = xm + NW * 64;       // [NW][64]
+  float* xm = (float*)smem + sub * NW * 64 * (2 + 16 * C::DB);  // [NW][64]
+  float* xl = xm + NW * 64;                                     // [NW][64]
   f32x4* xa = (f32x4*)(xl + NW * 64);  // [NW][4 DB][64]: columns 8 y + 4 h .. + 3 of row l32
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    if (32 * (rt0 + m) >= R) break;  // (every wave)
+    if (WPT == 1 && 32 * (rt0 + m) >= R) break;  // (every wave)
     const float l_tot = l_run[m] + swap_halves(l_run[m]);
     __syncthreads();
     xm[wave * 64 + lane] = m_run[m] - lift;  // what l and acc are relative to
@@ -522,21 +546,29 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   }
 }
 
-template <class T, int CODE, int D, int MT>
+template <class T, int CODE, int D, int NW, int WPT, int MT, int ST>
 void launch_rows(QuantTreeArgs a, hipStream_t st) {
-  a.t.nrt = (int)((((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32 + MT - 1) / MT);
-  const dim3 grid((unsigned)((a.t.nchunk + 7) / 8 * 8 * a.t.nrt)), block(QuantCfg<D>::NW * 64);
-  if (a.t.p.cap > 0.f) hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, MT, true>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, MT, false>), grid, block, 0, st, a);
+  a.t.nrt = (int)((((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32 + WPT * MT - 1) / (WPT * MT));
+  const dim3 grid((unsigned)((a.t.nchunk + 7) / 8 * 8 * a.t.nrt)), block(NW * WPT * 64);
+  if (a.t.p.cap > 0.f) hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, NW, WPT, MT, ST, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, NW, WPT, MT, ST, false>), grid, block, 0, st, a);
 }
 
 template <class T, int CODE, int D>
 void launch_code(const QuantTreeArgs& a, hipStream_t st) {
-  const int mt = quant_row_tiles(D, ((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32);
-  if constexpr (D <= 64) {
-    if (mt == 2) launch_rows<T, CODE, D, 2>(a, st);
+  const int share = quant_row_tiles(D, ((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32);
+  if constexpr (D == 128) {
+    if (share == 2) launch_rows<T, CODE, D, 4, 2, 1, 4>(a, st);
+    else launch_rows<T, CODE, D, 8, 1, 1, 2>(a, st);
+  } else if constexpr (D == 64) {
+    if (share == 2) launch_rows<T, CODE, D, 4, 2, 1, 4>(a, st);
+    else launch_rows<T, CODE, D, 4, 1, 1, 4>(a, st);
+  } else if constexpr (D == 32) {
+    if (share == 2) launch_rows<T, CODE, D, 4, 1, 2, 4>(a, st);
+    else launch_rows<T, CODE, D, 4, 1, 1, 4>(a, st);
+  } else {
+    launch_rows<T, CODE, D, 4, 1, 1, 2>(a, st);
   }
-  if (mt == 1) launch_rows<T, CODE, D, 1>(a, st);
 }
 
 template <class T, int D>
