@@ -102,28 +102,6 @@ __device__ __forceinline__ typename Mfma<T>::v8 operand8(int lo, int hi) {
   return as_v8<typename Mfma<T>::v8>(v);
 }
 
-// acc *= s where the accumulators stay in their half of the register file: a multiply of
-// its own would have all of them moved back and forth around the branch it is in, in every
-// iteration.  The waits are those between an MFMA and a read of its result, and between
-// the last write and an MFMA.
-__device__ __forceinline__ void scale_acc(f32x16& a, float s) {
-#pragma unroll
-  for (int r = 0; r < 16; r += 4) {
-    float x0, x1, x2, x3, y0 = a[r], y1 = a[r + 1], y2 = a[r + 2], y3 = a[r + 3];
-    asm volatile(
-        "s_nop 15\n\ts_nop 3\n\t"
-        "v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\t"
-        "v_accvgpr_read_b32 %6, %2\n\tv_accvgpr_read_b32 %7, %3\n\ts_nop 1\n\t"
-        "v_mul_f32_e32 %4, %8, %4\n\tv_mul_f32_e32 %5, %8, %5\n\t"
-        "v_mul_f32_e32 %6, %8, %6\n\tv_mul_f32_e32 %7, %8, %7\n\ts_nop 1\n\t"
-        "v_accvgpr_write_b32 %0, %4\n\tv_accvgpr_write_b32 %1, %5\n\t"
-        "v_accvgpr_write_b32 %2, %6\n\tv_accvgpr_write_b32 %3, %7\n\ts_nop 3"
-        : "+a"(y0), "+a"(y1), "+a"(y2), "+a"(y3), "=&v"(x0), "=&v"(x1), "=&v"(x2), "=&v"(x3)
-        : "v"(s));
-    a[r] = y0, a[r + 1] = y1, a[r + 2] = y2, a[r + 3] = y3;
-  }
-}
-
 // Transposed 8 x 8-bit read: lane i of 16 gets byte i % 8 at the addresses of lanes
 // 2 t + i / 8, t = 0 .. 7.
 __device__ __forceinline__ i32x2 lds_read_tr8(const void* p) {
@@ -131,27 +109,21 @@ __device__ __forceinline__ i32x2 lds_read_tr8(const void* p) {
       (__attribute__((address_space(3))) i32x2*)((__attribute__((address_space(3))) char*)p));
 }
 
-// Accumulators of two row tiles have only that half to be in.
-template <int MT>
-__device__ __forceinline__ void rescale(f32x16& a, float s) {
-  if constexpr (MT > 1) scale_acc(a, s);
-  else scale_inplace(a, s);
-}
-
-template <class T, int CODE, int D, int NW, int WPT, int MT, int ST, bool CAP>
-__global__ __launch_bounds__(NW * WPT * 64) __attribute__((amdgpu_waves_per_eu(D >= 256 || MT > 1 ? 1 : 2)))
+// WPT neighbouring waves, a row tile each, share their key tiles (as in tree_attn.hip).
+template <class T, int CODE, int D, int NW, int WPT, int ST, bool CAP>
+__global__ __launch_bounds__(NW * WPT * 64) __attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : 2)))
 void quant_attn_kernel(QuantTreeArgs qa) {
   using C = QuantCfg<D>;
   typedef typename Mfma<T>::v8 V8;
+  typedef _Float16 W;  // the weights' type
+  constexpr bool REST = __is_same(T, _Float16);  // and what their rounding leaves
   constexpr int EW = C::E / WPT;                 // copies a wave makes of a K or V tile
   constexpr int EC = 2 * EW + 1;                 // and of a stage, with scales
   constexpr int SCB = WPT > 1 ? 256 : 128;       // bytes from K's scales to V's
   constexpr int STB = 2 * C::TB + 2 * SCB;       // bytes of a stage
   constexpr int CROWS = WPT * C::RPC;            // rows of the waves' copies
   constexpr int PK = C::PK > WPT ? C::PK / WPT : 1, PV = C::PV > WPT ? C::PV / WPT : 1;
-  static_assert(WPT <= 2 && C::E % WPT == 0 && NW * ST * STB <= 160 * 1024, "stages");
-  typedef _Float16 W;  // the weights' type
-  constexpr bool REST = __is_same(T, _Float16);  // and what their rounding leaves
+  static_assert(WPT <= 2 && C::E % WPT == 0 && ST >= WPT + 1 && NW * ST * STB <= 160 * 1024, "stages");
   constexpr int kCombine = NW * WPT * 64 * 4 * (2 + 16 * C::DB);
   __shared__ __attribute__((aligned(1024))) char smem[NW * ST * STB > kCombine ? NW * ST * STB : kCombine];
 
@@ -165,10 +137,10 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   // (chunk, row tiles): as in tree_attn.hip
   int rt0 = 0, x = blockIdx.x;
   if (a.nrt > 1) {
-    rt0 = blockIdx.x / 8 % a.nrt * (WPT * MT);
+    rt0 = blockIdx.x / 8 % a.nrt * WPT;
     x = blockIdx.x / (8 * a.nrt) * 8 + blockIdx.x % 8;
   }
-  rt0 += sub * MT;
+  rt0 += sub;
   const TreeChunk ck = tree_chunk(a, x, NW);
   if (ck.b < 0) return;
   const int b = ck.b, hk = ck.hk, s = ck.s, ns = ck.ns;
@@ -177,24 +149,15 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   sq.t0 = __builtin_amdgcn_readfirstlane(sq.t0);
   if (rt0 == 0 && s == 0 && tid == 0 && a.counts) a.counts[b * p.Hkv + hk] = sq.bad ? 1 : ns;
 
-  // packed query rows of this lane: head, drafted token
+  // packed query row of this lane: head, drafted token
   const int R = p.G * p.Sq;
-  int hq[MT], qi[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int r = min(32 * (rt0 + m) + l32, R - 1);
-    hq[m] = hk * p.G + r % p.G;
-    qi[m] = r / p.G;
-  }
+  const int r = min(32 * rt0 + l32, R - 1);
+  const int hq = hk * p.G + r % p.G, qi = r / p.G;
   if (sq.bad) {
-    if (s == 0) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (32 * (rt0 + m) + l32 >= R) continue;
-        T* out = (T*)a.o.data + b * a.o.sb + hq[m] * a.o.sh + (int64_t)qi[m] * a.o.ss;
-        for (int d = wave * 2 + h; d < D; d += NW * 2) out[d] = from_f32<T>(__builtin_nanf(""));
-        if (wave == 0 && h == 0) a.lse[((int64_t)b * p.Hq + hq[m]) * p.Sq + qi[m]] = __builtin_nanf("");
-      }
+    if (s == 0 && 32 * rt0 + l32 < R) {
+      T* out = (T*)a.o.data + b * a.o.sb + hq * a.o.sh + (int64_t)qi * a.o.ss;
+      for (int d = wave * 2 + h; d < D; d += NW * 2) out[d] = from_f32<T>(__builtin_nanf(""));
+      if (wave == 0 && h == 0) a.lse[((int64_t)b * p.Hq + hq) * p.Sq + qi] = __builtin_nanf("");
     }
     return;
   }
@@ -217,6 +180,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
 #pragma unroll
   for (int e = 0; e < PV; ++e) vvo[e] = (e * CROWS + crow) * vss + swz_v8<C::CPR>(e * CROWS + crow, cchunk) * 16;
   const unsigned wbase = lds_addr_of(smem) + wave * (ST * STB);
+  // this wave's LDS reads have returned: the buffer they read may be refilled
   auto reads_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
 
   // this wave's tiles: first + NW * j, j < nt
@@ -227,7 +191,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   const uint64_t vp = (uint64_t)((const char*)a.v.data + b * a.v.sb + hk * a.v.sh);
   // (alone a wave copies both tensors' scales, 32 lanes each, of two waves each one's)
   const float* scales = ((WPT > 1 ? sub : h) ? qa.v_scales : qa.k_scales) + ((int64_t)b * p.Hkv + hk) * p.Skv;
-  // K, V and scales of tile j of this wave into its stage
+  // K, and V with the scales, of tile j of this wave into its stage
   auto issue_k = [&](int j) {
     const int t = first + NW * j;
     const unsigned dst = wbase + j % ST * STB + sub * 1024;
@@ -267,25 +231,16 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   }
 
   // Q: lane half h has elements 32 kc + 16 h .. + 15 of its row, the codes' order
-  i32x4 qf[MT][2 * C::KC];
+  i32x4 qf[2 * C::KC];
+  const char* src = (const char*)((const T*)a.q.data + b * a.q.sb + hq * a.q.sh + (int64_t)qi * a.q.ss) + 32 * h;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const char* src = (const char*)((const T*)a.q.data + b * a.q.sb + hq[m] * a.q.sh + (int64_t)qi[m] * a.q.ss) + 32 * h;
-#pragma unroll
-    for (int kc = 0; kc < 2 * C::KC; ++kc) qf[m][kc] = ld_global16(src + 64 * (kc >> 1) + 16 * (kc & 1));
-  }
+  for (int kc = 0; kc < 2 * C::KC; ++kc) qf[kc] = ld_global16(src + 64 * (kc >> 1) + 16 * (kc & 1));
   // Row qi sees the cached keys [row_lo, n); the tiles that hold only keys every row
   // sees need no mask.
-  int row_lo[MT], full_lo = 0;
-#pragma unroll
-  for (int m = 0; m < MT; ++m) row_lo[m] = 0;
+  int row_lo = 0, full_lo = 0;
   if (p.window > 0) {
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int depth = a.depths ? max(a.depths[(int64_t)b * p.Sq + qi[m]], 0) : qi[m];
-      row_lo[m] = max(n - (p.window - min(depth, p.window)), 0);
-      full_lo = max(full_lo, row_lo[m]);
-    }
+    const int depth = a.depths ? max(a.depths[(int64_t)b * p.Sq + qi], 0) : qi;
+    full_lo = row_lo = max(n - (p.window - min(depth, p.window)), 0);
 #pragma unroll
     for (int y = 32; y; y >>= 1) full_lo = max(full_lo, __shfl_xor(full_lo, y));
     full_lo = __builtin_amdgcn_readfirstlane(full_lo);
@@ -299,79 +254,82 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   }
   // wait for Q here, once: see fwd_split.hip
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int kc = 0; kc < 2 * C::KC; ++kc) {
+    qf[kc] ^= i32x4{flip, flip, flip, flip};
+    pin(qf[kc]);
+  }
+  wait_vmcnt<0>();  // (and the first tile)
 #pragma unroll
-    for (int kc = 0; kc < 2 * C::KC; ++kc) {
-      qf[m][kc] ^= i32x4{flip, flip, flip, flip};
-      pin(qf[m][kc]);
-    }
-#pragma unroll
-  for (int j = 1; j < (WPT > 1 ? ST - 1 : ST); ++j)
+  for (int j = 1; j < ST; ++j)
     if (j < nt) {
       issue_k(j);
-      issue_v(j);
+      if (WPT == 1 || j < ST - 1) issue_v(j);
     }
 
-  f32x16 acc[MT][C::DB];
-  float m_run[MT], l_run[MT];
+  f32x16 acc[C::DB];
+  float m_run = kNegInf, l_run = 0.f;
+#pragma unroll
+  for (int db = 0; db < C::DB; ++db) acc[db] = f32x16{};
   // weights are 2^(x - m_run + lift), and rel = 2^lift times a scale is at most 1
   float lift = 90.f, rel = 0x1p90f;
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    m_run[m] = kNegInf, l_run[m] = 0.f;
-#pragma unroll
-    for (int db = 0; db < C::DB; ++db) acc[m][db] = f32x16{};
-  }
 
-  // tile j landed, later ones in flight (at most `most` of them)
-  auto landed = [&](int j, auto most) {
-    constexpr int N = most;
-    const int left = nt - 1 - j;
-    if (left >= N) wait_vmcnt<N * EC>();
-    else if (N > 2 && left == 2) wait_vmcnt<(N > 2 ? 2 : 0) * EC>();
-    else if (N > 1 && left == 1) wait_vmcnt<(N > 1 ? 1 : 0) * EC>();
+  // K of tile j + 1, and all that was issued before it, lands.  What may be in flight
+  // behind it: V of that tile and up to ST - 2 whole tiles; of waves that share tiles, K and
+  // V of ST - 2 tiles in the order V, K, as far as there are tiles.
+  auto landed = [&](int j) {
+    constexpr int N = ST - 2, X = WPT > 1 ? 0 : EW + 1;
+    static_assert(N <= 2, "stages");
+    const int more = nt - 2 - j;  // tiles behind tile j + 1
+    if (more >= N) wait_vmcnt<N * EC + X>();
+    else if (N > 1 && more == 1) wait_vmcnt<(WPT > 1 ? 2 * EC - EW : EC + X)>();
+    else if (more == 0) wait_vmcnt<EW + 1>();
     else wait_vmcnt<0>();
   };
+  // K's fragments of tile j, and S^T from them: codes alone
+  auto read_k = [&](int j, i32x4 (&kf)[C::KC]) {
+    const char* sK = smem + wave * (ST * STB) + j % ST * STB;
+#pragma unroll
+    for (int kc = 0; kc < C::KC; ++kc) kf[kc] = lds_read16(sK + koff[kc]);
+  };
+  auto scores = [&](const i32x4 (&kf)[C::KC]) {
+    f32x16 sc = f32x16{};
+#pragma unroll
+    for (int kc = 0; kc < C::KC; ++kc) {
+      sc = Mfma<T>::mma(operand8<T, CODE>(kf[kc][0], kf[kc][1]), as_v8<V8>(qf[2 * kc]), sc);
+      sc = Mfma<T>::mma(operand8<T, CODE>(kf[kc][2], kf[kc][3]), as_v8<V8>(qf[2 * kc + 1]), sc);
+    }
+    return sc;
+  };
+
   const int steps = WPT == 1 ? nt : __builtin_amdgcn_readfirstlane((ck.count + NW - 1) / NW);
+  if constexpr (WPT > 1) {
+    __builtin_amdgcn_s_barrier();  // every wave's copies of its first tile
+    asm volatile("" ::: "memory");
+  }
+  i32x4 kf[C::KC];
+  read_k(0, kf);
+  f32x16 sc = scores(kf);
   for (int j = 0; j < steps; ++j) {
     const int n0 = (first + NW * j) * C::BN;
+    // K of tile j + 1 and V of tile j land; what has been read is refilled
     if constexpr (WPT > 1) {
-      // this wave's copies of tile j have landed and its reads of tile j - 1 have returned ...
-      landed(j, std::integral_constant<int, ST - 2>{});
+      // this wave's copies have landed and its reads of tile j - 1 have returned ...
+      landed(j);
       reads_done();
       __builtin_amdgcn_s_barrier();  // ... and every wave's
       asm volatile("" ::: "memory");
-      if (j + ST - 1 < nt) {
-        issue_k(j + ST - 1);
-        issue_v(j + ST - 1);
-      }
+      if (j + ST - 1 < nt) issue_v(j + ST - 1);
+      if (j + ST < nt) issue_k(j + ST);
       if (j >= nt || 32 * rt0 >= R) continue;  // (the last step of waves with one tile less; waves without rows)
     } else {
-      landed(j, std::integral_constant<int, ST - 1>{});
-    }
-    const char* sK = smem + wave * (ST * STB) + j % ST * STB;
-    const char* sV = sK + C::TB;
-    const char* sS = sV + C::TB + 16 * h;
-
-    f32x16 sc[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) sc[m] = f32x16{};
-#pragma unroll
-    for (int kc = 0; kc < C::KC; ++kc) {
-      const i32x4 kf = lds_read16(sK + koff[kc]);
-      const V8 k0 = operand8<T, CODE>(kf[0], kf[1]), k1 = operand8<T, CODE>(kf[2], kf[3]);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        sc[m] = Mfma<T>::mma(k0, as_v8<V8>(qf[m][2 * kc]), sc[m]);
-        sc[m] = Mfma<T>::mma(k1, as_v8<V8>(qf[m][2 * kc + 1]), sc[m]);
-      }
-    }
-    if constexpr (WPT == 1) {
-      if (j + ST < nt) {  // K's half of the stage is free
+      landed(j);
+      if (j + ST < nt) {
         reads_done();
         issue_k(j + ST);
       }
     }
+    const char* sV = smem + wave * (ST * STB) + j % ST * STB + C::TB;
+    const char* sS = sV + C::TB + 16 * h;
     // scales of this lane's keys: element e is key n0 + 8(e/4) + 4h + e%4
     f32x16 ks, vs;
 #pragma unroll
@@ -380,6 +338,14 @@ void quant_attn_kernel(QuantTreeArgs qa) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) ks[4 * i + e] = __int_as_float(k4[e]), vs[4 * i + e] = __int_as_float(v4[e]);
     }
+    // ... and all else that the tile reads, which is there when it is used
+    read_k(j + 1, kf);
+    i32x2 vf[2][C::DB];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int db = 0; db < C::DB; ++db) vf[c][db] = lds_read_tr8(sV + 16 * c * D + voff[db]);
+    asm volatile("" ::: "memory");
     float top, top2;
     max16_partial(vs, top, top2);
     top = max2(top, top2);
@@ -388,94 +354,82 @@ void quant_attn_kernel(QuantTreeArgs qa) {
       // the power of two above the largest scale, as far as there is one
       const int expo = (int)(__float_as_uint(top) >> 23) & 255, field = min(max(253 - expo, 1), 217);
       const float now = __int_as_float(field << 23), turn = now / rel;
+      l_run *= turn;
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        l_run[m] *= turn;
-#pragma unroll
-        for (int db = 0; db < C::DB; ++db) rescale<MT>(acc[m][db], turn);
-      }
+      for (int db = 0; db < C::DB; ++db) scale_inplace(acc[db], turn);
       rel = now;
       lift = (float)(field - 127);
     }
-
-    auto softmax = [&](auto which) {  // (a loop over them is not unrolled)
-      constexpr int m = which;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sc[m][e] *= ks[e];
-      if constexpr (CAP) {
-        soft_cap(sc[m], p);
+    for (int e = 0; e < 16; ++e) sc[e] *= ks[e];
+    if constexpr (CAP) {
+      soft_cap(sc, p);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sc[m][e] *= p.cap_log2;
-      }
-      if (n0 < full_lo || n0 + C::BN > n) {
-        // this lane's keys, relative to its first: e, and hidden before lo or from hi on
-        const int lo = row_lo[m] - n0 - 4 * h, hi = n + (mask ? p.Sq : qi[m] + 1) - n0 - 4 * h;
+      for (int e = 0; e < 16; ++e) sc[e] *= p.cap_log2;
+    }
+    if (n0 < full_lo || n0 + C::BN > n) {
+      // this lane's keys, relative to its first: e, and hidden before lo or from hi on
+      const int lo = row_lo - n0 - 4 * h, hi = n + (mask ? p.Sq : qi + 1) - n0 - 4 * h;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if ((unsigned)(8 * (e >> 2) + (e & 3) - lo) >= (unsigned)max(hi - lo, 0)) sc[e] = kNegInf;
+      if (mask && n0 + C::BN > n) {  // all of the tile's mask bytes at once
+        const unsigned char* mrow = mask + (int64_t)qi * p.Sq;
+        const int u0 = n0 + 4 * h - n;
+        unsigned char mb[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mb[e] = mrow[min(max(u0 + 8 * (e >> 2) + (e & 3), 0), p.Sq - 1)];
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if ((unsigned)(8 * (e >> 2) + (e & 3) - lo) >= (unsigned)max(hi - lo, 0)) sc[m][e] = kNegInf;
-        if (mask && n0 + C::BN > n) {  // all of the tile's mask bytes at once
-          const unsigned char* mrow = mask + (int64_t)qi[m] * p.Sq;
-          const int u0 = n0 + 4 * h - n;
-          unsigned char mb[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) mb[e] = mrow[min(max(u0 + 8 * (e >> 2) + (e & 3), 0), p.Sq - 1)];
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (u0 + 8 * (e >> 2) + (e & 3) >= 0 && mb[e] == 0) sc[m][e] = kNegInf;
-        }
-      }
-      float mx, mx2;
-      max16_partial(sc[m], mx, mx2);
-      mx = max2(mx, mx2);
-      if constexpr (!CAP) mx *= c2;
-      mx = fmaxf(mx, swap_halves(mx));
-      if (mx != mx) mx = kNegInf;
-      const bool grow = mx > m_run[m] + kTreeRescale;
-      if (__builtin_amdgcn_ballot_w64(grow)) {
-        const float m_new = grow ? mx : m_run[m];
-        const float alpha = grow ? fast_exp2(m_run[m] - m_new) : 1.f;
-        l_run[m] *= alpha;
-#pragma unroll
-        for (int db = 0; db < C::DB; ++db) rescale<MT>(acc[m][db], alpha);
-        m_run[m] = m_new;
-      }
-      const float m_use = (m_run[m] == kNegInf ? 0.f : m_run[m]) - lift;
-      float rs[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        float pe;
-        if constexpr (!CAP) pe = fast_exp2(__builtin_fmaf(sc[m][e], c2, -m_use));
-        else pe = fast_exp2(sc[m][e] - m_use);
-        rs[e & 3] += pe;
-        sc[m][e] = pe * vs[e];
-      }
-      l_run[m] += (rs[0] + rs[1]) + (rs[2] + rs[3]);
-    };
-    softmax(std::integral_constant<int, 0>{});
-    if constexpr (MT > 1) softmax(std::integral_constant<int, 1>{});
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      Mfma<W>::v8 pb[MT], pl[MT];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        pb[m] = pack8<W>(sc[m], 8 * c);
-        if constexpr (REST) {
-#pragma unroll
-          for (int t = 0; t < 8; ++t) pl[m][t] = (W)(sc[m][8 * c + t] - (float)pb[m][t]);
-        }
-      }
-      const char* vr = sV + 16 * c * D;
-#pragma unroll
-      for (int db = 0; db < C::DB; ++db) {
-        const i32x2 w = lds_read_tr8(vr + voff[db]);
-        const Mfma<W>::v8 v = operand8<W, CODE>(w[0], w[1]);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          acc[m][db] = Mfma<W>::mma(v, pb[m], acc[m][db]);
-          if constexpr (REST) acc[m][db] = Mfma<W>::mma(v, pl[m], acc[m][db]);
-        }
+          if (u0 + 8 * (e >> 2) + (e & 3) >= 0 && mb[e] == 0) sc[e] = kNegInf;
       }
     }
+    float mx, mx2;
+    max16_partial(sc, mx, mx2);
+    mx = max2(mx, mx2);
+    if constexpr (!CAP) mx *= c2;
+    mx = fmaxf(mx, swap_halves(mx));
+    if (mx != mx) mx = kNegInf;
+    const bool grow = mx > m_run + kTreeRescale;
+    if (__builtin_amdgcn_ballot_w64(grow)) {
+      const float m_new = grow ? mx : m_run;
+      const float alpha = grow ? fast_exp2(m_run - m_new) : 1.f;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < C::DB; ++db) scale_inplace(acc[db], alpha);
+      m_run = m_new;
+    }
+    const float m_use = (m_run == kNegInf ? 0.f : m_run) - lift;
+
+    // From here on one block: the next tile's scores (behind the last one of what is
+    // there, and not used) between this one's weights, whose product follows.
+    const f32x16 next = scores(kf);
+    float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      float pe;
+      if constexpr (!CAP) pe = fast_exp2(__builtin_fmaf(sc[e], c2, -m_use));
+      else pe = fast_exp2(sc[e] - m_use);
+      rs[e & 3] += pe;
+      sc[e] = pe * vs[e];
+    }
+    l_run += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const Mfma<W>::v8 pb = pack8<W>(sc, 8 * c);
+      Mfma<W>::v8 pl;
+      if constexpr (REST) {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) pl[t] = (W)(sc[8 * c + t] - (float)pb[t]);
+      }
+#pragma unroll
+      for (int db = 0; db < C::DB; ++db) {
+        const Mfma<W>::v8 v = operand8<W, CODE>(vf[c][db][0], vf[c][db][1]);
+        acc[db] = Mfma<W>::mma(v, pb, acc[db]);
+        if constexpr (REST) acc[db] = Mfma<W>::mma(v, pl, acc[db]);
+      }
+    }
+    sc = next;
     if constexpr (WPT == 1) {
       if (j + ST < nt) {
         reads_done();
@@ -489,85 +443,75 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   float* xm = (float*)smem + sub * NW * 64 * (2 + 16 * C::DB);  // [NW][64]
   float* xl = xm + NW * 64;                                     // [NW][64]
   f32x4* xa = (f32x4*)(xl + NW * 64);  // [NW][4 DB][64]: columns 8 y + 4 h .. + 3 of row l32
+  const float l_tot = l_run + swap_halves(l_run);
+  __syncthreads();
+  xm[wave * 64 + lane] = m_run - lift;  // what l and acc are relative to
+  xl[wave * 64 + lane] = l_tot;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    if (WPT == 1 && 32 * (rt0 + m) >= R) break;  // (every wave)
-    const float l_tot = l_run[m] + swap_halves(l_run[m]);
-    __syncthreads();
-    xm[wave * 64 + lane] = m_run[m] - lift;  // what l and acc are relative to
-    xl[wave * 64 + lane] = l_tot;
+  for (int y = 0; y < 4 * C::DB; ++y) {
+    const f32x16& v = acc[y / 4];
+    const int e = y % 4 * 4;
+    xa[(wave * 4 * C::DB + y) * 64 + lane] = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+  }
+  __syncthreads();
+  float mw[NW], mall = kNegInf;
 #pragma unroll
-    for (int y = 0; y < 4 * C::DB; ++y) {
-      const f32x16& v = acc[m][y / 4];
-      const int e = y % 4 * 4;
-      xa[(wave * 4 * C::DB + y) * 64 + lane] = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
-    }
-    __syncthreads();
-    float mw[NW], mall = kNegInf;
+  for (int w = 0; w < NW; ++w) {
+    mw[w] = xm[w * 64 + lane];
+    mall = fmaxf(mall, mw[w]);
+  }
+  float al[NW], L = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      mw[w] = xm[w * 64 + lane];
-      mall = fmaxf(mall, mw[w]);
-    }
-    float al[NW], L = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      // a wave whose maximum stayed -inf has weights of 0, or NaN scores
-      const float lw = xl[w * 64 + lane];
-      al[w] = mw[w] == kNegInf ? (lw == 0.f ? 0.f : 1.f) : fast_exp2(mw[w] - mall);
-      L = __builtin_fmaf(al[w], lw, L);
-    }
-    const bool empty = L == 0.f;  // no key; NaN (a NaN query row or key) is not
-    const float inv = empty ? 0.f : 1.0f / L;
-    if (32 * (rt0 + m) + l32 < R) {
-      const int64_t row = ((int64_t)b * p.Hq + hq[m]) * p.Sq + qi[m];
-      float* po = a.part_o + (row * a.nsplit + s) * D + 4 * h;
-      T* out = (T*)a.o.data + b * a.o.sb + hq[m] * a.o.sh + (int64_t)qi[m] * a.o.ss + 4 * h;
+  for (int w = 0; w < NW; ++w) {
+    // a wave whose maximum stayed -inf has weights of 0, or NaN scores
+    const float lw = xl[w * 64 + lane];
+    al[w] = mw[w] == kNegInf ? (lw == 0.f ? 0.f : 1.f) : fast_exp2(mw[w] - mall);
+    L = __builtin_fmaf(al[w], lw, L);
+  }
+  const bool empty = L == 0.f;  // no key; NaN (a NaN query row or key) is not
+  const float inv = empty ? 0.f : 1.0f / L;
+  if (32 * rt0 + l32 < R) {
+    const int64_t row = ((int64_t)b * p.Hq + hq) * p.Sq + qi;
+    float* po = a.part_o + (row * a.nsplit + s) * D + 4 * h;
+    T* out = (T*)a.o.data + b * a.o.sb + hq * a.o.sh + (int64_t)qi * a.o.ss + 4 * h;
 #pragma unroll 2
-      for (int y = wave; y < 4 * C::DB; y += NW) {
-        f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int y = wave; y < 4 * C::DB; y += NW) {
+      f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          const f32x4 v = xa[(w * 4 * C::DB + y) * 64 + lane];
+      for (int w = 0; w < NW; ++w) {
+        const f32x4 v = xa[(w * 4 * C::DB + y) * 64 + lane];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(al[w], v[e], o[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] *= inv;
-        if (ns > 1) *(f32x4*)(po + 8 * y) = o;
-        else st_global8(out + 8 * y, pack4<T>(o[0], o[1], o[2], o[3]));
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(al[w], v[e], o[e]);
       }
-      if (wave == 0 && h == 0) {
-        const float lse = empty ? kNegInf : mall + log2f(L);
-        if (ns > 1) a.part_lse[row * a.nsplit + s] = lse;
-        else a.lse[row] = lse * kLn2;
-      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= inv;
+      if (ns > 1) *(f32x4*)(po + 8 * y) = o;
+      else st_global8(out + 8 * y, pack4<T>(o[0], o[1], o[2], o[3]));
+    }
+    if (wave == 0 && h == 0) {
+      const float lse = empty ? kNegInf : mall + log2f(L);
+      if (ns > 1) a.part_lse[row * a.nsplit + s] = lse;
+      else a.lse[row] = lse * kLn2;
     }
   }
 }
 
-template <class T, int CODE, int D, int NW, int WPT, int MT, int ST>
+template <class T, int CODE, int D, int NW, int WPT, int ST>
 void launch_rows(QuantTreeArgs a, hipStream_t st) {
-  a.t.nrt = (int)((((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32 + WPT * MT - 1) / (WPT * MT));
+  a.t.nrt = (int)((((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32 + WPT - 1) / WPT);
   const dim3 grid((unsigned)((a.t.nchunk + 7) / 8 * 8 * a.t.nrt)), block(NW * WPT * 64);
-  if (a.t.p.cap > 0.f) hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, NW, WPT, MT, ST, true>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, NW, WPT, MT, ST, false>), grid, block, 0, st, a);
+  if (a.t.p.cap > 0.f) hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, NW, WPT, ST, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, NW, WPT, ST, false>), grid, block, 0, st, a);
 }
 
 template <class T, int CODE, int D>
 void launch_code(const QuantTreeArgs& a, hipStream_t st) {
   const int share = quant_row_tiles(D, ((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32);
-  if constexpr (D == 128) {
-    if (share == 2) launch_rows<T, CODE, D, 4, 2, 1, 4>(a, st);
-    else launch_rows<T, CODE, D, 8, 1, 1, 2>(a, st);
-  } else if constexpr (D == 64) {
-    if (share == 2) launch_rows<T, CODE, D, 4, 2, 1, 4>(a, st);
-    else launch_rows<T, CODE, D, 4, 1, 1, 4>(a, st);
-  } else if constexpr (D == 32) {
-    if (share == 2) launch_rows<T, CODE, D, 4, 1, 2, 4>(a, st);
-    else launch_rows<T, CODE, D, 4, 1, 1, 4>(a, st);
+  if constexpr (D == 64 || D == 128) {
+    if (share == 2) launch_rows<T, CODE, D, 4, 2, 4>(a, st);
+    else launch_rows<T, CODE, D, D == 128 ? 8 : 4, 1, D == 128 ? 2 : 4>(a, st);
   } else {
-    launch_rows<T, CODE, D, 4, 1, 1, 2>(a, st);
+    launch_rows<T, CODE, D, 4, 1, D == 32 ? 4 : 2>(a, st);
   }
 }
 
