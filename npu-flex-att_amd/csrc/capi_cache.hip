@@ -206,6 +206,7 @@ int check_tree(const flexatt_tree* p) {
 
 int check_quant_tree(const flexatt_tree* p) {
   FLEXATT_TRY(check_tree(p));
+  if (p->tree_mask && p->tokens > 1 << 15) return FLEXATT_ERANGE;  // (offsets in a mask are 32 bits)
   return p->dtype == FLEXATT_F32 ? FLEXATT_EDTYPE : FLEXATT_OK;
 }
 

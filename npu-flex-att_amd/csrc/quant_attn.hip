@@ -102,6 +102,32 @@ __device__ __forceinline__ typename Mfma<T>::v8 operand8(int lo, int hi) {
   return as_v8<typename Mfma<T>::v8>(v);
 }
 
+// acc *= s.  Accumulators of head dim 256 are kept in the other half of the register file:
+// a multiply of its own would have all of them moved there and back around the branch it
+// is in, in every iteration.  The caller has waited for the last MFMA's result; the wait at
+// the end is that between a write and an MFMA.
+template <int D>
+__device__ __forceinline__ void rescale(f32x16& a, float s) {
+  if constexpr (D < 256) {
+    scale_inplace(a, s);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      float x0, x1, x2, x3, y0 = a[r], y1 = a[r + 1], y2 = a[r + 2], y3 = a[r + 3];
+      asm volatile(
+          "v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\t"
+          "v_accvgpr_read_b32 %6, %2\n\tv_accvgpr_read_b32 %7, %3\n\ts_nop 1\n\t"
+          "v_mul_f32_e32 %4, %8, %4\n\tv_mul_f32_e32 %5, %8, %5\n\t"
+          "v_mul_f32_e32 %6, %8, %6\n\tv_mul_f32_e32 %7, %8, %7\n\ts_nop 1\n\t"
+          "v_accvgpr_write_b32 %0, %4\n\tv_accvgpr_write_b32 %1, %5\n\t"
+          "v_accvgpr_write_b32 %2, %6\n\tv_accvgpr_write_b32 %3, %7\n\ts_nop 3"
+          : "+a"(y0), "+a"(y1), "+a"(y2), "+a"(y3), "=&v"(x0), "=&v"(x1), "=&v"(x2), "=&v"(x3)
+          : "v"(s));
+      a[r] = y0, a[r + 1] = y1, a[r + 2] = y2, a[r + 3] = y3;
+    }
+  }
+}
+
 // Transposed 8 x 8-bit read: lane i of 16 gets byte i % 8 at the addresses of lanes
 // 2 t + i / 8, t = 0 .. 7.
 __device__ __forceinline__ i32x2 lds_read_tr8(const void* p) {
@@ -225,16 +251,15 @@ void quant_attn_kernel(QuantTreeArgs qa) {
     }
     load_lds4(scales + min(t * C::BN + l32, last), wbase + j % ST * STB + 2 * C::TB + sub * SCB);
   };
-  if (nt > 0) {
-    issue_k(0);
-    issue_v(0);
-  }
-
   // Q: lane half h has elements 32 kc + 16 h .. + 15 of its row, the codes' order
   i32x4 qf[2 * C::KC];
   const char* src = (const char*)((const T*)a.q.data + b * a.q.sb + hq * a.q.sh + (int64_t)qi * a.q.ss) + 32 * h;
 #pragma unroll
   for (int kc = 0; kc < 2 * C::KC; ++kc) qf[kc] = ld_global16(src + 64 * (kc >> 1) + 16 * (kc & 1));
+  if (nt > 0) {
+    issue_k(0);
+    issue_v(0);
+  }
   // Row qi sees the cached keys [row_lo, n); the tiles that hold only keys every row
   // sees need no mask.
   int row_lo = 0, full_lo = 0;
@@ -259,12 +284,11 @@ void quant_attn_kernel(QuantTreeArgs qa) {
     pin(qf[kc]);
   }
   wait_vmcnt<0>();  // (and the first tile)
-#pragma unroll
-  for (int j = 1; j < ST; ++j)
-    if (j < nt) {
-      issue_k(j);
-      if (WPT == 1 || j < ST - 1) issue_v(j);
-    }
+#pragma unroll 1  // (a short call's time is its code's)
+  for (int j = 1; j < min(nt, ST); ++j) {
+    issue_k(j);
+    if (WPT == 1 || j < ST - 1) issue_v(j);
+  }
 
   f32x16 acc[C::DB];
   float m_run = kNegInf, l_run = 0.f;
@@ -339,26 +363,17 @@ void quant_attn_kernel(QuantTreeArgs qa) {
       for (int e = 0; e < 4; ++e) ks[4 * i + e] = __int_as_float(k4[e]), vs[4 * i + e] = __int_as_float(v4[e]);
     }
     // ... and all else that the tile reads, which is there when it is used
-    read_k(j + 1, kf);
     i32x2 vf[2][C::DB];
+    auto read_v = [&] {
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int db = 0; db < C::DB; ++db) vf[c][db] = lds_read_tr8(sV + 16 * c * D + voff[db]);
-    asm volatile("" ::: "memory");
-    float top, top2;
-    max16_partial(vs, top, top2);
-    top = max2(top, top2);
-    top = fmaxf(top, swap_halves(top));
-    if (__builtin_amdgcn_readfirstlane(top * rel > 1.f)) {
-      // the power of two above the largest scale, as far as there is one
-      const int expo = (int)(__float_as_uint(top) >> 23) & 255, field = min(max(253 - expo, 1), 217);
-      const float now = __int_as_float(field << 23), turn = now / rel;
-      l_run *= turn;
-#pragma unroll
-      for (int db = 0; db < C::DB; ++db) scale_inplace(acc[db], turn);
-      rel = now;
-      lift = (float)(field - 127);
+        for (int db = 0; db < C::DB; ++db) vf[c][db] = lds_read_tr8(sV + 16 * c * D + voff[db]);
+    };
+    if constexpr (D < 256) {  // (registers)
+      read_k(j + 1, kf);
+      read_v();
+      asm volatile("" ::: "memory");
     }
 #pragma unroll
     for (int e = 0; e < 16; ++e) sc[e] *= ks[e];
@@ -374,11 +389,11 @@ void quant_attn_kernel(QuantTreeArgs qa) {
       for (int e = 0; e < 16; ++e)
         if ((unsigned)(8 * (e >> 2) + (e & 3) - lo) >= (unsigned)max(hi - lo, 0)) sc[e] = kNegInf;
       if (mask && n0 + C::BN > n) {  // all of the tile's mask bytes at once
-        const unsigned char* mrow = mask + (int64_t)qi * p.Sq;
+        const unsigned mrow = (unsigned)qi * (unsigned)p.Sq;
         const int u0 = n0 + 4 * h - n;
         unsigned char mb[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mb[e] = mrow[min(max(u0 + 8 * (e >> 2) + (e & 3), 0), p.Sq - 1)];
+        for (int e = 0; e < 16; ++e) mb[e] = mask[mrow + (unsigned)min(max(u0 + 8 * (e >> 2) + (e & 3), 0), p.Sq - 1)];
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (u0 + 8 * (e >> 2) + (e & 3) >= 0 && mb[e] == 0) sc[e] = kNegInf;
@@ -390,19 +405,36 @@ void quant_attn_kernel(QuantTreeArgs qa) {
     if constexpr (!CAP) mx *= c2;
     mx = fmaxf(mx, swap_halves(mx));
     if (mx != mx) mx = kNegInf;
-    const bool grow = mx > m_run + kTreeRescale;
-    if (__builtin_amdgcn_ballot_w64(grow)) {
+    float top, top2;
+    max16_partial(vs, top, top2);
+    top = max2(top, top2);
+    top = fmaxf(top, swap_halves(top));
+    const bool grow = mx > m_run + kTreeRescale, over = __builtin_amdgcn_readfirstlane(top * rel > 1.f);
+    if (over || __builtin_amdgcn_ballot_w64(grow)) {
+      // (over: 2^lift becomes the power of two above the largest scale, as far as there is one)
+      const int expo = (int)(__float_as_uint(top) >> 23) & 255;
+      const int field = over ? min(max(253 - expo, 1), 217) : (int)lift + 127;
+      const float now = __int_as_float(field << 23);
       const float m_new = grow ? mx : m_run;
-      const float alpha = grow ? fast_exp2(m_run - m_new) : 1.f;
-      l_run *= alpha;
+      const float alpha = (grow ? fast_exp2(m_run - m_new) : 1.f) * (now / rel);
+      if (j > 0) {  // (the first tile finds zeros)
+        l_run *= alpha;
+        settle(acc[0]);
 #pragma unroll
-      for (int db = 0; db < C::DB; ++db) scale_inplace(acc[db], alpha);
+        for (int db = 0; db < C::DB; ++db) rescale<D>(acc[db], alpha);
+      }
       m_run = m_new;
+      rel = now;
+      lift = (float)(field - 127);
     }
     const float m_use = (m_run == kNegInf ? 0.f : m_run) - lift;
 
     // From here on one block: the next tile's scores (behind the last one of what is
     // there, and not used) between this one's weights, whose product follows.
+    if constexpr (D == 256) {
+      read_k(j + 1, kf);
+      read_v();
+    }
     const f32x16 next = scores(kf);
     float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
