@@ -105,26 +105,25 @@ struct NormRotaryArgs {
   float eps;
   int norm, w_wide;
   int kind;      // 0, or enum flexatt_code: the cache's rows are bytes
-  int q_groups;  // groups of q heads (set by the launcher)
+  int q_groups, k_groups;  // groups of q heads and of k heads (set by the launcher)
 };
 
 // The gradient's workgroups: `columns` of tokens times the groups of hpt heads, q's and
-// k's apart, about 1024 workgroups (four a CU) where there are tokens for them.
+// k's apart, as many as three a CU, which run at once (registers; bf16 B=2 S=4096 Hq=32
+// Hkv=8 D=128: 768 of them, 16 heads each, 50 us, 1280 56).
 struct NormGradPlan {
   int columns, hpt, q_groups, k_groups;
 };
 inline NormGradPlan norm_grad_plan(int B, int S, int Hq, int Hkv, int D, int es) {
+  constexpr int64_t kMost = 768;
   NormGradPlan p;
   const int64_t per = 256 / (D * es / 32), nb = ((int64_t)B * S + per - 1) / per;
-  const int heads = Hq + Hkv;
-  int64_t groups = (1024 + nb - 1) / nb;
-  if (groups > heads) groups = heads;
-  p.hpt = 1;
-  while (2 * p.hpt * groups <= heads) p.hpt *= 2;
-  p.q_groups = (Hq + p.hpt - 1) / p.hpt;
-  p.k_groups = (Hkv + p.hpt - 1) / p.hpt;
-  int64_t most = 2048 / (p.q_groups + p.k_groups);
-  if (most < 1) most = 1;
+  for (p.hpt = 1;; p.hpt *= 2) {
+    p.q_groups = (Hq + p.hpt - 1) / p.hpt;
+    p.k_groups = (Hkv + p.hpt - 1) / p.hpt;
+    if (nb * (p.q_groups + p.k_groups) <= kMost || (p.q_groups <= 1 && p.k_groups <= 1) || p.hpt >= 1 << 20) break;
+  }
+  const int64_t groups = p.q_groups + p.k_groups, most = kMost > groups ? kMost / groups : 1;
   p.columns = (int)(nb < most ? nb : most);
   return p;
 }

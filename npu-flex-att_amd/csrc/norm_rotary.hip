@@ -158,54 +158,52 @@ __device__ __forceinline__ unsigned code4(int kind, float a, float b, float c, f
   return (p & 255) | (q & 255) << 8 | (r & 255) << 16 | s << 24;
 }
 
-// Head hh of token (b, s): q (which 0), k (1) or v (2), and where it goes.
-struct RowOf {
-  const char* src;
-  char* dst;         // nullptr: outside the cache, nothing written
-  float* scale;      // of a row of 8 bits
-};
-__device__ __forceinline__ RowOf row_of(const NormRotaryArgs& n, int which, int hh, int b, int s, int64_t slot, int es,
-                                        bool coded) {
-  const RotaryArgs& a = n.r;
-  const View& x = which == 0 ? a.q : which == 1 ? a.k : a.v;
-  const MutView& y = which == 0 ? a.qo : which == 1 ? a.ko : a.vo;
-  const bool cached = which != 0 && a.cache_rows > 0;
-  RowOf r;
-  r.src = (const char*)x.data + (b * x.sb + hh * x.sh + s * x.ss) * es;
-  r.dst = nullptr;
-  r.scale = nullptr;
-  if (cached && (slot < 0 || slot >= a.cache_rows)) return r;
-  r.dst = (char*)y.data + (b * y.sb + hh * y.sh + (cached ? slot : (int64_t)s) * y.ss) * (coded && cached ? 1 : es);
-  if (coded && cached) r.scale = (which == 1 ? n.k_scales : n.v_scales) + ((int64_t)b * a.Hkv + hh) * a.cache_rows + slot;
-  return r;
-}
-
+// A workgroup has some heads of q, of k or of v (grid.y: the groups of a.hpt of each) for
+// its tokens.  A thread's first rows are on their way before it forms its sines, and the
+// next ones while it works on a pair.
 template <class T, int D, int MODE, bool CODED>
 __global__ __launch_bounds__(kThreads) void norm_rotary_kernel(NormRotaryArgs n) {
   using C = NormCfg<T, D>;
   using P = Place<T, D, MODE>;
   typedef typename P::vec vec;
-  constexpr int E = C::E, UPR = C::UPR;
+  constexpr int E = C::E, UPR = C::UPR, U = 2, ES = (int)sizeof(T);
   const RotaryArgs& a = n.r;
   const int64_t tok = (int64_t)blockIdx.x * C::TPB + threadIdx.x / UPR;
   if (tok >= (int64_t)a.B * a.S) return;  // (whole rows of threads)
+  const int which = (int)blockIdx.y < n.q_groups ? 0 : (int)blockIdx.y < n.q_groups + n.k_groups ? 1 : 2;
+  const int lo = ((int)blockIdx.y - (which == 0 ? 0 : n.q_groups + (which == 2 ? n.k_groups : 0))) * a.hpt;
+  const int rows = min(a.hpt, (which ? a.Hkv : a.Hq) - lo);
   int b, s;
   int64_t slot;
   double pos;
   token_of(a, tok, b, s, slot, pos);
   const P at(a, threadIdx.x % UPR);
-  float cs[E], sn[E];
-  at.turns(a, pos, cs, sn);
 
-  const int h0 = blockIdx.y * a.hpt, h1 = min(h0 + a.hpt, a.heads);
-#pragma unroll 1
-  for (int which = 0; which < 3; ++which) {
-    const int from = which == 0 ? 0 : which == 1 ? a.Hq : a.Hq + a.Hkv;
-    const int lo = max(h0, from), hi = min(h1, which == 0 ? a.Hq : from + a.Hkv);
-    if (lo >= hi) continue;
-    const bool norm = n.norm && which != 2;
-    // y = (a ac - b bs, b bc + a as), times r
-    float ac[E], as[E], bc[E], bs[E];
+  const auto of = [&](auto q, auto k, auto v) { return which == 0 ? q : which == 1 ? k : v; };
+  const View vx = {of(a.q.data, a.k.data, a.v.data), of(a.q.sb, a.k.sb, a.v.sb), of(a.q.sh, a.k.sh, a.v.sh),
+                   of(a.q.ss, a.k.ss, a.v.ss)};
+  const MutView vy = {of(a.qo.data, a.ko.data, a.vo.data), of(a.qo.sb, a.ko.sb, a.vo.sb), of(a.qo.sh, a.ko.sh, a.vo.sh),
+                      of(a.qo.ss, a.ko.ss, a.vo.ss)};
+  const bool cached = which != 0 && a.cache_rows > 0, coded = CODED && cached;
+  const char* src = (const char*)vx.data + (b * vx.sb + lo * vx.sh + s * vx.ss) * ES;
+  const bool kept = !cached || (slot >= 0 && slot < a.cache_rows);  // (a row outside the cache is not written)
+  char* dst = (char*)vy.data + (b * vy.sb + lo * vy.sh + (cached ? slot : (int64_t)s) * vy.ss) * (coded ? 1 : ES);
+  float* scales = nullptr;
+  if (coded) scales = (which == 1 ? n.k_scales : n.v_scales) + ((int64_t)b * a.Hkv + lo) * a.cache_rows + slot;
+  vec x[U], y[U], nx[U], ny[U];
+  auto fetch = [&](int r0, vec (&p)[U], vec (&q)[U]) {
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (r0 + i < rows) at.load(src + (r0 + i) * vx.sh * ES, p[i], q[i]);
+  };
+  fetch(0, x, y);
+
+  const bool norm = n.norm && which != 2;
+  // y = (a ac - b bs, b bc + a as), times r
+  float ac[E], as[E], bc[E], bs[E];
+  if (which != 2) {
+    float cs[E], sn[E];
+    at.turns(a, pos, cs, sn);
     const void* w = which == 0 ? n.wq : n.wk;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -213,85 +211,82 @@ __global__ __launch_bounds__(kThreads) void norm_rotary_kernel(NormRotaryArgs n)
       const float wb = norm ? weight_at<T>(w, n.w_wide, at.second(e)) : 1.f;
       ac[e] = wa * cs[e], as[e] = wa * sn[e], bc[e] = wb * cs[e], bs[e] = wb * sn[e];
     }
-    constexpr int U = 4;  // heads loaded before the first is stored
-    for (int hh = lo; hh < hi; hh += U) {
-      vec x[U], y[U];
-      RowOf row[U];
+  }
+  for (int r0 = 0; r0 < rows; r0 += U) {
+    fetch(r0 + U, nx, ny);
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        if (hh + i >= hi) break;
-        row[i] = row_of(n, which, hh + i - from, b, s, slot, sizeof(T), CODED);
-        at.load(row[i].src, x[i], y[i]);
+    for (int i = 0; i < U; ++i) {
+      if (r0 + i >= rows) break;
+      char* to = dst + (r0 + i) * vy.sh * (coded ? 1 : ES);
+      if (!CODED && which == 2) {
+        if (kept) at.store(to, x[i], y[i]);
+        continue;
       }
+      float ya[E], yb[E], sq = 0.f;
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        if (hh + i >= hi) break;
-        if (!CODED && which == 2) {
-          if (row[i].dst) at.store(row[i].dst, x[i], y[i]);
+      for (int e = 0; e < E; ++e) {
+        const float p = P::a_of(x[i], y[i], e), q = P::b_of(x[i], y[i], e);
+        if (which == 2) {
+          ya[e] = p, yb[e] = q;
           continue;
         }
-        float ya[E], yb[E], sq = 0.f;
+        sq = __builtin_fmaf(p, p, sq);
+        sq = __builtin_fmaf(q, q, sq);
+        const bool t = at.turned(e);
+        ya[e] = t ? __builtin_fmaf(p, ac[e], -(q * bs[e])) : p * ac[e];
+        yb[e] = t ? __builtin_fmaf(q, bc[e], p * as[e]) : q * bc[e];
+      }
+      if (norm) {
+        const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(row_sum<UPR>(sq), 1.0f / D, n.eps));
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float p = P::a_of(x[i], y[i], e), q = P::b_of(x[i], y[i], e);
-          sq = __builtin_fmaf(p, p, sq);
-          sq = __builtin_fmaf(q, q, sq);
-          const bool t = which != 2 && at.turned(e);
-          ya[e] = t ? __builtin_fmaf(p, ac[e], -(q * bs[e])) : which == 2 ? p : p * ac[e];
-          yb[e] = t ? __builtin_fmaf(q, bc[e], p * as[e]) : which == 2 ? q : q * bc[e];
+        for (int e = 0; e < E; ++e) ya[e] *= r, yb[e] *= r;
+      }
+      if (!coded) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) P::put(x[i], y[i], e, ya[e], yb[e]);
+        if (kept) at.store(to, x[i], y[i]);
+        continue;
+      }
+      unsigned top = 0;  // largest size; infinities and NaN are larger than numbers
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        top = max(top, max(__float_as_uint(ya[e]) & 0x7fffffffu, __float_as_uint(yb[e]) & 0x7fffffffu));
+      top = row_max<UPR>(top);
+      const bool fine = top < 0x7f800000u;
+      // (the largest numbers a little less, so that code * scale is one)
+      const float size = fminf(fmaxf(__uint_as_float(top), 0x1p-100f), 0x1.fffffp127f);
+      const float scale = size / (n.kind == FLEXATT_E4M3 ? 448.f : 127.f);
+      const float inv = 1.0f / scale;
+#pragma unroll
+      for (int e = 0; e < E; ++e) ya[e] = fine ? ya[e] * inv : 0.f, yb[e] = fine ? yb[e] * inv : 0.f;
+      if (!kept) continue;
+      if (at.u == 0) scales[(int64_t)(r0 + i) * a.cache_rows] = fine ? scale : __builtin_nanf("");
+      if constexpr (MODE == kAny) {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const unsigned c = code4(n.kind, ya[e], yb[e], ya[e + 1], yb[e + 1]);
+          to[at.first(e)] = (char)c, to[at.second(e)] = (char)(c >> 8);
+          to[at.first(e + 1)] = (char)(c >> 16), to[at.second(e + 1)] = (char)(c >> 24);
         }
-        if (norm) {
-          const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(row_sum<UPR>(sq), 1.0f / D, n.eps));
+      } else if constexpr (MODE == kInter) {  // 2 E neighbours
+        unsigned c[E / 2];
 #pragma unroll
-          for (int e = 0; e < E; ++e) ya[e] *= r, yb[e] *= r;
-        }
-        if (CODED && which != 0) {
-          unsigned top = 0;  // largest size; infinities and NaN are larger than numbers
+        for (int e = 0; e < E / 2; ++e) c[e] = code4(n.kind, ya[2 * e], yb[2 * e], ya[2 * e + 1], yb[2 * e + 1]);
+        if constexpr (E == 8) *(i32x4*)(to + at.c0) = i32x4{(int)c[0], (int)c[1], (int)c[2], (int)c[3]};
+        else *(i32x2*)(to + at.c0) = i32x2{(int)c[0], (int)c[1]};
+      } else {
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            top = max(top, max(__float_as_uint(ya[e]) & 0x7fffffffu, __float_as_uint(yb[e]) & 0x7fffffffu));
-          top = row_max<UPR>(top);
-          const bool fine = top < 0x7f800000u;
-          // (the largest numbers a little less, so that code * scale is one)
-          const float size = fminf(fmaxf(__uint_as_float(top), 0x1p-100f), 0x1.fffffp127f);
-          const float scale = size / (n.kind == FLEXATT_E4M3 ? 448.f : 127.f);
-          const float inv = 1.0f / scale;
-#pragma unroll
-          for (int e = 0; e < E; ++e) ya[e] = fine ? ya[e] * inv : 0.f, yb[e] = fine ? yb[e] * inv : 0.f;
-          if (row[i].dst) {
-            char* to = row[i].dst;
-            if (at.u == 0) *row[i].scale = fine ? scale : __builtin_nanf("");
-            if constexpr (MODE == kAny) {
-#pragma unroll
-              for (int e = 0; e < E; e += 2) {
-                const unsigned c = code4(n.kind, ya[e], yb[e], ya[e + 1], yb[e + 1]);
-                to[at.first(e)] = (char)c, to[at.second(e)] = (char)(c >> 8);
-                to[at.first(e + 1)] = (char)(c >> 16), to[at.second(e + 1)] = (char)(c >> 24);
-              }
-            } else if constexpr (MODE == kInter) {  // 2 E neighbours
-              unsigned c[E / 2];
-#pragma unroll
-              for (int e = 0; e < E / 2; ++e) c[e] = code4(n.kind, ya[2 * e], yb[2 * e], ya[2 * e + 1], yb[2 * e + 1]);
-              if constexpr (E == 8) *(i32x4*)(to + at.c0) = i32x4{(int)c[0], (int)c[1], (int)c[2], (int)c[3]};
-              else *(i32x2*)(to + at.c0) = i32x2{(int)c[0], (int)c[1]};
-            } else {
-#pragma unroll
-              for (int g = 0; g < 2; ++g) {
-                const float* v = g ? yb : ya;
-                char* d = to + (g ? at.c1 : at.c0);
-                const unsigned c = code4(n.kind, v[0], v[1], v[2], v[3]);
-                if constexpr (E == 8) *(i32x2*)d = i32x2{(int)c, (int)code4(n.kind, v[4], v[5], v[6], v[7])};
-                else *(int*)d = (int)c;
-              }
-            }
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e) P::put(x[i], y[i], e, ya[e], yb[e]);
-          if (row[i].dst) at.store(row[i].dst, x[i], y[i]);
+        for (int g = 0; g < 2; ++g) {
+          const float* v = g ? yb : ya;
+          char* d = to + (g ? at.c1 : at.c0);
+          const unsigned c = code4(n.kind, v[0], v[1], v[2], v[3]);
+          if constexpr (E == 8) *(i32x2*)d = i32x2{(int)c, (int)code4(n.kind, v[4], v[5], v[6], v[7])};
+          else *(int*)d = (int)c;
         }
       }
     }
+#pragma unroll
+    for (int i = 0; i < U; ++i) x[i] = nx[i], y[i] = ny[i];
   }
 }
 
@@ -439,7 +434,10 @@ hipError_t launch(NormRotaryArgs n, hipStream_t st) {
   if (groups > a.heads) groups = a.heads;
   a.hpt = (int)((a.heads + groups - 1) / groups);
   if (a.hpt > 2) a.hpt = (a.hpt + 3) / 4 * 4;
-  const dim3 grid((unsigned)nb, (unsigned)((a.heads + a.hpt - 1) / a.hpt)), block(kThreads);
+  n.q_groups = (a.Hq + a.hpt - 1) / a.hpt;
+  n.k_groups = (a.Hkv + a.hpt - 1) / a.hpt;
+  const int v_groups = a.cache_rows > 0 ? n.k_groups : 0;
+  const dim3 grid((unsigned)nb, (unsigned)(n.q_groups + n.k_groups + v_groups)), block(kThreads);
   switch (mode_of<T, D>(a)) {
     case kPlain: hipLaunchKernelGGL((norm_rotary_kernel<T, D, kPlain, CODED>), grid, block, 0, st, n); break;
     case kInter: hipLaunchKernelGGL((norm_rotary_kernel<T, D, kInter, CODED>), grid, block, 0, st, n); break;
