@@ -228,14 +228,14 @@ struct TreePlan {
   int slots, nchunk, min_tiles, nsplit;
 };
 int64_t row_tiles(const flexatt_tree* p) { return ((int64_t)(p->heads_q / p->heads_kv) * p->tokens + 31) / 32; }
-// `share`: row tiles of a workgroup; `per_cu`: workgroups that fit a CU.
-TreePlan plan_of(const flexatt_tree* p, int share, int per_cu) {
+// `share`: row tiles of a workgroup; `fit`: workgroups that run at once.
+TreePlan plan_of(const flexatt_tree* p, int share, int64_t fit) {
   TreePlan t;
   const int64_t groups = (row_tiles(p) + share - 1) / share;
   // a chunk's row tiles are on one of the 8 XCDs (tree_attn_kernel): whole chunks of each
   // (fp32 B=2 Hq=8 Hkv=2 T=53 caches of 22374 D=128, 7 row tiles: 36 chunks, five on some
   // XCDs for 32 CUs, 192 us, 32 chunks 117)
-  const int64_t fit = per_cu * cus(), slots = groups <= fit / 8 ? fit / 8 / groups * 8 : fit / groups;
+  const int64_t slots = groups <= fit / 8 ? fit / 8 / groups * 8 : fit / groups;
   const int64_t bh = (int64_t)p->batch * p->heads_kv, tiles = (p->cache_rows + 31) / 32;
   // a cache of up to 512 rows whole: what the chunks save the merge costs (bf16 B=1 Hq=32
   // Hkv=8 T=8 D=128, 500 rows 13.4 -> 11.3 us, 1000 rows 14.0 -> 14.9; fp32 D=64, 500 rows
@@ -259,14 +259,19 @@ TreePlan plan_of(const flexatt_tree* p, int share, int per_cu) {
 }
 TreePlan tree_plan(const flexatt_tree* p) {
   const int rowb = p->head_dim * (int)elt_size(p->dtype);
-  return plan_of(p, tree_share(rowb, (int)elt_size(p->dtype), row_tiles(p)), rowb >= 256 ? 1 : 2);
+  return plan_of(p, tree_share(rowb, (int)elt_size(p->dtype), row_tiles(p)), (rowb >= 256 ? 1 : 2) * (int64_t)cus());
 }
 TreePlan quant_plan(const flexatt_tree* p) {
   const int share = quant_row_tiles(p->head_dim, row_tiles(p));
-  return plan_of(p, share, p->head_dim >= 128 || share > 1 ? 1 : 2);
+  return plan_of(p, share, (p->head_dim >= 128 || share > 1 ? 1 : 2) * (int64_t)cus());
 }
-// The launch behind a shared prefix: its rows are those of all sequences, and its chunks
-// get their share of the workgroups that run at once, by key tiles times row tiles.
+// The launch behind a shared prefix, whose rows are those of all sequences: `np` chunks of
+// the prefix, and of each sequence's own cache as TreePlan has them.  Where one round of
+// workgroups can have it all, the two that make the longest chunk shortest (in steps of
+// the waves; bf16 B=4 Hq=32 Hkv=8 T=1 D=128, a prefix of 16000 rows, caches of 1000: 27 us
+// with eight workgroups in a second round, 21 without); else the prefix gets its share of a
+// round, by key tiles times row tiles (more of it, or less: 72 -> 76 and 81 us for 32
+// sequences of 4 tokens behind 16383 rows).
 struct PrefixPlan {
   TreePlan own;
   int np;
@@ -274,17 +279,32 @@ struct PrefixPlan {
 PrefixPlan prefix_plan(const flexatt_tree* p, int prefix_rows) {
   const int rowb = p->head_dim * (int)elt_size(p->dtype);
   const int64_t rows = (int64_t)(p->heads_q / p->heads_kv) * p->tokens, all = (rows * p->batch + 31) / 32;
-  const int share = tree_share(rowb, (int)elt_size(p->dtype), all), per_cu = rowb >= 256 ? 1 : 2;
+  const int share = tree_share(rowb, (int)elt_size(p->dtype), all);
+  const int64_t groups = (all + share - 1) / share, own_groups = ((rows + 31) / 32 + share - 1) / share;
+  const int64_t tiles = (prefix_rows + 31) / 32, own_tiles = (p->cache_rows + 31) / 32;
+  const int64_t slots = (rowb >= 256 ? 1 : 2) * (int64_t)cus(), waves = rowb > 512 ? 2 : share == 4 ? 2 : 4;
+  const int64_t least = 8, most = (tiles + least - 1) / least < 64 ? (tiles + least - 1) / least : 64;
+  const int64_t per = groups * p->heads_kv, own_per = own_groups * p->heads_kv * p->batch;
   PrefixPlan t;
-  t.own = plan_of(p, share, per_cu);
-  const int64_t groups = (all + share - 1) / share, tiles = (prefix_rows + 31) / 32;
-  const int64_t mine = groups * tiles, others = ((rows + 31) / 32 + share - 1) / share * p->batch * ((p->cache_rows + 31) / 32);
-  const int64_t slots = per_cu * cus();
-  int64_t np = (slots * mine / (mine + others) + groups * p->heads_kv / 2) / (groups * p->heads_kv);
-  const int64_t most = (tiles + 7) / 8;
-  if (np > most) np = most;
-  if (np > 64) np = 64;
-  t.np = np < 1 ? 1 : (int)np;
+  t.own = plan_of(p, share, slots);
+  int64_t np = 0, best = INT64_MAX;
+  for (int64_t ns = 1; ns <= (own_tiles + least - 1) / least && ns * own_per + per <= slots; ++ns) {
+    int64_t n = (slots - ns * own_per) / per;
+    if (n > most) n = most;
+    const int64_t x = (tiles + n * waves - 1) / (n * waves), y = (own_tiles + ns * waves - 1) / (ns * waves);
+    const int64_t cost = x > y ? x : y;
+    if (cost >= best) continue;
+    best = cost;
+    np = n;
+    t.own.nsplit = (int)ns;
+    t.own.slots = t.own.nchunk = (int)(ns * p->heads_kv * p->batch);
+  }
+  if (np == 0) {
+    const int64_t mine = groups * tiles, others = own_groups * p->batch * own_tiles;
+    np = (slots * mine / (mine + others) + per / 2) / per;
+    np = np < 1 ? 1 : np > most ? most : np;
+  }
+  t.np = (int)np;
   return t;
 }
 size_t tree_rows(const flexatt_tree* p) { return (size_t)p->batch * p->heads_q * p->tokens; }
