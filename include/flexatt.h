@@ -451,21 +451,24 @@ typedef struct flexatt_norm {
   const void* k_weight; /* device [D]; NULL when heads_kv is 0 */
 } flexatt_norm;
 
-/* As flexatt_rotary_apply.  An output may be its own input. */
+/* As flexatt_rotary_apply (FLEXATT_ERANGE: also more than 2^30 heads).  An output may be its
+ * own input. */
 int flexatt_norm_rotary_apply(const flexatt_rotary* r, const flexatt_norm* n, const flexatt_tensor* q,
                               const flexatt_tensor* k, const flexatt_tensor* q_out, const flexatt_tensor* k_out,
                               void* stream);
 
 /* Its gradients: dq, dk and the weights' (device [D] of weight_dtype, sums over all rows
  * in 32 bits) from q, k and the gradients of q_out and k_out.  k, k_grad, dk and dk_weight
- * are NULL when heads_kv is 0.  `workspace` as in flexatt_tree_fwd. */
+ * are NULL when heads_kv is 0.  `workspace` as in flexatt_tree_fwd.  No output, nor the
+ * workspace, may lie within an input or another of them. */
 size_t flexatt_norm_rotary_grad_workspace(const flexatt_rotary* r);
 int flexatt_norm_rotary_grad(const flexatt_rotary* r, const flexatt_norm* n, const flexatt_tensor* q,
                              const flexatt_tensor* k, const flexatt_tensor* q_grad, const flexatt_tensor* k_grad,
                              const flexatt_tensor* dq, const flexatt_tensor* dk, void* dq_weight, void* dk_weight,
                              void* workspace, size_t workspace_bytes, void* stream);
 
-/* As flexatt_rotary_append. */
+/* As flexatt_rotary_append; weights, inv_freq and positions may not lie within the span of
+ * the cache either. */
 int flexatt_norm_rotary_append(const flexatt_rotary* r, const flexatt_norm* n, const flexatt_tensor* q,
                                const flexatt_tensor* k, const flexatt_tensor* v, const flexatt_tensor* q_out,
                                const flexatt_tensor* k_cache, const flexatt_tensor* v_cache, int32_t cache_rows,
@@ -509,9 +512,10 @@ int flexatt_dequant_rows(const flexatt_dequant* p, const flexatt_tensor* k_cache
                          const float* k_scales, const float* v_scales, const flexatt_tensor* k_out,
                          const flexatt_tensor* v_out, void* stream);
 
-/* flexatt_tree_fwd over such a cache, for dtype fp16 and bf16 (else FLEXATT_EDTYPE).  The
- * scores are q . code times the key's scale; weights times the values' scales, relative to
- * the largest of these, are rounded to fp16 for the second product. */
+/* flexatt_tree_fwd over such a cache, for dtype fp16 and bf16 (else FLEXATT_EDTYPE), a
+ * tree_mask for up to 2^15 tokens (else FLEXATT_ERANGE).  The scores are q . code times the
+ * key's scale; weights times the values' scales, relative to the largest of these, are
+ * rounded to fp16 for the second product (for fp16, to two numbers of it). */
 size_t flexatt_quant_tree_fwd_workspace(const flexatt_tree* p);
 int flexatt_quant_tree_fwd(const flexatt_tree* p, int32_t code, const flexatt_tensor* q, const flexatt_tensor* k_cache,
                            const flexatt_tensor* v_cache, const float* k_scales, const float* v_scales,

@@ -85,6 +85,29 @@ int check_norm(const flexatt_rotary* r, const flexatt_norm* n) {
   return FLEXATT_OK;
 }
 
+// The launch of norm_rotary.hip: a workgroup has 256 / (D / (32 / size)) tokens, and of many
+// tokens all heads of q, k or v; few tokens make some thousand workgroups at most.
+int check_norm_launch(const flexatt_rotary* r, bool append) {
+  if ((int64_t)r->heads_q + r->heads_kv > 1 << 30) return FLEXATT_ERANGE;
+  const int64_t per = 256 / (r->head_dim * (int)elt_size(r->dtype) / 32), kinds = (r->heads_q > 0) + (r->heads_kv > 0) * (append ? 2 : 1);
+  return check_launch(((int64_t)r->batch * r->seqlen + per - 1) / per * kinds, 256);
+}
+
+// What a call reads besides its tensors, within `out`.
+bool within(const flexatt_rotary* r, const flexatt_norm* n, Span out) {
+  if (r->rotary_dim > 0 && overlap(span_of(r->inv_freq, (size_t)r->rotary_dim / 2 * 8), out)) return true;
+  if (r->positions) {
+    const int64_t x = (r->batch - 1) * r->position_stride_b, y = (r->seqlen - 1) * r->position_stride_s, es = r->position_bytes;
+    const uintptr_t at = (uintptr_t)r->positions;
+    const Span all = {at + (uintptr_t)(((x < 0 ? x : 0) + (y < 0 ? y : 0)) * es),
+                      at + (uintptr_t)(((x > 0 ? x : 0) + (y > 0 ? y : 0) + 1) * es)};
+    if (overlap(all, out)) return true;
+  }
+  if (!n) return false;
+  const size_t bytes = r->head_dim * elt_size(n->weight_dtype);
+  return (n->q_weight && overlap(span_of(n->q_weight, bytes), out)) || (n->k_weight && overlap(span_of(n->k_weight, bytes), out));
+}
+
 NormRotaryArgs norm_args(const RotaryArgs& r, const flexatt_norm* n) {
   NormRotaryArgs a = {};
   a.r = r;
@@ -269,7 +292,7 @@ TreePlan quant_plan(const flexatt_tree* p) {
 // the prefix, and of each sequence's own cache as TreePlan has them.  Where one round of
 // workgroups can have it all, the two that make the longest chunk shortest (in steps of
 // the waves; bf16 B=4 Hq=32 Hkv=8 T=1 D=128, a prefix of 16000 rows, caches of 1000: 27 us
-// with eight workgroups in a second round, 21 without); else the prefix gets its share of a
+// with eight workgroups in a second round, 22 without); else the prefix gets its share of a
 // round, by key tiles times row tiles (more of it, or less: 72 -> 76 and 81 us for 32
 // sequences of 4 tokens behind 16383 rows).
 struct PrefixPlan {
@@ -457,6 +480,7 @@ int flexatt_norm_rotary_apply(const flexatt_rotary* r, const flexatt_norm* n, co
                               void* stream) {
   FLEXATT_TRY(check_rotary(r, false));
   FLEXATT_TRY(check_norm(r, n));
+  FLEXATT_TRY(check_norm_launch(r, false));
   FLEXATT_TRY(check_tensor(q, r->dtype));
   FLEXATT_TRY(check_out_tensor(q_out, r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
   if (r->heads_kv == 0 && (k || k_out)) return FLEXATT_EINVAL;
@@ -499,6 +523,21 @@ int flexatt_norm_rotary_grad(const flexatt_rotary* r, const flexatt_norm* n, con
   if ((uintptr_t)workspace % 16) return FLEXATT_ELAYOUT;
   for (const void* w : {dq_weight, dk_weight})
     if ((uintptr_t)w % elt_size(n->weight_dtype)) return FLEXATT_ELAYOUT;
+  // (workgroups still read the inputs while others write the outputs)
+  const auto span = [&](const flexatt_tensor* t, int heads) {
+    return t ? span_of(t, r->dtype, r->batch, heads, r->seqlen, r->head_dim) : Span{};
+  };
+  const size_t weight = r->head_dim * elt_size(n->weight_dtype);
+  const Span outs[] = {span(dq, r->heads_q), span(dk, r->heads_kv), span_of(dq_weight, weight),
+                       span_of(dk_weight, dk_weight ? weight : 0), span_of(workspace, flexatt_norm_rotary_grad_workspace(r))};
+  const Span ins[] = {span(q, r->heads_q), span(k, r->heads_kv), span(q_grad, r->heads_q), span(k_grad, r->heads_kv)};
+  for (const Span& y : outs) {
+    if (within(r, n, y)) return FLEXATT_ELAYOUT;
+    for (const Span& x : ins)
+      if (overlap(x, y)) return FLEXATT_ELAYOUT;
+    for (const Span& x : outs)
+      if (&x != &y && overlap(x, y)) return FLEXATT_ELAYOUT;
+  }
   NormRotaryArgs g = norm_args(a, n);
   g.gq = view(q_grad);
   if (r->heads_kv > 0) g.gk = view(k_grad);
@@ -514,7 +553,10 @@ int flexatt_norm_rotary_append(const flexatt_rotary* r, const flexatt_norm* n, c
                                const int32_t* lengths, void* stream) {
   FLEXATT_TRY(check_rotary(r, true));
   FLEXATT_TRY(check_norm(r, n));
+  FLEXATT_TRY(check_norm_launch(r, true));
   FLEXATT_TRY(check_append(r, q, k, v, q_out, k_cache, v_cache, (int64_t)elt_size(r->dtype), cache_rows, lengths));
+  for (const flexatt_tensor* y : {k_cache, v_cache})
+    if (within(r, n, span_of(y, r->dtype, r->batch, r->heads_kv, cache_rows, r->head_dim))) return FLEXATT_ELAYOUT;
   const RotaryArgs a = append_args(r, q, k, v, q_out, k_cache, v_cache, cache_rows, lengths);
   return (int)kNorm[head_index(r->head_dim)](r->dtype, norm_args(a, n), (hipStream_t)stream);
 }
@@ -526,6 +568,7 @@ int flexatt_quant_append(const flexatt_rotary* r, const flexatt_norm* n, int32_t
   FLEXATT_TRY(check_rotary(r, true));
   if (!is_code(code) || r->inverse) return FLEXATT_EINVAL;
   if (n) FLEXATT_TRY(check_norm(r, n));
+  FLEXATT_TRY(check_norm_launch(r, true));
   FLEXATT_TRY(check_append(r, q, k, v, q_out, k_cache, v_cache, 1, cache_rows, lengths));
   if (!k_scales || !v_scales) return FLEXATT_EINVAL;
   if ((uintptr_t)k_scales % 4 || (uintptr_t)v_scales % 4) return FLEXATT_ELAYOUT;
@@ -540,6 +583,9 @@ int flexatt_quant_append(const flexatt_rotary* r, const flexatt_norm* n, int32_t
                         span_bytes(k_cache, 1, r->batch, r->heads_kv, cache_rows, r->head_dim),
                         span_bytes(v_cache, 1, r->batch, r->heads_kv, cache_rows, r->head_dim)})
     if (overlap(x, ks) || overlap(x, vs)) return FLEXATT_ELAYOUT;
+  for (const Span& y : {ks, vs, span_bytes(k_cache, 1, r->batch, r->heads_kv, cache_rows, r->head_dim),
+                        span_bytes(v_cache, 1, r->batch, r->heads_kv, cache_rows, r->head_dim)})
+    if (within(r, n, y)) return FLEXATT_ELAYOUT;
   NormRotaryArgs a = norm_args(append_args(r, q, k, v, q_out, k_cache, v_cache, cache_rows, lengths), n);
   a.kind = code;
   a.k_scales = k_scales;
@@ -553,9 +599,8 @@ int flexatt_dequant_rows(const flexatt_dequant* p, const flexatt_tensor* k_cache
   if (!p) return FLEXATT_EINVAL;
   FLEXATT_TRY(check_sizes(p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim));
   if (!is_code(p->code) || (p->fill & ~1) || p->reserved != 0 || !p->lengths) return FLEXATT_EINVAL;
-  // (rows of a workgroup: dequant.hip)
-  const int64_t rows = 256 / (p->head_dim * (int)elt_size(p->dtype) / 16);
-  FLEXATT_TRY(check_launch((int64_t)p->batch * p->heads_kv * ((p->cache_rows + rows - 1) / rows), 256));
+  const int64_t bh = (int64_t)p->batch * p->heads_kv, rows = dequant_rows(p->head_dim * (int)elt_size(p->dtype), bh, p->cache_rows);
+  FLEXATT_TRY(check_launch(bh * ((p->cache_rows + rows - 1) / rows), 256));
   FLEXATT_TRY(check_view(k_cache, 1));
   FLEXATT_TRY(check_view(v_cache, 1));
   FLEXATT_TRY(check_out_tensor(k_out, p->dtype, p->batch, p->heads_kv, p->cache_rows, p->head_dim));

@@ -78,15 +78,11 @@ __global__ __launch_bounds__(kThreads) void dequant_kernel(DequantArgs a, int ch
 template <class T, int D>
 hipError_t launch_d(const DequantArgs& a, hipStream_t st) {
   constexpr int RPB = kThreads / (D / (16 / (int)sizeof(T)));
-  const int64_t bh = (int64_t)a.B * a.H, rows = a.C;
-  // four rows a thread where that leaves four workgroups a CU, else one
-  if (bh * ((rows + 4 * RPB - 1) / (4 * RPB)) >= 1024) {
-    const int chunks = (int)((rows + 4 * RPB - 1) / (4 * RPB));
-    hipLaunchKernelGGL((dequant_kernel<T, D, 4>), dim3((unsigned)(bh * chunks)), dim3(kThreads), 0, st, a, chunks);
-  } else {
-    const int chunks = (int)((rows + RPB - 1) / RPB);
-    hipLaunchKernelGGL((dequant_kernel<T, D, 1>), dim3((unsigned)(bh * chunks)), dim3(kThreads), 0, st, a, chunks);
-  }
+  const int64_t bh = (int64_t)a.B * a.H;
+  const int rows = dequant_rows(D * (int)sizeof(T), bh, a.C), chunks = (a.C + rows - 1) / rows;
+  const dim3 grid((unsigned)(bh * chunks));
+  if (rows == RPB) hipLaunchKernelGGL((dequant_kernel<T, D, 1>), grid, dim3(kThreads), 0, st, a, chunks);
+  else hipLaunchKernelGGL((dequant_kernel<T, D, 4>), grid, dim3(kThreads), 0, st, a, chunks);
   return hipGetLastError();
 }
 

@@ -137,6 +137,12 @@ struct DequantArgs {
   int B, H, C, D, kind;
   int fill;  // 1: rows behind the length are zeroed
 };
+// Rows of one of its workgroups, of rowb output bytes: four rounds of its threads where
+// that leaves four workgroups a CU, else one.
+inline int dequant_rows(int rowb, int64_t bh, int64_t cache_rows) {
+  const int once = 256 / (rowb / 16);
+  return bh * ((cache_rows + 4 * once - 1) / (4 * once)) >= 1024 ? 4 * once : once;
+}
 
 // Attention of a tree of drafted tokens over a cache (tree_attn.hip).
 struct TreeArgs {

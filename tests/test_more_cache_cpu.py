@@ -214,3 +214,62 @@ def test_oracle_gradient_is_the_forwards(inter):
     dx, dw = torch.autograd.grad(y, (x, w), gy)
     (ox, _), (ow, _) = orc.norm_rotary_grad(x.detach(), w.detach(), gy, f, at, inter, m, 1e-3)
     assert torch.allclose(dx, ox, rtol=1e-12, atol=1e-13) and torch.allclose(dw, ow, rtol=1e-12, atol=1e-13)
+
+
+@pytest.mark.parametrize("Hq,Hkv,S,apply,append", [
+    (1, 1, 1 << 26, -6, -6), (1, 1, (1 << 26) - 8, -5, -6), (1, 1, 44739240, -5, -5), (1, 1, 44739248, -5, -6),
+    (1 << 30, 1, 1, -6, -6), ((1 << 30) - 1, 1, 1, -5, -5)])
+def test_norm_launch_limits_of_keys_and_values(Hq, Hkv, S, apply, append):
+    """Eight tokens of 1 KB a workgroup, for q, k and v each: 2^24 of 256 threads are one too many."""
+    lib, n = L.load(), L.Norm(L.F32, 1e-6, FAKE, FAKE)
+    r = L.Rotary(L.F32, 1, Hq, Hkv, S, 256, 0, 0, 0, 1.0, None, None, 0, 0, 0, 0)
+    assert lib.flexatt_norm_rotary_apply(r, n, ODD, ODD, ODD, ODD, None) == apply
+    assert lib.flexatt_norm_rotary_append(r, n, ODD, ODD, ODD, ODD, ODD, ODD, 100, FAKE, None) == append
+    assert lib.flexatt_quant_append(r, n, L.INT8, ODD, ODD, ODD, ODD, ODD, ODD, FAKE, FAKE, 100, FAKE, None) == append
+    assert lib.flexatt_quant_append(r, None, L.INT8, ODD, ODD, ODD, ODD, ODD, ODD, FAKE, FAKE, 100, FAKE, None) == append
+
+
+def test_what_an_append_reads_lies_apart_from_the_cache():
+    lib, kc, vc = L.load(), _t(2, 100, at=FAR), _t(2, 100, at=2 * FAR)
+    wide = 2 * 2 * 100 * 128  # bytes of a cache of 16 bits, half of it one of 8
+
+    def both(r=None, n=None):
+        r, n = _rotary(**(r or {})), _norm(**(n or {}))
+        a = lib.flexatt_norm_rotary_append(r, n, _t(4), _t(), _t(), _t(4), kc, vc, 100, FAKE, None)
+        return a, lib.flexatt_quant_append(r, n, L.INT8, _t(4), _t(), _t(), _t(4), kc, vc, 3 * FAR, 4 * FAR, 100, FAKE, None)
+
+    for at in (FAR, 2 * FAR, FAR + wide // 2 - 8, 2 * FAR + wide // 2 - 8, FAR - 8):
+        assert both(r=dict(inv_freq=at)) == both(n=dict(q_weight=at)) == both(n=dict(k_weight=at)) == (-5, -5)
+        assert both(r=dict(positions=at, position_bytes=8, position_stride_s=1)) == (-5, -5)
+    # positions whose sequences lie one behind the other, or backwards
+    assert both(r=dict(positions=FAR - 64, position_bytes=8, position_stride_b=8, position_stride_s=1)) == (-5, -5)
+    assert both(r=dict(positions=FAR + wide // 2, position_bytes=4, position_stride_b=0, position_stride_s=-1)) == (-5, -5)
+    for at in (3 * FAR, 4 * FAR, 4 * FAR + 2 * 2 * 100 * 4 - 8):
+        assert both(r=dict(inv_freq=at))[1] == both(n=dict(q_weight=at))[1] == both(n=dict(k_weight=at))[1] == -5
+
+
+def test_norm_gradients_lie_apart():
+    lib, r, n = L.load(), _rotary(inv_freq=20 * FAR), _norm(q_weight=21 * FAR, k_weight=22 * FAR)
+    ok = dict(q=_t(4, at=FAR), k=_t(2, at=2 * FAR), gq=_t(4, at=3 * FAR), gk=_t(2, at=4 * FAR), dq=_t(4, at=5 * FAR),
+              dk=_t(2, at=6 * FAR), wq=7 * FAR, wk=8 * FAR, ws=9 * FAR, size=1 << 30)
+    call = lambda **kw: lib.flexatt_norm_rotary_grad(r, n, *dict(ok, **kw).values(), None)  # noqa: E731
+    for name, heads in (("dq", 4), ("dk", 2)):
+        for other in (1, 2, 3, 4, 5 if name == "dk" else 6, 7, 8, 9, 20, 21, 22):
+            assert call(**{name: _t(heads, at=other * FAR)}) == -5, (name, other)
+    for name in ("wq", "wk", "ws"):
+        for other in (1, 2, 3, 4, 5, 6, 20, 21, 22):
+            assert call(**{name: other * FAR}) == -5, (name, other)
+    assert call(wk=7 * FAR) == call(ws=7 * FAR) == call(ws=8 * FAR - 16) == -5
+
+
+def test_mask_and_read_back_limits():
+    lib, p = L.load(), _tree(batch=1, heads_q=1, heads_kv=1, tokens=1 << 15, cache_rows=1 << 16, tree_mask=FAKE, mask_batch=1)
+    run = lambda: lib.flexatt_quant_tree_fwd(p, L.INT8, ODD, ODD, ODD, FAKE, FAKE, ODD, FAKE, FAKE, 1 << 40, None)  # noqa: E731
+    assert run() == -5
+    p.tokens += 1
+    assert run() == -6 and lib.flexatt_quant_tree_fwd_workspace(p) == 2 ** 64 - 1
+    p.tree_mask, p.mask_batch = None, 0
+    assert run() == -5
+    for rows, code in ((1 << 27, -6), ((1 << 27) - 16, -5)):  # 16 rows of 1 KB a workgroup
+        d = _dequant(dtype=L.F32, head_dim=256, batch=1, cache_rows=rows)
+        assert lib.flexatt_dequant_rows(d, ODD, ODD, FAKE, FAKE, ODD, ODD, None) == code
