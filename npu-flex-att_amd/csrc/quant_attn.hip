@@ -65,6 +65,10 @@ __device__ __forceinline__ int swz_v8(int r, int c) {
   else return c ^ ((r & 7) << 1);
 }
 
+// What 2^lift times a scale may reach: weights reach 2^8 before the maximum follows
+// (kTreeRescale), and fp16 ends at 2^16.
+constexpr float kMostScale = 0x1p7f;
+
 // Eight codes as an MFMA operand of T.
 template <class T, int CODE>
 __device__ __forceinline__ typename Mfma<T>::v8 operand8(int lo, int hi) {
@@ -294,7 +298,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   float m_run = kNegInf, l_run = 0.f;
 #pragma unroll
   for (int db = 0; db < C::DB; ++db) acc[db] = f32x16{};
-  // weights are 2^(x - m_run + lift), and rel = 2^lift times a scale is at most 1
+  // weights are 2^(x - m_run + lift), and rel = 2^lift times a scale is at most kMostScale
   float lift = 90.f, rel = 0x1p90f;
 
   // K of tile j + 1, and all that was issued before it, lands.  What may be in flight
@@ -409,11 +413,11 @@ void quant_attn_kernel(QuantTreeArgs qa) {
     max16_partial(vs, top, top2);
     top = max2(top, top2);
     top = fmaxf(top, swap_halves(top));
-    const bool grow = mx > m_run + kTreeRescale, over = __builtin_amdgcn_readfirstlane(top * rel > 1.f);
+    const bool grow = mx > m_run + kTreeRescale, over = __builtin_amdgcn_readfirstlane(top * rel > kMostScale);
     if (over || __builtin_amdgcn_ballot_w64(grow)) {
-      // (over: 2^lift becomes the power of two above the largest scale, as far as there is one)
+      // (over: the largest power of two with which the largest scale is below 2^7)
       const int expo = (int)(__float_as_uint(top) >> 23) & 255;
-      const int field = over ? min(max(253 - expo, 1), 217) : (int)lift + 127;
+      const int field = over ? min(max(260 - expo, 1), 217) : (int)lift + 127;
       const float now = __int_as_float(field << 23);
       const float m_new = grow ? mx : m_run;
       const float alpha = (grow ? fast_exp2(m_run - m_new) : 1.f) * (now / rel);

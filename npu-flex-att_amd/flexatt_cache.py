@@ -189,9 +189,11 @@ def quantized_tree_attention(query, key_cache, value_cache, key_scales, value_sc
     """:func:`tree_attention` over a cache of 8 bits, for float16 and bfloat16 queries; the
     other arguments and results are the same.
 
-    Scores are products with the codes times the key's scale, in 32 bits.  A weight times
-    its value's scale is rounded to float16, relative to the largest scale.  Scales of rows that a token does
-    not see must be finite, as their values.
+    Scores are products with the codes times the key's scale, in 32 bits.  A weight times its
+    value's scale is rounded to float16 (for float16 queries to two of them), in which the
+    largest scale is 2 ** 6 at least: a value 2 ** 20 times smaller than the largest keeps
+    eleven bits of a weight of 1.  A ``tree_mask`` is of 2 ** 15 tokens at most.  Scales of
+    rows that a token does not see must be finite, as their values.
     """
     return _lib.native().quant_tree_attention(query, key_cache, value_cache, key_scales, value_scales, lengths, tree_mask,
                                               sliding_window, depths, scale, soft_cap, return_lse)
