@@ -290,31 +290,35 @@ TreePlan quant_plan(const flexatt_tree* p) {
 }
 // The launch behind a shared prefix, whose rows are those of all sequences: `np` chunks of
 // the prefix, and of each sequence's own cache as TreePlan has them.  Where one round of
-// workgroups can have it all, the two that make the longest chunk shortest (in steps of
-// the waves; bf16 B=4 Hq=32 Hkv=8 T=1 D=128, a prefix of 16000 rows, caches of 1000: 27 us
-// with eight workgroups in a second round, 22 without); else the prefix gets its share of a
-// round, by key tiles times row tiles (more of it, or less: 72 -> 76 and 81 us for 32
-// sequences of 4 tokens behind 16383 rows).
+// workgroups can have it all, the two that make the longest chunk shortest, in steps of the
+// waves (bf16 B=4 Hq=32 Hkv=8 T=1 D=128, a prefix of 16000 rows, caches of 1000: 27 us with
+// eight workgroups in a second round, 22 without); else the prefix gets its share of a
+// round, by key tiles times row tiles or, with eight row tiles a workgroup, by their times
+// (64 sequences of one token behind 4000 rows, caches of 600: 44 -> 40 us).
 struct PrefixPlan {
   TreePlan own;
   int np;
+  bool wide;
 };
 PrefixPlan prefix_plan(const flexatt_tree* p, int prefix_rows) {
   const int rowb = p->head_dim * (int)elt_size(p->dtype);
   const int64_t rows = (int64_t)(p->heads_q / p->heads_kv) * p->tokens, all = (rows * p->batch + 31) / 32;
-  const int share = tree_share(rowb, (int)elt_size(p->dtype), all);
-  const int64_t groups = (all + share - 1) / share, own_groups = ((rows + 31) / 32 + share - 1) / share;
+  const bool wide = prefix_wide(rowb, (int)elt_size(p->dtype), all, row_tiles(p));
+  const int share = wide ? 8 : tree_share(rowb, (int)elt_size(p->dtype), all), own_share = wide ? 1 : share;
+  const int64_t groups = (all + share - 1) / share, own_groups = (row_tiles(p) + own_share - 1) / own_share;
   const int64_t tiles = (prefix_rows + 31) / 32, own_tiles = (p->cache_rows + 31) / 32;
-  const int64_t slots = (rowb >= 256 ? 1 : 2) * (int64_t)cus(), waves = rowb > 512 ? 2 : share == 4 ? 2 : 4;
+  const int64_t slots = (rowb >= 256 || wide ? 1 : 2) * (int64_t)cus();
+  const int64_t waves = wide ? 1 : rowb > 512 ? 2 : share == 4 ? 2 : 4, own_waves = wide ? 8 : waves;
   const int64_t least = 8, most = (tiles + least - 1) / least < 64 ? (tiles + least - 1) / least : 64;
   const int64_t per = groups * p->heads_kv, own_per = own_groups * p->heads_kv * p->batch;
   PrefixPlan t;
-  t.own = plan_of(p, share, slots);
+  t.own = plan_of(p, own_share, slots);
+  t.wide = wide;
   int64_t np = 0, best = INT64_MAX;
   for (int64_t ns = 1; ns <= (own_tiles + least - 1) / least && ns * own_per + per <= slots; ++ns) {
     int64_t n = (slots - ns * own_per) / per;
     if (n > most) n = most;
-    const int64_t x = (tiles + n * waves - 1) / (n * waves), y = (own_tiles + ns * waves - 1) / (ns * waves);
+    const int64_t x = (tiles + n * waves - 1) / (n * waves), y = (own_tiles + ns * own_waves - 1) / (ns * own_waves);
     const int64_t cost = x > y ? x : y;
     if (cost >= best) continue;
     best = cost;
@@ -322,7 +326,13 @@ PrefixPlan prefix_plan(const flexatt_tree* p, int prefix_rows) {
     t.own.nsplit = (int)ns;
     t.own.slots = t.own.nchunk = (int)(ns * p->heads_kv * p->batch);
   }
-  if (np == 0) {
+  if (np == 0 && wide) {
+    // in times of a prefix tile: a chunk of it costs five more, a sequence's own workgroup
+    // eight and a quarter of each tile; as many chunks as make one no longer than all work's
+    // share of a CU
+    const int64_t own = own_per * (32 + own_tiles);  // (quarters)
+    for (np = 1; np < most && (tiles / np + 5) * slots * 4 > np * per * (tiles / np + 5) * 4 + own;) ++np;
+  } else if (np == 0) {
     const int64_t mine = groups * tiles, others = own_groups * p->batch * own_tiles;
     np = (slots * mine / (mine + others) + per / 2) / per;
     np = np < 1 ? 1 : np > most ? most : np;
@@ -701,6 +711,7 @@ int flexatt_prefix_fwd(const flexatt_tree* p, int32_t prefix_rows, const flexatt
   PrefixArgs a = {};
   a.t = tree_args(p, plan.own, q, k_cache, v_cache, o, lse, nullptr);
   a.np = plan.np;
+  a.wide = plan.wide;
   a.pitch = plan.np + plan.own.nsplit;
   a.t.part_o = (float*)workspace;
   a.t.part_lse = a.t.part_o + tree_rows(p) * a.pitch * p->head_dim;

@@ -174,6 +174,7 @@ struct PrefixArgs {
   int pitch;  // partials of a row, np + t.nsplit
   int npre;   // workgroups of the prefix, the first of the launch (set by the launcher)
   int nrtp;   // groups of the prefix's row tiles, B * G * T rows (set by the launcher)
+  int wide;   // eight row tiles of the prefix a workgroup
 };
 
 // The same over a cache of 8 bits (quant_attn.hip): t.k and t.v are bytes.
@@ -219,6 +220,14 @@ struct EvictArgs {
 inline int tree_share(int row_bytes, int elt_bytes, int64_t tiles) {
   if (elt_bytes != 2 || row_bytes > 256 || tiles < 2) return 1;
   return row_bytes > 128 && (tiles + 3) / 4 * 4 * 6 <= (tiles + 1) / 2 * 2 * 7 ? 4 : 2;
+}
+
+// Whether a workgroup has eight row tiles of a shared prefix, of `all`, and a sequence's own
+// rows are `own` (tree_attn.hip): 16-bit rows of 256 bytes, where eight pad by a sixth at
+// most (bf16 Hq=32 Hkv=8 D=128, 128 sequences of 2 tokens behind 8000 rows 82 -> 68 us, 64
+// of 1 behind 4000 46 -> 40; D=64, 28 row tiles behind 8000 rows 26 -> 31).
+inline bool prefix_wide(int row_bytes, int elt_bytes, int64_t all, int64_t own) {
+  return elt_bytes == 2 && row_bytes == 256 && own <= 2 && (all + 7) / 8 * 8 * 6 <= all * 7;
 }
 
 typedef hipError_t (*TreeLauncher)(const TreeArgs&, hipStream_t);

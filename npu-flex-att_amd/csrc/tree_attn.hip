@@ -79,8 +79,7 @@ struct TreeCfg {
   static constexpr int PV = RPC >= VROWS ? 1 : VROWS / RPC;  // and V's
   static constexpr int NW = ROWB <= 512 ? 4 : 2;      // waves per workgroup
   static constexpr int ST = ROWB <= 256 ? 2 : 1;      // stages
-  static constexpr int WAVEB = ST * 2 * TB;
-  static_assert(E * 1024 == TB && NW * WAVEB <= 160 * 1024 && E % PK == 0 && E % PV == 0, "tiles");
+  static_assert(E * 1024 == TB && NW * ST * 2 * TB <= 160 * 1024 && E % PK == 0 && E % PV == 0, "tiles");
 };
 
 // V tiles of 32-bit elements are read one element per lane, 32 of a row by each
@@ -124,20 +123,24 @@ __device__ __forceinline__ const TreeArgs& tree_of(const PrefixArgs& a) { return
 // WPT neighbouring waves, a row tile each, share their key tiles: each copies its share of
 // a tile, and a barrier a tile keeps them in step.
 //
-// PRE: the sequences share a prefix.  The launch's first workgroups have its chunks, whose
-// rows are those of all sequences (b, token, head, the head innermost), so that a key of
-// it is read once for all of them; the others have the sequences' own caches.
-template <class T, int D, int NW, int WPT, bool CAP, bool PRE>
-__global__ __launch_bounds__(NW * WPT * 64)
-__attribute__((amdgpu_waves_per_eu(D * sizeof(T) >= 256 ? (WPT == 1 ? 1 : 2) : WPT == 1 ? 2 : 4)))
-void tree_attn_kernel(ArgsOf<PRE> args) {
+// Behind a shared prefix the launch's first workgroups have its chunks, whose rows are
+// those of all sequences (b, token, head, the head innermost), so that a key of it is read
+// once for all of them; the others have the sequences' own caches.
+enum { kTree, kBoth, kOwn };  // no prefix; a workgroup of either kind; of the second alone
+template <class T, int D, int NW, int WPT, int ST>
+constexpr int tree_lds() {
+  constexpr int combine = NW * WPT * 64 * 4 * (2 + 16 * TreeCfg<T, D>::DB), tiles = NW * ST * 2 * TreeCfg<T, D>::TB;
+  return tiles > combine ? tiles : combine;
+}
+template <class T, int D, int NW, int WPT, int ST, bool CAP, int KIND>
+__device__ __forceinline__ void tree_work(const ArgsOf<KIND != kTree>& args, char* smem, int block) {
+  constexpr bool PRE = KIND != kTree;
   const TreeArgs& a = tree_of(args);
   using C = TreeCfg<T, D>;
-  constexpr int ST = C::ST, EC = C::E / WPT;  // copies a wave makes of a tile
+  constexpr int EC = C::E / WPT;  // copies a wave makes of a tile
+  constexpr int WAVEB = ST * 2 * C::TB;
   constexpr int PK = C::PK > WPT ? C::PK / WPT : 1, PV = C::PV > WPT ? C::PV / WPT : 1, CROWS = WPT * C::RPC;
   static_assert(WPT == 1 || (ST == 2 && C::E % WPT == 0), "shared tiles");
-  constexpr int kCombine = NW * WPT * 64 * 4 * (2 + 16 * C::DB);
-  __shared__ __attribute__((aligned(1024))) char smem[NW * C::WAVEB > kCombine ? NW * C::WAVEB : kCombine];
 
   const Shape& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -149,17 +152,19 @@ void tree_attn_kernel(ArgsOf<PRE> args) {
   // and started together (as rows of a two-dimensional grid, started one after the
   // other, they find the chunk gone from L2: fp16 B=4 Hq=28 Hkv=4 T=64, caches of
   // 16384 D=64, 58 -> 74 us)
-  int rt0 = 0, x = blockIdx.x;
+  int rt0 = 0, x = block;
   bool shared = false;  // a chunk of the prefix
   if constexpr (PRE) {
-    shared = x < args.npre;
-    if (!shared) x -= args.npre;
+    if constexpr (KIND == kBoth) {
+      shared = x < args.npre;
+      if (!shared) x -= args.npre;
+    }
     const int nrt = shared ? args.nrtp : a.nrt, i = x;
     rt0 = i / 8 % nrt * WPT;
     x = i / (8 * nrt) * 8 + i % 8;
   } else if (a.nrt > 1) {
-    rt0 = blockIdx.x / 8 % a.nrt * WPT;
-    x = blockIdx.x / (8 * a.nrt) * 8 + blockIdx.x % 8;
+    rt0 = block / 8 % a.nrt * WPT;
+    x = block / (8 * a.nrt) * 8 + block % 8;
   }
   rt0 += sub;
   TreeChunk ck;
@@ -167,7 +172,7 @@ void tree_attn_kernel(ArgsOf<PRE> args) {
   if (PRE && shared) {
     if constexpr (PRE) {
       if (x >= p.Hkv * args.np) return;
-      ck = prefix_chunk(args, x);
+      ck = prefix_chunk<1>(args, x);
       sq = TreeSeq{args.P, 0, 0, false};
     }
   } else {
@@ -216,7 +221,7 @@ void tree_attn_kernel(ArgsOf<PRE> args) {
   for (int e = 0; e < PK; ++e) kvo[e] = (e * CROWS + crow) * kss + swz_col<C::CPR>(e * CROWS + crow, cchunk) * 16;
 #pragma unroll
   for (int e = 0; e < PV; ++e) vvo[e] = (e * CROWS + crow) * vss + swz_v<T, C::CPR>(e * CROWS + crow, cchunk) * 16;
-  const unsigned wbase = lds_addr_of(smem) + wave * C::WAVEB;
+  const unsigned wbase = lds_addr_of(smem) + wave * WAVEB;
   // this wave's LDS reads have returned: the buffer they read may be refilled
   auto reads_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
 
@@ -351,7 +356,7 @@ void tree_attn_kernel(ArgsOf<PRE> args) {
     } else {
       wait_vmcnt<EC>();  // K of tile j landed (its V, issued later, may be in flight)
     }
-    const char* sK = smem + wave * C::WAVEB + (ST == 2 ? (j & 1) * 2 * C::TB : 0);
+    const char* sK = smem + wave * WAVEB + (ST == 2 ? (j & 1) * 2 * C::TB : 0);
     const char* sV = sK + C::TB;
     const int n0 = t * C::BN;
 
@@ -515,6 +520,278 @@ void tree_attn_kernel(ArgsOf<PRE> args) {
   }
 }
 
+template <class T, int D, int NW, int WPT, bool CAP, bool PRE>
+__global__ __launch_bounds__(NW * WPT * 64)
+__attribute__((amdgpu_waves_per_eu(D * sizeof(T) >= 256 ? (WPT == 1 ? 1 : 2) : WPT == 1 ? 2 : 4)))
+void tree_attn_kernel(ArgsOf<PRE> args) {
+  constexpr int ST = TreeCfg<T, D>::ST;
+  __shared__ __attribute__((aligned(1024))) char smem[tree_lds<T, D, NW, WPT, ST>()];
+  tree_work<T, D, NW, WPT, ST, CAP, PRE ? kBoth : kTree>(args, smem, blockIdx.x);
+}
+
+// The prefix with eight row tiles a workgroup, a wave each, where there are as many: 64-key
+// tiles copied by all eight waves into four stages, three ahead, and the two waves of a SIMD
+// a phase apart, one in its products (O += P V of a tile and the scores of the next) while
+// the other has its softmax, with a barrier after each phase.  16384 prefix rows more for 128
+// tokens of Hq=32 Hkv=8 D=128 are 45 us with four waves that share 32-key tiles, 37 here
+// (0.92 PFLOP/s; the regular forward reaches 1.07 at fp16).
+template <class T, int D, bool CAP>
+__device__ __forceinline__ void prefix_rows(const PrefixArgs& args, char* smem) {
+  using C = TreeCfg<T, D>;
+  typedef typename Mfma<T>::v8 V8;
+  constexpr int BN = 64, NB = 2, TILEB = BN * C::ROWB, E = TILEB / 8192, CROWS = 8 * E * C::RPC, AHEAD = 2;
+  static_assert(CROWS == BN && NB * C::KC == 4 * C::DB, "tiles");
+  const TreeArgs& a = args.t;
+  const Shape& p = a.p;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rt = (int)blockIdx.x / 8 % args.nrtp * 8 + wave, x = (int)blockIdx.x / (8 * args.nrtp) * 8 + (int)blockIdx.x % 8;
+  if (x >= p.Hkv * args.np) return;
+  const TreeChunk ck = prefix_chunk<2>(args, x);
+  const int hk = ck.hk, first = ck.first / 2, nv = (ck.count + 1) / 2;
+
+  // packed query row of this lane: head, drafted token, sequence
+  const int R = p.B * p.G * p.Sq, r = min(32 * rt + l32, R - 1);
+  const int hq = hk * p.G + r % p.G, qb = r / p.G / p.Sq, qi = r / p.G - qb * p.Sq;
+  i32x4 qf[C::KC];
+  const char* src = (const char*)((const T*)a.q.data + qb * a.q.sb + hq * a.q.sh + (int64_t)qi * a.q.ss) + 16 * h;
+#pragma unroll
+  for (int kc = 0; kc < C::KC; ++kc) qf[kc] = ld_global16(src + 32 * kc);
+
+  int koff[C::KC], voff[C::DB];
+  const int tr_row = 4 * h + ((lane & 15) >> 2), tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+  for (int kc = 0; kc < C::KC; ++kc) koff[kc] = l32 * C::ROWB + swz_col<C::CPR>(l32, 2 * kc + h) * 16;
+#pragma unroll
+  for (int db = 0; db < C::DB; ++db)
+    voff[db] = tr_row * C::ROWB + swz_tr<C::CPR>(tr_row, 4 * db + (tr_col >> 3)) * 16 + (tr_col & 7) * 2;
+  const unsigned kss = (unsigned)(args.k.ss * (int)sizeof(T)), vss = (unsigned)(args.v.ss * (int)sizeof(T));
+  const int crow = wave * E * C::RPC + lane / C::CPR, cchunk = lane % C::CPR;
+  unsigned kvo[E], vvo[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int row = crow + e * C::RPC;
+    kvo[e] = row * kss + swz_col<C::CPR>(row, cchunk) * 16;
+    vvo[e] = row * vss + swz_v<T, C::CPR>(row, cchunk) * 16;
+  }
+  const unsigned lds0 = lds_addr_of(smem) + wave * E * 1024;
+  const uint64_t kp = (uint64_t)((const T*)args.k.data + hk * args.k.sh), vp = (uint64_t)((const T*)args.v.data + hk * args.v.sh);
+  // Tile v of the chunk into stage v % 4; behind the last one that again, so that every wait
+  // is for the same number of copies.
+  auto issue = [&](int v) {
+    const unsigned dst = lds0 + (v & 3) * 2 * TILEB;
+    const int n0 = (first + min(v, nv - 1)) * BN;
+    const uint64_t kb = kp + (uint64_t)n0 * kss, vb = vp + (uint64_t)n0 * vss;
+    if (n0 + BN <= args.P) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        load_lds16_base(kvo[e], kb, dst + e * 1024);
+        load_lds16_base(vvo[e], vb, dst + e * 1024 + TILEB);
+      }
+    } else {  // rows behind the last one repeat it
+#pragma unroll 1
+      for (int e = 0; e < E; ++e) {
+        const int row = crow + e * C::RPC, at = min(row, args.P - 1 - n0);
+        load_lds16_base(at * kss + swz_col<C::CPR>(row, cchunk) * 16, kb, dst + e * 1024);
+        load_lds16_base(at * vss + swz_v<T, C::CPR>(row, cchunk) * 16, vb, dst + e * 1024 + TILEB);
+      }
+    }
+  };
+  auto landed = [] { wait_vmcnt<2 * E>(); };
+
+  if (nv > 0) {
+    issue(0);
+    issue(1);
+  }
+
+  // rows of the prefix this lane's row sees: from row_lo on (tree_work)
+  int row_lo = 0, full_lo = 0;
+  if (p.window > 0) {
+    const int depth = a.depths ? max(a.depths[(int64_t)qb * p.Sq + qi], 0) : qi;
+    const int past = args.P + min(max(a.lengths[qb], 0), p.Skv);
+    full_lo = row_lo = max(past - (p.window - min(depth, p.window)), 0);
+#pragma unroll
+    for (int y = 32; y; y >>= 1) full_lo = max(full_lo, __shfl_xor(full_lo, y));
+    full_lo = __builtin_amdgcn_readfirstlane(full_lo);
+  }
+  float c2 = p.scale_log2;
+  int flip = 0;
+  if constexpr (!CAP) {
+    if (c2 < 0.f) flip = (int)0x80008000;
+    c2 = c2 == 0.f ? 1e-30f : fabsf(c2);
+  }
+#pragma unroll
+  for (int kc = 0; kc < C::KC; ++kc) {
+    qf[kc] ^= i32x4{flip, flip, flip, flip};
+    pin(qf[kc]);
+  }
+
+  f32x16 acc[C::DB], sc[NB];
+  V8 P[2 * NB];
+  float m_run = kNegInf, l_run = 0.f;
+#pragma unroll
+  for (int db = 0; db < C::DB; ++db) acc[db] = f32x16{};
+  auto softmax = [&](int n0) {
+    if constexpr (CAP) {
+#pragma unroll
+      for (int bb = 0; bb < NB; ++bb) {
+        soft_cap(sc[bb], p);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[bb][e] *= p.cap_log2;
+      }
+    }
+    if (n0 < full_lo || n0 + BN > args.P) {
+      const int lo = row_lo - n0 - 4 * h, hi = args.P - n0 - 4 * h;
+#pragma unroll
+      for (int bb = 0; bb < NB; ++bb) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if ((unsigned)(32 * bb + 8 * (e >> 2) + (e & 3) - lo) >= (unsigned)max(hi - lo, 0)) sc[bb][e] = kNegInf;
+        pin(sc[bb]);  // finished inside the branch (no selects after it)
+      }
+    }
+    float mp[4];
+#pragma unroll
+    for (int bb = 0; bb < NB; ++bb) max16_partial(sc[bb], mp[2 * bb], mp[2 * bb + 1]);
+    float mx = max2(max3(mp[0], mp[1], mp[2]), mp[3]);
+    if constexpr (!CAP) mx *= c2;
+    mx = fmaxf(mx, swap_halves(mx));
+    if (mx != mx) mx = kNegInf;
+    const bool grow = mx > m_run + kTreeRescale;
+    if (__builtin_amdgcn_ballot_w64(grow)) {
+      const float m_new = grow ? mx : m_run;
+      const float alpha = grow ? fast_exp2(m_run - m_new) : 1.f;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < C::DB; ++db) scale_inplace(acc[db], alpha);
+      m_run = m_new;
+    }
+    const float m_use = (m_run == kNegInf) ? 0.f : m_run;
+    float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int bb = 0; bb < NB; ++bb) {
+      f32x16 pe;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if constexpr (!CAP) pe[e] = fast_exp2(__builtin_fmaf(sc[bb][e], c2, -m_use));
+        else pe[e] = fast_exp2(sc[bb][e] - m_use);
+        rs[e & 3] += pe[e];
+      }
+      P[2 * bb] = pack8<T>(pe, 0);
+      P[2 * bb + 1] = pack8<T>(pe, 8);
+    }
+    l_run += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+    // done before the barrier
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) pin(P[i]);
+    pin(l_run);
+  };
+  // what a phase reads is read after the barrier that ends its producer
+  auto pin_s = [&] {
+#pragma unroll
+    for (int bb = 0; bb < NB; ++bb) pin(sc[bb]);
+  };
+  auto pin_p = [&] {
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) pin(P[i]);
+  };
+  // O += P V of tile v and the scores of tile w (either < 0: not), their MFMAs in turn so
+  // that neither waits for its own, LDS reads AHEAD pairs before them
+  auto products = [&](int v, int w, auto both) {
+    const char* sV = smem + (v & 3) * 2 * TILEB + TILEB;
+    const char* sK = smem + (w & 3) * 2 * TILEB;
+    if (both || w >= 0) {
+#pragma unroll
+      for (int bb = 0; bb < NB; ++bb) sc[bb] = f32x16{};
+    }
+#pragma unroll
+    for (int i = 0; i < NB * C::KC; ++i) {
+      if (both || v >= 0) {
+        const int db = i % C::DB, c = i / C::DB;
+        const char* vr = sV + 16 * c * C::ROWB + voff[db];
+        const i16x4 lo = lds_read_tr4(vr), hi = lds_read_tr4(vr + 8 * C::ROWB);
+        acc[db] = Mfma<T>::mma(cat_tr<V8>(lo, hi), P[c], acc[db]);
+      }
+      if (both || w >= 0) {
+        const int bb = i % NB, kc = i / NB;
+        sc[bb] = Mfma<T>::mma(as_v8<V8>(lds_read16(sK + bb * 32 * C::ROWB + koff[kc])), as_v8<V8>(qf[kc]), sc[bb]);
+      }
+    }
+    if constexpr (both) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 3 * AHEAD, 2);
+#pragma unroll
+      for (int i = 0; i < NB * C::KC - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 2);
+        __builtin_amdgcn_sched_group_barrier(0x100, 3, 2);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 2 * AHEAD, 2);
+    }
+  };
+
+  // Stage v % 4 has tile v from its copy, issued when the products of tiles v - 4 and v - 3
+  // begin, which is after the barrier behind every wave's last read of tile v - 4.
+  if (nv > 0) {
+    const bool late = wave >= 4;
+    landed();
+    __syncthreads();
+    if (late) __syncthreads();  // the second half starts a phase later
+    issue(2);
+    products(-1, 0, std::false_type{});
+    landed();
+    __syncthreads();
+    pin_s();
+    for (int v = 0; v + 1 < nv; ++v) {
+      softmax((first + v) * BN);
+      landed();
+      __syncthreads();
+      pin_p();
+      __builtin_amdgcn_s_setprio(1);
+      issue(v + 3);
+      products(v, v + 1, std::true_type{});
+      __builtin_amdgcn_s_setprio(0);
+      landed();
+      __syncthreads();
+      pin_s();
+    }
+    softmax((first + nv - 1) * BN);
+    landed();
+    __syncthreads();
+    pin_p();
+    products(nv - 1, -1, std::false_type{});
+    wait_vmcnt<0>();  // no copy may land after the workgroup's LDS is released
+    __syncthreads();
+    if (!late) __syncthreads();  // the first half matches the second's count
+  }
+
+  const float L = l_run + swap_halves(l_run);
+  const bool empty = L == 0.f;  // no key; NaN is not
+  const float inv = empty ? 0.f : 1.0f / L;
+  if (32 * rt + l32 < R) {
+    const int64_t place = (((int64_t)qb * p.Hq + hq) * p.Sq + qi) * args.pitch + ck.s;
+    float* po = a.part_o + place * D + 4 * h;
+#pragma unroll
+    for (int y = 0; y < 4 * C::DB; ++y) {
+      const f32x16& v = acc[y / 4];
+      const int e = y % 4 * 4;
+      *(f32x4*)(po + 8 * y) = f32x4{v[e] * inv, v[e + 1] * inv, v[e + 2] * inv, v[e + 3] * inv};
+    }
+    if (h == 0) a.part_lse[place] = empty ? kNegInf : m_run + log2f(L);
+  }
+}
+constexpr int kWide = 8;  // waves of its workgroup
+
+// With it the sequences' own caches, a row tile or two each: a wave takes every eighth tile
+// (a wave in four had rows where four waves share their tiles: own caches of 1000 rows alone
+// 34 -> 32 us).
+template <class T, int D, bool CAP>
+__global__ __launch_bounds__(kWide * 64) __attribute__((amdgpu_waves_per_eu(2)))
+void prefix_wide_kernel(PrefixArgs args) {
+  constexpr int ST = 1, own = tree_lds<T, D, kWide, 1, ST>(), all = 4 * 2 * 64 * D * (int)sizeof(T);
+  __shared__ __attribute__((aligned(1024))) char smem[own > all ? own : all];
+  if ((int)blockIdx.x < args.npre) prefix_rows<T, D, CAP>(args, smem);
+  else tree_work<T, D, kWide, 1, ST, CAP, kOwn>(args, smem, blockIdx.x - args.npre);
+}
+
 template <class T, int D, int WPT>
 void launch_tree_share(TreeArgs a, hipStream_t st) {
   constexpr int NW = WPT == 4 ? TreeCfg<T, D>::NW / 2 : TreeCfg<T, D>::NW;
@@ -555,9 +832,26 @@ void launch_prefix_share(PrefixArgs a, hipStream_t st) {
 }
 
 template <class T, int D>
+void launch_prefix_wide(PrefixArgs a, hipStream_t st) {
+  const int64_t rows = (int64_t)a.t.p.G * a.t.p.Sq;
+  a.t.nrt = (int)((rows + 31) / 32);
+  a.nrtp = (int)(((rows * a.t.p.B + 31) / 32 + kWide - 1) / kWide);
+  a.npre = (a.t.p.Hkv * a.np + 7) / 8 * 8 * a.nrtp;
+  const dim3 grid((unsigned)(a.npre + (a.t.nchunk + 7) / 8 * 8 * a.t.nrt)), block(kWide * 64);
+  if (a.t.p.cap > 0.f) hipLaunchKernelGGL((prefix_wide_kernel<T, D, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((prefix_wide_kernel<T, D, false>), grid, block, 0, st, a);
+}
+
+template <class T, int D>
 hipError_t launch_prefix(const PrefixArgs& a, hipStream_t st) {
   using C = TreeCfg<T, D>;
-  const int share = tree_share(C::ROWB, sizeof(T), ((int64_t)a.t.p.B * a.t.p.G * a.t.p.Sq + 31) / 32);
+  int share = tree_share(C::ROWB, sizeof(T), ((int64_t)a.t.p.B * a.t.p.G * a.t.p.Sq + 31) / 32);
+  if constexpr (sizeof(T) == 2 && C::ROWB == 256) {
+    if (a.wide) {
+      launch_prefix_wide<T, D>(a, st);
+      share = 0;
+    }
+  }
   if constexpr (sizeof(T) == 2 && C::ROWB <= 256) {
     if constexpr (C::ROWB == 256) {
       if (share == 4) launch_prefix_share<T, D, 4>(a, st);

@@ -1,5 +1,6 @@
-// What the attention kernels over a K/V cache share (tree_attn.hip, quant_attn.hip, prefix_attn.hip): a sequence's key
-// tiles and how they are cut into chunks, tile copies to LDS, and the merge of the chunks' partials.
+// What the attention kernels over a K/V cache share (tree_attn.hip, quant_attn.hip): a
+// sequence's key tiles and how they are cut into chunks, tile copies to LDS, and the merge of
+// the chunks' partials.
 #pragma once
 #include "flexatt_device.h"
 #include "flexatt_kernels.h"
@@ -89,7 +90,8 @@ __device__ __forceinline__ TreeChunk tree_chunk(const TreeArgs& a, int x, int nw
 }
 
 // The chunk x < Hkv np of a shared prefix.  A window leaves its last rows only: as many as
-// the sequence with the fewest cached tokens reaches.
+// the sequence with the fewest cached tokens reaches.  Chunks are whole multiples of UNIT tiles.
+template <int UNIT>
 __device__ __forceinline__ TreeChunk prefix_chunk(const PrefixArgs& a, int x) {
   const int t1 = (a.P + 31) / 32;
   int t0 = 0;
@@ -97,14 +99,14 @@ __device__ __forceinline__ TreeChunk prefix_chunk(const PrefixArgs& a, int x) {
     const int lane = threadIdx.x & 63, B = a.t.p.B;
     unsigned need = 0;
     for (int b = lane; b < B; b += 64) need = max(need, (unsigned)max(a.t.p.window - tree_seq(a.t, b).n, 0));
-    t0 = (a.P - (int)min(wave_max(need), (unsigned)a.P)) / 32;
+    t0 = (a.P - (int)min(wave_max(need), (unsigned)a.P)) / (32 * UNIT) * UNIT;
   }
   TreeChunk r;
   r.b = 0;
   r.hk = x / a.np;
   r.s = x - r.hk * a.np;
   r.ns = a.np;
-  const int each = (t1 - t0 + a.np - 1) / a.np;
+  const int each = (t1 - t0 + a.np * UNIT - 1) / (a.np * UNIT) * UNIT;
   r.first = t0 + r.s * each;
   r.count = max(min(each, t1 - r.first), 0);
   return r;

@@ -170,3 +170,48 @@ def test_empty_and_refused(gpu_device):
                dict(prefix_key=pk[:1], prefix_value=pv[:1]), dict(query=q[:, :7])):
         with pytest.raises(AssertionError):
             fc.shared_prefix_attention(**dict(ok, **kw))
+
+
+MANY = [
+    # dtype, B, Hq, Hkv, T, P, C, lengths, mask, window, cap, scale: eight row tiles of the prefix and more
+    (BF, 64, 8, 1, 1, 1500, 40, [i % 40 for i in range(64)], None, 0, 0.0, None),
+    (FH, 30, 8, 1, 8, 700, 30, [i % 22 for i in range(30)], "batch", 0, 0.0, None),     # two row tiles a sequence
+    (BF, 32, 16, 2, 1, 63, 70, [2 * i for i in range(32)], None, 50, 0.0, None),       # windows that end in the prefix or behind
+    (FH, 64, 4, 1, 1, 1, 9, [i % 9 for i in range(64)], None, 0, 30.0, 0.11),
+    (BF, 63, 4, 1, 1, 2049, 40, [i % 44 - 2 for i in range(63)], None, 1000, 0.0, None),  # sequences that do not fit
+    (FH, 43, 12, 2, 2, 640, 20, [i % 19 for i in range(43)], "shared", 333, 20.0, -0.2),
+    (BF, 16, 16, 1, 1, 8200, 3, [i % 3 for i in range(16)], None, 0, 0.0, 0.0),
+    (BF, 100, 10, 2, 3, 129, 300, [3 * i - 3 for i in range(100)], "holes", 70, 0.0, -0.09),
+]
+
+
+@pytest.mark.parametrize("i", range(len(MANY)))
+def test_many_sequences(gpu_device, i):
+    dtype, B, Hq, Hkv, T, P, C, n, mask, window, cap, scale = MANY[i]
+    q, kc, vc = (draw(s + i, B, h, r, 128, dtype, "bsnd") for s, h, r in ((1, Hq, T), (50, Hkv, C), (90, Hkv, C)))
+    big = torch.full((2, Hkv, P + 40, 128), float("nan"), dtype=dtype, device="cuda")  # a prefix shorter than its buffer
+    big[0, :, 3:3 + P], big[1, :, 3:3 + P] = draw(130 + i, 1, Hkv, P, 128, dtype)[0], draw(170 + i, 1, Hkv, P, 128, dtype)[0]
+    pk, pv = big[0, :, 3:3 + P], big[1, :, 3:3 + P]
+    m = depths = None
+    if mask:
+        made = [tree(T, 7 * i + b, mask) for b in range(B if mask in ("batch", "holes") else 1)]
+        m = torch.stack([x for x, _ in made])
+        depths = torch.stack([d for _, d in made]).expand(B, T)
+    lengths = torch.tensor(n, dtype=torch.int32)
+    args = (q, pk, pv, kc, vc, lengths.cuda())
+    kw = dict(tree_mask=None if m is None else m.cuda(), depths=None if m is None else depths.cuda(), sliding_window=window,
+              soft_cap=cap, scale=scale)
+    o, lse = fc.shared_prefix_attention(*args, return_lse=True, **kw)
+    ro, rl, to, tl = oracle(q, pk, pv, kc, vc, lengths, m, depths, dict(sliding_window=window, scale=scale, soft_cap=cap), dtype)
+    fits = (lengths >= 0) & (lengths + T <= C)
+    check("o", o[fits.cuda()], ro[fits], to[fits])
+    check("lse", lse[fits.cuda()], rl[fits], tl[fits])
+    assert bool(o[~fits.cuda()].isnan().all()) and bool(lse[~fits.cuda()].isnan().all())
+    again = fc.shared_prefix_attention(*args, return_lse=True, **kw)
+    assert torch.equal(o[fits.cuda()], again[0][fits.cuda()]) and torch.equal(lse[fits.cuda()], again[1][fits.cuda()])
+    if i == 0:
+        q[5, 3] = float("nan")  # a row that is not a number leaves the others
+        x = fc.shared_prefix_attention(*args, **kw)
+        assert bool(x[5, 3].isnan().all())
+        x[5, 3] = o[5, 3]
+        assert torch.equal(x, o)
