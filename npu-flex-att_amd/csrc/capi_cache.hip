@@ -285,8 +285,7 @@ TreePlan tree_plan(const flexatt_tree* p) {
   return plan_of(p, tree_share(rowb, (int)elt_size(p->dtype), row_tiles(p)), (rowb >= 256 ? 1 : 2) * (int64_t)cus());
 }
 TreePlan quant_plan(const flexatt_tree* p) {
-  const int share = quant_row_tiles(p->head_dim, row_tiles(p));
-  return plan_of(p, share, (p->head_dim >= 128 || share > 1 ? 1 : 2) * (int64_t)cus());
+  return plan_of(p, 1, (p->head_dim >= 128 ? 1 : 2) * (int64_t)cus());
 }
 // The launch behind a shared prefix, whose rows are those of all sequences: `np` chunks of
 // the prefix, and of each sequence's own cache as TreePlan has them.  Where one round of

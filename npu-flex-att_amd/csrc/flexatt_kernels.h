@@ -231,9 +231,6 @@ inline bool prefix_wide(int row_bytes, int elt_bytes, int64_t all, int64_t own) 
 }
 
 typedef hipError_t (*TreeLauncher)(const TreeArgs&, hipStream_t);
-// Row tiles of one wave of the attention over a cache of 8 bits: two share what a tile's
-// conversion costs, where registers hold them (quant_attn.hip).
-inline int quant_row_tiles(int head_dim, int64_t tiles) { return (head_dim == 64 || head_dim == 128) && tiles > 1 ? 2 : 1; }
 
 typedef hipError_t (*PrefixLauncher)(const PrefixArgs&, hipStream_t);
 typedef hipError_t (*QuantTreeLauncher)(const QuantTreeArgs&, hipStream_t);

@@ -12,17 +12,31 @@
 //    whose weights the scores' accumulators hold.
 // p s' is rounded to fp16 for either type of queries, in which codes are exact: its half
 // step of 2^-11 is far under that of bf16 outputs (bf16 weights: rms errors of 1.3 to 1.6
-// times the output's rounding alone).  For fp16 outputs, where it would be as much as
-// theirs (1.3 to 1.5 times), what the rounding leaves is the operand of MFMAs of its own,
-// which a wave that waits for memory has time for.  fp16's range: weights are taken
-// relative to the running maximum less `lift`, so that 2^lift times the largest scale a
-// wave has met is at most 1; sums and accumulators follow both.
+// times the output's rounding alone, fp16 ones 1.01).  For fp16 outputs, where it would be as
+// much as theirs (1.3 to 1.5 times), what the rounding leaves is the operand of MFMAs of its
+// own, which a wave that waits for memory has time for.  fp16's range: weights are taken
+// relative to the running maximum less `lift`, with 2^lift times the largest scale a wave has
+// met between 2^6 and 2^7; sums and accumulators follow both.
 //
-// A wave has one row tile of 32 packed query rows, or two (MT) that share the tile's LDS
-// reads and conversions, and every NW-th 32-key tile of its workgroup's chunk, copied to
-// its own LDS stages without barriers, the scales with one copy more.
+// A wave has one row tile of 32 packed query rows and every NW-th 32-key tile of its
+// workgroup's chunk in LDS stages of its own, without barriers, the scales with one copy
+// more.  The scores of the next tile, whose conversions and MFMAs wait for nothing, stand
+// between this one's weights and in front of its second product, and a tile's LDS reads at its
+// start (bf16 e4m3 B=8 Hq=32 Hkv=8 D=128, caches of 24576 to 32768: T=1 100 -> 96 us).  Row
+// tiles are workgroups of their own, whose chunk comes from the XCD's L2 after the first:
+// waves that share a tile's copies wait for each other (T=16, two row tiles, 122 and 125 us;
+// T=24 270 -> 180, T=16 over one cache of 4096 17.9 -> 15.2).
 //
-// Bound by HBM for long caches and few rows, by the softmax's VALU work for many.
+// Bound by HBM for long caches and few rows; by the softmax's VALU work, with the conversions
+// a half of all cycles at T=16, for more; by latency for short ones, whose code is fetched
+// once for a few tiles.  Both calls above read 470 MB, 4.9 and 3.9 TB/s.
+//   fp16 the same, T=16: 147 us (with the rest's MFMAs)
+//   fp16 int8 B=4 Hq=28 Hkv=4 T=64, caches of 16384: D=128 147 us; bf16 D=64 104
+//   bf16 e4m3 B=4 Hq=16 Hkv=8 T=1, caches of 16000, D=256: 58 us
+//   fp16 int8 B=2 Hq=16 Hkv=8 T=8, window 4096, soft-cap 50, D=256: 26 us (the merge 4.8)
+//   bf16 e4m3 B=1 Hq=32 Hkv=8 T=1, a cache of 4096, D=128: 13.4 us (9.3 and the merge 4)
+// Equal shares of all key tiles for the workgroups, in place of equal chunks of each
+// sequence, shorten the longest by an eighth and change nothing (T=16 121 -> 123).
 #include <type_traits>
 
 #include "flexatt_device.h"
@@ -139,38 +153,32 @@ __device__ __forceinline__ i32x2 lds_read_tr8(const void* p) {
       (__attribute__((address_space(3))) i32x2*)((__attribute__((address_space(3))) char*)p));
 }
 
-// WPT neighbouring waves, a row tile each, share their key tiles (as in tree_attn.hip).
-template <class T, int CODE, int D, int NW, int WPT, int ST, bool CAP>
-__global__ __launch_bounds__(NW * WPT * 64) __attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : 2)))
+template <class T, int CODE, int D, int NW, int ST, bool CAP>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(D >= 256 ? 1 : 2)))
 void quant_attn_kernel(QuantTreeArgs qa) {
   using C = QuantCfg<D>;
   typedef typename Mfma<T>::v8 V8;
   typedef _Float16 W;  // the weights' type
   constexpr bool REST = __is_same(T, _Float16);  // and what their rounding leaves
-  constexpr int EW = C::E / WPT;                 // copies a wave makes of a K or V tile
-  constexpr int EC = 2 * EW + 1;                 // and of a stage, with scales
-  constexpr int SCB = WPT > 1 ? 256 : 128;       // bytes from K's scales to V's
+  constexpr int EC = 2 * C::E + 1;               // copies of a stage: K, V and the scales
+  constexpr int SCB = 128;                       // bytes from K's scales to V's
   constexpr int STB = 2 * C::TB + 2 * SCB;       // bytes of a stage
-  constexpr int CROWS = WPT * C::RPC;            // rows of the waves' copies
-  constexpr int PK = C::PK > WPT ? C::PK / WPT : 1, PV = C::PV > WPT ? C::PV / WPT : 1;
-  static_assert(WPT <= 2 && C::E % WPT == 0 && ST >= WPT + 1 && NW * ST * STB <= 160 * 1024, "stages");
-  constexpr int kCombine = NW * WPT * 64 * 4 * (2 + 16 * C::DB);
+  static_assert(ST >= 2 && NW * ST * STB <= 160 * 1024, "stages");
+  constexpr int kCombine = NW * 64 * 4 * (2 + 16 * C::DB);
   __shared__ __attribute__((aligned(1024))) char smem[NW * ST * STB > kCombine ? NW * ST * STB : kCombine];
 
   const TreeArgs& a = qa.t;
   const Shape& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid / (WPT * 64));  // its key tiles
-  const int sub = WPT > 1 ? __builtin_amdgcn_readfirstlane((tid >> 6) % WPT) : 0;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // its key tiles
   const int h = lane >> 5, l32 = lane & 31;
 
   // (chunk, row tiles): as in tree_attn.hip
   int rt0 = 0, x = blockIdx.x;
   if (a.nrt > 1) {
-    rt0 = blockIdx.x / 8 % a.nrt * WPT;
+    rt0 = blockIdx.x / 8 % a.nrt;
     x = blockIdx.x / (8 * a.nrt) * 8 + blockIdx.x % 8;
   }
-  rt0 += sub;
   const TreeChunk ck = tree_chunk(a, x, NW);
   if (ck.b < 0) return;
   const int b = ck.b, hk = ck.hk, s = ck.s, ns = ck.ns;
@@ -203,12 +211,12 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   }
   // this lane's offsets in a tile's copies
   const unsigned kss = (unsigned)a.k.ss, vss = (unsigned)a.v.ss;
-  const int crow = lane / C::CPR + sub * C::RPC, cchunk = lane % C::CPR;
-  unsigned kvo[PK], vvo[PV];
+  const int crow = lane / C::CPR, cchunk = lane % C::CPR;
+  unsigned kvo[C::PK], vvo[C::PV];
 #pragma unroll
-  for (int e = 0; e < PK; ++e) kvo[e] = (e * CROWS + crow) * kss + swz_k8<C::CPR>(e * CROWS + crow, cchunk) * 16;
+  for (int e = 0; e < C::PK; ++e) kvo[e] = (e * C::RPC + crow) * kss + swz_k8<C::CPR>(e * C::RPC + crow, cchunk) * 16;
 #pragma unroll
-  for (int e = 0; e < PV; ++e) vvo[e] = (e * CROWS + crow) * vss + swz_v8<C::CPR>(e * CROWS + crow, cchunk) * 16;
+  for (int e = 0; e < C::PV; ++e) vvo[e] = (e * C::RPC + crow) * vss + swz_v8<C::CPR>(e * C::RPC + crow, cchunk) * 16;
   const unsigned wbase = lds_addr_of(smem) + wave * (ST * STB);
   // this wave's LDS reads have returned: the buffer they read may be refilled
   auto reads_done = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
@@ -219,41 +227,41 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   const int nt = __builtin_amdgcn_readfirstlane(max((ck.count - wave + NW - 1) / NW, 0));
   const uint64_t kp = (uint64_t)((const char*)a.k.data + b * a.k.sb + hk * a.k.sh);
   const uint64_t vp = (uint64_t)((const char*)a.v.data + b * a.v.sb + hk * a.v.sh);
-  // (alone a wave copies both tensors' scales, 32 lanes each, of two waves each one's)
-  const float* scales = ((WPT > 1 ? sub : h) ? qa.v_scales : qa.k_scales) + ((int64_t)b * p.Hkv + hk) * p.Skv;
+  // (both tensors' scales in one copy, 32 lanes each)
+  const float* scales = (h ? qa.v_scales : qa.k_scales) + ((int64_t)b * p.Hkv + hk) * p.Skv;
   // K, and V with the scales, of tile j of this wave into its stage
   auto issue_k = [&](int j) {
     const int t = first + NW * j;
-    const unsigned dst = wbase + j % ST * STB + sub * 1024;
+    const unsigned dst = wbase + j % ST * STB;
     const uint64_t base = kp + (uint64_t)(t * C::BN) * kss;
     if (t * C::BN + C::BN - 1 <= last) {
 #pragma unroll
-      for (int e = 0; e < EW; ++e)
-        load_lds16_base(kvo[e % PK], base + (uint64_t)(e / PK * PK * CROWS) * kss, dst + e * (WPT * 1024));
+      for (int e = 0; e < C::E; ++e)
+        load_lds16_base(kvo[e % C::PK], base + (uint64_t)(e / C::PK * C::PK * C::RPC) * kss, dst + e * 1024);
     } else {  // rows behind the last one repeat it
 #pragma unroll 1
-      for (int e = 0; e < EW; ++e) {
-        const int kr = e * CROWS + crow;
-        load_lds16_base(min(kr, last - t * C::BN) * kss + swz_k8<C::CPR>(kr, cchunk) * 16, base, dst + e * (WPT * 1024));
+      for (int e = 0; e < C::E; ++e) {
+        const int kr = e * C::RPC + crow;
+        load_lds16_base(min(kr, last - t * C::BN) * kss + swz_k8<C::CPR>(kr, cchunk) * 16, base, dst + e * 1024);
       }
     }
   };
   auto issue_v = [&](int j) {
     const int t = first + NW * j;
-    const unsigned dst = wbase + j % ST * STB + C::TB + sub * 1024;
+    const unsigned dst = wbase + j % ST * STB + C::TB;
     const uint64_t base = vp + (uint64_t)(t * C::BN) * vss;
     if (t * C::BN + C::BN - 1 <= last) {
 #pragma unroll
-      for (int e = 0; e < EW; ++e)
-        load_lds16_base(vvo[e % PV], base + (uint64_t)(e / PV * PV * CROWS) * vss, dst + e * (WPT * 1024));
+      for (int e = 0; e < C::E; ++e)
+        load_lds16_base(vvo[e % C::PV], base + (uint64_t)(e / C::PV * C::PV * C::RPC) * vss, dst + e * 1024);
     } else {
 #pragma unroll 1
-      for (int e = 0; e < EW; ++e) {
-        const int kr = e * CROWS + crow;
-        load_lds16_base(min(kr, last - t * C::BN) * vss + swz_v8<C::CPR>(kr, cchunk) * 16, base, dst + e * (WPT * 1024));
+      for (int e = 0; e < C::E; ++e) {
+        const int kr = e * C::RPC + crow;
+        load_lds16_base(min(kr, last - t * C::BN) * vss + swz_v8<C::CPR>(kr, cchunk) * 16, base, dst + e * 1024);
       }
     }
-    load_lds4(scales + min(t * C::BN + l32, last), wbase + j % ST * STB + 2 * C::TB + sub * SCB);
+    load_lds4(scales + min(t * C::BN + l32, last), wbase + j % ST * STB + 2 * C::TB);
   };
   // Q: lane half h has elements 32 kc + 16 h .. + 15 of its row, the codes' order
   i32x4 qf[2 * C::KC];
@@ -291,7 +299,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
 #pragma unroll 1  // (a short call's time is its code's)
   for (int j = 1; j < min(nt, ST); ++j) {
     issue_k(j);
-    if (WPT == 1 || j < ST - 1) issue_v(j);
+    issue_v(j);
   }
 
   f32x16 acc[C::DB];
@@ -302,15 +310,14 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   float lift = 90.f, rel = 0x1p90f;
 
   // K of tile j + 1, and all that was issued before it, lands.  What may be in flight
-  // behind it: V of that tile and up to ST - 2 whole tiles; of waves that share tiles, K and
-  // V of ST - 2 tiles in the order V, K, as far as there are tiles.
+  // behind it, as far as there are tiles: V of that tile and up to ST - 2 whole tiles.
   auto landed = [&](int j) {
-    constexpr int N = ST - 2, X = WPT > 1 ? 0 : EW + 1;
+    constexpr int N = ST - 2, X = C::E + 1;
     static_assert(N <= 2, "stages");
     const int more = nt - 2 - j;  // tiles behind tile j + 1
     if (more >= N) wait_vmcnt<N * EC + X>();
-    else if (N > 1 && more == 1) wait_vmcnt<(WPT > 1 ? 2 * EC - EW : EC + X)>();
-    else if (more == 0) wait_vmcnt<EW + 1>();
+    else if (N > 1 && more == 1) wait_vmcnt<EC + X>();
+    else if (more == 0) wait_vmcnt<X>();
     else wait_vmcnt<0>();
   };
   // K's fragments of tile j, and S^T from them: codes alone
@@ -329,32 +336,16 @@ void quant_attn_kernel(QuantTreeArgs qa) {
     return sc;
   };
 
-  const int steps = WPT == 1 ? nt : __builtin_amdgcn_readfirstlane((ck.count + NW - 1) / NW);
-  if constexpr (WPT > 1) {
-    __builtin_amdgcn_s_barrier();  // every wave's copies of its first tile
-    asm volatile("" ::: "memory");
-  }
   i32x4 kf[C::KC];
   read_k(0, kf);
   f32x16 sc = scores(kf);
-  for (int j = 0; j < steps; ++j) {
+  for (int j = 0; j < nt; ++j) {
     const int n0 = (first + NW * j) * C::BN;
     // K of tile j + 1 and V of tile j land; what has been read is refilled
-    if constexpr (WPT > 1) {
-      // this wave's copies have landed and its reads of tile j - 1 have returned ...
-      landed(j);
+    landed(j);
+    if (j + ST < nt) {
       reads_done();
-      __builtin_amdgcn_s_barrier();  // ... and every wave's
-      asm volatile("" ::: "memory");
-      if (j + ST - 1 < nt) issue_v(j + ST - 1);
-      if (j + ST < nt) issue_k(j + ST);
-      if (j >= nt || 32 * rt0 >= R) continue;  // (the last step of waves with one tile less; waves without rows)
-    } else {
-      landed(j);
-      if (j + ST < nt) {
-        reads_done();
-        issue_k(j + ST);
-      }
+      issue_k(j + ST);
     }
     const char* sV = smem + wave * (ST * STB) + j % ST * STB + C::TB;
     const char* sS = sV + C::TB + 16 * h;
@@ -466,18 +457,16 @@ void quant_attn_kernel(QuantTreeArgs qa) {
       }
     }
     sc = next;
-    if constexpr (WPT == 1) {
-      if (j + ST < nt) {
-        reads_done();
-        issue_v(j + ST);
-      }
+    if (j + ST < nt) {
+      reads_done();
+      issue_v(j + ST);
     }
   }
 
   // The (m, l, acc) of a row tile's NW waves combined in wave order through LDS (every
   // wave's copies have landed: its last tile waited for vmcnt 0), then O / l and LSE.
-  float* xm = (float*)smem + sub * NW * 64 * (2 + 16 * C::DB);  // [NW][64]
-  float* xl = xm + NW * 64;                                     // [NW][64]
+  float* xm = (float*)smem;  // [NW][64]
+  float* xl = xm + NW * 64;  // [NW][64]
   f32x4* xa = (f32x4*)(xl + NW * 64);  // [NW][4 DB][64]: columns 8 y + 4 h .. + 3 of row l32
   const float l_tot = l_run + swap_halves(l_run);
   __syncthreads();
@@ -532,23 +521,16 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   }
 }
 
-template <class T, int CODE, int D, int NW, int WPT, int ST>
-void launch_rows(QuantTreeArgs a, hipStream_t st) {
-  a.t.nrt = (int)((((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32 + WPT - 1) / WPT);
-  const dim3 grid((unsigned)((a.t.nchunk + 7) / 8 * 8 * a.t.nrt)), block(NW * WPT * 64);
-  if (a.t.p.cap > 0.f) hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, NW, WPT, ST, true>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, NW, WPT, ST, false>), grid, block, 0, st, a);
-}
-
+// Eight waves of two stages at head dim 128, where LDS leaves a CU one workgroup (four of
+// four: T=1 over the long caches above 96 -> 101 us, B=16 over 2000 rows 17 -> 20); four below,
+// two workgroups of them; two stages at 256, for LDS.
 template <class T, int CODE, int D>
-void launch_code(const QuantTreeArgs& a, hipStream_t st) {
-  const int share = quant_row_tiles(D, ((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32);
-  if constexpr (D == 64 || D == 128) {
-    if (share == 2) launch_rows<T, CODE, D, 4, 2, 4>(a, st);
-    else launch_rows<T, CODE, D, D == 128 ? 8 : 4, 1, D == 128 ? 2 : 4>(a, st);
-  } else {
-    launch_rows<T, CODE, D, 4, 1, D == 32 ? 4 : 2>(a, st);
-  }
+void launch_code(QuantTreeArgs a, hipStream_t st) {
+  constexpr int NW = D == 128 ? 8 : 4, ST = D >= 128 ? 2 : 4;
+  a.t.nrt = (int)(((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32);
+  const dim3 grid((unsigned)((a.t.nchunk + 7) / 8 * 8 * a.t.nrt)), block(NW * 64);
+  if (a.t.p.cap > 0.f) hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, NW, ST, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, NW, ST, false>), grid, block, 0, st, a);
 }
 
 template <class T, int D>

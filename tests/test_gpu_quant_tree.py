@@ -198,3 +198,33 @@ def test_empty_and_refused(gpu_device):
         fc.quantized_tree_attention(**dict(ok, query=q[:, :7]))
     with pytest.raises(AssertionError):
         fc.quantized_tree_attention(**dict(ok, query=q[..., :64].contiguous()))
+
+
+UNEVEN = [
+    # dtype, cache, B, Hq, Hkv, T, C, D, lengths, window
+    (BF, F8, 2, 16, 8, 256, 20300, 64, [20000, 12000], 0),      # workgroups whose share ends in the next head's tiles
+    (FH, I8, 3, 8, 8, 200, 9000, 128, [8800, 4100, 6400], 0),
+    (BF, I8, 4, 8, 4, 160, 9000, 64, [8840, -1, 4500, 8840], 0),  # one that does not fit among them
+    (FH, F8, 3, 8, 4, 250, 20000, 128, [19000, 2000, 5000], 9000),
+    (BF, F8, 9, 16, 4, 16, 9000, 128, [8000, 8100, 0, 8984, 5000, 5100, 33, 1, 7000], 0),
+]
+
+
+@pytest.mark.parametrize("i", range(len(UNEVEN)))
+def test_sequences_of_uneven_lengths(gpu_device, i):
+    dtype, kind, B, Hq, Hkv, T, C, D, n, window = UNEVEN[i]
+    q = draw(i, B, Hq, T, D, dtype)
+    (kc, ks), (vc, vs) = cache(50 + i, B, Hkv, C, D, kind), cache(90 + i, B, Hkv, C, D, kind, 1.0)
+    lengths = torch.tensor(n, dtype=torch.int32)
+    args = (q, kc, vc, ks, vs, lengths.cuda())
+    o, lse = fc.quantized_tree_attention(*args, sliding_window=window, return_lse=True)
+    fits = lengths >= 0
+    for b in range(B):
+        if not fits[b]:
+            assert bool(o[b].isnan().all()) and bool(lse[b].isnan().all())
+            continue
+        ro, rl, to, tl = orc.quantized_tree_attention(*(x[b:b + 1].cpu() for x in args), window=window, dtype=dtype)
+        check("o", o[b:b + 1], ro, to)
+        check("lse", lse[b:b + 1], rl, tl)
+    again = fc.quantized_tree_attention(*args, sliding_window=window, return_lse=True)
+    assert torch.equal(o[fits.cuda()], again[0][fits.cuda()]) and torch.equal(lse[fits.cuda()], again[1][fits.cuda()])
