@@ -9,17 +9,26 @@
 // so one pass over x and gy has both sums of a row, of x^2 and of g w x, before it needs
 // either.
 //
-// A row of 8 bits: s = max(amax, 2^-100) / top, top = 448 (e4m3) or 127 (int8), in 32 bits,
-// and codes round(y / s), to the nearest, of two the even one; y is rounded nowhere
-// before.  |y| / s is top (1 + 2^-19) at most, which rounds to top: nothing is clamped.  A
-// row with an infinity or NaN gets codes of 0 and a scale of NaN: it reads back as NaN.
+// A row of 8 bits: s = max(amax, 2^-100) / top in 32 bits, top = 448 (e4m3) or 127 (int8), and
+// codes round(y / s), to the nearest, of two the even one.  y, amax and y / s are in 64 bits,
+// sines and norm included (for e4m3 y / s is rounded to 32 bits on its way): next to the border of two codes an error of y is one of a whole
+// step, and 32 bits gave a key's code in some 10^5 the wrong neighbour; the quotients of
+// values of 8 or 11 bits lie on borders, where an approximate one decides by its own rounding.
+// y / s is top (1 + 2^-24) at most, which rounds to top: nothing is clamped.  A row with an
+// infinity, NaN or a value beyond 32 bits gets codes of 0 and a scale of NaN: it reads back
+// as NaN.
 //
-// Bound by memory.  As in rotary.hip a thread has 2 x 16 bytes of a token's heads and the
-// sines of them, and walks over heads; a row's threads, 2 to 32 lanes next to each other,
-// join its sums by lane shifts.  What a thread multiplies by, weights times sines, is
-// formed once for all its heads.  The weights' gradients are added up in registers over
+// Bound by memory for long inputs.  As in rotary.hip a thread has 2 x 16 bytes of a token's
+// heads and the sines of them, and walks over heads; a row's threads, 2 to 32 lanes next to
+// each other, join its sums by lane shifts.  What a thread multiplies by, weights times sines,
+// is formed once for all its heads.  The weights' gradients are added up in registers over
 // the heads and tokens of a workgroup, in 32 bits, and over the workgroups by a second
 // launch, in a fixed order.
+//   bf16 B=2 S=4096 Hq=32 Hkv=8 D=128: 37 us, 4.5 TB/s, its gradient 50 us, 5.0 TB/s, and 4
+//   fp16 B=4 S=777 Hq=28 Hkv=4 D=64 into a cache of int8: 11 us, 30 MB and the latency
+// Short inputs are one launch and its latency, 4 to 5 us.
+#include <float.h>
+
 #include "flexatt_device.h"
 #include "flexatt_kernels.h"
 #include "rotary_device.h"
@@ -60,15 +69,24 @@ __device__ __forceinline__ float row_sum(float x) {
   if constexpr (N >= 32) x += __shfl_xor(x, 16);
   return x;
 }
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double x) {
+  const i32x2 w = __builtin_bit_cast(i32x2, x);
+  return __builtin_bit_cast(double, i32x2{__builtin_amdgcn_update_dpp(w[0], w[0], CTRL, 0xf, 0xf, false),
+                                          __builtin_amdgcn_update_dpp(w[1], w[1], CTRL, 0xf, 0xf, false)});
+}
+// The same in 64 bits of two numbers at once, a sum and a maximum (numbers alone).
 template <int N>
-__device__ __forceinline__ unsigned row_max(unsigned x) {
-  const auto step = [&](float y) { x = max(x, __float_as_uint(y)); };
-  step(dpp_f<0xB1>(__uint_as_float(x)));
-  if constexpr (N >= 4) step(dpp_f<0x4E>(__uint_as_float(x)));
-  if constexpr (N >= 8) step(dpp_f<0x141>(__uint_as_float(x)));
-  if constexpr (N >= 16) step(dpp_f<0x140>(__uint_as_float(x)));
-  if constexpr (N >= 32) x = max(x, (unsigned)__shfl_xor((int)x, 16));
-  return x;
+__device__ __forceinline__ void row_join(double& sum, double& top) {
+  const auto step = [&](double a, double b) {
+    sum += a;
+    top = fmax(top, b);
+  };
+  step(dpp_d<0xB1>(sum), dpp_d<0xB1>(top));
+  if constexpr (N >= 4) step(dpp_d<0x4E>(sum), dpp_d<0x4E>(top));
+  if constexpr (N >= 8) step(dpp_d<0x141>(sum), dpp_d<0x141>(top));
+  if constexpr (N >= 16) step(dpp_d<0x140>(sum), dpp_d<0x140>(top));
+  if constexpr (N >= 32) step(__shfl_xor(sum, 16), __shfl_xor(top, 16));
 }
 
 // A thread's place in a row: its pairs' elements, whether they are turned, their sines.
@@ -138,6 +156,27 @@ struct Place {
       if (turned(e)) turn_of(pos, a.inv_freq[pair(e)], a.mag, 1.f, cs[e], sn[e]);
     }
   }
+  // (|x| <= pi / 4; the series' rest is under 4e-13)
+  __device__ __forceinline__ void turns(const RotaryArgs& a, double pos, double (&cs)[E], double (&sn)[E]) const {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      cs[e] = 1.0, sn[e] = 0.0;
+      if (!turned(e)) continue;
+      const double q = pos * (a.inv_freq[pair(e)] * 0.63661977236758134308), n = __builtin_rint(q);
+      const double x = (q - n) * 1.57079632679489661923, z = x * x;
+      const int k = (int)(n - 4.0 * __builtin_floor(n * 0.25));
+      double u = 1.0 / 6227020800, v = 1.0 / 479001600;
+      u = __builtin_fma(u, z, -1.0 / 39916800), v = __builtin_fma(v, z, -1.0 / 3628800);
+      u = __builtin_fma(u, z, 1.0 / 362880), v = __builtin_fma(v, z, 1.0 / 40320);
+      u = __builtin_fma(u, z, -1.0 / 5040), v = __builtin_fma(v, z, -1.0 / 720);
+      u = __builtin_fma(u, z, 1.0 / 120), v = __builtin_fma(v, z, 1.0 / 24);
+      u = __builtin_fma(u, z, -1.0 / 6), v = __builtin_fma(v, z, -0.5);
+      const double sp = __builtin_fma(u * z, x, x), cp = __builtin_fma(v, z, 1.0);
+      const double c = (k & 1) ? sp : cp, s = (k & 1) ? cp : sp;
+      cs[e] = ((k == 1 || k == 2) ? -c : c) * (double)a.mag;
+      sn[e] = ((k & 2) ? -s : s) * (double)a.mag;
+    }
+  }
 };
 
 template <class T>
@@ -145,17 +184,15 @@ __device__ __forceinline__ float weight_at(const void* w, int wide, int i) {
   return wide ? ((const float*)w)[i] : to_f32(((const T*)w)[i]);
 }
 
-// Two codes of 8 bits, of values that are at most the kind's largest in size.
-__device__ __forceinline__ unsigned code4(int kind, float a, float b, float c, float d) {
+// Four codes of 8 bits, of values that round to the kind's largest in size at most.
+__device__ __forceinline__ unsigned code4(int kind, double a, double b, double c, double d) {
   if (kind == FLEXATT_E4M3) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32((float)a, (float)b, 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32((float)c, (float)d, w, true);
   }
-  // x + 1.5 2^23 rounds x to a whole number, whose low byte is the code
-  constexpr float kWhole = 12582912.f;
-  const unsigned p = __float_as_uint(a + kWhole), q = __float_as_uint(b + kWhole);
-  const unsigned r = __float_as_uint(c + kWhole), s = __float_as_uint(d + kWhole);
-  return (p & 255) | (q & 255) << 8 | (r & 255) << 16 | s << 24;
+  // x + 1.5 2^52 rounds x to a whole number, whose low byte is the code
+  const auto whole = [](double x) { return (unsigned)__builtin_bit_cast(i32x2, x + 0x1.8p52)[0]; };
+  return (whole(a) & 255) | (whole(b) & 255) << 8 | (whole(c) & 255) << 16 | whole(d) << 24;
 }
 
 // A workgroup has some heads of q, of k or of v (grid.y: the groups of a.hpt of each) for
@@ -166,7 +203,9 @@ __global__ __launch_bounds__(kThreads) void norm_rotary_kernel(NormRotaryArgs n)
   using C = NormCfg<T, D>;
   using P = Place<T, D, MODE>;
   typedef typename P::vec vec;
-  constexpr int E = C::E, UPR = C::UPR, U = 2, ES = (int)sizeof(T);
+  // rows on their way at once (codes: two take registers that a fourth wave needs, B=4 S=777
+  // D=64 22.3 -> 24.2 us with the read-back)
+  constexpr int E = C::E, UPR = C::UPR, U = CODED ? 1 : 2, ES = (int)sizeof(T);
   const RotaryArgs& a = n.r;
   const int64_t tok = (int64_t)blockIdx.x * C::TPB + threadIdx.x / UPR;
   if (tok >= (int64_t)a.B * a.S) return;  // (whole rows of threads)
@@ -199,68 +238,67 @@ __global__ __launch_bounds__(kThreads) void norm_rotary_kernel(NormRotaryArgs n)
   fetch(0, x, y);
 
   const bool norm = n.norm && which != 2;
+  const void* w = which == 0 ? n.wq : n.wk;
   // y = (a ac - b bs, b bc + a as), times r
-  float ac[E], as[E], bc[E], bs[E];
-  if (which != 2) {
-    float cs[E], sn[E];
-    at.turns(a, pos, cs, sn);
-    const void* w = which == 0 ? n.wq : n.wk;
+  if (coded) {
+    if (!kept) return;  // (whole rows of threads)
+    double ac[E], as[E], bc[E], bs[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float wa = norm ? weight_at<T>(w, n.w_wide, at.first(e)) : 1.f;
-      const float wb = norm ? weight_at<T>(w, n.w_wide, at.second(e)) : 1.f;
-      ac[e] = wa * cs[e], as[e] = wa * sn[e], bc[e] = wb * cs[e], bs[e] = wb * sn[e];
-    }
-  }
-  for (int r0 = 0; r0 < rows; r0 += U) {
-    fetch(r0 + U, nx, ny);
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (r0 + i >= rows) break;
-      char* to = dst + (r0 + i) * vy.sh * (coded ? 1 : ES);
-      if (!CODED && which == 2) {
-        if (kept) at.store(to, x[i], y[i]);
-        continue;
-      }
-      float ya[E], yb[E], sq = 0.f;
+    for (int e = 0; e < E; ++e) ac[e] = bc[e] = 1.0, as[e] = bs[e] = 0.0;
+    if (which != 2) {
+      double cs[E], sn[E];
+      at.turns(a, pos, cs, sn);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float p = P::a_of(x[i], y[i], e), q = P::b_of(x[i], y[i], e);
-        if (which == 2) {
-          ya[e] = p, yb[e] = q;
-          continue;
-        }
-        sq = __builtin_fmaf(p, p, sq);
-        sq = __builtin_fmaf(q, q, sq);
-        const bool t = at.turned(e);
-        ya[e] = t ? __builtin_fmaf(p, ac[e], -(q * bs[e])) : p * ac[e];
-        yb[e] = t ? __builtin_fmaf(q, bc[e], p * as[e]) : q * bc[e];
+        const double wa = norm ? weight_at<T>(w, n.w_wide, at.first(e)) : 1.f;
+        const double wb = norm ? weight_at<T>(w, n.w_wide, at.second(e)) : 1.f;
+        ac[e] = wa * cs[e], as[e] = wa * sn[e], bc[e] = wb * cs[e], bs[e] = wb * sn[e];
       }
-      if (norm) {
-        const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(row_sum<UPR>(sq), 1.0f / D, n.eps));
+    }
+    for (int r0 = 0; r0 < rows; ++r0) {
+      fetch(r0 + 1, nx, ny);
+      double ya[E], yb[E], sq = 0.0, top = 0.0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) ya[e] *= r, yb[e] *= r;
+      for (int e = 0; e < E; ++e) {
+        const double p = P::a_of(x[0], y[0], e), q = P::b_of(x[0], y[0], e);
+        sq = __builtin_fma(p, p, sq);
+        sq = __builtin_fma(q, q, sq);
+        ya[e] = __builtin_fma(p, ac[e], -(q * bs[e]));
+        yb[e] = __builtin_fma(q, bc[e], p * as[e]);
+        top = fmax(top, fmax(fabs(ya[e]), fabs(yb[e])));
       }
-      if (!coded) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) P::put(x[i], y[i], e, ya[e], yb[e]);
-        if (kept) at.store(to, x[i], y[i]);
-        continue;
+      row_join<UPR>(sq, top);
+      double r = 1.0, root = 1.0;
+      if (norm) {  // r = m^-1/2: of the one in 32 bits one step more leaves 2e-14
+        const double m = __builtin_fma(sq, 1.0 / D, (double)n.eps);
+        r = __builtin_amdgcn_rsqf((float)m);
+        r *= __builtin_fma(-0.5 * m * r, r, 1.5);
+        root = m * r;
       }
-      unsigned top = 0;  // largest size; infinities and NaN are larger than numbers
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        top = max(top, max(__float_as_uint(ya[e]) & 0x7fffffffu, __float_as_uint(yb[e]) & 0x7fffffffu));
-      top = row_max<UPR>(top);
-      const bool fine = top < 0x7f800000u;
+      top *= r;
+      // (sq: of an infinity or NaN it is none of the numbers that 32 bits give)
+      const bool fine = sq < 0x1p300 && top <= (double)FLT_MAX;
       // (the largest numbers a little less, so that code * scale is one)
-      const float size = fminf(fmaxf(__uint_as_float(top), 0x1p-100f), 0x1.fffffp127f);
-      const float scale = size / (n.kind == FLEXATT_E4M3 ? 448.f : 127.f);
-      const float inv = 1.0f / scale;
+      const double size = fmin(fmax(top, 0x1p-100), 0x1.fffffp127);
+      const float scale = (float)(size * (n.kind == FLEXATT_E4M3 ? 1.0 / 448 : 1.0 / 127));
+      // y r / scale: the quotient by (scale / r), with its rest (exact where r is 1)
+      const double by = (double)scale * root;
+      double inv = __builtin_amdgcn_rcpf(scale);
+      inv *= __builtin_fma(-inv, (double)scale, 2.0) * r;
 #pragma unroll
-      for (int e = 0; e < E; ++e) ya[e] = fine ? ya[e] * inv : 0.f, yb[e] = fine ? yb[e] * inv : 0.f;
-      if (!kept) continue;
-      if (at.u == 0) scales[(int64_t)(r0 + i) * a.cache_rows] = fine ? scale : __builtin_nanf("");
+      for (int e = 0; e < E; ++e) {
+        const auto over = [&](double v) {
+          const double t = v * inv;
+          return __builtin_fma(__builtin_fma(-t, by, v), inv, t);
+        };
+        ya[e] = over(ya[e]), yb[e] = over(yb[e]);
+      }
+      if (!fine) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) ya[e] = yb[e] = 0.0;
+      }
+      char* to = dst + r0 * vy.sh;
+      if (at.u == 0) scales[(int64_t)r0 * a.cache_rows] = fine ? scale : __builtin_nanf("");
       if constexpr (MODE == kAny) {
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
@@ -277,13 +315,54 @@ __global__ __launch_bounds__(kThreads) void norm_rotary_kernel(NormRotaryArgs n)
       } else {
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const float* v = g ? yb : ya;
+          const double* v = g ? yb : ya;
           char* d = to + (g ? at.c1 : at.c0);
           const unsigned c = code4(n.kind, v[0], v[1], v[2], v[3]);
           if constexpr (E == 8) *(i32x2*)d = i32x2{(int)c, (int)code4(n.kind, v[4], v[5], v[6], v[7])};
           else *(int*)d = (int)c;
         }
       }
+      x[0] = nx[0], y[0] = ny[0];
+    }
+    return;
+  }
+  float ac[E], as[E], bc[E], bs[E];
+  if (which != 2) {
+    float cs[E], sn[E];
+    at.turns(a, pos, cs, sn);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float wa = norm ? weight_at<T>(w, n.w_wide, at.first(e)) : 1.f;
+      const float wb = norm ? weight_at<T>(w, n.w_wide, at.second(e)) : 1.f;
+      ac[e] = wa * cs[e], as[e] = wa * sn[e], bc[e] = wb * cs[e], bs[e] = wb * sn[e];
+    }
+  }
+  for (int r0 = 0; r0 < rows; r0 += U) {
+    fetch(r0 + U, nx, ny);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (r0 + i >= rows) break;
+      char* to = dst + (r0 + i) * vy.sh * ES;
+      if (which != 2) {
+        float ya[E], yb[E], sq = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float p = P::a_of(x[i], y[i], e), q = P::b_of(x[i], y[i], e);
+          sq = __builtin_fmaf(p, p, sq);
+          sq = __builtin_fmaf(q, q, sq);
+          const bool t = at.turned(e);
+          ya[e] = t ? __builtin_fmaf(p, ac[e], -(q * bs[e])) : p * ac[e];
+          yb[e] = t ? __builtin_fmaf(q, bc[e], p * as[e]) : q * bc[e];
+        }
+        if (norm) {
+          const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(row_sum<UPR>(sq), 1.0f / D, n.eps));
+#pragma unroll
+          for (int e = 0; e < E; ++e) ya[e] *= r, yb[e] *= r;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) P::put(x[i], y[i], e, ya[e], yb[e]);
+      }
+      if (kept) at.store(to, x[i], y[i]);
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) x[i] = nx[i], y[i] = ny[i];

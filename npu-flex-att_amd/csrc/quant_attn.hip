@@ -27,14 +27,16 @@
 // waves that share a tile's copies wait for each other (T=16, two row tiles, 122 and 125 us;
 // T=24 270 -> 180, T=16 over one cache of 4096 17.9 -> 15.2).
 //
-// Bound by HBM for long caches and few rows; by the softmax's VALU work, with the conversions
-// a half of all cycles at T=16, for more; by latency for short ones, whose code is fetched
-// once for a few tiles.  Both calls above read 470 MB, 4.9 and 3.9 TB/s.
-//   fp16 the same, T=16: 147 us (with the rest's MFMAs)
-//   fp16 int8 B=4 Hq=28 Hkv=4 T=64, caches of 16384: D=128 147 us; bf16 D=64 104
-//   bf16 e4m3 B=4 Hq=16 Hkv=8 T=1, caches of 16000, D=256: 58 us
-//   fp16 int8 B=2 Hq=16 Hkv=8 T=8, window 4096, soft-cap 50, D=256: 26 us (the merge 4.8)
-//   bf16 e4m3 B=1 Hq=32 Hkv=8 T=1, a cache of 4096, D=128: 13.4 us (9.3 and the merge 4)
+// Bound by HBM for one row tile over long caches (4.9 TB/s there), by the work on a tile from
+// two on: at T=16 VALU instructions, of which the conversions are a third, issue in 0.56 of
+// the cycles and MFMAs run in 0.27, and a wave waits for 0.31 of its time, for what is not
+// known (copies further ahead and fewer instructions changed nothing); by latency for short
+// caches, whose code is fetched once for a few tiles.
+//   fp16 e4m3 the same caches, T=16: 147 us (with the rest's MFMAs)
+//   fp16 int8 B=4 Hq=28 Hkv=4 T=64, caches of 16384: 142 us; bf16 D=64 93
+//   bf16 e4m3 B=4 Hq=16 Hkv=8 T=1, caches of 16000, D=256: 57 us
+//   fp16 int8 B=2 Hq=16 Hkv=8 T=16, window 4096, soft-cap 50, D=256: 26 us
+//   bf16 e4m3 B=1 Hq=32 Hkv=8 T=1, a cache of 4097, D=128: 12 to 14 us (9.3 and the merge 4)
 // Equal shares of all key tiles for the workgroups, in place of equal chunks of each
 // sequence, shorten the longest by an eighth and change nothing (T=16 121 -> 123).
 #include <type_traits>

@@ -235,3 +235,45 @@ def test_in_a_graph_and_versions(gpu_device):
         back = fc.dequantize_cache(*mine, dtype=FH)
         assert torch.equal(y, want) and torch.equal(n, mine[4])
         assert torch.equal(out[0], back[0]) and torch.equal(out[1], back[1])
+
+
+def nearest(y, s, code, kind):
+    """How far codes are from being the nearest of y / s (float64), in half steps."""
+    t, c = y / s[..., None], code.float().double()
+    if kind == I8:
+        return ((t - c).abs() / 0.5).max().item()
+    step = torch.exp2(torch.floor(torch.log2(t.abs().clamp(min=2.0 ** -6))) - 3)  # of e4m3 where t is
+    return ((t - c).abs() / (step / 2)).max().item()
+
+
+@pytest.mark.parametrize("kind", [F8, I8])
+@pytest.mark.parametrize("dtype", [BF, FH, FS])
+def test_codes_at_borders(gpu_device, kind, dtype):
+    """Values are divided by their scale exactly, ties go to the even code; keys are off by far less than 32 bits are.
+
+    e4m3 is rounded from a quotient of 32 bits, 2^-24 of at most 32 half steps off: 2^-19 of a half step.  64 bits leave 1e-11 of a row's largest size (positions up to 3e5 times 2^-53 and the series' 4e-13), 448 and 127 times
+    that on the codes' scale, against half steps of at least 2^-10 and 2^-1."""
+    B, H, S, D = 2, 4, 500, 128
+    k, v = draw(1, B, H, S, D, dtype), draw(2, B, H, S, D, dtype)
+    v[0, :, ::3] = (v[0, :, ::3] * 64).round().clamp(-126, 126) / 2  # whole halves
+    v[0, :, ::3, 5] = 127.0 if kind == I8 else 448.0  # and a scale of 1
+    v[1, :, ::5, 7] = 254.0 if kind == I8 else 28.0   # or 2, or 1/16
+    kc, vc, ks, vs = caches(3, B, H, S, D, kind)
+    f, w = rot.rotary_frequencies(D, device="cuda")[0], weight(4, D, dtype)
+    pos = (torch.arange(S) * 601 % 300000).expand(B, S).contiguous()
+    fc.quantized_append(k[:, :0], k, v, kc, vc, ks, vs, torch.zeros(B, dtype=torch.int32, device="cuda"), f,
+                        positions=pos.cuda(), query_weight=w, key_weight=w, eps=1e-4)
+    x = v.double()
+    s = (x.abs().amax(dim=-1).clamp(min=2.0 ** -100) / orc.TOP[kind]).float()
+    t = (x / s.double()[..., None])
+    want = t.round().to(I8) if kind == I8 else None
+    assert torch.equal(vs, s) and (want is None or torch.equal(vc, want))
+    once = 2.0 ** -19 if kind == F8 else 0.0
+    assert nearest(x, s.double(), vc, kind) <= 1.0 + once
+    if kind == F8:  # a tie's code is even
+        tie = (t - vc.float().double()).abs() * 2 == torch.exp2(torch.floor(torch.log2(t.abs().clamp(min=2.0 ** -6))) - 3)
+        assert int(tie.sum()) > 100 and bool((bits(vc)[tie] % 2 == 0).all())
+    y, _ = orc.norm_rotary(k.cpu().double(), w.cpu().double(), f.cpu(), pos, False, 1.0, float(torch.tensor(1e-4)))
+    size = y.abs().amax(dim=-1) / orc.TOP[kind]
+    assert bool(((ks.cpu().double() - size).abs() <= size * (2.0 ** -24 + 2e-11)).all())
+    assert nearest(y, ks.cpu().double(), kc.cpu(), kind) <= 1.0 + once + 1e-11 * (448 * 2 ** 10 if kind == F8 else 127 * 2)
