@@ -476,8 +476,9 @@ int flexatt_norm_rotary_append(const flexatt_rotary* r, const flexatt_norm* n, c
 
 /* Caches of 8 bits.  A row (one position of one head) is D codes and one fp32 scale s =
  * max(amax, 2^-100) / top, of its values' largest size amax and the largest code top:
- * codes are y / s to the nearest, of two the even one, and stand for code * s.  The values
- * are rounded nowhere before.  A row with an infinity or NaN has codes 0 and scale NaN.
+ * codes are y / s to the nearest, of two the even one, and stand for code * s.  y, amax and
+ * y / s are in 64 bits (for e4m3 the quotient is rounded to 32 on its way).  A row with an
+ * infinity, NaN or a value beyond 32 bits has codes 0 and scale NaN.
  * Code tensors are [B, Hkv, cache_rows, D] views of bytes (strides in bytes, multiples of
  * 16), scales contiguous fp32 [B, Hkv, cache_rows]. */
 enum flexatt_code {

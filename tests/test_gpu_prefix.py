@@ -215,3 +215,30 @@ def test_many_sequences(gpu_device, i):
         assert bool(x[5, 3].isnan().all())
         x[5, 3] = o[5, 3]
         assert torch.equal(x, o)
+
+
+def test_many_sequences_in_a_graph(gpu_device):
+    """Captured once and replayed as lengths and queries change, on another stream too: what an eager call gives."""
+    B, T, P, C = 64, 1, 900, 50
+    q, kc, vc = (draw(s, B, h, r, 128, FH, "bsnd") for s, h, r in ((1, 16, T), (50, 4, C), (90, 4, C)))
+    pk, pv = draw(130, 1, 4, P, 128, FH)[0], draw(170, 1, 4, P, 128, FH)[0]
+    n = torch.arange(B, dtype=torch.int32, device="cuda") % 40
+    args = (q, pk, pv, kc, vc, n)
+    want = fc.shared_prefix_attention(*args, sliding_window=700)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = fc.shared_prefix_attention(*args, sliding_window=700)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fc.shared_prefix_attention(*args, sliding_window=700, return_lse=True)
+    for turn in range(3):
+        q.copy_(draw(10 + turn, B, 16, T, 128, FH))
+        n.copy_(torch.arange(B, dtype=torch.int32) * (7 + turn) % 49)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = fc.shared_prefix_attention(*args, sliding_window=700, return_lse=True)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
