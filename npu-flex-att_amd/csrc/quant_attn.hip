@@ -28,12 +28,12 @@
 // T=24 270 -> 180, T=16 over one cache of 4096 17.9 -> 15.2).
 //
 // Bound by HBM for one row tile over long caches (4.9 TB/s there), by the work on a tile from
-// two on: at T=16 VALU instructions, of which the conversions are a third, issue in 0.56 of
-// the cycles and MFMAs run in 0.27, and a wave waits for 0.31 of its time, for what is not
-// known (copies further ahead and fewer instructions changed nothing); by latency for short
-// caches, whose code is fetched once for a few tiles.
-//   fp16 e4m3 the same caches, T=16: 147 us (with the rest's MFMAs)
-//   fp16 int8 B=4 Hq=28 Hkv=4 T=64, caches of 16384: 142 us; bf16 D=64 93
+// two on: at T=16, 119 us, VALU instructions, of which the conversions are a third, issue in
+// 0.56 of the cycles and MFMAs run in 0.27, and a wave waits for 0.31 of its time, for what is
+// not known (copies further ahead and fewer instructions changed nothing, a raised priority
+// of the products 5%); by latency for short caches, whose code is fetched once for a few tiles.
+//   fp16 e4m3 the same caches, T=16: 141 us (with the rest's MFMAs)
+//   fp16 int8 B=4 Hq=28 Hkv=4 T=64, caches of 16384: 132 us; bf16 D=64 86
 //   bf16 e4m3 B=4 Hq=16 Hkv=8 T=1, caches of 16000, D=256: 57 us
 //   fp16 int8 B=2 Hq=16 Hkv=8 T=16, window 4096, soft-cap 50, D=256: 26 us
 //   bf16 e4m3 B=1 Hq=32 Hkv=8 T=1, a cache of 4097, D=128: 12 to 14 us (9.3 and the merge 4)
@@ -432,6 +432,9 @@ void quant_attn_kernel(QuantTreeArgs qa) {
       read_k(j + 1, kf);
       read_v();
     }
+    // (ahead of the SIMD's other wave: bf16 e4m3 B=8 T=16 125 -> 119 us, fp16 int8 B=4 T=64
+    // D=128 143 -> 132; the part in front of it raised instead 122 and 144)
+    __builtin_amdgcn_s_setprio(1);
     const f32x16 next = scores(kf);
     float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -458,6 +461,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
         if constexpr (REST) acc[db] = Mfma<W>::mma(v, pl, acc[db]);
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     sc = next;
     if (j + ST < nt) {
       reads_done();
