@@ -180,26 +180,43 @@ def code_tolerance(y, slack, scale, code):
 
 def quantized_tree_attention(q, kc, vc, ks, vs, lengths, mask=None, window=0, depths=None, scale=None, cap=0.0,
                              dtype=torch.bfloat16):
-    """O, LSE and their tolerances: those of :func:`tree_attention` over codes * scales.
+    """O, LSE and their tolerances: those of :func:`tree_attention` over codes * scales, but for what the second product
+    rounds.
 
-    The scales add two roundings to a score, 2^-23 of it, and one to a weight.  A weight times its value's scale is
-    rounded to fp16 where p was rounded to the type, relative to a power of two at most twice the largest scale; the
-    numbers under 2^-14 have the step 2^-24: (n + T) 2^-24 times the largest scale and code."""
+    The scales add two roundings to a score, 2^-23 of it.  A weight's exponent is at most 64 in log2 units, rounded at
+    2^-19, and the exponential, the scale and the partials at 2^-20 together.  The weight times its value's scale is rounded
+    to fp16: 2^-11 of it, 2^-22 for fp16 queries, whose rest is a second operand.  It is held relative to the largest scale
+    S that the row has met, S between 2^6 and 2^7, and to a largest weight of at least 2^-1/2, so half of fp16's smallest
+    step, 2^-25, is S 2^-30.5 for a code of 1: (n + T) S top 2^-30.5 over the row's sum of weights, relative to the largest.
+    An accumulator takes two MFMAs of sixteen products from every fourth 32-key tile: (n + T) / 4 + 16 roundings at 2^-24
+    with the joins.  All but the smallest step's are shares of the sum of weights times |values|."""
+    B, Hq, T, D = q.shape
+    G, C, top = Hq // kc.shape[1], kc.shape[2], TOP[kc.dtype]
+    seen = [0 <= int(n) <= C - T for n in lengths]
     k, v = kc.double() * ks.double()[..., None], vc.double() * vs.double()[..., None]
-    O, LSE, tO, tL = tree_attention(q, k, v, lengths, mask, window, depths, scale, cap, dtype, torch.float16)
-    G, T = q.shape[1] // kc.shape[1], q.shape[2]
-    top = TOP[kc.dtype]
-    for b in range(q.shape[0]):
-        n = int(lengths[b])
-        if n < 0 or n + T > kc.shape[2]:
+    O, LSE, tO, tL = tree_attention(q, k, v, lengths, mask, window, depths, scale, cap, dtype)
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    for b in range(B):
+        if not seen[b]:
             continue
-        for h in range(q.shape[1]):
-            x = (q[b, h].double().abs() @ k[b, h // G, :n + T].abs().T).amax() * (abs(scale) if scale is not None else
-                                                                                 1.0 / math.sqrt(q.shape[3]))
-            vmax = v[b, h // G, :n + T].abs().max()
-            tO[b, h] += 2 * x * 2.0 ** -23 * vmax + vmax * 2.0 ** -22
-            tO[b, h] += (n + T) * 2.0 ** -24 * vs[b, h // G, :n + T].double().max() * top
-            tL[b, h] += x * 2.0 ** -23
+        n = int(lengths[b])
+        m = None if mask is None else mask[b % mask.shape[0]] if mask.dim() == 3 else mask
+        ok = tree_allowed(n, T, C, m, window, None if depths is None else depths[b])[:, :n + T]
+        for h in range(Hq):
+            kk, vv, s = k[b, h // G, :n + T], v[b, h // G, :n + T], vs[b, h // G, :n + T].double()
+            x, e = _scores(q[b, h].double(), kk, scale, cap)
+            size = (q[b, h].double().abs() @ kk.abs().T * abs(scale)).masked_fill(~ok, 0.0).amax(dim=-1)
+            e = e.masked_fill(~ok, 0.0).amax(dim=-1) + size * 2.0 ** -23
+            x = x.masked_fill(~ok, float("-inf"))
+            w = torch.exp(x - x.amax(dim=-1, keepdim=True)).nan_to_num(nan=0.0)
+            row = w.sum(dim=-1).clamp(min=1.0)
+            part = (w @ vv.abs()) / row[:, None]
+            half = 2.0 ** -22 if dtype == torch.float16 else 2.0 ** -11
+            share = half + 2 * e + 2.0 ** -19 + 2.0 ** -20 + ((n + T) / 4 + 16) * 2.0 ** -24
+            largest = torch.where(ok, s[None], torch.zeros(())).amax(dim=-1)
+            least = (n + T) * 2.0 ** -30.5 * largest * top / row
+            tO[b, h] = rounded(O[b, h], part * share[:, None] + least[:, None], dtype)
+            tL[b, h] += size * 2.0 ** -23 + 2.0 ** -19
     return O, LSE, tO, tL
 
 
