@@ -54,13 +54,14 @@ def _scores(q, k, scale, cap):
     return x, err + x.abs() * 2.0 ** -22
 
 
-def tree_attention(q, kc, vc, lengths, mask=None, window=0, depths=None, scale=None, cap=0.0, dtype=torch.bfloat16,
-                   weights=None):
+def tree_attention(q, kc, vc, lengths, mask=None, window=0, depths=None, scale=None, cap=0.0, dtype=torch.bfloat16):
     """O, LSE and their tolerances; mask [T, T] or [B, T, T], depths [B, T] or None.
 
-    P is rounded to the type, or to ``weights``, before P V (fp32: not at all): half a step of each weight, and for fp16, whose weights
-    under 2^-14 have the step 2^-24, n 2^-25 in all beside a largest weight of at least 1.  A score error e scales a
-    weight by exp(e) and so the row sum: 2 e max|v|."""
+    P is rounded to the type before P V (fp32: not at all): half a step of each weight, and for fp16, whose weights under
+    2^-14 have the step 2^-24, 2^-25 of each value, over the row's sum of weights relative to a largest of at least 1.  A
+    score error e scales a weight by exp(e) and so the row sum: 2 e; exponentials and partials are at 2^-20, and an
+    accumulator rounds at most once for two keys (fp32: two products a time, of half the tiles; 16 bits: sixteen): (n + T) /
+    2 + 16 roundings at 2^-24.  All but fp16's smallest step are shares of the sum of weights times |values|."""
     B, Hq, T, D = q.shape
     Hkv, C = kc.shape[1:3]
     G = Hq // Hkv
@@ -68,8 +69,7 @@ def tree_attention(q, kc, vc, lengths, mask=None, window=0, depths=None, scale=N
     O = torch.zeros(B, Hq, T, D, dtype=torch.float64)
     LSE = torch.full((B, Hq, T), float("-inf"), dtype=torch.float64)
     tO, tL = torch.zeros_like(O), torch.zeros_like(LSE)
-    weights = weights or dtype
-    half = 0.0 if weights == torch.float32 else EPS[weights] / 2
+    half = 0.0 if dtype == torch.float32 else EPS[dtype] / 2
     for b in range(B):
         n = int(lengths[b])
         if n < 0 or n + T > C:
@@ -84,14 +84,14 @@ def tree_attention(q, kc, vc, lengths, mask=None, window=0, depths=None, scale=N
             lse = torch.logsumexp(x, dim=-1)
             some = ok.any(dim=-1)
             p = torch.exp(x - torch.where(some, lse, torch.zeros_like(lse))[:, None])
-            o = p @ v
             e = e.masked_fill(~ok, 0.0).amax(dim=-1)
-            vmax = torch.where(ok[:, :, None], v.abs()[None], torch.zeros(())).amax(dim=(1, 2))
-            O[b, h] = o
+            share = half + 2 * e + 2.0 ** -20 + ((n + T) / 2 + 16) * 2.0 ** -24
+            loose = (p @ v.abs()) * share[:, None]
+            if dtype == torch.float16:  # (p.amax: the largest weight over the row's sum)
+                loose = loose + (ok.double() @ v.abs()) * p.amax(dim=-1, keepdim=True) * 2.0 ** -25
+            O[b, h] = p @ v
             LSE[b, h] = lse
-            flat = (n + T) * 2.0 ** -25 if weights == torch.float16 else 0.0
-            loose = ((half + 2 * e + flat + 2.0 ** -20) * vmax)[:, None].expand_as(o)
-            tO[b, h] = rounded(o, loose, dtype)
+            tO[b, h] = rounded(O[b, h], loose, dtype)
             tL[b, h] = e + torch.where(some, lse.abs(), torch.zeros_like(lse)) * 2.0 ** -21 + 2.0 ** -20
     return O, LSE, tO, tL
 

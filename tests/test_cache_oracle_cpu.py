@@ -67,3 +67,30 @@ def test_rounded_weights_are_within_the_bounds(i, rest):
     assert bool(((got - o).abs() <= to).all()) or (dtype == FH and not rest)
     ratio = rms(got.to(dtype).double() - o) / rms(o.to(dtype).double() - o)
     assert ratio <= 1.05 if dtype == BF or rest else ratio > 1.15
+
+
+TREES = [
+    # dtype, Hq, Hkv, T, P, C, D, length
+    (BF, 4, 1, 2, 8000, 1100, 128, 1000), (FH, 2, 1, 1, 16383, 700, 128, 600), (FH, 2, 1, 20, 5000, 300, 64, 256),
+    (BF, 2, 1, 4, 100, 20000, 64, 19000), (torch.float32, 1, 1, 3, 2000, 300, 256, 290), (FH, 2, 1, 1, 1, 300, 32, 299),
+]
+
+
+@pytest.mark.parametrize("i", range(len(TREES)))
+def test_bounds_of_tree_and_prefix_are_far_below_the_output(i):
+    """bf16's weights are off by half a step of 2^-8, which is what its bound is for many keys: half of the output."""
+    dtype, Hq, Hkv, T, P, C, D, n = TREES[i]
+    g = torch.Generator().manual_seed(i)
+    q, pk, pv, kc, vc = (torch.randn(*s, D, generator=g).to(dtype)
+                         for s in ((1, Hq, T), (Hkv, P), (Hkv, P), (1, Hkv, C), (1, Hkv, C)))
+    o, lse, to, tl = orc.prefix_attention(q, pk, pv, kc, vc, [n], dtype=dtype)
+    assert rms(to) <= rms(o) / (2 if dtype == BF else 8) and bool((tl < 2e-3).all())
+    k, v = torch.cat((pk[None], kc), dim=2), torch.cat((pv[None], vc), dim=2)
+    same = orc.tree_attention(q, k, v, [P + n], dtype=dtype)
+    assert all(torch.equal(a, b) for a, b in zip((o, lse, to, tl), same))
+    x = (q[0].double().unflatten(0, (Hkv, Hq // Hkv)) @ k[0, :, None, :P + n + T].double().transpose(-1, -2)) / D ** 0.5
+    ok = torch.arange(P + n + T)[None] <= P + n + torch.arange(T)[:, None]
+    p = torch.exp(x.masked_fill(~ok, float("-inf")) - x.amax(dim=-1, keepdim=True))
+    w = p.double() if dtype == torch.float32 else p.to(dtype).double()
+    got = (w @ v[0, :, None, :P + n + T].double() / p.sum(dim=-1, keepdim=True)).flatten(0, 1)[None]
+    assert bool(((got - o).abs() <= to).all())
