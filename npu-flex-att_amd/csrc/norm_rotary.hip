@@ -269,9 +269,9 @@ __global__ __launch_bounds__(kThreads) void norm_rotary_kernel(NormRotaryArgs n)
       }
       row_join<UPR>(sq, top);
       double r = 1.0, root = 1.0;
-      if (norm) {  // r = m^-1/2: of the one in 32 bits one step more leaves 2e-14
+      if (norm) {  // r = m^-1/2, m of any size: of the approximate one in 64 bits one step more leaves 2e-14
         const double m = __builtin_fma(sq, 1.0 / D, (double)n.eps);
-        r = __builtin_amdgcn_rsqf((float)m);
+        r = __builtin_amdgcn_rsq(m);
         r *= __builtin_fma(-0.5 * m * r, r, 1.5);
         root = m * r;
       }
