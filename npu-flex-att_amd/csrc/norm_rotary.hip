@@ -255,6 +255,13 @@ __global__ __launch_bounds__(kThreads) void norm_rotary_kernel(NormRotaryArgs n)
         ac[e] = wa * cs[e], as[e] = wa * sn[e], bc[e] = wb * cs[e], bs[e] = wb * sn[e];
       }
     }
+    // A weight, or an angle's frequency, that is an infinity or NaN makes every row one that is
+    // not of numbers (0 times an infinity too), which the maximum of the rows would not show.
+    double odd = 0.0, none = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) odd += 0.0 * ac[e] + 0.0 * as[e] + 0.0 * bc[e] + 0.0 * bs[e];
+    row_join<UPR>(odd, none);
+    const bool sound = odd == 0.0;
     for (int r0 = 0; r0 < rows; ++r0) {
       fetch(r0 + 1, nx, ny);
       double ya[E], yb[E], sq = 0.0, top = 0.0;
@@ -277,7 +284,7 @@ __global__ __launch_bounds__(kThreads) void norm_rotary_kernel(NormRotaryArgs n)
       }
       top *= r;
       // (sq: of an infinity or NaN it is none of the numbers that 32 bits give)
-      const bool fine = sq < 0x1p300 && top <= (double)FLT_MAX;
+      const bool fine = sound && sq < 0x1p300 && top <= (double)FLT_MAX;
       // (the largest numbers a little less, so that code * scale is one)
       const double size = fmin(fmax(top, 0x1p-100), 0x1.fffffp127);
       const float scale = (float)(size * (n.kind == FLEXATT_E4M3 ? 1.0 / 448 : 1.0 / 127));
