@@ -442,8 +442,8 @@ int flexatt_evict_rows(const flexatt_evict* p, const flexatt_tensor* k_cache, co
                        float* scores_out, int32_t* slots, int32_t* lengths_out, void* stream);
 
 /* Queries and keys normalised for each head, then turned: y = R (x w / sqrt(mean x^2 +
- * eps)), the mean over the head's D elements in 32 bits, R the rotation of
- * flexatt_rotary (inverse 0).  Rounded once. */
+ * eps)), the mean over the head's D elements in 32 bits (of a row whose mean passes them,
+ * scaled by a power of two), R the rotation of flexatt_rotary (inverse 0).  Rounded once. */
 typedef struct flexatt_norm {
   int32_t weight_dtype; /* FLEXATT_F32, or the call's dtype */
   float eps;            /* a normal number above 0 */

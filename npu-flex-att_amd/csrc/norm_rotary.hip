@@ -89,6 +89,17 @@ __device__ __forceinline__ void row_join(double& sum, double& top) {
   if constexpr (N >= 32) step(__shfl_xor(sum, 16), __shfl_xor(top, 16));
 }
 
+// A row whose mean square passes 32 bits (elements of 2^64 and more, which fp16 has not) is
+// normalised 2^-72 times as large: r x is the same.  Whether the wave has one: a branch that no
+// other row takes, free beside the loads (bf16 B=2 S=4096 Hq=32 Hkv=8 D=128, forward and gradient:
+// 91 us with it and without).
+constexpr float kInf = __builtin_inff(), kLess = 0x1p-72f;
+template <class T>
+__device__ __forceinline__ bool passes(float m) {
+  if constexpr (__is_same(T, _Float16)) return false;
+  else return __builtin_amdgcn_ballot_w64(m == kInf) != 0;
+}
+
 // A thread's place in a row: its pairs' elements, whether they are turned, their sines.
 template <class T, int D, int MODE>
 struct Place {
@@ -148,6 +159,12 @@ struct Place {
     } else {
       x[e] = from_f32<T>(a), y[e] = from_f32<T>(b);
     }
+  }
+  // The row 2^-72 times as large, where its mean square m passes 32 bits.
+  static __device__ __forceinline__ void shrink(vec& x, vec& y, float m) {
+    const float s = m == kInf ? kLess : 1.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) put(x, y, e, a_of(x, y, e) * s, b_of(x, y, e) * s);
   }
   __device__ __forceinline__ void turns(const RotaryArgs& a, double pos, float (&cs)[E], float (&sn)[E]) const {
 #pragma unroll
@@ -351,18 +368,25 @@ __global__ __launch_bounds__(kThreads) void norm_rotary_kernel(NormRotaryArgs n)
       if (r0 + i >= rows) break;
       char* to = dst + (r0 + i) * vy.sh * ES;
       if (which != 2) {
-        float ya[E], yb[E], sq = 0.f;
+        float ya[E], yb[E], m = 0.f;
+        for (bool again = false;; again = true) {
+          float sq = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float p = P::a_of(x[i], y[i], e), q = P::b_of(x[i], y[i], e);
-          sq = __builtin_fmaf(p, p, sq);
-          sq = __builtin_fmaf(q, q, sq);
-          const bool t = at.turned(e);
-          ya[e] = t ? __builtin_fmaf(p, ac[e], -(q * bs[e])) : p * ac[e];
-          yb[e] = t ? __builtin_fmaf(q, bc[e], p * as[e]) : q * bc[e];
+          for (int e = 0; e < E; ++e) {
+            const float p = P::a_of(x[i], y[i], e), q = P::b_of(x[i], y[i], e);
+            sq = __builtin_fmaf(p, p, sq);
+            sq = __builtin_fmaf(q, q, sq);
+            const bool t = at.turned(e);
+            ya[e] = t ? __builtin_fmaf(p, ac[e], -(q * bs[e])) : p * ac[e];
+            yb[e] = t ? __builtin_fmaf(q, bc[e], p * as[e]) : q * bc[e];
+          }
+          if (!norm) break;
+          m = __builtin_fmaf(row_sum<UPR>(sq), 1.0f / D, again && m == kInf ? n.eps * kLess * kLess : n.eps);
+          if (again || !passes<T>(m)) break;
+          at.shrink(x[i], y[i], m);
         }
         if (norm) {
-          const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(row_sum<UPR>(sq), 1.0f / D, n.eps));
+          const float r = __builtin_amdgcn_rsqf(m);
 #pragma unroll
           for (int e = 0; e < E; ++e) ya[e] *= r, yb[e] *= r;
         }
@@ -377,9 +401,11 @@ __global__ __launch_bounds__(kThreads) void norm_rotary_kernel(NormRotaryArgs n)
 }
 
 // Gradients.  A workgroup has the heads of one weight (grid.y: groups of a.hpt q heads,
-// then of k heads) and every grid.x-th set of tokens.
+// then of k heads) and every grid.x-th set of tokens.  Three waves a SIMD are what its plan
+// counts on (neighbouring pairs in bf16 else take the registers of two: D=128 94 -> 99 us).
 template <class T, int D, int MODE>
-__global__ __launch_bounds__(kThreads) void norm_rotary_grad_kernel(NormRotaryArgs n) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(MODE == kAny ? 2 : 3)))
+void norm_rotary_grad_kernel(NormRotaryArgs n) {
   using C = NormCfg<T, D>;
   using P = Place<T, D, MODE>;
   typedef typename P::vec vec;
@@ -426,27 +452,35 @@ __global__ __launch_bounds__(kThreads) void norm_rotary_grad_kernel(NormRotaryAr
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         if (hh + i >= hi) break;
-        float ga[E], gb[E], sq = 0.f, dot = 0.f;
+        float ga[E], gb[E], ms = 0.f, dot, down = 1.f;  // (x of a row that is shrunk: r x is as it was)
+        for (bool again = false;; again = true) {
+          float sq = 0.f;
+          dot = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float p = P::a_of(x[i], y[i], e), q = P::b_of(x[i], y[i], e);
-          const float u = P::a_of(gx[i], gy[i], e), v = P::b_of(gx[i], gy[i], e);
-          const bool t = at.turned(e);
-          ga[e] = t ? __builtin_fmaf(u, cs[e], v * sn[e]) : u;
-          gb[e] = t ? __builtin_fmaf(v, cs[e], -(u * sn[e])) : v;
-          sq = __builtin_fmaf(p, p, sq);
-          sq = __builtin_fmaf(q, q, sq);
-          dot = __builtin_fmaf(ga[e] * wa[e], p, dot);
-          dot = __builtin_fmaf(gb[e] * wb[e], q, dot);
+          for (int e = 0; e < E; ++e) {
+            const float p = P::a_of(x[i], y[i], e), q = P::b_of(x[i], y[i], e);
+            const float u = P::a_of(gx[i], gy[i], e), v = P::b_of(gx[i], gy[i], e);
+            const bool t = at.turned(e);
+            ga[e] = t ? __builtin_fmaf(u, cs[e], v * sn[e]) : u;
+            gb[e] = t ? __builtin_fmaf(v, cs[e], -(u * sn[e])) : v;
+            sq = __builtin_fmaf(p, p, sq);
+            sq = __builtin_fmaf(q, q, sq);
+            dot = __builtin_fmaf(ga[e] * wa[e], p, dot);
+            dot = __builtin_fmaf(gb[e] * wb[e], q, dot);
+          }
+          ms = __builtin_fmaf(row_sum<UPR>(sq), 1.0f / D, n.eps * down * down);
+          if (again || !passes<T>(ms)) break;
+          at.shrink(x[i], y[i], ms);
+          if (ms == kInf) down = kLess;
         }
-        const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(row_sum<UPR>(sq), 1.0f / D, n.eps));
+        const float r = __builtin_amdgcn_rsqf(ms), rd = r * down;
         const float m = row_sum<UPR>(dot) * (1.0f / D) * r * r;  // mean(g w x r) r
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const float p = P::a_of(x[i], y[i], e), q = P::b_of(x[i], y[i], e);
           da[e] = __builtin_fmaf(ga[e] * r, p, da[e]);
           db[e] = __builtin_fmaf(gb[e] * r, q, db[e]);
-          P::put(gx[i], gy[i], e, r * __builtin_fmaf(-m, p, ga[e] * wa[e]), r * __builtin_fmaf(-m, q, gb[e] * wb[e]));
+          P::put(gx[i], gy[i], e, rd * __builtin_fmaf(-m, p, ga[e] * wa[e]), rd * __builtin_fmaf(-m, q, gb[e] * wb[e]));
         }
         at.store(pd, gx[i], gy[i]);
         pd += vd.sh * (int)sizeof(T);

@@ -101,7 +101,7 @@ def norm_rotary_embedding(query, key, query_weight, key_weight, inv_freq, positi
 
     A head's row ``x`` becomes the rotation (as :func:`rotary_embedding` gives it, with its
     arguments) of ``x * weight / sqrt(mean(x ** 2) + eps)``, rounded once: squares, sums and
-    the norm are in 32 bits.  ``query_weight`` and ``key_weight``: [D], both of query's
+    the norm are in 32 bits, of rows whose mean square passes them scaled by a power of two.  ``query_weight`` and ``key_weight``: [D], both of query's
     dtype or both float32 (a model whose weights are offsets passes ``1 + w``).  Without a
     key, key and key_weight are None.
 
