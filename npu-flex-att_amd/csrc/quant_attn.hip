@@ -14,9 +14,12 @@
 // step of 2^-11 is far under that of bf16 outputs (bf16 weights: rms errors of 1.3 to 1.6
 // times the output's rounding alone, fp16 ones 1.01).  For fp16 outputs, where it would be as
 // much as theirs (1.3 to 1.5 times), what the rounding leaves is the operand of MFMAs of its
-// own, which a wave that waits for memory has time for.  fp16's range: weights are taken
-// relative to the running maximum less `lift`, with 2^lift times the largest scale a wave has
-// met between 2^6 and 2^7; sums and accumulators follow both.
+// own, which a wave that waits for memory has time for.  fp16's range: what is rounded is the
+// weight relative to the running maximum, times 2^lift, with 2^lift times the largest scale a
+// wave has met between 2^6 and 2^7, and so are the accumulators; the sum of weights is relative
+// to the maximum alone, since values of zeros (scales of 2^-109) beside ones of 2^75 would leave
+// 32 bits with it.  2^lift is part of the weights' exponents up to 2^-32 and 2^32, of the scales
+// beyond.  The running maximum is a whole number, so that sums and accumulators follow it exactly.
 //
 // A wave has one row tile of 32 packed query rows and every NW-th 32-key tile of its
 // workgroup's chunk in LDS stages of its own, without barriers, the scales with one copy
@@ -81,9 +84,11 @@ __device__ __forceinline__ int swz_v8(int r, int c) {
   else return c ^ ((r & 7) << 1);
 }
 
-// What 2^lift times a scale may reach: weights reach 2^8 before the maximum follows
+// What 2^lift times a scale may reach: weights reach 2^8.5 before the maximum follows
 // (kTreeRescale), and fp16 ends at 2^16.
 constexpr float kMostScale = 0x1p7f;
+// The part of a lift that the weights' exponents have.
+constexpr float kMostUp = 32.f;
 
 // Eight codes as an MFMA operand of T.
 template <class T, int CODE>
@@ -121,6 +126,9 @@ __device__ __forceinline__ typename Mfma<T>::v8 operand8(int lo, int hi) {
                    __builtin_bit_cast(int, p[3])};
   return as_v8<typename Mfma<T>::v8>(v);
 }
+
+// x 2^n, n a whole number.
+__device__ __forceinline__ float ldexp(float x, float n) { return __builtin_amdgcn_ldexpf(x, (int)n); }
 
 // acc *= s.  Accumulators of head dim 256 are kept in the other half of the register file:
 // a multiply of its own would have all of them moved there and back around the branch it
@@ -166,7 +174,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   constexpr int SCB = 128;                       // bytes from K's scales to V's
   constexpr int STB = 2 * C::TB + 2 * SCB;       // bytes of a stage
   static_assert(ST >= 2 && NW * ST * STB <= 160 * 1024, "stages");
-  constexpr int kCombine = NW * 64 * 4 * (2 + 16 * C::DB);
+  constexpr int kCombine = NW * 64 * 4 * (3 + 16 * C::DB);
   __shared__ __attribute__((aligned(1024))) char smem[NW * ST * STB > kCombine ? NW * ST * STB : kCombine];
 
   const TreeArgs& a = qa.t;
@@ -308,8 +316,10 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   float m_run = kNegInf, l_run = 0.f;
 #pragma unroll
   for (int db = 0; db < C::DB; ++db) acc[db] = f32x16{};
-  // weights are 2^(x - m_run + lift), and rel = 2^lift times a scale is at most kMostScale
-  float lift = 90.f, rel = 0x1p90f;
+  // acc is relative to 2^(m_run - lift), l_run to 2^m_run; weights are 2^(x - m_run + up), up the
+  // lift as far as kMostUp, and 2^lift times a scale is at most kMostScale
+  float lift = 126.f, up = kMostUp;
+  bool far = true;  // up is not all of it
 
   // K of tile j + 1, and all that was issued before it, lands.  What may be in flight
   // behind it, as far as there are tiles: V of that tile and up to ST - 2 whole tiles.
@@ -406,25 +416,31 @@ void quant_attn_kernel(QuantTreeArgs qa) {
     max16_partial(vs, top, top2);
     top = max2(top, top2);
     top = fmaxf(top, swap_halves(top));
-    const bool grow = mx > m_run + kTreeRescale, over = __builtin_amdgcn_readfirstlane(top * rel > kMostScale);
+    const bool grow = mx > m_run + kTreeRescale;
+    const bool over = __builtin_amdgcn_readfirstlane(ldexp(top, lift) > kMostScale);
     if (over || __builtin_amdgcn_ballot_w64(grow)) {
       // (over: the largest power of two with which the largest scale is below 2^7)
       const int expo = (int)(__float_as_uint(top) >> 23) & 255;
-      const int field = over ? min(max(260 - expo, 1), 217) : (int)lift + 127;
-      const float now = __int_as_float(field << 23);
-      const float m_new = grow ? mx : m_run;
-      const float alpha = (grow ? fast_exp2(m_run - m_new) : 1.f) * (now / rel);
+      const float now = over ? (float)min(max(133 - expo, -126), 126) : lift;
+      const float m_new = grow ? __builtin_rintf(mx) : m_run;
+      const float step = grow ? fast_exp2(m_run - m_new) : 1.f;
       if (j > 0) {  // (the first tile finds zeros)
-        l_run *= alpha;
+        const float alpha = ldexp(step, now - lift);
+        l_run *= step;
         settle(acc[0]);
 #pragma unroll
         for (int db = 0; db < C::DB; ++db) rescale<D>(acc[db], alpha);
       }
       m_run = m_new;
-      rel = now;
-      lift = (float)(field - 127);
+      lift = now;
+      up = fminf(fmaxf(lift, -kMostUp), kMostUp);
+      far = up != lift;
     }
-    const float m_use = (m_run == kNegInf ? 0.f : m_run) - lift;
+    if (far) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) vs[e] = ldexp(vs[e], lift - up);
+    }
+    const float m_use = (m_run == kNegInf ? 0.f : m_run) - up;
 
     // From here on one block: the next tile's scores (behind the last one of what is
     // there, and not used) between this one's weights, whose product follows.
@@ -445,7 +461,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
       rs[e & 3] += pe;
       sc[e] = pe * vs[e];
     }
-    l_run += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+    l_run += ldexp((rs[0] + rs[1]) + (rs[2] + rs[3]), -up);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const Mfma<W>::v8 pb = pack8<W>(sc, 8 * c);
@@ -473,11 +489,13 @@ void quant_attn_kernel(QuantTreeArgs qa) {
   // wave's copies have landed: its last tile waited for vmcnt 0), then O / l and LSE.
   float* xm = (float*)smem;  // [NW][64]
   float* xl = xm + NW * 64;  // [NW][64]
-  f32x4* xa = (f32x4*)(xl + NW * 64);  // [NW][4 DB][64]: columns 8 y + 4 h .. + 3 of row l32
+  float* xu = xl + NW * 64;  // [NW][64]
+  f32x4* xa = (f32x4*)(xu + NW * 64);  // [NW][4 DB][64]: columns 8 y + 4 h .. + 3 of row l32
   const float l_tot = l_run + swap_halves(l_run);
   __syncthreads();
-  xm[wave * 64 + lane] = m_run - lift;  // what l and acc are relative to
+  xm[wave * 64 + lane] = m_run;
   xl[wave * 64 + lane] = l_tot;
+  xu[wave * 64 + lane] = m_run - lift;
 #pragma unroll
   for (int y = 0; y < 4 * C::DB; ++y) {
     const f32x16& v = acc[y / 4];
@@ -485,22 +503,24 @@ void quant_attn_kernel(QuantTreeArgs qa) {
     xa[(wave * 4 * C::DB + y) * 64 + lane] = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
   }
   __syncthreads();
-  float mw[NW], mall = kNegInf;
+  float mw[NW], uw[NW], mall = kNegInf, uall = kNegInf;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
     mw[w] = xm[w * 64 + lane];
+    uw[w] = xu[w * 64 + lane];
     mall = fmaxf(mall, mw[w]);
+    uall = fmaxf(uall, uw[w]);
   }
   float al[NW], L = 0.f;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
     // a wave whose maximum stayed -inf has weights of 0, or NaN scores
-    const float lw = xl[w * 64 + lane];
-    al[w] = mw[w] == kNegInf ? (lw == 0.f ? 0.f : 1.f) : fast_exp2(mw[w] - mall);
-    L = __builtin_fmaf(al[w], lw, L);
+    const float lw = xl[w * 64 + lane], none = lw == 0.f ? 0.f : 1.f;
+    al[w] = mw[w] == kNegInf ? none : fast_exp2(uw[w] - uall);
+    L = __builtin_fmaf(mw[w] == kNegInf ? none : fast_exp2(mw[w] - mall), lw, L);
   }
   const bool empty = L == 0.f;  // no key; NaN (a NaN query row or key) is not
-  const float inv = empty ? 0.f : 1.0f / L;
+  const float inv = empty ? 0.f : 1.0f / L, back = empty ? 0.f : uall - mall;
   if (32 * rt0 + l32 < R) {
     const int64_t row = ((int64_t)b * p.Hq + hq) * p.Sq + qi;
     float* po = a.part_o + (row * a.nsplit + s) * D + 4 * h;
@@ -515,7 +535,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
         for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(al[w], v[e], o[e]);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] *= inv;
+      for (int e = 0; e < 4; ++e) o[e] = ldexp(o[e] * inv, back);
       if (ns > 1) *(f32x4*)(po + 8 * y) = o;
       else st_global8(out + 8 * y, pack4<T>(o[0], o[1], o[2], o[3]));
     }
