@@ -515,8 +515,8 @@ int flexatt_dequant_rows(const flexatt_dequant* p, const flexatt_tensor* k_cache
 
 /* flexatt_tree_fwd over such a cache, for dtype fp16 and bf16 (else FLEXATT_EDTYPE), a
  * tree_mask for up to 2^15 tokens (else FLEXATT_ERANGE).  The scores are q . code times the
- * key's scale; weights times the values' scales, relative to the largest of these, are
- * rounded to fp16 for the second product (for fp16, to two numbers of it). */
+ * key's scale; weights times the values' scales, relative to the largest of these that the
+ * row sees, are rounded to fp16 for the second product (for fp16, to two numbers of it). */
 size_t flexatt_quant_tree_fwd_workspace(const flexatt_tree* p);
 int flexatt_quant_tree_fwd(const flexatt_tree* p, int32_t code, const flexatt_tensor* q, const flexatt_tensor* k_cache,
                            const flexatt_tensor* v_cache, const float* k_scales, const float* v_scales,

@@ -15,8 +15,9 @@
 // times the output's rounding alone, fp16 ones 1.01).  For fp16 outputs, where it would be as
 // much as theirs (1.3 to 1.5 times), what the rounding leaves is the operand of MFMAs of its
 // own, which a wave that waits for memory has time for.  fp16's range: what is rounded is the
-// weight relative to the running maximum, times 2^lift, with 2^lift times the largest scale a
-// wave has met between 2^6 and 2^7, and so are the accumulators; the sum of weights is relative
+// weight relative to the running maximum, times 2^lift, with 2^lift times the largest scale that
+// a row has met in a wave between 2^6 and 2^7, and so are the accumulators (scales that a row
+// does not see are 0 for it, whatever they are); the sum of weights is relative
 // to the maximum alone, since values of zeros (scales of 2^-109) beside ones of 2^75 would leave
 // 32 bits with it.  2^lift is part of the weights' exponents up to 2^-32 and 2^32, of the scales
 // beyond.  The running maximum is a whole number, so that sums and accumulators follow it exactly.
@@ -394,7 +395,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
       const int lo = row_lo - n0 - 4 * h, hi = n + (mask ? p.Sq : qi + 1) - n0 - 4 * h;
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        if ((unsigned)(8 * (e >> 2) + (e & 3) - lo) >= (unsigned)max(hi - lo, 0)) sc[e] = kNegInf;
+        if ((unsigned)(8 * (e >> 2) + (e & 3) - lo) >= (unsigned)max(hi - lo, 0)) sc[e] = kNegInf, vs[e] = 0.f;
       if (mask && n0 + C::BN > n) {  // all of the tile's mask bytes at once
         const unsigned mrow = (unsigned)qi * (unsigned)p.Sq;
         const int u0 = n0 + 4 * h - n;
@@ -403,7 +404,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
         for (int e = 0; e < 16; ++e) mb[e] = mask[mrow + (unsigned)min(max(u0 + 8 * (e >> 2) + (e & 3), 0), p.Sq - 1)];
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (u0 + 8 * (e >> 2) + (e & 3) >= 0 && mb[e] == 0) sc[e] = kNegInf;
+          if (u0 + 8 * (e >> 2) + (e & 3) >= 0 && mb[e] == 0) sc[e] = kNegInf, vs[e] = 0.f;
       }
     }
     float mx, mx2;
@@ -416,9 +417,8 @@ void quant_attn_kernel(QuantTreeArgs qa) {
     max16_partial(vs, top, top2);
     top = max2(top, top2);
     top = fmaxf(top, swap_halves(top));
-    const bool grow = mx > m_run + kTreeRescale;
-    const bool over = __builtin_amdgcn_readfirstlane(ldexp(top, lift) > kMostScale);
-    if (over || __builtin_amdgcn_ballot_w64(grow)) {
+    const bool grow = mx > m_run + kTreeRescale, over = ldexp(top, lift) > kMostScale;
+    if (__builtin_amdgcn_ballot_w64(grow || over)) {
       // (over: the largest power of two with which the largest scale is below 2^7)
       const int expo = (int)(__float_as_uint(top) >> 23) & 255;
       const float now = over ? (float)min(max(133 - expo, -126), 126) : lift;
@@ -434,7 +434,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
       m_run = m_new;
       lift = now;
       up = fminf(fmaxf(lift, -kMostUp), kMostUp);
-      far = up != lift;
+      far = __builtin_amdgcn_ballot_w64(up != lift) != 0;
     }
     if (far) {
 #pragma unroll

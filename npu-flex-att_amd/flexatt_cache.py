@@ -191,9 +191,10 @@ def quantized_tree_attention(query, key_cache, value_cache, key_scales, value_sc
 
     Scores are products with the codes times the key's scale, in 32 bits.  A weight times its
     value's scale is rounded to float16 (for float16 queries to two of them), in which the
-    largest scale is 2 ** 6 at least: a value 2 ** 20 times smaller than the largest keeps
-    eleven bits of a weight of 1.  A ``tree_mask`` is of 2 ** 15 tokens at most.  Scales of
-    rows that a token does not see must be finite, as their values.
+    largest scale that the token sees is 2 ** 6 at least: a value 2 ** 20 times smaller than
+    the largest keeps eleven bits of a weight of 1.  A ``tree_mask`` is of 2 ** 15 tokens at
+    most.  Scales of rows that a token does not see may be anything, their codes anything but
+    float8_e4m3fn's NaN.
     """
     return _lib.native().quant_tree_attention(query, key_cache, value_cache, key_scales, value_scales, lengths, tree_mask,
                                               sliding_window, depths, scale, soft_cap, return_lse)
