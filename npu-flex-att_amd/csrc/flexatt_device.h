@@ -303,6 +303,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 __device__ __forceinline__ void settle(f32x16& a) {
   asm volatile("s_nop 15\n\ts_nop 2" : "+v"(a));
 }
+__device__ __forceinline__ void settle(f32x16& a, f32x16& b) {
+  asm volatile("s_nop 15\n\ts_nop 2" : "+v"(a), "+v"(b));
+}
 // Max of 16 accumulator values as 7 instructions, leaving two partials.
 __device__ __forceinline__ void max16_partial(const f32x16& s, float& f, float& g) {
   const float a = max3(s[0], s[1], s[2]), b = max3(s[3], s[4], s[5]), c = max3(s[6], s[7], s[8]);

@@ -654,6 +654,7 @@ __device__ __forceinline__ void prefix_rows(const PrefixArgs& args, char* smem) 
         pin(sc[bb]);  // finished inside the branch (no selects after it)
       }
     }
+    if constexpr (!CAP) settle(sc[0], sc[1]);  // (as in tree_work)
     float mp[4];
 #pragma unroll
     for (int bb = 0; bb < NB; ++bb) max16_partial(sc[bb], mp[2 * bb], mp[2 * bb + 1]);
