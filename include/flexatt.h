@@ -514,20 +514,22 @@ int flexatt_dequant_rows(const flexatt_dequant* p, const flexatt_tensor* k_cache
                          const flexatt_tensor* v_out, void* stream);
 
 /* flexatt_tree_fwd over such a cache, for dtype fp16 and bf16 (else FLEXATT_EDTYPE), a
- * tree_mask for up to 2^15 tokens (else FLEXATT_ERANGE).  The scores are q . code times the
- * key's scale; weights times the values' scales, relative to the largest of these that the
- * row sees, are rounded to fp16 for the second product (for fp16, to two numbers of it). */
+ * tree_mask for up to 2^15 tokens, and no more workgroups than a launch can have (else
+ * FLEXATT_ERANGE).  The scores are q . code times the key's scale; weights times the values'
+ * scales, relative to the largest of these that the row sees, are rounded to fp16 for the
+ * second product (for fp16, to two numbers of it). */
 size_t flexatt_quant_tree_fwd_workspace(const flexatt_tree* p);
 int flexatt_quant_tree_fwd(const flexatt_tree* p, int32_t code, const flexatt_tensor* q, const flexatt_tensor* k_cache,
                            const flexatt_tensor* v_cache, const float* k_scales, const float* v_scales,
                            const flexatt_tensor* o, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
 /* flexatt_tree_fwd behind a prefix of `prefix_rows` rows (>= 1; with cache_rows at most
- * 2^30, else FLEXATT_ESHAPE) that all sequences share: the keys of a token are the
- * prefix's, then those flexatt_tree_fwd gives it.  A cached row j of sequence b is at
- * position prefix_rows + j, a row of the prefix at its own: a window leaves the rows of the
- * prefix with prefix_rows + n + depths[b][t] - j <= W.  prefix_k and prefix_v are [Hkv,
- * prefix_rows, D] views (stride_b is not used), of rows as those of the cache. */
+ * 2^30, else FLEXATT_ESHAPE; FLEXATT_ERANGE: also more workgroups than a launch can have)
+ * that all sequences share: the keys of a token are the prefix's, then those flexatt_tree_fwd
+ * gives it.  A cached row j of sequence b is at position prefix_rows + j, a row of the prefix
+ * at its own: a window leaves the rows of the prefix with prefix_rows + n + depths[b][t] - j
+ * <= W.  prefix_k and prefix_v are [Hkv, prefix_rows, D] views (stride_b is not used), of rows
+ * as those of the cache. */
 size_t flexatt_prefix_fwd_workspace(const flexatt_tree* p, int32_t prefix_rows);
 int flexatt_prefix_fwd(const flexatt_tree* p, int32_t prefix_rows, const flexatt_tensor* q,
                        const flexatt_tensor* prefix_k, const flexatt_tensor* prefix_v, const flexatt_tensor* k_cache,

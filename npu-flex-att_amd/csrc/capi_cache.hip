@@ -227,12 +227,6 @@ int check_tree(const flexatt_tree* p) {
   return FLEXATT_OK;
 }
 
-int check_quant_tree(const flexatt_tree* p) {
-  FLEXATT_TRY(check_tree(p));
-  if (p->tree_mask && p->tokens > 1 << 15) return FLEXATT_ERANGE;  // (offsets in a mask are 32 bits)
-  return p->dtype == FLEXATT_F32 ? FLEXATT_EDTYPE : FLEXATT_OK;
-}
-
 // [fp16, bf16][head index]
 const QuantTreeLauncher kQuantTree[2][4] = {
     {quant_attn_f16_d32, quant_attn_f16_d64, quant_attn_f16_d128, quant_attn_f16_d256},
@@ -287,6 +281,15 @@ TreePlan tree_plan(const flexatt_tree* p) {
 TreePlan quant_plan(const flexatt_tree* p) {
   return plan_of(p, 1, (p->head_dim >= 128 ? 1 : 2) * (int64_t)cus());
 }
+// A launch's workgroups: whole eights of chunks for each group of row tiles.
+int64_t workgroups(int64_t chunks, int64_t groups) { return (chunks + 7) / 8 * 8 * groups; }
+
+int check_quant_tree(const flexatt_tree* p) {
+  FLEXATT_TRY(check_tree(p));
+  if (p->tree_mask && p->tokens > 1 << 15) return FLEXATT_ERANGE;  // (offsets in a mask are 32 bits)
+  if (p->dtype == FLEXATT_F32) return FLEXATT_EDTYPE;
+  return check_launch(workgroups(quant_plan(p).nchunk, row_tiles(p)), quant_threads(p->head_dim));
+}
 // The launch behind a shared prefix, whose rows are those of all sequences: `np` chunks of
 // the prefix, and of each sequence's own cache as TreePlan has them.  Where one round of
 // workgroups can have it all, the two that make the longest chunk shortest, in steps of the
@@ -298,6 +301,8 @@ struct PrefixPlan {
   TreePlan own;
   int np;
   bool wide;
+  int64_t workgroups;
+  int threads;  // of one
 };
 PrefixPlan prefix_plan(const flexatt_tree* p, int prefix_rows) {
   const int rowb = p->head_dim * (int)elt_size(p->dtype);
@@ -337,6 +342,8 @@ PrefixPlan prefix_plan(const flexatt_tree* p, int prefix_rows) {
     np = np < 1 ? 1 : np > most ? most : np;
   }
   t.np = (int)np;
+  t.workgroups = workgroups(p->heads_kv * np, groups) + workgroups(t.own.nchunk, own_groups);
+  t.threads = wide || share > 1 ? 512 : rowb > 512 ? 128 : 256;
   return t;
 }
 size_t tree_rows(const flexatt_tree* p) { return (size_t)p->batch * p->heads_q * p->tokens; }
@@ -382,7 +389,8 @@ int check_prefix(const flexatt_tree* p, int32_t prefix_rows) {
   FLEXATT_TRY(check_tree(p));
   if (prefix_rows < 1) return FLEXATT_EINVAL;
   if ((int64_t)prefix_rows + p->cache_rows > 1 << 30) return FLEXATT_ESHAPE;
-  return FLEXATT_OK;
+  const PrefixPlan plan = prefix_plan(p, prefix_rows);
+  return check_launch(plan.workgroups, plan.threads);
 }
 
 int check_workspace(size_t need, const void* workspace, size_t bytes) {

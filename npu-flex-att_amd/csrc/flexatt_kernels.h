@@ -230,6 +230,9 @@ inline bool prefix_wide(int row_bytes, int elt_bytes, int64_t all, int64_t own) 
   return elt_bytes == 2 && row_bytes == 256 && own <= 2 && (all + 7) / 8 * 8 * 6 <= all * 7;
 }
 
+// Threads of a workgroup over a cache of 8 bits (quant_attn.hip).
+constexpr int quant_threads(int head_dim) { return head_dim == 128 ? 512 : 256; }
+
 typedef hipError_t (*TreeLauncher)(const TreeArgs&, hipStream_t);
 
 typedef hipError_t (*PrefixLauncher)(const PrefixArgs&, hipStream_t);

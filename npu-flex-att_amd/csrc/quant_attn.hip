@@ -552,7 +552,7 @@ void quant_attn_kernel(QuantTreeArgs qa) {
 // two workgroups of them; two stages at 256, for LDS.
 template <class T, int CODE, int D>
 void launch_code(QuantTreeArgs a, hipStream_t st) {
-  constexpr int NW = D == 128 ? 8 : 4, ST = D >= 128 ? 2 : 4;
+  constexpr int NW = quant_threads(D) / 64, ST = D >= 128 ? 2 : 4;
   a.t.nrt = (int)(((int64_t)a.t.p.G * a.t.p.Sq + 31) / 32);
   const dim3 grid((unsigned)((a.t.nchunk + 7) / 8 * 8 * a.t.nrt)), block(NW * 64);
   if (a.t.p.cap > 0.f) hipLaunchKernelGGL((quant_attn_kernel<T, CODE, D, NW, ST, true>), grid, block, 0, st, a);
