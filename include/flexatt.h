@@ -457,10 +457,10 @@ int flexatt_norm_rotary_apply(const flexatt_rotary* r, const flexatt_norm* n, co
                               const flexatt_tensor* k, const flexatt_tensor* q_out, const flexatt_tensor* k_out,
                               void* stream);
 
-/* Its gradients: dq, dk and the weights' (device [D] of weight_dtype, sums over all rows
- * in 32 bits) from q, k and the gradients of q_out and k_out.  k, k_grad, dk and dk_weight
- * are NULL when heads_kv is 0.  `workspace` as in flexatt_tree_fwd.  No output, nor the
- * workspace, may lie within an input or another of them. */
+/* Its gradients (FLEXATT_ERANGE alike): dq, dk and the weights' (device [D] of weight_dtype,
+ * sums over all rows in 32 bits) from q, k and the gradients of q_out and k_out.  k, k_grad,
+ * dk and dk_weight are NULL when heads_kv is 0.  `workspace` as in flexatt_tree_fwd.  No
+ * output, nor the workspace, may lie within an input or another of them. */
 size_t flexatt_norm_rotary_grad_workspace(const flexatt_rotary* r);
 int flexatt_norm_rotary_grad(const flexatt_rotary* r, const flexatt_norm* n, const flexatt_tensor* q,
                              const flexatt_tensor* k, const flexatt_tensor* q_grad, const flexatt_tensor* k_grad,

@@ -85,10 +85,15 @@ int check_norm(const flexatt_rotary* r, const flexatt_norm* n) {
   return FLEXATT_OK;
 }
 
+// (numbers of heads with a group's added to them fit 32 bits)
+int check_norm_heads(const flexatt_rotary* r) {
+  return (int64_t)r->heads_q + r->heads_kv > 1 << 30 ? FLEXATT_ERANGE : FLEXATT_OK;
+}
+
 // The launch of norm_rotary.hip: a workgroup has 256 / (D / (32 / size)) tokens, and of many
 // tokens all heads of q, k or v; few tokens make some thousand workgroups at most.
 int check_norm_launch(const flexatt_rotary* r, bool append) {
-  if ((int64_t)r->heads_q + r->heads_kv > 1 << 30) return FLEXATT_ERANGE;
+  FLEXATT_TRY(check_norm_heads(r));
   const int64_t per = 256 / (r->head_dim * (int)elt_size(r->dtype) / 32), kinds = (r->heads_q > 0) + (r->heads_kv > 0) * (append ? 2 : 1);
   return check_launch(((int64_t)r->batch * r->seqlen + per - 1) / per * kinds, 256);
 }
@@ -512,7 +517,7 @@ int flexatt_norm_rotary_apply(const flexatt_rotary* r, const flexatt_norm* n, co
 }
 
 size_t flexatt_norm_rotary_grad_workspace(const flexatt_rotary* r) {
-  if (check_rotary(r, false) != FLEXATT_OK) return SIZE_MAX;
+  if (check_rotary(r, false) != FLEXATT_OK || check_norm_heads(r) != FLEXATT_OK) return SIZE_MAX;
   const NormGradPlan p = norm_grad_plan(r->batch, r->seqlen, r->heads_q, r->heads_kv, r->head_dim, (int)elt_size(r->dtype));
   return (size_t)p.columns * (p.q_groups + p.k_groups) * r->head_dim * sizeof(float);
 }
@@ -523,6 +528,7 @@ int flexatt_norm_rotary_grad(const flexatt_rotary* r, const flexatt_norm* n, con
                              void* workspace, size_t workspace_bytes, void* stream) {
   FLEXATT_TRY(check_rotary(r, false));
   FLEXATT_TRY(check_norm(r, n));
+  FLEXATT_TRY(check_norm_heads(r));
   FLEXATT_TRY(check_tensor(q, r->dtype));
   FLEXATT_TRY(check_tensor(q_grad, r->dtype));
   FLEXATT_TRY(check_out_tensor(dq, r->dtype, r->batch, r->heads_q, r->seqlen, r->head_dim));
