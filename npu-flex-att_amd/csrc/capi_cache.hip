@@ -712,6 +712,10 @@ int flexatt_prefix_fwd(const flexatt_tree* p, int32_t prefix_rows, const flexatt
                        size_t workspace_bytes, void* stream) {
   FLEXATT_TRY(check_prefix(p, prefix_rows));
   FLEXATT_TRY(check_tensor(q, p->dtype));
+  if (!prefix_k || !prefix_v) return FLEXATT_EINVAL;
+  flexatt_tensor pk = *prefix_k, pv = *prefix_v;
+  pk.stride_b = pv.stride_b = 0;  // (no batch)
+  prefix_k = &pk, prefix_v = &pv;
   for (const flexatt_tensor* x : {prefix_k, prefix_v, k_cache, v_cache}) {
     FLEXATT_TRY(check_tensor(x, p->dtype));
     const int rows = x == prefix_k || x == prefix_v ? prefix_rows : p->cache_rows;  // (as flexatt_tree_fwd)
