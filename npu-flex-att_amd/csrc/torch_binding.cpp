@@ -390,13 +390,17 @@ struct NormRotary : torch::autograd::Function<NormRotary> {
                          const Tensor& h) {
       return norm_rotate_grad(x, w, g, y, v, h, saved[4], pos, interleaved, magnitude, eps);
     };
-    if (gq.defined() && gk.defined()) {
+    // (not for a frozen query or key, or one that this pass does not ask for; the tensors are inputs 0 to 3, or 0 and 1)
+    const bool keyed = saved[1].defined();
+    const bool q = gq.defined() && (ctx->needs_input_grad(0) || ctx->needs_input_grad(keyed ? 2 : 1));
+    const bool k = gk.defined() && (ctx->needs_input_grad(1) || ctx->needs_input_grad(3));
+    if (q && k) {
       const NormGrads r = run(saved[0], saved[2], gq, saved[1], saved[3], gk);
       out[0] = r.dx, out[2] = r.dw, out[1] = r.dy, out[3] = r.dv;
-    } else if (gq.defined()) {
+    } else if (q) {
       const NormGrads r = run(saved[0], saved[2], gq, Tensor(), Tensor(), Tensor());
       out[0] = r.dx, out[2] = r.dw;
-    } else if (gk.defined()) {
+    } else if (k) {
       const NormGrads r = run(saved[1], saved[3], gk, Tensor(), Tensor(), Tensor());
       out[1] = r.dx, out[3] = r.dw;
     }
