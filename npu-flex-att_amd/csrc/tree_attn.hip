@@ -32,7 +32,13 @@
 // unrounded ones), which over many keys averages out to about what O's own rounding is:
 // the rms error of bf16 outputs is 1.8e-3 to 2.3e-3 of their rms, 1.7e-3 the output's
 // rounding alone, of fp16 ones 2.9e-4 and 2.1e-4; the same rounding in a plain fp32
-// computation gives the same errors to three digits.
+// computation gives the same errors to three digits.  Behind a shared prefix, where a wave
+// has a row tile alone (few sequences) and waits for memory, what the rounding leaves is an
+// operand of MFMAs of its own: errors of 1.3 to 1.4 times the output's rounding become 1.00,
+// at 2% (B=4 T=1 behind 16000 rows 21.9 -> 22.3 us, 2048 rows of B=8 14.8 -> 14.9).  Where
+// waves share key tiles it costs 5 to 13% (D=128 12 sequences behind 8000 rows 18.4 -> 19.9
+// us, D=64 16 of 8 tokens 25.8 -> 29.3) and eight row tiles a workgroup are bound by their
+// MFMAs, so there P is rounded as above.
 // What bounds it: K and V from HBM for long caches and few rows; from some hundred
 // rows per KV head on the softmax's VALU work and the MFMAs; latency for short caches.
 // Of that the instructions are the larger part: a launch finds the instruction cache
@@ -139,6 +145,7 @@ constexpr int tree_lds() {
 template <class T, int D, int NW, int WPT, int ST, bool CAP, int KIND>
 __device__ __forceinline__ void tree_work(const ArgsOf<KIND != kTree>& args, char* smem, int block) {
   constexpr bool PRE = KIND != kTree;
+  constexpr bool REST = KIND == kBoth && WPT == 1 && sizeof(T) == 2;  // (what P's rounding leaves is a second operand)
   const TreeArgs& a = tree_of(args);
   using C = TreeCfg<T, D>;
   constexpr int EC = C::E / WPT;  // copies a wave makes of a tile
@@ -449,12 +456,19 @@ __device__ __forceinline__ void tree_work(const ArgsOf<KIND != kTree>& args, cha
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const V8 pb = pack8<T>(pe, 8 * c);
+        V8 pl;
+        if constexpr (REST) {
+#pragma unroll
+          for (int t = 0; t < 8; ++t) pl[t] = from_f32<T>(pe[8 * c + t] - to_f32(pb[t]));
+        }
         const char* vr = sV + 16 * c * C::ROWB;
 #pragma unroll
         for (int db = 0; db < C::DB; ++db) {
           const i16x4 lo = lds_read_tr4(vr + voff[db]);
           const i16x4 hi = lds_read_tr4(vr + 8 * C::ROWB + voff[db]);
-          acc[db] = Mfma<T>::mma(cat_tr<V8>(lo, hi), pb, acc[db]);
+          const V8 v = cat_tr<V8>(lo, hi);
+          acc[db] = Mfma<T>::mma(v, pb, acc[db]);
+          if constexpr (REST) acc[db] = Mfma<T>::mma(v, pl, acc[db]);
         }
       }
     }

@@ -149,6 +149,10 @@ def shared_prefix_attention(query, prefix_key, prefix_value, key_cache, value_ca
     position ``P + j``: append to it with ``positions`` that say so.  The other arguments
     and results are those of :func:`tree_attention`; ``sliding_window`` W counts positions,
     so it keeps row ``j`` of the prefix where ``P + lengths[b] + depths[b][t] - j <= W``.
+
+    Weights are rounded to the type for the second product, as there, but not where all
+    sequences' query rows of a KV head (B, T and Hq / Hkv multiplied) are 32 or fewer, or with
+    a head dim of 256: what the rounding leaves is added.
     """
     return _lib.native().prefix_attention(query, prefix_key, prefix_value, key_cache, value_cache, lengths, tree_mask,
                                           sliding_window, depths, scale, soft_cap, return_lse)
