@@ -462,6 +462,9 @@ void quant_attn_kernel(QuantTreeArgs qa) {
       sc[e] = pe * vs[e];
     }
     l_run += ldexp((rs[0] + rs[1]) + (rs[2] + rs[3]), -up);
+    // (products are numbers of 32 bits from here on: one rounded to fp16 in a fused step and, for
+    // its rest, again by way of 32 bits, is another number in 1 of 10^4)
+    if constexpr (REST) pin(sc);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const Mfma<W>::v8 pb = pack8<W>(sc, 8 * c);
