@@ -26,3 +26,23 @@ def test_error_beside_the_outputs_rounding(gpu_device, dtype, cap, B, Hq, Hkv, T
     ref = orc.prefix_attention(*(x.cpu() for x in (q, pk, pv, kc, vc)), n, cap=cap, dtype=dtype)[0]
     rms = lambda x: x.square().mean().sqrt().item()  # noqa: E731
     assert rms(o - ref) <= most * rms(ref.to(dtype).double() - ref)
+
+
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("dtype", [BF, FH])
+@pytest.mark.parametrize("D,P,T,n", [(128, 70, 3, 50), (64, 40, 2, 20), (256, 150, 4, 90), (32, 17, 1, 12)])
+def test_each_weight(gpu_device, dtype, cap, D, P, T, n):
+    """A value of its own column for each key: an output is that key's weight, which has lost nothing but the output's
+    rounding."""
+    B, Hq, Hkv, C = 2, 8, 2, n + T
+    q, kc, pk = draw(1, B, Hq, T, D, dtype), draw(2, B, Hkv, C, D, dtype), draw(3, 1, Hkv, P, D, dtype)[0]
+    pv, vc = torch.zeros(Hkv, P, D), torch.zeros(B, Hkv, C, D)
+    pv[:, torch.arange(P), torch.arange(P)] = 1.0
+    vc[:, :, torch.arange(C), P + torch.arange(C)] = 1.0
+    pv, vc = pv.to(dtype).cuda(), vc.to(dtype).cuda()
+    lengths = torch.full((B,), n, dtype=torch.int32)
+    o = fc.shared_prefix_attention(q, pk, pv, kc, vc, lengths.cuda(), soft_cap=cap)
+    ref, _, _, _ = orc.prefix_attention(*(x.cpu() for x in (q, pk, pv, kc, vc)), lengths, cap=cap, dtype=dtype)
+    eps = torch.finfo(dtype).eps  # half a step, and scores' errors of some 2^-16 each
+    least = 2.0 ** -24 if dtype == FH else 0.0
+    assert bool(((o.cpu().double() - ref).abs() <= ref * (eps / 2 + 2.0 ** -14) + least).all())
