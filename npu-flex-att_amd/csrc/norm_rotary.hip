@@ -11,12 +11,12 @@
 //
 // A row of 8 bits: s = max(amax, 2^-100) / top in 32 bits, top = 448 (e4m3) or 127 (int8), and
 // codes round(y / s), to the nearest, of two the even one.  y, amax and y / s are in 64 bits,
-// sines and norm included (for e4m3 y / s is rounded to 32 bits on its way): next to the border of two codes an error of y is one of a whole
-// step, and 32 bits gave a key's code in some 10^5 the wrong neighbour; the quotients of
-// values of 8 or 11 bits lie on borders, where an approximate one decides by its own rounding.
-// y / s is top (1 + 2^-24) at most, which rounds to top: nothing is clamped.  A row with an
-// infinity, NaN or a value beyond 32 bits gets codes of 0 and a scale of NaN: it reads back
-// as NaN.
+// sines and norm included (for e4m3 y / s is rounded to 32 bits on its way): next to the border
+// of two codes an error of y is one of a whole step, and 32 bits gave a key's code in some 10^5
+// the wrong neighbour; the quotients of values of 8 or 11 bits lie on borders, where an
+// approximate one decides by its own rounding.  y / s is top (1 + 2^-24) at most, which rounds
+// to top: nothing is clamped.  A row with an infinity, NaN or a value beyond 32 bits, be it by a
+// weight or a frequency, gets codes of 0 and a scale of NaN: it reads back as NaN.
 //
 // Bound by memory for long inputs.  As in rotary.hip a thread has 2 x 16 bytes of a token's
 // heads and the sines of them, and walks over heads; a row's threads, 2 to 32 lanes next to

@@ -29,15 +29,15 @@
 // start (bf16 e4m3 B=8 Hq=32 Hkv=8 D=128, caches of 24576 to 32768: T=1 100 -> 96 us).  Row
 // tiles are workgroups of their own, whose chunk comes from the XCD's L2 after the first:
 // waves that share a tile's copies wait for each other (T=16, two row tiles, 122 and 125 us;
-// T=24 270 -> 180, T=16 over one cache of 4096 17.9 -> 15.2).
+// T=24 270 -> 180, 171 now, T=16 over one cache of 4096 17.9 -> 15.2).
 //
 // Bound by HBM for one row tile over long caches (4.9 TB/s there), by the work on a tile from
-// two on: at T=16, 119 us, VALU instructions, of which the conversions are a third, issue in
-// 0.56 of the cycles and MFMAs run in 0.27, and a wave waits for 0.31 of its time, for what is
-// not known (copies further ahead and fewer instructions changed nothing, a raised priority
+// two on: at T=16, 117 us, VALU instructions, of which the conversions are a third, issue in
+// 0.52 of the cycles and MFMAs run in 0.25, and a wave cannot issue for 0.29 of its time, for what
+// is not known (copies further ahead and fewer instructions changed nothing, a raised priority
 // of the products 5%); by latency for short caches, whose code is fetched once for a few tiles.
-//   fp16 e4m3 the same caches, T=16: 141 us (with the rest's MFMAs)
-//   fp16 int8 B=4 Hq=28 Hkv=4 T=64, caches of 16384: 132 us; bf16 D=64 86
+//   fp16 e4m3 the same caches, T=16: 136 us (with the rest's MFMAs; VALU 0.59, MFMAs 0.34)
+//   fp16 int8 B=4 Hq=28 Hkv=4 T=64, caches of 16384: 126 us; bf16 D=64 81
 //   bf16 e4m3 B=4 Hq=16 Hkv=8 T=1, caches of 16000, D=256: 57 us
 //   fp16 int8 B=2 Hq=16 Hkv=8 T=16, window 4096, soft-cap 50, D=256: 26 us
 //   bf16 e4m3 B=1 Hq=32 Hkv=8 T=1, a cache of 4097, D=128: 12 to 14 us (9.3 and the merge 4)

@@ -134,7 +134,7 @@ __device__ __forceinline__ const TreeArgs& tree_of(const PrefixArgs& a) { return
 // once for all of them; the others have the sequences' own caches.  Every row has partials of
 // the prefix's chunks and of its own, joined as above.  Bound by latency for few rows, by the
 // products for many, whose workgroups stand beside those of the own caches, which wait for
-// memory (bf16 Hq=32 Hkv=8 D=128: B=8 T=1 behind 2048 rows, caches of 60 to 300: 13.8 us, the
+// memory (bf16 Hq=32 Hkv=8 D=128: B=8 T=1 behind 2048 rows, caches of 60 to 300: 14.2 us, the
 // merge 4; fp16 B=32 T=4 behind 16383, caches of 300 to 1024: 66 to 74 us, the merge 7).
 enum { kTree, kBoth, kOwn };  // no prefix; a workgroup of either kind; of the second alone
 template <class T, int D, int NW, int WPT, int ST>

@@ -166,7 +166,8 @@ def quantized_append(query, key, value, key_cache, value_cache, key_scales, valu
     A row's scale is its largest size (at least 2 ** -100) over the largest code, 448
     (float8_e4m3fn) or 127 (int8), and its codes are the values over the scale, rounded to
     the nearest, of two the even one; keys are rounded nowhere before, and what decides a
-    code is in 64 bits.  A row with an infinity or NaN gets codes of 0 and a scale of NaN.
+    code is in 64 bits.  A row with an infinity or NaN, be it by a weight or a frequency, gets
+    codes of 0 and a scale of NaN.
     Rows of the cache and its scales that no token goes to are left as they were; the new
     tokens, both caches and both scales share no memory.
     """

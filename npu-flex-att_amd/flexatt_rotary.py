@@ -101,9 +101,9 @@ def norm_rotary_embedding(query, key, query_weight, key_weight, inv_freq, positi
 
     A head's row ``x`` becomes the rotation (as :func:`rotary_embedding` gives it, with its
     arguments) of ``x * weight / sqrt(mean(x ** 2) + eps)``, rounded once: squares, sums and
-    the norm are in 32 bits, of rows whose mean square passes them scaled by a power of two.  ``query_weight`` and ``key_weight``: [D], both of query's
-    dtype or both float32 (a model whose weights are offsets passes ``1 + w``).  Without a
-    key, key and key_weight are None.
+    the norm are in 32 bits, of rows whose mean square passes them scaled by a power of two.
+    ``query_weight`` and ``key_weight``: [D], both of query's dtype or both float32 (a model
+    whose weights are offsets passes ``1 + w``).  Without a key, key and key_weight are None.
 
     Differentiable in query, key and both weights, in reverse mode and once: a backward pass
     with ``create_graph`` is refused.  The weights' gradients are sums over all rows in 32
